@@ -410,6 +410,59 @@ int q4fc_emb_q8c_quant(const float* table, int64_t V, int64_t E, int8_t* codes, 
 int q4fc_emb_q8c(const void* ids, int ids_are_i32, int64_t n, const int8_t* codes, const float* scales, int64_t V,
                  int64_t E, float* out, int64_t ldo, q4fc_stream_t stream);
 
+/* ---- rows grouped by an id: experts and adapters ------------------------------------------------------------------
+ * No counterpart in the reference, whose every FC gives all rows the same weights.  Where the weights depend on the row
+ * (the experts that a router chose for a token, the adapter of a request), rows of one group are computed together; the
+ * plan that sorts them is made once and serves every such call of a step.
+ *
+ *   q4fc_groups_bytes   size of a plan for `rows` ids out of [0, n_groups); 0 for a size beyond the limits below.
+ *   q4fc_group_rows     ids: int32 or int64 [rows] on the device.  A negative id stands for no group; an id >= n_groups
+ *                       too, and sets the device status word that q4fc_fc_check_status(NULL, ..) reads.
+ *   q4fc_route_top_k    the router of a layer of experts and the plan of its choice.  logits: fp32 [tokens][ld].  Per
+ *                       token p = softmax over the experts in fp32; ids (int32 [tokens][top_k]) are the top_k experts of
+ *                       the largest logits, the lowest index first where they are equal; weights (fp32, the same shape)
+ *                       their p, or with renormalize != 0 p divided by the sum of the chosen ones.  An expert whose
+ *                       logit is -inf is closed: never chosen; where too few are open the remaining slots have id -1
+ *                       and weight 0.  A NaN logit is never chosen either and makes the token's weights NaN.
+ * The plan is device memory of q4fc_groups_bytes bytes, 16-byte aligned, written whole by each call: int32 words
+ * [0, 16) for the library, [16, 16 + n_groups + 1) the first place in `order` of each group (and of the rows without one),
+ * then, from the next multiple of four words on, order[rows]: the row numbers sorted by group, stable, those without a
+ * group last.  Limits: n_groups <= 1024, rows <= 2^23, top_k <= 32 and <= experts; beyond them Q4FC_ELIMIT. */
+size_t q4fc_groups_bytes(int64_t rows, int64_t n_groups);
+int q4fc_group_rows(const void* ids, int ids_are_i32, int64_t rows, int64_t n_groups, void* groups, q4fc_stream_t stream);
+int q4fc_route_top_k(const float* logits, int64_t tokens, int64_t experts, int64_t ld, int64_t top_k, int renormalize,
+                     float* weights, int32_t* ids, void* groups, q4fc_stream_t stream);
+
+/* FC by expert (a layer of experts behind a router).  Per (token, slot) pair the product is that of q4fc_fc:
+ * h[t][s] = quantized(x) . W[id of the pair], with x the token's row, or with x_per_slot a row of the pair's own.
+ * Without weights y is fp32 [tokens * top_k][ldy], the pairs' products; with weights (fp32 [tokens][top_k]) y is
+ * [tokens][ldy] and y[t] = sum over the slots, in their order, of weights[t][s] * h[t][s].  A pair without an expert (id -1,
+ * or one out of range) counts as a row of zeros.  With silu_mul a row of x is gate[K], then up[K], and what is quantized
+ * is silu(gate) * up as in q4fc_silu_mul_quant: gate and up projections packed as one weight tensor of 2 K columns feed the
+ * down projection directly.
+ * groups: the plan of the tokens * top_k ids, made with n_groups = experts.  most_rows: no expert has more pairs, as far as
+ * the caller knows (tokens, where a token's experts differ, as q4fc_route_top_k chooses them), or 0.  Anything the plan
+ * says beyond it is an error of the caller's that leaves outputs unwritten.
+ * ws: q4fc_experts_workspace_bytes bytes of scratch, 256-byte aligned; nothing is kept in it between calls, calls that may
+ * overlap need separate ones.  Sums have a fixed order that depends on the sizes, the counts of rows per expert and the card.
+ * flags: Q4FC_FLAG_NIBBLE_SIGNED. */
+typedef struct q4fc_experts_call {
+    const float* x;      /* fp32 [tokens][ldx], or with x_per_slot [tokens * top_k][ldx] */
+    int64_t tokens, top_k, K, ldx;
+    int x_per_slot, silu_mul;
+    const void* wq;      /* packed [experts][Ng][Kg][BS] */
+    int64_t experts, Ng, Kg, N;
+    int qtype, group_k;
+    const void* groups;
+    int64_t most_rows;
+    const float* weights; /* NULL, or fp32 [tokens][top_k] */
+    float* y;
+    int64_t ldy;
+} q4fc_experts_call;
+size_t q4fc_experts_workspace_bytes(int64_t tokens, int64_t top_k, int64_t K, int64_t N, int group_k, int64_t experts,
+                                    int weighted);
+int q4fc_fc_experts(const q4fc_experts_call* call, void* ws, size_t ws_bytes, unsigned flags, q4fc_stream_t stream);
+
 /* Reads and clears the device status word kept at the start of a workspace
  * (host-synchronous: waits for `stream`).  ws = NULL reads the word that decode
  * calls made without a workspace share (one per device).  Returns Q4FC_OK or

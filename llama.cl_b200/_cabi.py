@@ -31,6 +31,7 @@ SYMBOLS = (
     "q4fc_silu_mul_quant", "q4fc_quant_x_q8_batch",
     "q4fc_fc_chain_create", "q4fc_fc_chain_run", "q4fc_fc_chain_check", "q4fc_fc_chain_destroy",
     "q4fc_q8c_pack", "q4fc_q8c_workspace_bytes", "q4fc_q8c_fc", "q4fc_emb_q8c_quant", "q4fc_emb_q8c",
+    "q4fc_groups_bytes", "q4fc_group_rows", "q4fc_route_top_k", "q4fc_experts_workspace_bytes", "q4fc_fc_experts",
 )
 
 
@@ -115,6 +116,31 @@ class FcCall(C.Structure):
     ]
 
 
+class ExpertsCall(C.Structure):
+    """``q4fc_experts_call`` of include/q4fc_b200.h."""
+    _fields_ = [
+        ("x", C.c_void_p),
+        ("tokens", C.c_int64),
+        ("top_k", C.c_int64),
+        ("K", C.c_int64),
+        ("ldx", C.c_int64),
+        ("x_per_slot", C.c_int),
+        ("silu_mul", C.c_int),
+        ("wq", C.c_void_p),
+        ("experts", C.c_int64),
+        ("Ng", C.c_int64),
+        ("Kg", C.c_int64),
+        ("N", C.c_int64),
+        ("qtype", C.c_int),
+        ("group_k", C.c_int),
+        ("groups", C.c_void_p),
+        ("most_rows", C.c_int64),
+        ("weights", C.c_void_p),
+        ("y", C.c_void_p),
+        ("ldy", C.c_int64),
+    ]
+
+
 _lib = None
 
 
@@ -166,6 +192,13 @@ def lib() -> C.CDLL:
     L.q4fc_q8c_fc.argtypes = [vp, i64, i64, i64, vp, vp, i64, i64, i64, vp, i64, vp, sz, vp]
     L.q4fc_emb_q8c_quant.argtypes = [vp, i64, i64, vp, vp, vp]
     L.q4fc_emb_q8c.argtypes = [vp, i32, i64, vp, vp, i64, i64, vp, i64, vp]
+    L.q4fc_groups_bytes.restype = sz
+    L.q4fc_groups_bytes.argtypes = [i64, i64]
+    L.q4fc_group_rows.argtypes = [vp, i32, i64, i64, vp, vp]
+    L.q4fc_route_top_k.argtypes = [vp, i64, i64, i64, i64, i32, vp, vp, vp, vp]
+    L.q4fc_experts_workspace_bytes.restype = sz
+    L.q4fc_experts_workspace_bytes.argtypes = [i64, i64, i64, i64, i32, i64, i32]
+    L.q4fc_fc_experts.argtypes = [C.POINTER(ExpertsCall), vp, sz, u32, vp]
     L.q4fc_tp_site_bytes.restype = sz
     if L.q4fc_tp_site_bytes() != C.sizeof(TpSite):
         raise RuntimeError(f"q4fc_tp_site is {L.q4fc_tp_site_bytes()} bytes in the library, {C.sizeof(TpSite)} here")

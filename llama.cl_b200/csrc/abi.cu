@@ -7,7 +7,7 @@
 #include <cstring>
 #include <mutex>
 
-#include "common.cuh"
+#include "groups.cuh"
 
 namespace q4fc {
 
@@ -97,6 +97,27 @@ int check_fc_args(const char* who, const float* x, int64_t rows, int64_t K, int6
             set_error("%s: packed weights need 16-byte alignment, x and y 4-byte", who);
             return Q4FC_EALIGN;
         }
+    }
+    return Q4FC_OK;
+}
+
+int check_groups(const char* who, int64_t rows, int64_t n_groups, const void* groups) {
+    if (rows < 0 || n_groups < 1) {
+        set_error("%s: negative or empty size (rows=%lld n_groups=%lld)", who, (long long)rows, (long long)n_groups);
+        return Q4FC_EINVAL;
+    }
+    if (n_groups > kMaxGroups || rows > kMaxGroupRows) {
+        set_error("%s: n_groups=%lld exceeds %lld, or rows=%lld 2^23", who, (long long)n_groups, (long long)kMaxGroups,
+                  (long long)rows);
+        return Q4FC_ELIMIT;
+    }
+    if (!groups) {
+        set_error("%s: null plan", who);
+        return Q4FC_EINVAL;
+    }
+    if (!aligned(groups, 16)) {
+        set_error("%s: the plan needs 16-byte alignment", who);
+        return Q4FC_EALIGN;
     }
     return Q4FC_OK;
 }
@@ -482,6 +503,96 @@ int q4fc_fc(const float* x, int64_t rows, int64_t K, int64_t ldx, const void* wq
     if (rows <= kMaxDecodeRows)
         return q4fc_fc_decode(x, rows, K, ldx, wq, Ng, Kg, qtype, group_k, N, y, ldy, ws, ws_bytes, flags, stream);
     return q4fc_fc_prefill(x, rows, K, ldx, wq, Ng, Kg, qtype, group_k, N, y, ldy, ws, ws_bytes, flags, stream);
+}
+
+size_t q4fc_groups_bytes(int64_t rows, int64_t n_groups) {
+    if (rows < 0 || n_groups < 1 || n_groups > kMaxGroups || rows > kMaxGroupRows) return 0;
+    return (size_t)group_plan(nullptr, rows, n_groups).bytes;
+}
+
+int q4fc_group_rows(const void* ids, int ids_are_i32, int64_t rows, int64_t n_groups, void* groups, q4fc_stream_t stream) {
+    if (int rc = check_groups("group_rows", rows, n_groups, groups)) return rc;
+    if (rows > 0 && (!ids || !aligned(ids, ids_are_i32 ? 4 : 8))) {
+        set_error("group_rows: null or misaligned ids");
+        return Q4FC_EINVAL;
+    }
+    return launch_group_rows(ids, ids_are_i32 != 0, rows, n_groups, groups, static_cast<cudaStream_t>(stream));
+}
+
+int q4fc_route_top_k(const float* logits, int64_t tokens, int64_t experts, int64_t ld, int64_t top_k, int renormalize,
+                     float* weights, int32_t* ids, void* groups, q4fc_stream_t stream) {
+    if (top_k < 1 || top_k > experts || tokens < 0) {
+        set_error("route_top_k: top_k=%lld outside 1..%lld experts, or tokens=%lld", (long long)top_k, (long long)experts,
+                  (long long)tokens);
+        return Q4FC_EINVAL;
+    }
+    if (top_k > 32 || tokens > kMaxGroupRows) {
+        set_error("route_top_k: top_k=%lld exceeds 32, or tokens=%lld 2^23", (long long)top_k, (long long)tokens);
+        return Q4FC_ELIMIT;
+    }
+    if (int rc = check_groups("route_top_k", tokens * top_k, experts, groups)) return rc;
+    if (tokens > 0 && (!logits || !weights || !ids || ld < experts || !aligned(logits, 4) || !aligned(weights, 4) || !aligned(ids, 4))) {
+        set_error("route_top_k: null or misaligned logits, weights or ids, or a leading dimension smaller than the row");
+        return Q4FC_EINVAL;
+    }
+    return launch_route_top_k(logits, tokens, experts, ld, top_k, renormalize != 0, weights, ids, groups,
+                              static_cast<cudaStream_t>(stream));
+}
+
+size_t q4fc_experts_workspace_bytes(int64_t tokens, int64_t top_k, int64_t K, int64_t N, int group_k, int64_t experts,
+                                    int weighted) {
+    if (tokens < 0 || top_k < 1 || top_k > 32 || tokens > kMaxGroupRows / top_k || K <= 0 || N < 0 || K > 0x7fffffffLL ||
+        N > 0x7fffffffLL || (group_k != 32 && group_k != 128) || experts < 1 || experts > kMaxGroups)
+        return 0;
+    return align_up(experts_scratch_bytes(tokens * top_k, K, N, group_k, experts, weighted != 0), 256) + 256;
+}
+
+int q4fc_fc_experts(const q4fc_experts_call* call, void* ws, size_t ws_bytes, unsigned flags, q4fc_stream_t stream) {
+    if (!call) {
+        set_error("fc_experts: null call");
+        return Q4FC_EINVAL;
+    }
+    const q4fc_experts_call& c = *call;
+    if (c.tokens < 0 || c.top_k < 1 || c.most_rows < 0) {
+        set_error("fc_experts: negative or empty size (tokens=%lld top_k=%lld most_rows=%lld)", (long long)c.tokens,
+                  (long long)c.top_k, (long long)c.most_rows);
+        return Q4FC_EINVAL;
+    }
+    if (c.top_k > 32 || c.tokens > kMaxGroupRows) {
+        set_error("fc_experts: top_k=%lld exceeds 32, or tokens=%lld 2^23", (long long)c.top_k, (long long)c.tokens);
+        return Q4FC_ELIMIT;
+    }
+    const int64_t rows = c.tokens * c.top_k;
+    if (int rc = check_groups("fc_experts", rows, c.experts, c.groups)) return rc;
+    // (a row of gate and up is as long as two)
+    if (int rc = check_fc_args("fc_experts", c.x, rows, c.K, c.silu_mul && c.ldx < 2 * c.K ? 0 : c.ldx, c.wq, c.Ng, c.Kg, c.qtype,
+                               c.group_k, c.N, c.y, c.ldy))
+        return rc;
+    if (rows == 0 || c.N == 0) return Q4FC_OK;
+    if (c.weights && !aligned(c.weights, 4)) {
+        set_error("fc_experts: misaligned weights");
+        return Q4FC_EALIGN;
+    }
+    if (c.K > 0x3fffffffLL || c.N > 0x3fffffffLL || c.Ng > 0x7fffffffLL / 32) {
+        set_error("fc_experts: K=%lld or N=%lld beyond the limit", (long long)c.K, (long long)c.N);
+        return Q4FC_ELIMIT;
+    }
+    const size_t need = q4fc_experts_workspace_bytes(c.tokens, c.top_k, c.K, c.N, c.group_k, c.experts, c.weights != nullptr);
+    if (!ws || ws_bytes < need) {
+        set_error("fc_experts: workspace of %zu bytes given, %zu needed", ws ? ws_bytes : 0, need);
+        return Q4FC_EWORKSPACE;
+    }
+    if (!aligned(ws, 256)) {
+        set_error("fc_experts: workspace needs 256-byte alignment");
+        return Q4FC_EALIGN;
+    }
+    ExpertsCall e = {};
+    e.x = c.x, e.rows = rows, e.K = c.K, e.ldx = c.ldx, e.per_row = c.x_per_slot ? 1 : c.top_k, e.gated = c.silu_mul != 0;
+    e.wq = static_cast<const uint8_t*>(c.wq), e.Ng = c.Ng, e.Kg = c.Kg, e.qtype = c.qtype, e.G = c.group_k, e.N = c.N;
+    e.plan = group_plan(const_cast<void*>(c.groups), rows, c.experts), e.n = c.experts;
+    e.most_rows = c.most_rows > 0 && c.most_rows < rows ? c.most_rows : rows;
+    e.y = c.y, e.ldy = c.ldy, e.flags = flags, e.scratch = static_cast<uint8_t*>(ws);
+    return launch_fc_experts(e, c.weights, c.top_k, static_cast<cudaStream_t>(stream));
 }
 
 size_t q4fc_tp_site_bytes(void) { return sizeof(q4fc_tp_site); }

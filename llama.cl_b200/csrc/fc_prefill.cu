@@ -61,8 +61,10 @@
 
 #include <atomic>
 #include <cfloat>
+#include <cmath>
 #include <mutex>
 
+#include "groups.cuh"
 #include "prefill_common.cuh"
 
 namespace cg = cooperative_groups;
@@ -313,7 +315,7 @@ __device__ __forceinline__ void merge_sums(uint64_t (&run)[2][8], uint32_t at, u
     if (two) store(run[1], at + step);
 }
 
-template <int FMT, int G, int TM, int FOLD>
+template <int FMT, int G, int TM, int FOLD, bool GROUPED>
 __global__ void __launch_bounds__(PrefillShape<FMT, G, TM, FOLD>::kThreads, TM == 128 ? 1 : 2)
     fc_prefill_kernel(const PrefillParams p, const __grid_constant__ CUtensorMap codes_map) {
     using S = PrefillShape<FMT, G, TM, FOLD>;
@@ -346,8 +348,13 @@ __global__ void __launch_bounds__(PrefillShape<FMT, G, TM, FOLD>::kThreads, TM =
     int n_tile = (int)(blockIdx.x / cs) + p.n_off, m_tile = (int)blockIdx.y + p.m_off;
     if (n_tile >= p.n_tiles) n_tile -= p.n_tiles, m_tile++;
     if (m_tile > p.m_end || (m_tile == p.m_end && n_tile >= p.n_end)) return;  // (the whole cluster)
-    const int64_t n0 = (int64_t)n_tile * kTileN, m0 = (int64_t)m_tile * TM;
-    const int live = (int)min((int64_t)TM, p.rows - m0);  // rows of this tile that exist
+    if (GROUPED && m_tile >= __ldcg(p.tile_count)) {
+        if (m_tile == 0) pdl_wait_prior_grid();  // no tile at all: this launch's end still stands for the quantizer's
+        return;
+    }
+    const RowTile tile = row_tile<GROUPED, TM>(p, m_tile);
+    const int64_t n0 = (int64_t)n_tile * kTileN, m0 = tile.m0;
+    const int live = tile.live;  // rows of this tile that exist
     const int nstage = (p.Kg + GPS - 1) / GPS;
     const int it0 = (int)((int64_t)nstage * rank / cs), it1 = (int)((int64_t)nstage * (rank + 1) / cs);
     const int iters = it1 - it0;
@@ -496,6 +503,11 @@ __global__ void __launch_bounds__(PrefillShape<FMT, G, TM, FOLD>::kThreads, TM =
                     for (int j = 0; j < 8; j++) {
                         float lo, hi;
                         unpack2(acc[h][j], lo, hi);
+                        if (GROUPED) {
+                            if (mc + 2 * j < live) y_row<GROUPED>(p, m0 + mc + 2 * j)[n] = lo;
+                            if (mc + 2 * j + 1 < live) y_row<GROUPED>(p, m0 + mc + 2 * j + 1)[n] = hi;
+                            continue;
+                        }
                         if (FMT == kQ8C) lo = __fmul_rn(ws, lo), hi = __fmul_rn(ws, hi);
                         if (mc + 2 * j < live) *dst = lo;
                         dst += p.ldy;
@@ -522,7 +534,7 @@ __global__ void __launch_bounds__(PrefillShape<FMT, G, TM, FOLD>::kThreads, TM =
         const int pw = warp - kUnpackWarp;
         const int nb = n_tile * 4 + pw;
         const bool stripe_live = nb < p.Ng;  // (columns beyond the weights: nothing is read, nothing is stored)
-        const uint8_t* stripe = p.wq + (int64_t)nb * p.Kg * BS;
+        const uint8_t* stripe = tile.wq + (int64_t)nb * p.Kg * BS;
         auto issue_raw = [&](int i) {
             const int it = it0 + i, slot = (i % S::kRaw) * 4 + pw;
             const uint32_t bytes = (uint32_t)(min(GPS, p.Kg - it * GPS) * BS);
@@ -709,7 +721,7 @@ __global__ void __launch_bounds__(PrefillShape<FMT, G, TM, FOLD>::kThreads, TM =
                 for (int c = 0; c < 4; c++) {
                     const int64_t n = n0 + lane + 32 * c;
                     if (n < p.N)
-                        p.y[(m0 + m) * p.ldy + n] = FMT == kQ8C ? __fmul_rn(__ldg(p.wscales + n), out[c]) : out[c];
+                        y_row<GROUPED>(p, m0 + m)[n] = FMT == kQ8C ? __fmul_rn(__ldg(p.wscales + n), out[c]) : out[c];
                 }
             }
         }
@@ -777,13 +789,13 @@ int make_codes_map(CUtensorMap* map, const int8_t* codes, int64_t rows, int64_t 
     return Q4FC_OK;
 }
 
-template <int FMT, int G, int TM, int FOLD = 0>
+template <int FMT, int G, int TM, int FOLD = 0, bool GROUPED = false>
 int launch_prefill_variant(const PrefillParams& p, const CUtensorMap& map, dim3 grid, cudaStream_t s) {
     using S = PrefillShape<FMT, G, TM, FOLD>;
     static std::atomic<bool> attr_done[64] = {};  // set once per device; a second setter repeats the same call
     int dev = 0;
     Q4FC_CUDA_OK(cudaGetDevice(&dev));
-    auto* fn = fc_prefill_kernel<FMT, G, TM, FOLD>;
+    auto* fn = fc_prefill_kernel<FMT, G, TM, FOLD, GROUPED>;
     if (dev >= 64 || !attr_done[dev]) {
         Q4FC_CUDA_OK(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem));
         Q4FC_CUDA_OK(cudaFuncSetAttribute(fn, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared));
@@ -1083,6 +1095,80 @@ int launch_fc_prefill(const float* x, int64_t rows, int64_t K, int64_t ldx, cons
     // the reference's 1/16 activation scale of Q4_0 pairs with its x16 nibble shift; neither is materialised
     return launch_gemm(qtype == 1 ? kQ4_1 : sgn ? kQ4_0Signed : kQ4_0, G, x, rows, K, ldx,
                        reinterpret_cast<int8_t*>(base + l.codes), reinterpret_cast<float*>(base + l.sc), wide, p, s);
+}
+
+// ---- experts: the rows sorted by the weights they take ------------------------------------------------------------------------------
+namespace {
+
+// Row tiles in use as the host can know them, when every expert is as likely: the experts that `rows` pairs reach, and half a tile more
+// for each of these than the rows fill.
+float likely_tiles(int size, int64_t rows, int64_t n) {
+    const double used = n * (1.0 - exp(rows * log1p(-1.0 / n)));
+    const double filled = (double)rows / size + 0.5 * used;
+    return (float)(n == 1 ? (rows + size - 1) / size : used > filled ? used : filled);
+}
+struct GroupedPlan {
+    int which;  // of the plan's tiles
+    bool f16;
+    int split;
+    size_t codes, sc, bytes;  // scratch
+};
+// The wide kernel where experts have more than 64 rows in the mean.
+int grouped_tiles(int64_t rows, int64_t n) { return rows > 64 * n ? kTiles128 : kTiles64; }
+GroupedPlan grouped_scratch(int64_t rows, int64_t Kg, int G, int64_t n) {
+    GroupedPlan g = {};
+    g.which = grouped_tiles(rows, n), g.f16 = g.which == kTiles128 && wide_codes_f16(G);
+    g.sc = align_up((size_t)(rows * Kg * G) * (g.f16 ? 2 : 1), 256);
+    g.bytes = g.sc + align_up((size_t)(most_tiles(g.which, rows, n) * tile_rows(g.which) * Kg) * 2 * 4, 256);
+    return g;
+}
+template <int FMT, int G>
+int launch_grouped(int which, const PrefillParams& p, const CUtensorMap& map, dim3 grid, cudaStream_t s) {
+    return which == kTiles128 ? launch_prefill_wide_grouped(FMT, G, p, map, grid, s)
+                              : launch_prefill_variant<FMT, G, 64, 0, true>(p, map, grid, s);
+}
+
+}  // namespace
+
+size_t experts_gemm_scratch(int64_t rows, int64_t Kg, int G, int64_t n) { return grouped_scratch(rows, Kg, G, n).bytes; }
+
+int launch_experts_gemm(const ExpertsCall& c, GroupQuant q, cudaStream_t s) {
+    const DeviceInfo* di = device_info();
+    if (!di) return Q4FC_ECUDA;
+    const GroupedPlan g = grouped_scratch(c.rows, c.Kg, c.G, c.n);
+    const int64_t Kp = c.Kg * c.G, n_tiles = (c.N + kTileN - 1) / kTileN, m_tiles = most_tiles(g.which, c.rows, c.n);
+    if (Kp > 0x3fffffffLL || n_tiles > 0x7fffffffLL / kMaxSplit || m_tiles > kMaxTileRows) {
+        set_error("fc_experts: %lld rows, K=%lld, N=%lld exceed the grid or coordinate limit", (long long)c.rows, (long long)c.K,
+                  (long long)c.N);
+        return Q4FC_ELIMIT;
+    }
+    const bool sgn = (c.flags & Q4FC_FLAG_NIBBLE_SIGNED) && c.qtype == 0;
+    const int fmt = c.qtype == 1 ? kQ4_1 : sgn ? kQ4_0Signed : kQ4_0, nstage = (int)((Kp + kStageK - 1) / kStageK);
+    q.codes = reinterpret_cast<int8_t*>(c.scratch), q.sc = reinterpret_cast<float*>(c.scratch + g.sc);
+    q.tile0 = c.plan.tile0[g.which], q.log2tile = g.which == kTiles128 ? 7 : 6, q.sums = fmt == kQ4_1, q.isum = 0;
+    if (int rc = launch_quant_x_group(q, c.G, g.f16, s)) return rc;
+    CUtensorMap map = {};
+    if (int rc = make_codes_map(&map, q.codes, c.rows, g.f16 ? 2 * Kp : Kp, tile_rows(g.which))) return rc;
+    PrefillParams p = {};
+    p.status = ring_status_word();
+    if (!p.status) return Q4FC_ECUDA;
+    p.wq = c.wq, p.sc = q.sc, p.y = c.y, p.rows = c.rows, p.N = c.N, p.ldy = c.ldy;
+    p.Ng = (int)c.Ng, p.Kg = (int)c.Kg, p.n_tiles = (int)n_tiles, p.m_end = (int)m_tiles, p.part = kWhole;
+    p.tiles = c.plan.tiles[g.which], p.tile_count = c.plan.counts + g.which, p.order = c.plan.order;
+    p.group_bytes = c.Ng * c.Kg * block_bytes(c.qtype, c.G);
+    // few tiles: K divided over clusters, as for as many tiles of one weight tensor
+    p.split = 1;
+    const float tiles = likely_tiles(tile_rows(g.which), c.rows, c.n);
+    const int64_t places = (g.which == kTiles128 ? 1 : 2) * di->sm_count;
+    if (tiles * (float)n_tiles < (float)places) {
+        const TilePlan t = plan_tiles(tile_rows(g.which), fmt, c.G, (int)n_tiles, (int64_t)(tiles + 0.5f) * tile_rows(g.which),
+                                      nstage, cluster_room(di), di->sm_count);
+        p.split = t.split;
+    }
+    const dim3 grid((unsigned)(n_tiles * p.split), (unsigned)m_tiles);
+    if (fmt == kQ4_1) return c.G == 32 ? launch_grouped<kQ4_1, 32>(g.which, p, map, grid, s) : launch_grouped<kQ4_1, 128>(g.which, p, map, grid, s);
+    if (fmt == kQ4_0) return c.G == 32 ? launch_grouped<kQ4_0, 32>(g.which, p, map, grid, s) : launch_grouped<kQ4_0, 128>(g.which, p, map, grid, s);
+    return c.G == 32 ? launch_grouped<kQ4_0Signed, 32>(g.which, p, map, grid, s) : launch_grouped<kQ4_0Signed, 128>(g.which, p, map, grid, s);
 }
 
 size_t q8c_prefill_scale_bytes(int64_t rows, int64_t Kg) { return scale_bytes(rows, Kg, 1); }

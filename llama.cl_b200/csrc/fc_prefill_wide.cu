@@ -184,7 +184,7 @@ __device__ __forceinline__ void accumulate(uint64_t (&acc)[W / 2], const uint32_
 
 // FOLD: the running sums move to a second place, once, after p.fold stages of 128 k (0.9 us with adding them at the end; see fold_of in
 // fc_prefill.cu)
-template <int FMT, int G, bool FOLD>
+template <int FMT, int G, bool FOLD, bool GROUPED>
 __global__ void __launch_bounds__(kThreads, 1) fc_prefill_wide_kernel(const PrefillParams p, const __grid_constant__ CUtensorMap codes_map) {
     using S = WideShape<FMT, G>;
     constexpr int BS = S::kBlock;
@@ -211,8 +211,13 @@ __global__ void __launch_bounds__(kThreads, 1) fc_prefill_wide_kernel(const Pref
     int n_tile = (int)(blockIdx.x / cs) + p.n_off, m_tile = (int)blockIdx.y + p.m_off;
     if (n_tile >= p.n_tiles) n_tile -= p.n_tiles, m_tile++;
     if (m_tile > p.m_end || (m_tile == p.m_end && n_tile >= p.n_end)) return;  // (the whole cluster)
-    const int64_t n0 = (int64_t)n_tile * kTileN, m0 = (int64_t)m_tile * TM;
-    const int live = (int)min((int64_t)TM, p.rows - m0);  // rows of this tile that exist
+    if (GROUPED && m_tile >= __ldcg(p.tile_count)) {
+        if (m_tile == 0) pdl_wait_prior_grid();  // no tile at all: this launch's end still stands for the quantizer's
+        return;
+    }
+    const RowTile tile = row_tile<GROUPED, TM>(p, m_tile);
+    const int64_t n0 = (int64_t)n_tile * kTileN, m0 = tile.m0;
+    const int live = tile.live;  // rows of this tile that exist
     const int nstage = (p.Kg + GPS - 1) / GPS;
     const int it0 = (int)((int64_t)nstage * rank / cs), it1 = (int)((int64_t)nstage * (rank + 1) / cs);
     const int iters = it1 - it0;
@@ -247,7 +252,7 @@ __global__ void __launch_bounds__(kThreads, 1) fc_prefill_wide_kernel(const Pref
             const uint32_t bytes = (uint32_t)(min(GPS, p.Kg - (it0 + i) * GPS) * BS), bar = bar_raw + 8 * i;
             if (j == 0) mbar_expect_tx(bar, bytes * stripes);
             bulk_g2s(smem0 + S::kSlotOff + i * S::kSlotBytes + j * S::kRawStripe,
-                     p.wq + ((int64_t)(n_tile * 4 + j) * p.Kg + (int64_t)(it0 + i) * GPS) * BS, bytes, bar);
+                     tile.wq + ((int64_t)(n_tile * 4 + j) * p.Kg + (int64_t)(it0 + i) * GPS) * BS, bytes, bar);
         }
     }
     if (warp == kMmaWarp) {
@@ -428,6 +433,11 @@ __global__ void __launch_bounds__(kThreads, 1) fc_prefill_wide_kernel(const Pref
                     for (int j = 0; j < W / 2; j++) {
                         float lo, hi;
                         unpack2(acc[h][j], lo, hi);
+                        if (GROUPED) {
+                            if (mc + 2 * j < live) y_row<GROUPED>(p, m0 + mc + 2 * j)[n] = lo;
+                            if (mc + 2 * j + 1 < live) y_row<GROUPED>(p, m0 + mc + 2 * j + 1)[n] = hi;
+                            continue;
+                        }
                         if (mc + 2 * j < live) *dst = lo;
                         dst += p.ldy;
                         if (mc + 2 * j + 1 < live) *dst = hi;
@@ -495,7 +505,7 @@ __global__ void __launch_bounds__(kThreads, 1) fc_prefill_wide_kernel(const Pref
     } else {
         // =================== loader: packed weights, codes and scales of the rows ===================
         if (elect_one()) {
-            const uint8_t* stripes = p.wq + (int64_t)n_tile * 4 * p.Kg * BS;
+            const uint8_t* stripes = tile.wq + (int64_t)n_tile * 4 * p.Kg * BS;
             const int live_stripes = min(4, p.Ng - n_tile * 4);  // (columns beyond the weights: nothing is read, nothing is stored)
             auto load_raw = [&](int i) {
                 const int it = it0 + i, slot = i % S::kSlots;
@@ -584,7 +594,7 @@ __global__ void __launch_bounds__(kThreads, 1) fc_prefill_wide_kernel(const Pref
 #pragma unroll
                 for (int c = 0; c < 4; c++) {
                     const int64_t n = n0 + lane + 32 * c;
-                    if (n < p.N) p.y[(m0 + m) * p.ldy + n] = out[c];
+                    if (n < p.N) y_row<GROUPED>(p, m0 + m)[n] = out[c];
                 }
             }
         }
@@ -611,13 +621,13 @@ __global__ void __launch_bounds__(kThreads, 1) fc_prefill_wide_kernel(const Pref
     }
 }
 
-template <int FMT, int G, bool FOLD>
+template <int FMT, int G, bool FOLD, bool GROUPED = false>
 int launch_variant(const PrefillParams& p, const CUtensorMap& map, dim3 grid, cudaStream_t s) {
     using S = WideShape<FMT, G>;
     static std::atomic<bool> attr_done[64] = {};  // set once per device; a second setter repeats the same call
     int dev = 0;
     Q4FC_CUDA_OK(cudaGetDevice(&dev));
-    auto* fn = fc_prefill_wide_kernel<FMT, G, FOLD>;
+    auto* fn = fc_prefill_wide_kernel<FMT, G, FOLD, GROUPED>;
     if (dev >= 64 || !attr_done[dev]) {
         Q4FC_CUDA_OK(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, S::template kSmem<FOLD>));
         Q4FC_CUDA_OK(cudaFuncSetAttribute(fn, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared));
@@ -653,6 +663,12 @@ int launch_prefill_wide(int fmt, int G, const PrefillParams& p, const CUtensorMa
     if (fmt == kQ4_1) return G == 32 ? launch_fold<kQ4_1, 32>(p, map, grid, s) : launch_fold<kQ4_1, 128>(p, map, grid, s);
     if (fmt == kQ4_0) return G == 32 ? launch_fold<kQ4_0, 32>(p, map, grid, s) : launch_fold<kQ4_0, 128>(p, map, grid, s);
     return G == 32 ? launch_fold<kQ4_0Signed, 32>(p, map, grid, s) : launch_fold<kQ4_0Signed, 128>(p, map, grid, s);
+}
+
+int launch_prefill_wide_grouped(int fmt, int G, const PrefillParams& p, const CUtensorMap& map, dim3 grid, cudaStream_t s) {
+    if (fmt == kQ4_1) return G == 32 ? launch_variant<kQ4_1, 32, false, true>(p, map, grid, s) : launch_variant<kQ4_1, 128, false, true>(p, map, grid, s);
+    if (fmt == kQ4_0) return G == 32 ? launch_variant<kQ4_0, 32, false, true>(p, map, grid, s) : launch_variant<kQ4_0, 128, false, true>(p, map, grid, s);
+    return G == 32 ? launch_variant<kQ4_0Signed, 32, false, true>(p, map, grid, s) : launch_variant<kQ4_0Signed, 128, false, true>(p, map, grid, s);
 }
 
 }  // namespace q4fc

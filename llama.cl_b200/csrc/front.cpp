@@ -389,6 +389,131 @@ PyObject* embedding(PyObject*, PyObject* const* a, Py_ssize_t n) {
     FRONT_END
 }
 
+// ---- rows grouped by an id -----------------------------------------------------------------------------------------------
+// a plan for `rows` ids out of n_groups, as a new tensor of int32 words
+Tensor new_plan(int64_t rows, int64_t n_groups, const at::Device& dev, const char* what) {
+    const size_t bytes = q4fc_groups_bytes(rows, n_groups);
+    if (bytes == 0)
+        fail(std::string(what) + ": " + std::to_string(rows) + " rows of " + std::to_string(n_groups) +
+             " groups: expected 1 to 1024 groups and at most 2^23 rows");
+    return at::detail::empty_cuda({(int64_t)(bytes / 4)}, at::kInt, dev, std::nullopt);
+}
+PyObject* wrap(Tensor t) {
+    PyObject* r = THPVariable_Wrap(std::move(t));
+    if (!r) throw PyFailed();
+    return r;
+}
+
+// group_rows(ids, n_groups) -> plan
+PyObject* group_rows(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    if (!nargs_ok(n, 2)) return nullptr;
+    FRONT_BEGIN
+    if (!THPVariable_Check(a[0])) fail(std::string("ids: expected a torch.Tensor, got ") + Py_TYPE(a[0])->tp_name);
+    const Tensor& ids = THPVariable_Unpack(a[0]);
+    if (ids.scalar_type() != at::kInt && ids.scalar_type() != at::kLong) fail("ids: must be int32 or int64, got " + attr_str(a[0], "dtype"));
+    if (!ids.is_cuda()) fail("ids: tensor must live on a CUDA device (there is no CPU path)");
+    if (!ids.is_contiguous()) fail("ids: tensor must be dense row-major (contiguous)");
+    const int64_t groups = as_int(a[1]), rows = ids.numel();
+    c10::cuda::CUDAGuard guard(ids.device());
+    Tensor plan = new_plan(rows, groups, ids.device(), "group_rows");
+    void* pp = plan.data_ptr();
+    ret = wrap(std::move(plan));
+    const void* ip = ids.data_ptr();
+    const int i32 = ids.scalar_type() == at::kInt;
+    cudaStream_t stream = c10::cuda::getCurrentCUDAStream(ids.device().index()).stream();
+    check(without_gil([&] { return q4fc_group_rows(ip, i32, rows, groups, pp, stream); }), "group_rows");
+    FRONT_END
+}
+
+// route_top_k(logits, top_k, renormalize) -> (weights, ids, plan)
+PyObject* route_top_k(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    if (!nargs_ok(n, 3)) return nullptr;
+    FRONT_BEGIN
+    if (!THPVariable_Check(a[0])) fail(std::string("logits: expected a torch.Tensor, got ") + Py_TYPE(a[0])->tp_name);
+    const int64_t rank = THPVariable_Unpack(a[0]).dim();
+    const Tensor& x = tensor(a[0], "logits", at::kFloat, rank < 2 ? 2 : rank);
+    const int64_t E = x.size(-1), k = as_int(a[1]);
+    if (k < 1 || k > E || k > 32)
+        fail("route_top_k: top_k=" + std::to_string(k) + " outside 1.." + std::to_string(E < 32 ? E : 32) + " (" + std::to_string(E) + " experts)");
+    const int64_t tokens = E ? x.numel() / E : 0;
+    at::DimVector shape(x.sizes().begin(), x.sizes().end());
+    shape.back() = k;
+    c10::cuda::CUDAGuard guard(x.device());
+    Tensor plan = new_plan(tokens * k, E, x.device(), "route_top_k");
+    Tensor weights = empty_f32(shape, x.device());
+    Tensor ids = at::detail::empty_cuda(shape, at::kInt, x.device(), std::nullopt);
+    const float* xp = static_cast<const float*>(x.data_ptr());
+    float* wp = static_cast<float*>(weights.data_ptr());
+    int32_t* ip = static_cast<int32_t*>(ids.data_ptr());
+    void* pp = plan.data_ptr();
+    const int renormalize = truth(a[2]);
+    cudaStream_t stream = c10::cuda::getCurrentCUDAStream(x.device().index()).stream();
+    check(without_gil([&] { return q4fc_route_top_k(xp, tokens, E, E, k, renormalize, wp, ip, pp, stream); }), "route_top_k");
+    ret = PyTuple_New(3);
+    if (!ret) throw PyFailed();
+    PyTuple_SET_ITEM(ret, 0, wrap(std::move(weights)));
+    PyTuple_SET_ITEM(ret, 1, wrap(std::move(ids)));
+    PyTuple_SET_ITEM(ret, 2, wrap(std::move(plan)));
+    FRONT_END
+}
+
+// a plan as made here for these ids
+void* plan_of(PyObject* o, int64_t rows, int64_t n_groups, const at::Device& dev) {
+    const Tensor& t = tensor(o, "groups.buf", at::kInt, 1);
+    if (t.numel() * 4 != (int64_t)q4fc_groups_bytes(rows, n_groups)) fail("groups: not a plan of " + std::to_string(rows) + " rows");
+    if (t.device() != dev) fail("input and groups live on different devices");
+    return t.data_ptr();
+}
+
+// fc_experts(input, wei_quantized, N, ids, n_groups, most_rows, plan, weights, silu_mul, nibble_signed, out)
+PyObject* fc_experts(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    if (!nargs_ok(n, 11)) return nullptr;
+    FRONT_BEGIN
+    if (!THPVariable_Check(a[0])) fail(std::string("input: expected a torch.Tensor, got ") + Py_TYPE(a[0])->tp_name);
+    const int64_t rank = THPVariable_Unpack(a[0]).dim();
+    const Tensor& x = tensor(a[0], "input", at::kFloat, rank == 4 ? 4 : 3);
+    const Tensor& w = tensor(a[1], "wei_quantized", at::kChar, 4);
+    if (!THPVariable_Check(a[3])) fail("groups.ids: expected a torch.Tensor");
+    const Tensor& ids = THPVariable_Unpack(a[3]);
+    if (w.device() != x.device()) fail("input and wei_quantized live on different devices");
+    if (ids.dim() != 3 || ids.size(0) != x.size(0) || ids.size(1) != x.size(1) || (rank == 4 && ids.size(2) != x.size(2)))
+        fail("groups: ids of shape " + shape_text(ids.sizes()) + " do not fit the input " + shape_text(x.sizes()));
+    q4fc_experts_call c = {};
+    c.tokens = ids.size(0) * ids.size(1), c.top_k = ids.size(2), c.x_per_slot = rank == 4, c.silu_mul = truth(a[8]);
+    c.experts = w.size(0), c.Ng = w.size(1), c.Kg = w.size(2);
+    variant_of(w.size(3), &c.qtype, &c.group_k);
+    c.ldx = x.size(-1), c.K = c.silu_mul ? c.ldx / 2 : c.ldx;
+    if (c.silu_mul && c.ldx % 2) fail("input: rows of gate and up are even, got " + std::to_string(c.ldx));
+    c.N = to_int(a[2]);
+    if (c.N < 0) fail("fc_Q4A_experts: negative N");
+    if (as_int(a[4]) != c.experts)
+        fail("groups: a plan of " + std::to_string(as_int(a[4])) + " groups for " + std::to_string(c.experts) + " experts");
+    if (c.top_k < 1) fail("groups: ids without a slot");
+    c.most_rows = as_int(a[5]);
+    c10::cuda::CUDAGuard guard(x.device());
+    c.groups = plan_of(a[6], c.tokens * c.top_k, c.experts, x.device());
+    at::DimVector shape(ids.sizes().begin(), ids.sizes().end());
+    if (a[7] != Py_None) {
+        const Tensor& weights = tensor(a[7], "weights", at::kFloat, 3);
+        if (weights.sizes() != ids.sizes()) fail("weights: expected shape " + shape_text(ids.sizes()) + ", got " + shape_text(weights.sizes()));
+        if (weights.device() != x.device()) fail("input and weights live on different devices");
+        c.weights = static_cast<const float*>(weights.data_ptr());
+        shape.pop_back();
+    }
+    shape.push_back(c.N);
+    c.x = static_cast<const float*>(x.data_ptr()), c.wq = w.data_ptr();
+    c.y = output(a[10], shape, x.device(), &ret), c.ldy = c.N;
+    if (a[10] != Py_None && THPVariable_Unpack(a[10]).device() != x.device()) fail("input and out live on different devices");
+    const size_t need = q4fc_experts_workspace_bytes(c.tokens, c.top_k, c.K, c.N, c.group_k, c.experts, c.weights != nullptr);
+    // scratch of this call's own, from torch's allocator: calls on several streams and captured graphs never share it
+    Tensor ws = at::detail::empty_cuda({(int64_t)need}, at::kByte, x.device(), std::nullopt);
+    void* wp = ws.data_ptr();
+    cudaStream_t stream = c10::cuda::getCurrentCUDAStream(x.device().index()).stream();
+    const unsigned flags = truth(a[9]) ? Q4FC_FLAG_NIBBLE_SIGNED : 0u;
+    check(without_gil([&] { return q4fc_fc_experts(&c, wp, need, flags, stream); }), "fc_Q4A_experts");
+    FRONT_END
+}
+
 // ---- prepared argument blocks: fc_batch(address, n, qtype, group_k, flags, device), quant_batch(address, n, group_k,
 //      want_isum, flags, device) ------------------------------------------------------------------------------------------
 PyObject* fc_batch(PyObject*, PyObject* const* a, Py_ssize_t n) {
@@ -478,6 +603,9 @@ PyMethodDef methods[] = {
     {"pack", reinterpret_cast<PyCFunction>(pack), METH_FASTCALL, nullptr},
     {"q8c_fc", reinterpret_cast<PyCFunction>(q8c_fc), METH_FASTCALL, nullptr},
     {"embedding", reinterpret_cast<PyCFunction>(embedding), METH_FASTCALL, nullptr},
+    {"group_rows", reinterpret_cast<PyCFunction>(group_rows), METH_FASTCALL, nullptr},
+    {"route_top_k", reinterpret_cast<PyCFunction>(route_top_k), METH_FASTCALL, nullptr},
+    {"fc_experts", reinterpret_cast<PyCFunction>(fc_experts), METH_FASTCALL, nullptr},
     {"fc_batch", reinterpret_cast<PyCFunction>(fc_batch), METH_FASTCALL, nullptr},
     {"quant_batch", reinterpret_cast<PyCFunction>(quant_batch), METH_FASTCALL, nullptr},
     {"graph_step", reinterpret_cast<PyCFunction>(graph_step), METH_FASTCALL, nullptr},

@@ -1,0 +1,308 @@
+// Rows grouped by an id, and the router in front of a layer of experts.  No counterpart in the reference, whose every FC
+// gives all rows the same weights (ops/op_fc.hpp:286-426).
+//
+//   route:  p = softmax(logits) over the experts of a token; its top_k largest, the lowest index first where they are
+//           equal; an expert whose logit is -inf is closed and never chosen (id -1, weight 0 where none is left).
+//           Weights p, or p over the sum of the chosen ones.  The choice compares logits, no exponentials.
+//   group:  a stable counting sort of the (token, slot) pairs by expert, or of rows by adapter (groups.cuh).
+//
+// Route: a warp per token, a lane holds every 32nd logit.  A step of the choice is two warp reductions, of the largest key
+// and of the lowest index that has it; only the winner looks for its next.
+// Group: one cluster.  Each warp owns a contiguous piece of the rows and its own bins in shared memory, so that equal ids
+// need no atomics whose order would decide places: it counts its piece (lanes with equal ids find one another with
+// match.any, the first adds), the bins of all warps and CTAs are summed in order, and it walks its piece again with its
+// places.  The same from run to run.
+#include <cooperative_groups.h>
+
+#include <atomic>
+#include <type_traits>
+
+#include "groups.cuh"
+
+namespace cg = cooperative_groups;
+
+namespace q4fc {
+namespace {
+
+constexpr int kThreads = 1024, kWarps = kThreads / 32;
+constexpr int kCluster = 8;               // CTAs that share a long list
+constexpr uint32_t kClosed = 0x007fffffu;  // key of -inf; finite numbers are above
+
+// order-preserving, -0 and 0 equal; NaN below everything
+__device__ __forceinline__ uint32_t key_of(float x) {
+    const uint32_t b = __float_as_uint(x + 0.0f);
+    return x != x ? 0u : b ^ ((b >> 31) ? 0xffffffffu : 0x80000000u);
+}
+__device__ __forceinline__ float value_of(uint32_t key) {
+    return __uint_as_float(key ^ ((key >> 31) ? 0x80000000u : 0xffffffffu));
+}
+
+struct RouteArgs {
+    const float* logits;
+    int64_t tokens, ld;
+    int experts, top_k, renormalize;
+    float* weights;
+    int32_t* ids;
+};
+
+// One token, by one warp; NV logits a lane.
+template <int NV>
+__device__ __forceinline__ void route_token(const RouteArgs& a, int64_t token, int lane) {
+    const float* src = a.logits + token * a.ld;
+    uint32_t key[NV];
+    bool nan = false;
+    uint32_t best = 0;
+#pragma unroll
+    for (int i = 0; i < NV; i++) {
+        const int e = lane + 32 * i;
+        const float x = e < a.experts ? ld_after_wait(src + e) : -INFINITY;
+        key[i] = key_of(x);
+        nan |= x != x;
+        best = max(best, key[i]);
+    }
+    nan = __any_sync(0xffffffffu, nan);
+    const uint32_t top = __reduce_max_sync(0xffffffffu, best);
+    const float most = value_of(top);
+    float total = 0.0f;
+    if (!a.renormalize && top > kClosed) {
+#pragma unroll
+        for (int i = 0; i < NV; i++)
+            if (key[i] >= kClosed) total += expf(value_of(key[i]) - most);  // (-inf: 0)
+#pragma unroll
+        for (int off = 16; off > 0; off >>= 1) total += __shfl_xor_sync(0xffffffffu, total, off);
+    }
+    int id = -1;       // of slot `lane`
+    float mine = 0.0f;
+    for (int s = 0; s < a.top_k; s++) {
+        const uint32_t k = __reduce_max_sync(0xffffffffu, best);
+        if (k <= kClosed) break;
+        int at = 0x7fffffff;
+        if (best == k) {
+#pragma unroll
+            for (int i = NV - 1; i >= 0; i--)
+                if (key[i] == k) at = lane + 32 * i;
+        }
+        at = __reduce_min_sync(0xffffffffu, (unsigned)at);
+        const float w = expf(value_of(k) - most);
+        if (a.renormalize) total += w;
+        if (lane == s) id = at, mine = w;
+        if (lane == (at & 31)) {
+            best = 0;
+#pragma unroll
+            for (int i = 0; i < NV; i++) {
+                if (i == at >> 5) key[i] = 0;
+                best = max(best, key[i]);
+            }
+        }
+    }
+    if (lane < a.top_k) {
+        a.ids[token * a.top_k + lane] = id;
+        a.weights[token * a.top_k + lane] = nan ? __uint_as_float(0x7fc00000u) : id < 0 ? 0.0f : __fdiv_rn(mine, total);
+    }
+}
+
+template <int NV>
+__global__ void __launch_bounds__(256) route_kernel(const RouteArgs a) {
+    pdl_wait_prior_grid();
+    pdl_launch_dependents();
+    const int64_t token = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+    if (token < a.tokens) route_token<NV>(a, token, threadIdx.x & 31);
+}
+
+struct GroupArgs {
+    const void* ids;
+    int i32;
+    int64_t rows, piece;  // rows of a warp
+    int n;
+    GroupPlan plan;
+    int* status;
+};
+// ROUTE: the warps choose the experts of their own tokens first (NV logits a lane)
+template <int NV>
+__global__ void __launch_bounds__(kThreads, 1) group_kernel(const GroupArgs a, const RouteArgs route) {
+    extern __shared__ uint32_t bins[];  // [warp][n + 1]
+    __shared__ uint32_t sums[kMaxGroups + 1];             // this CTA's rows of each group
+    __shared__ uint32_t first[kMaxGroups + 1];            // its first place of each group
+    __shared__ uint32_t start[kMaxGroups + 1];            // the group's first place
+    __shared__ int tile0[kTileSizes][kMaxGroups + 1];     // first tile of each group
+    __shared__ uint32_t warp_sum[4][kWarps];
+    cg::cluster_group cluster = cg::this_cluster();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int ctas = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+    const int nb = a.n + 1;  // bins; the last one is of rows without a group
+    uint32_t* mine = bins + warp * nb;
+    for (int i = threadIdx.x; i < kWarps * nb; i += kThreads) bins[i] = 0;
+    pdl_wait_prior_grid();
+    pdl_launch_dependents();
+    __syncthreads();
+    const int64_t begin = min(a.rows, ((int64_t)rank * kWarps + warp) * a.piece), end = min(a.rows, begin + a.piece);
+    if constexpr (NV > 0) {
+        for (int64_t t = begin / route.top_k; t < end / route.top_k; t++) route_token<NV>(route, t, lane);
+        __syncwarp();  // (a warp's own ids are what it sorts)
+    }
+    auto bin_of = [&](int64_t i) {
+        const int64_t id = a.i32 ? (int64_t)__ldcg(static_cast<const int*>(a.ids) + i)
+                                 : (int64_t)__ldcg(static_cast<const long long*>(a.ids) + i);
+        if (id >= a.n) atomicOr(a.status, kStatusBadId);
+        return id >= 0 && id < a.n ? (int)id : a.n;
+    };
+    for (int64_t i0 = begin; i0 < end; i0 += 32) {
+        const bool there = i0 + lane < end;
+        const int b = there ? bin_of(i0 + lane) : -1;
+        const uint32_t same = __match_any_sync(0xffffffffu, b);
+        if (there && (same & ((1u << lane) - 1)) == 0) mine[b] += __popc(same);
+        __syncwarp();
+    }
+    __syncthreads();
+    for (int b = threadIdx.x; b < nb; b += kThreads) {  // warps in order
+        uint32_t sum = 0;
+        for (int w = 0; w < kWarps; w++) {
+            const uint32_t c = bins[w * nb + b];
+            bins[w * nb + b] = sum;
+            sum += c;
+        }
+        sums[b] = sum;
+    }
+    cluster.sync();
+    // group b = threadIdx.x (kMaxGroups = kThreads of them): its rows, those of the CTAs in front, its first place and tiles
+    uint32_t all = 0, front = 0;
+    if ((int)threadIdx.x < a.n)
+        for (int c = 0; c < ctas; c++) {
+            const uint32_t v = cluster.map_shared_rank(sums, c)[threadIdx.x];
+            all += v;
+            if (c < rank) front += v;
+        }
+    uint32_t none_front = 0;  // of rows without a group
+    if (threadIdx.x == 0)
+        for (int c = 0; c < rank; c++) none_front += cluster.map_shared_rank(sums, c)[a.n];
+    uint32_t v[4] = {all, (all + 7) / 8, (all + 63) / 64, (all + 127) / 128};
+    uint32_t own[4] = {v[0], v[1], v[2], v[3]};
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1)
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const uint32_t o = __shfl_up_sync(0xffffffffu, v[j], off);
+            if (lane >= off) v[j] += o;
+        }
+    if (lane == 31)
+        for (int j = 0; j < 4; j++) warp_sum[j][warp] = v[j];
+    __syncthreads();
+    uint32_t total[4];
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        const uint32_t w = warp_sum[j][lane];  // (32 warps)
+        total[j] = __reduce_add_sync(0xffffffffu, w);
+        v[j] += __reduce_add_sync(0xffffffffu, lane < warp ? w : 0u) - own[j];  // in front of this group
+    }
+    if ((int)threadIdx.x < a.n) {
+        first[threadIdx.x] = v[0] + front, start[threadIdx.x] = v[0];
+        for (int j = 0; j < kTileSizes; j++) tile0[j][threadIdx.x] = (int)v[j + 1];
+        if (rank == 0) {
+            a.plan.offsets[threadIdx.x] = (int)v[0];
+            for (int j = 0; j < kTileSizes; j++) a.plan.tile0[j][threadIdx.x] = (int)v[j + 1];
+        }
+    }
+    if (threadIdx.x == 0) {
+        first[a.n] = total[0] + none_front, start[a.n] = total[0];
+        for (int j = 0; j < kTileSizes; j++) tile0[j][a.n] = (int)total[j + 1];
+        if (rank == 0) {
+            a.plan.offsets[a.n] = (int)total[0];
+            for (int j = 0; j < kTileSizes; j++) a.plan.tile0[j][a.n] = (int)total[j + 1];
+            for (int j = 0; j < 16; j++) a.plan.counts[j] = j < kTileSizes ? (int)total[j + 1] : 0;
+        }
+    }
+    __syncthreads();
+    // the rows' places
+    for (int64_t i0 = begin; i0 < end; i0 += 32) {
+        const bool there = i0 + lane < end;
+        const int b = there ? bin_of(i0 + lane) : -1;
+        const uint32_t same = __match_any_sync(0xffffffffu, b), below = same & ((1u << lane) - 1);
+        const uint32_t at = there ? mine[b] : 0;
+        __syncwarp();
+        if (there) {
+            const uint32_t place = first[b] + at + __popc(below);
+            a.plan.order[place] = (int)(i0 + lane), a.plan.group_of[place] = b;
+            if (below == 0) mine[b] = at + __popc(same);
+        }
+        __syncwarp();
+    }
+    // tiles: the group of tile i is the last whose first tile is not behind it
+    for (int j = 0; j < kTileSizes; j++) {
+        const int size = tile_rows(j);
+        for (int i = rank * kThreads + threadIdx.x; i < (int)total[j + 1]; i += ctas * kThreads) {
+            int lo = 0, hi = a.n;  // tile0[lo] <= i < tile0[hi]
+            while (hi - lo > 1) {
+                const int mid = (lo + hi) / 2;
+                if (tile0[j][mid] <= i) lo = mid; else hi = mid;
+            }
+            const int at = (i - tile0[j][lo]) * size;
+            a.plan.tiles[j][i] = make_int4(lo, (int)start[lo] + at, min(size, (int)(start[lo + 1] - start[lo]) - at), 0);
+        }
+    }
+    cluster.sync();  // nobody leaves while its sums are being read
+}
+
+template <int NV>
+int launch_group_variant(const GroupArgs& a, const RouteArgs& route, int ctas, cudaStream_t s) {
+    static std::atomic<bool> attr_done[64] = {};  // set once per device; a second setter repeats the same call
+    auto* fn = group_kernel<NV>;
+    const size_t most = kWarps * (kMaxGroups + 1) * sizeof(uint32_t);
+    int dev = 0;
+    Q4FC_CUDA_OK(cudaGetDevice(&dev));
+    if (dev >= 64 || !attr_done[dev]) {
+        Q4FC_CUDA_OK(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most));
+        if (dev < 64) attr_done[dev] = true;
+    }
+    DependentLaunch l(dim3((unsigned)ctas), kThreads, s);
+    cudaLaunchAttribute attrs[2] = {l.attr, {}};
+    attrs[1].id = cudaLaunchAttributeClusterDimension;
+    attrs[1].val.clusterDim.x = (unsigned)ctas, attrs[1].val.clusterDim.y = attrs[1].val.clusterDim.z = 1;
+    l.cfg.attrs = attrs, l.cfg.numAttrs = 2;
+    l.cfg.dynamicSmemBytes = kWarps * (size_t)(a.n + 1) * sizeof(uint32_t);
+    Q4FC_CUDA_OK(cudaLaunchKernelEx(&l.cfg, fn, a, route));
+    return Q4FC_OK;
+}
+// NV: logits a lane holds, for as many experts
+template <typename F>
+int with_lanes(int experts, F f) {
+    if (experts <= 32) return f(std::integral_constant<int, 1>{});
+    if (experts <= 64) return f(std::integral_constant<int, 2>{});
+    if (experts <= 128) return f(std::integral_constant<int, 4>{});
+    if (experts <= 256) return f(std::integral_constant<int, 8>{});
+    return f(std::integral_constant<int, 32>{});
+}
+int group_args(GroupArgs* a, const void* ids, int i32, int64_t rows, int64_t n, void* groups, int ctas, int64_t together) {
+    a->ids = ids, a->i32 = i32, a->rows = rows, a->n = (int)n, a->plan = group_plan(groups, rows, n);
+    const int64_t warps = (int64_t)ctas * kWarps;
+    a->piece = (rows / together + warps - 1) / warps * together;
+    a->status = ring_status_word();
+    return a->status ? Q4FC_OK : Q4FC_ECUDA;
+}
+
+}  // namespace
+
+int launch_group_rows(const void* ids, int ids_are_i32, int64_t rows, int64_t n, void* groups, cudaStream_t s) {
+    GroupArgs a = {};
+    const int ctas = rows > 2048 ? kCluster : 1;
+    if (int rc = group_args(&a, ids, ids_are_i32, rows, n, groups, ctas, 1)) return rc;
+    return launch_group_variant<0>(a, RouteArgs{}, ctas, s);
+}
+
+int launch_route_top_k(const float* logits, int64_t tokens, int64_t experts, int64_t ld, int64_t top_k, int renormalize,
+                       float* weights, int32_t* ids, void* groups, cudaStream_t s) {
+    RouteArgs route = {logits, tokens, ld, (int)experts, (int)top_k, renormalize, weights, ids};
+    GroupArgs a = {};
+    const int64_t rows = tokens * top_k;
+    const bool inside = tokens <= 1024;
+    const int ctas = rows > 2048 || (inside && tokens > 64) ? kCluster : 1;
+    if (int rc = group_args(&a, ids, 1, rows, experts, groups, ctas, top_k)) return rc;
+    return with_lanes((int)experts, [&](auto nv) {
+        constexpr int NV = decltype(nv)::value;
+        if (inside) return launch_group_variant<NV>(a, route, ctas, s);
+        DependentLaunch l(dim3((unsigned)((tokens + 7) / 8)), 256, s);
+        Q4FC_CUDA_OK(cudaLaunchKernelEx(&l.cfg, route_kernel<NV>, route));
+        return launch_group_variant<0>(a, RouteArgs{}, ctas, s);
+    });
+}
+
+}  // namespace q4fc

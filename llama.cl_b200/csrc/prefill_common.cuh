@@ -25,12 +25,40 @@ struct PrefillParams {
     int n_end, m_end;    // and the one behind its last
     int fold;            // Q4: stages of 128 k of a running sum, 0: one sum over all of a CTA's stages
     int part;            // kWhole, or of two launches kFirst (whole rounds) and kRemainder (the tiles that are left)
+    // GROUPED: the rows are sorted by the weights they take (groups.cuh).  A row tile is one of the plan's, its rows of y are in
+    // `order`, and wq holds the weights of every group
+    const int4* tiles;
+    const int* tile_count;
+    const int* order;
+    int64_t group_bytes;
 };
 
 // 128-row tiles of Q4 weights (fc_prefill_wide.cu)
 int launch_prefill_wide(int fmt, int G, const PrefillParams& p, const CUtensorMap& map, dim3 grid, cudaStream_t s);
+int launch_prefill_wide_grouped(int fmt, int G, const PrefillParams& p, const CUtensorMap& map, dim3 grid, cudaStream_t s);
 
 #ifdef __CUDACC__
+// What a CTA computes: rows m0 .. m0 + live - 1 of the codes with the weights at wq.
+struct RowTile {
+    const uint8_t* wq;
+    int64_t m0;
+    int live;
+};
+template <bool GROUPED, int TM>
+__device__ __forceinline__ RowTile row_tile(const PrefillParams& p, int m_tile) {
+    if constexpr (GROUPED) {
+        const int4 t = __ldcg(p.tiles + m_tile);
+        return {p.wq + t.x * p.group_bytes, t.y, t.z};
+    } else {
+        const int64_t m0 = (int64_t)m_tile * TM;
+        return {p.wq, m0, (int)min((int64_t)TM, p.rows - m0)};
+    }
+}
+// row m of the codes in y
+template <bool GROUPED>
+__device__ __forceinline__ float* y_row(const PrefillParams& p, int64_t m) {
+    return p.y + (GROUPED ? (int64_t)__ldcg(p.order + m) : m) * p.ldy;
+}
 // one lane of a converged warp.  (The compiler knows that exactly one lane runs the branch and keeps descriptors in
 // uniform registers; behind `lane == 0` it cannot, and issuing an MMA takes about a third longer.)
 __device__ __forceinline__ bool elect_one() {

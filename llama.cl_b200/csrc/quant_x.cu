@@ -18,7 +18,7 @@
 // fused copy of this arithmetic (tree-ordered sums), the prefill path its own
 // kernel below; this one serves callers that want the quantized activations
 // themselves and the per-channel int8 FC on mma.sync (q8c.cu).
-#include "common.cuh"
+#include "groups.cuh"
 
 namespace q4fc {
 namespace {
@@ -111,6 +111,68 @@ __global__ void __launch_bounds__(kQxWarps * 32) quant_x_kernel(const float* __r
     }
 }
 
+// 128 k of a row, by one warp, in a form that the FC kernels read: lane l holds v[0..3] = x[k .. k + 3], 0 beyond K, of
+// k = 128 c + 4 l.  Codes and scales as in quant_x_kernel, group sums tree-ordered.  `codes`: the row's; `sc`: the row's
+// place in the first K group, `per` floats from there to its place in the next, the sum `sum_at` behind the scale.
+// isum: instead of the sum, the bits of the integer 8 * sum of codes.
+template <int G, bool F16>
+__device__ __forceinline__ void quantize_unit(const float (&v)[4], int64_t c, int lane, int64_t K, int64_t Kg, bool sums, bool isum,
+                                              int8_t* __restrict__ codes, float* __restrict__ sc, int64_t per, int64_t sum_at) {
+    constexpr int SEG = G / 4;    // lanes per group
+    constexpr int GPC = 128 / G;  // groups per 128-k chunk
+    const int64_t k = c * 128 + lane * 4;
+    const int64_t kb = c * GPC + lane / SEG;
+    const bool exists = kb < Kg;
+    const int len = exists ? (int)min((int64_t)G, K - kb * G) : 0;
+    const int body = len & ~7;
+    const int e0 = (lane % SEG) * 4;
+    float amax = 0.0f, sum = (v[0] + v[1]) + (v[2] + v[3]);
+#pragma unroll
+    for (int j = 0; j < 4; j++)
+        if (e0 + j < len) amax = fmaxf(amax, fabsf(v[j]));
+#pragma unroll
+    for (int off = SEG / 2; off > 0; off >>= 1) {
+        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, off));
+        sum += __shfl_xor_sync(0xffffffffu, sum, off);
+    }
+    const float d = div_const_rn(amax, 127.0f, 1.0f / 127.0f);
+    const float id = inv_or_zero(d);
+    int q[4] = {};
+#pragma unroll
+    for (int j = 0; j < 4; j++)
+        if (e0 + j < len) {
+            const float t = __fmul_rn(v[j], id);
+            q[j] = sat8(e0 + j < body ? __float2int_rn(t) : round_half_away(t));
+        }
+    if (isum) {
+        int s = q[0] + q[1] + q[2] + q[3];
+#pragma unroll
+        for (int off = SEG / 2; off > 0; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
+        sum = __int_as_float(8 * s);
+    }
+    uint32_t w[2];  // F16: four codes, as two lanes hold eight k: the even one takes k = 0,2,4,6 (see launch_quant_x_tile)
+    if constexpr (F16) {
+        uint32_t h[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) h[j] = __half_as_ushort(__int2half_rn(q[j] * ((lane & 1) ? 16 : 256)));
+        const uint32_t even = h[0] | h[2] << 16, odd = h[1] | h[3] << 16;
+        const uint32_t other = __shfl_xor_sync(0xffffffffu, (lane & 1) ? even : odd, 1);
+        w[0] = (lane & 1) ? other : even, w[1] = (lane & 1) ? odd : other;
+    }
+    if (exists) {
+        if constexpr (F16)
+            *reinterpret_cast<uint2*>(codes + k * 2) = make_uint2(w[0], w[1]);
+        else
+            *reinterpret_cast<uint32_t*>(codes + k) =
+                (q[0] & 0xFF) | (q[1] & 0xFF) << 8 | (q[2] & 0xFF) << 16 | (uint32_t)(q[3] & 0xFF) << 24;
+        if (e0 == 0) {
+            float* dst = sc + kb * per;
+            dst[0] = F16 ? __fmul_rn(d, 64.0f) : d;
+            if (sums) dst[sum_at] = sum;
+        }
+    }
+}
+
 // The prefill GEMM's quantizer: the codes and scales of quant_x_kernel, scales (and, `sums`, group sums, tree-ordered)
 // in the layout in which the GEMM's tiles of 2^log2tile rows read them: [row tile][Kg][scale | sum][row in tile].
 // The eight warps of a CTA take the same 128 k of eight neighbouring rows, whose scales share a 32-byte sector.
@@ -119,8 +181,6 @@ __global__ void __launch_bounds__(kQxWarps * 32) quant_x_tile_kernel(const float
                                                                      int64_t ldx, int64_t Kg, int vec_ok, int sums,
                                                                      int log2tile, int8_t* __restrict__ codes,
                                                                      float* __restrict__ sc) {
-    constexpr int SEG = G / 4;    // lanes per group
-    constexpr int GPC = 128 / G;  // groups per 128-k chunk
     pdl_wait_prior_grid();
     pdl_launch_dependents();      // the GEMM's weight copies run beside this launch
     const int lane = threadIdx.x & 31;
@@ -139,50 +199,60 @@ __global__ void __launch_bounds__(kQxWarps * 32) quant_x_tile_kernel(const float
         for (int j = 0; j < 4; j++)
             if (k + j < K) v[j] = ld_after_wait(src + j);
     }
-    const int64_t kb = c * GPC + lane / SEG;
-    const bool exists = kb < Kg;
-    const int len = exists ? (int)min((int64_t)G, K - kb * G) : 0;
-    const int body = len & ~7;
-    const int e0 = (lane % SEG) * 4;
-    float amax = 0.0f, sum = (v[0] + v[1]) + (v[2] + v[3]);  // (0 beyond K)
-#pragma unroll
-    for (int j = 0; j < 4; j++)
-        if (e0 + j < len) amax = fmaxf(amax, fabsf(v[j]));
-#pragma unroll
-    for (int off = SEG / 2; off > 0; off >>= 1) {
-        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, off));
-        sum += __shfl_xor_sync(0xffffffffu, sum, off);
+    const int64_t tile = (int64_t)1 << log2tile, per = tile << sums;
+    quantize_unit<G, F16>(v, c, lane, K, Kg, sums, false, codes + row * (Kg * G) * (F16 ? 2 : 1),
+                          sc + (row >> log2tile) * Kg * per + (row & (tile - 1)), per, tile);
+}
+
+// The quantizer of the experts' product: rows in the order of a plan (groups.cuh), codes in that order, scales by the
+// plan's tiles: for the decode kernel (tiles of 8 rows) as quant_x_pre_kernel has them, else as quant_x_tile_kernel.
+// A row of x serves `per_row` (token, slot) pairs, or one; `gated`: the value is silu(x[k]) * x[K + k].  An output row
+// without an expert is zeroed here.
+template <int G, bool F16>
+__global__ void __launch_bounds__(kQxWarps * 32) quant_x_group_kernel(const __grid_constant__ GroupQuant a) {
+    pdl_wait_prior_grid();
+    __threadfence();              // what is behind this launch reads the plan, too, before this launch has ended
+    pdl_launch_dependents();
+    const int lane = threadIdx.x & 31;
+    const int64_t row_sets = (a.rows + kQxWarps - 1) / kQxWarps;
+    const int64_t c = blockIdx.x / row_sets;
+    const int64_t place = (blockIdx.x - c * row_sets) * kQxWarps + (threadIdx.x >> 5);
+    if (place >= a.rows) return;
+    const int group = __ldcg(a.group_of + place);
+    const int64_t pair = __ldcg(a.order + place);
+    if (group >= a.n) {
+        if (c == 0)
+            for (int64_t n = lane; n < a.N; n += 32) a.y[pair * a.ldy + n] = 0.0f;
+        return;
     }
-    const float d = div_const_rn(amax, 127.0f, 1.0f / 127.0f);
-    const float id = inv_or_zero(d);
-    int q[4] = {};
+    const int first = __ldcg(a.offsets + group), tile0 = __ldcg(a.tile0 + group);
+    const int64_t k = c * 128 + lane * 4;
+    const float* src = a.x + (a.per_row > 1 ? pair / a.per_row : pair) * a.ldx + k;
+    float v[4] = {0.f, 0.f, 0.f, 0.f};
+    auto load = [&](const float* src, float (&v)[4]) {
+        if (a.vec_ok && k + 4 <= a.K) {
+            const float4 b = ld_after_wait(reinterpret_cast<const float4*>(src));
+            v[0] = b.x, v[1] = b.y, v[2] = b.z, v[3] = b.w;
+        } else {
 #pragma unroll
-    for (int j = 0; j < 4; j++)
-        if (e0 + j < len) {
-            const float t = __fmul_rn(v[j], id);
-            q[j] = sat8(e0 + j < body ? __float2int_rn(t) : round_half_away(t));
+            for (int j = 0; j < 4; j++)
+                if (k + j < a.K) v[j] = ld_after_wait(src + j);
         }
-    uint32_t w[2];  // F16: four codes, as two lanes hold eight k: the even one takes k = 0,2,4,6 (see launch_quant_x_tile)
-    if constexpr (F16) {
-        uint32_t h[4];
+    };
+    load(src, v);
+    if (a.gated) {
+        float up[4] = {0.f, 0.f, 0.f, 0.f};
+        load(src + a.K, up);
 #pragma unroll
-        for (int j = 0; j < 4; j++) h[j] = __half_as_ushort(__int2half_rn(q[j] * ((lane & 1) ? 16 : 256)));
-        const uint32_t even = h[0] | h[2] << 16, odd = h[1] | h[3] << 16;
-        const uint32_t other = __shfl_xor_sync(0xffffffffu, (lane & 1) ? even : odd, 1);
-        w[0] = (lane & 1) ? other : even, w[1] = (lane & 1) ? odd : other;
+        for (int j = 0; j < 4; j++) v[j] = __fmul_rn(up[j], __fdiv_rn(v[j], __fadd_rn(1.0f, expf(-v[j]))));
     }
-    if (exists) {
-        if constexpr (F16)
-            *reinterpret_cast<uint2*>(codes + (row * (Kg * G) + k) * 2) = make_uint2(w[0], w[1]);
-        else
-            *reinterpret_cast<uint32_t*>(codes + row * (Kg * G) + k) =
-                (q[0] & 0xFF) | (q[1] & 0xFF) << 8 | (q[2] & 0xFF) << 16 | (uint32_t)(q[3] & 0xFF) << 24;
-        if (e0 == 0) {
-            const int64_t tile = (int64_t)1 << log2tile, per = tile << sums;
-            float* dst = sc + ((row >> log2tile) * Kg + kb) * per + (row & (tile - 1));
-            dst[0] = F16 ? __fmul_rn(d, 64.0f) : d;
-            if (sums) dst[tile] = sum;
-        }
+    const int at = (int)place - first, tile = tile0 + (at >> a.log2tile), row = at & ((1 << a.log2tile) - 1);
+    int8_t* codes = a.codes + place * (a.Kg * G) * (F16 ? 2 : 1);
+    if (a.log2tile == 3)
+        quantize_unit<G, F16>(v, c, lane, a.K, a.Kg, true, a.isum, codes, a.sc + (int64_t)tile * a.Kg * 16 + 2 * row, 16, 1);
+    else {
+        const int64_t size = (int64_t)1 << a.log2tile, per = size << a.sums;
+        quantize_unit<G, F16>(v, c, lane, a.K, a.Kg, a.sums, false, codes, a.sc + (int64_t)tile * a.Kg * per + row, per, size);
     }
 }
 
@@ -437,6 +507,19 @@ int launch_quant_x_tile(const float* x, int64_t rows, int64_t K, int64_t ldx, in
     auto* kernel = G == 128 ? quant_x_tile_kernel<128, false> : f16 ? quant_x_tile_kernel<32, true> : quant_x_tile_kernel<32, false>;
     DependentLaunch l(dim3((unsigned)grid), kQxWarps * 32, s);
     Q4FC_CUDA_OK(cudaLaunchKernelEx(&l.cfg, kernel, x, rows, K, ldx, Kg, vec_ok, (int)sums, l2, codes, sc));
+    return Q4FC_OK;
+}
+
+int launch_quant_x_group(const GroupQuant& q, int G, bool f16, cudaStream_t s) {
+    if (q.rows == 0) return Q4FC_OK;
+    const int64_t grid = (q.rows + kQxWarps - 1) / kQxWarps * ((q.Kg * G + 127) / 128);
+    if (grid > 0x7fffffffLL) {
+        set_error("quant_x: %lld x %lld exceeds the grid limit", (long long)q.rows, (long long)q.K);
+        return Q4FC_ELIMIT;
+    }
+    auto* kernel = G == 128 ? quant_x_group_kernel<128, false> : f16 ? quant_x_group_kernel<32, true> : quant_x_group_kernel<32, false>;
+    DependentLaunch l(dim3((unsigned)grid), kQxWarps * 32, s);
+    Q4FC_CUDA_OK(cudaLaunchKernelEx(&l.cfg, kernel, q));
     return Q4FC_OK;
 }
 

@@ -24,7 +24,8 @@ from ._cabi import FLAG_NIBBLE_SIGNED, FLAG_PDL, FLAG_STREAMK, Q4_0, Q4_1
 
 __all__ = ["offline_FC_quant_Q4A", "offline_FC_dequant_Q4A", "fc_Q4A", "FC_dynamic_quantize_x",
            "fc_workspace", "Workspace", "fc_Q4A_multi", "FCBatch", "fc_Q4A_q8", "quantize_activations", "rmsnorm_quantize", "silu_mul_quantize",
-           "QuantizedActivations", "QuantizeBatch", "FCChain", "FC_quant_Q8C", "FC_evaluate_Q8C", "embedding_q8c_quant_w", "embedding_q8c", "check_device_status"]
+           "QuantizedActivations", "QuantizeBatch", "FCChain", "FC_quant_Q8C", "FC_evaluate_Q8C", "embedding_q8c_quant_w", "embedding_q8c", "check_device_status",
+           "RowGroups", "group_rows", "route_top_k", "fc_Q4A_experts"]
 
 
 def _index(device: torch.device) -> int:
@@ -637,6 +638,65 @@ def embedding_q8c(output: torch.Tensor, input: torch.Tensor, weight: torch.Tenso
     reference's argument order and in-place result (ops/op_embedding.hpp:108-137).  An id outside the table gives a
     row of zeros and makes ``check_device_status`` raise."""
     _front().embedding(input, weight, scales, output)
+
+
+# ---- FCs whose weights depend on the row: experts and adapters --------------------------------------------------------
+class RowGroups:
+    """The rows of a call sorted by the id of the weights they take (``q4fc_groups_*`` format): made by ``group_rows`` or
+    ``route_top_k``, and read by every call of a step that shares the choice.
+
+    ``ids``: the ids as given, int32 or int64 of any shape; ``n_groups``; ``most_rows``: no group has more rows."""
+
+    __slots__ = ("ids", "n_groups", "most_rows", "buf")
+
+    def __init__(self, ids: torch.Tensor, n_groups: int, most_rows: int, buf: torch.Tensor) -> None:
+        self.ids, self.n_groups, self.most_rows, self.buf = ids, n_groups, most_rows, buf
+
+    @property
+    def offsets(self) -> torch.Tensor:
+        """int32 ``[n_groups + 1]``: the first place in ``order`` of each group, and of the rows without one."""
+        return self.buf[16: 17 + self.n_groups]
+
+    @property
+    def order(self) -> torch.Tensor:
+        """int32 ``[rows]``: row numbers sorted by group, stable; those without a group last."""
+        first = 16 + (self.n_groups + 4) // 4 * 4
+        return self.buf[first: first + self.ids.numel()]
+
+
+def group_rows(ids: torch.Tensor, n_groups: int) -> RowGroups:
+    """Sorts rows by id.  ``ids``: int32 or int64 of any shape, ``0 <= id < n_groups``; a negative id stands for no
+    group, one beyond the last too and makes ``check_device_status`` raise.  At most 1024 groups."""
+    buf = _front().group_rows(ids, n_groups)
+    return RowGroups(ids, n_groups, ids.numel(), buf)
+
+
+def route_top_k(logits: torch.Tensor, top_k: int, *, renormalize: bool = True) -> tuple[torch.Tensor, RowGroups]:
+    """The router of a layer of experts: softmax of ``logits`` (fp32 ``[..., experts]``, at most 1024), the ``top_k``
+    (at most 32) largest of each token, and the plan for ``fc_Q4A_experts``.
+
+    Returns the weights, fp32 ``[..., top_k]`` -- with ``renormalize`` each token's sum to one -- and the groups, whose
+    ``ids`` are int32 ``[..., top_k]``.  Equal logits: the lower index first.  An expert whose logit is -inf is closed; where too
+    few are open the remaining slots have id -1 and weight 0.  A NaN makes the token's weights NaN."""
+    weights, ids, buf = _front().route_top_k(logits, top_k, renormalize)
+    return weights, RowGroups(ids, logits.shape[-1], ids.numel() // top_k, buf)
+
+
+def fc_Q4A_experts(input: torch.Tensor, wei_quantized: torch.Tensor, N: int, groups: RowGroups, *,
+                   weights: torch.Tensor | None = None, silu_mul: bool = False, nibble_signed: bool = False,
+                   out: torch.Tensor | None = None) -> torch.Tensor:
+    """``fc_Q4A`` with the weights that a router chose for each (token, slot) pair.
+
+    ``input``: fp32 ``[B, M, K]``, a row per token, or ``[B, M, top_k, K]``, a row per pair; ``wei_quantized``: int8
+    ``[experts, Ng, Kg, block_bytes]``, a packed tensor per expert; ``groups``: of ids ``[B, M, top_k]``
+    (``route_top_k``, ``group_rows``).  Returns the products, fp32 ``[B, M, top_k, N]``, or with ``weights`` (fp32
+    ``[B, M, top_k]``) their weighted sum over the slots, ``[B, M, N]``.  A pair without an expert gives zeros.
+
+    ``silu_mul``: a row of ``input`` is gate, then up, as one product with both projections packed as one tensor of
+    ``2 K`` columns leaves them, and ``silu(gate) * up`` is multiplied (``llmops.itrans`` and ``imul`` of the
+    reference, ops/op_misc.hpp:83-138)."""
+    return _front().fc_experts(input, wei_quantized, N, groups.ids, groups.n_groups, groups.most_rows, groups.buf, weights,
+                               silu_mul, nibble_signed, out)
 
 
 def check_device_status(device: torch.device | str | int | None = None) -> None:
