@@ -463,6 +463,36 @@ size_t q4fc_experts_workspace_bytes(int64_t tokens, int64_t top_k, int64_t K, in
                                     int weighted);
 int q4fc_fc_experts(const q4fc_experts_call* call, void* ws, size_t ws_bytes, unsigned flags, q4fc_stream_t stream);
 
+/* Low-rank adapters of many requests beside a shared projection: for every row m of a group i of the plan
+ *   y[m] += scales[i] * lora_b[i] . (lora_a[i] . x[m])
+ * with lora_a [adapters][rank][K], lora_b [adapters][N][rank], both of one dtype and dense, x as it is (not quantized) and
+ * sums in fp32 (products of fp32 numbers are off by 2^-22, of x with fp16 or bf16 too).  Rows without a group are left
+ * as they are.  scales: fp32 [adapters], or NULL for ones.  rank 1..256.
+ *   q4fc_lora_add  adds to the y that is there, of any projection.
+ *   q4fc_fc_lora   q4fc_fc into y and the adapters' part on top: the same results as the two calls.  (The adapters' first
+ *                  product runs beside the start of the projection.)  A wait that runs out sets the device status word
+ *                  that q4fc_fc_check_status(NULL, ..) reads.
+ * ws: scratch, 256-byte aligned, of q4fc_lora_workspace_bytes or q4fc_fc_lora_workspace_bytes bytes; it need not be
+ * zeroed, nothing is kept in it between calls, and calls that may overlap need separate ones. */
+enum { Q4FC_F32 = 0, Q4FC_F16 = 1, Q4FC_BF16 = 2 };
+typedef struct q4fc_lora_call {
+    const float* x;          /* fp32 [rows][ldx] */
+    int64_t rows, K, ldx;
+    const void* lora_a;
+    const void* lora_b;
+    int dtype;
+    int64_t adapters, rank, N;
+    const float* scales;
+    const void* groups;      /* the plan of the rows' ids, n_groups = adapters */
+    float* y;                /* fp32 [rows][ldy] */
+    int64_t ldy;
+} q4fc_lora_call;
+size_t q4fc_lora_workspace_bytes(int64_t rows, int64_t rank);
+int q4fc_lora_add(const q4fc_lora_call* call, void* ws, size_t ws_bytes, q4fc_stream_t stream);
+size_t q4fc_fc_lora_workspace_bytes(int64_t rows, int64_t rank, int64_t K, int64_t N, int qtype, int group_k);
+int q4fc_fc_lora(const q4fc_lora_call* call, const void* wq, int64_t Ng, int64_t Kg, int qtype, int group_k, void* ws,
+                 size_t ws_bytes, unsigned flags, q4fc_stream_t stream);
+
 /* Reads and clears the device status word kept at the start of a workspace
  * (host-synchronous: waits for `stream`).  ws = NULL reads the word that decode
  * calls made without a workspace share (one per device).  Returns Q4FC_OK or

@@ -32,6 +32,7 @@ SYMBOLS = (
     "q4fc_fc_chain_create", "q4fc_fc_chain_run", "q4fc_fc_chain_check", "q4fc_fc_chain_destroy",
     "q4fc_q8c_pack", "q4fc_q8c_workspace_bytes", "q4fc_q8c_fc", "q4fc_emb_q8c_quant", "q4fc_emb_q8c",
     "q4fc_groups_bytes", "q4fc_group_rows", "q4fc_route_top_k", "q4fc_experts_workspace_bytes", "q4fc_fc_experts",
+    "q4fc_lora_workspace_bytes", "q4fc_lora_add", "q4fc_fc_lora_workspace_bytes", "q4fc_fc_lora",
 )
 
 
@@ -141,6 +142,26 @@ class ExpertsCall(C.Structure):
     ]
 
 
+class LoraCall(C.Structure):
+    """``q4fc_lora_call`` of include/q4fc_b200.h."""
+    _fields_ = [
+        ("x", C.c_void_p),
+        ("rows", C.c_int64),
+        ("K", C.c_int64),
+        ("ldx", C.c_int64),
+        ("lora_a", C.c_void_p),
+        ("lora_b", C.c_void_p),
+        ("dtype", C.c_int),
+        ("adapters", C.c_int64),
+        ("rank", C.c_int64),
+        ("N", C.c_int64),
+        ("scales", C.c_void_p),
+        ("groups", C.c_void_p),
+        ("y", C.c_void_p),
+        ("ldy", C.c_int64),
+    ]
+
+
 _lib = None
 
 
@@ -199,6 +220,12 @@ def lib() -> C.CDLL:
     L.q4fc_experts_workspace_bytes.restype = sz
     L.q4fc_experts_workspace_bytes.argtypes = [i64, i64, i64, i64, i32, i64, i32]
     L.q4fc_fc_experts.argtypes = [C.POINTER(ExpertsCall), vp, sz, u32, vp]
+    L.q4fc_lora_workspace_bytes.restype = sz
+    L.q4fc_lora_workspace_bytes.argtypes = [i64, i64]
+    L.q4fc_lora_add.argtypes = [C.POINTER(LoraCall), vp, sz, vp]
+    L.q4fc_fc_lora_workspace_bytes.restype = sz
+    L.q4fc_fc_lora_workspace_bytes.argtypes = [i64, i64, i64, i64, i32, i32]
+    L.q4fc_fc_lora.argtypes = [C.POINTER(LoraCall), vp, i64, i64, i32, i32, vp, sz, u32, vp]
     L.q4fc_tp_site_bytes.restype = sz
     if L.q4fc_tp_site_bytes() != C.sizeof(TpSite):
         raise RuntimeError(f"q4fc_tp_site is {L.q4fc_tp_site_bytes()} bytes in the library, {C.sizeof(TpSite)} here")

@@ -122,6 +122,52 @@ int check_groups(const char* who, int64_t rows, int64_t n_groups, const void* gr
     return Q4FC_OK;
 }
 
+int lora_call(const char* who, const q4fc_lora_call* call, void* ws, size_t ws_bytes, LoraCall* out) {
+    if (!call) {
+        set_error("%s: null call", who);
+        return Q4FC_EINVAL;
+    }
+    const q4fc_lora_call& c = *call;
+    if (c.rows < 0 || c.K <= 0 || c.N < 0 || c.rank < 1) {
+        set_error("%s: negative or empty size (rows=%lld K=%lld N=%lld rank=%lld)", who, (long long)c.rows, (long long)c.K,
+                  (long long)c.N, (long long)c.rank);
+        return Q4FC_EINVAL;
+    }
+    if (int rc = check_groups(who, c.rows, c.adapters, c.groups)) return rc;
+    if (c.rank > 256 || c.K > 0x3fffffffLL || c.N > 0x3fffffffLL) {
+        set_error("%s: rank=%lld exceeds 256, or K=%lld or N=%lld is beyond the limit", who, (long long)c.rank, (long long)c.K,
+                  (long long)c.N);
+        return Q4FC_ELIMIT;
+    }
+    if (c.dtype != Q4FC_F32 && c.dtype != Q4FC_F16 && c.dtype != Q4FC_BF16) {
+        set_error("%s: unknown dtype %d of the adapters", who, c.dtype);
+        return Q4FC_EINVAL;
+    }
+    if (c.rows > 0 && c.N > 0) {
+        if (!c.x || !c.lora_a || !c.lora_b || !c.y || c.ldx < c.K || c.ldy < c.N) {
+            set_error("%s: null pointer, or a leading dimension smaller than the row", who);
+            return Q4FC_EINVAL;
+        }
+        const size_t each = c.dtype == Q4FC_F32 ? 4 : 2;
+        if (!aligned(c.x, 4) || !aligned(c.y, 4) || !aligned(c.lora_a, each) || !aligned(c.lora_b, each) || !aligned(c.scales, 4)) {
+            set_error("%s: misaligned pointer", who);
+            return Q4FC_EALIGN;
+        }
+        const size_t need = q4fc_lora_workspace_bytes(c.rows, c.rank);
+        if (!ws || ws_bytes < need) {
+            set_error("%s: workspace of %zu bytes given, %zu needed", who, ws ? ws_bytes : 0, need);
+            return Q4FC_EWORKSPACE;
+        }
+        if (!aligned(ws, 256)) {
+            set_error("%s: workspace needs 256-byte alignment", who);
+            return Q4FC_EALIGN;
+        }
+    }
+    *out = LoraCall{c.x, c.rows, c.K, c.ldx, c.lora_a, c.lora_b, c.dtype, c.adapters, c.rank, c.N, c.scales,
+                    group_plan(const_cast<void*>(c.groups), c.rows, c.adapters), c.y, c.ldy, ws};
+    return Q4FC_OK;
+}
+
 }  // namespace
 }  // namespace q4fc
 
@@ -593,6 +639,58 @@ int q4fc_fc_experts(const q4fc_experts_call* call, void* ws, size_t ws_bytes, un
     e.most_rows = c.most_rows > 0 && c.most_rows < rows ? c.most_rows : rows;
     e.y = c.y, e.ldy = c.ldy, e.flags = flags, e.scratch = static_cast<uint8_t*>(ws);
     return launch_fc_experts(e, c.weights, c.top_k, static_cast<cudaStream_t>(stream));
+}
+
+size_t q4fc_lora_workspace_bytes(int64_t rows, int64_t rank) {
+    if (rows < 0 || rows > kMaxGroupRows || rank < 1 || rank > 256) return 0;
+    return align_up(lora_scratch_bytes(rows, rank), 256) + 256;
+}
+
+int q4fc_lora_add(const q4fc_lora_call* call, void* ws, size_t ws_bytes, q4fc_stream_t stream) {
+    LoraCall c;
+    if (int rc = lora_call("lora_add", call, ws, ws_bytes, &c)) return rc;
+    if (c.rows == 0 || c.N == 0) return Q4FC_OK;
+    if (int rc = launch_lora_shrink(c, static_cast<cudaStream_t>(stream))) return rc;
+    return launch_lora_expand(c, static_cast<cudaStream_t>(stream));
+}
+
+size_t q4fc_fc_lora_workspace_bytes(int64_t rows, int64_t rank, int64_t K, int64_t N, int qtype, int group_k) {
+    const size_t lora = q4fc_lora_workspace_bytes(rows, rank);
+    if (lora == 0 || K <= 0 || N < 0 || !valid_variant(qtype, group_k)) return 0;
+    return lora + align_up(q4fc_fc_workspace_bytes(rows, K, N, qtype, group_k), 256);
+}
+
+int q4fc_fc_lora(const q4fc_lora_call* call, const void* wq, int64_t Ng, int64_t Kg, int qtype, int group_k, void* ws,
+                 size_t ws_bytes, unsigned flags, q4fc_stream_t stream) {
+    LoraCall c;
+    if (int rc = lora_call("fc_lora", call, ws, ws_bytes, &c)) return rc;
+    if (int rc = check_fc_args("fc_lora", c.x, c.rows, c.K, c.ldx, wq, Ng, Kg, qtype, group_k, c.N, c.y, c.ldy)) return rc;
+    if (flags & Q4FC_FLAG_STREAMK) {
+        set_error("fc_lora: Q4FC_FLAG_STREAMK is not available beside adapters");
+        return Q4FC_EINVAL;
+    }
+    if (c.rows == 0 || c.N == 0) return Q4FC_OK;
+    const size_t need = q4fc_fc_lora_workspace_bytes(c.rows, c.rank, c.K, c.N, qtype, group_k);
+    if (ws_bytes < need) {
+        set_error("fc_lora: workspace of %zu bytes given, %zu needed", ws_bytes, need);
+        return Q4FC_EWORKSPACE;
+    }
+    int* status = ring_status_word();
+    if (!status) return Q4FC_ECUDA;
+    const cudaStream_t s = static_cast<cudaStream_t>(stream);
+    const size_t lora = q4fc_lora_workspace_bytes(c.rows, c.rank);
+    uint8_t* fc_ws = static_cast<uint8_t*>(ws) + lora;
+    if (int rc = launch_lora_shrink(c, s)) return rc;
+    // (shrink writes no weights, and has let this launch begin only when everything in front of it was complete)
+    if (c.rows <= kMaxDecodeRows) {
+        if (int rc = launch_fc_decode_ring(c.x, (int)c.rows, c.K, c.ldx, static_cast<const uint8_t*>(wq), Ng, Kg, qtype, group_k, c.N,
+                                           c.y, c.ldy, flags | Q4FC_FLAG_PDL, s, fc_ws, need - lora, nullptr, nullptr, 0, status))
+            return rc;
+    } else if (int rc = launch_fc_prefill(c.x, c.rows, c.K, c.ldx, static_cast<const uint8_t*>(wq), Ng, Kg, qtype, group_k, c.N, c.y,
+                                          c.ldy, fc_ws, need - lora, flags, s, status)) {
+        return rc;
+    }
+    return launch_lora_expand(c, s);
 }
 
 size_t q4fc_tp_site_bytes(void) { return sizeof(q4fc_tp_site); }

@@ -74,7 +74,8 @@ int launch_fc_decode(const float* x, int rows, int64_t K, int64_t ldx, const uin
 int launch_fc_decode_ring(const float* x, int rows, int64_t K, int64_t ldx, const uint8_t* wq, int64_t Ng, int64_t Kg,
                           int qtype, int G, int64_t N, float* y, int64_t ldy, unsigned flags, cudaStream_t s,
                           void* ws = nullptr, size_t ws_bytes = 0, const void* xq = nullptr,
-                          const float* addend = nullptr, int64_t addend_ld = 0);
+                          const float* addend = nullptr, int64_t addend_ld = 0,
+                          int* status = nullptr);  // given: instead of the workspace's status word
 // several weight tensors on one input in one launch
 int launch_fc_decode_ring_multi(const float* x, int rows, int64_t K, int64_t ldx, int64_t Kg, int qtype, int G,
                                 const q4fc_fc_job* jobs, int njobs, unsigned flags, cudaStream_t s, void* ws,
@@ -125,7 +126,7 @@ int chain_destroy(void* chain);
 size_t prefill_workspace_bytes(int64_t rows, int64_t K, int64_t N, int qtype, int G);
 int launch_fc_prefill(const float* x, int64_t rows, int64_t K, int64_t ldx, const uint8_t* wq, int64_t Ng,
                       int64_t Kg, int qtype, int G, int64_t N, float* y, int64_t ldy, void* ws, size_t ws_bytes,
-                      unsigned flags, cudaStream_t s);
+                      unsigned flags, cudaStream_t s, int* status = nullptr);
 // the same GEMM over per-channel int8 weights; `sc`: scratch of q8c_prefill_scale_bytes
 size_t q8c_prefill_scale_bytes(int64_t rows, int64_t Kg);
 int launch_q8c_prefill(const float* x, int64_t rows, int64_t K, int64_t ldx, const int8_t* wq, const float* wscales,

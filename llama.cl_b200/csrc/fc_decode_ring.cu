@@ -34,9 +34,9 @@ int* ring_status_word() {
 
 int launch_fc_decode_ring(const float* x, int rows, int64_t K, int64_t ldx, const uint8_t* wq, int64_t Ng, int64_t Kg,
                           int qtype, int G, int64_t N, float* y, int64_t ldy, unsigned flags, cudaStream_t s, void* ws,
-                          size_t ws_bytes, const void* xq, const float* addend, int64_t addend_ld) {
+                          size_t ws_bytes, const void* xq, const float* addend, int64_t addend_ld, int* status) {
     const RingCall c = {x, ldx, xq, rows, K, Kg, wq, Ng, N, y, ldy, addend, addend_ld};
-    return launch_ring_impl<false>(&c, 1, qtype, G, flags, s, nullptr, ws, ws_bytes);
+    return launch_ring_impl<false>(&c, 1, qtype, G, flags, s, nullptr, ws, ws_bytes, status);
 }
 
 int launch_fc_decode_ring_multi(const float* x, int rows, int64_t K, int64_t ldx, int64_t Kg, int qtype, int G,

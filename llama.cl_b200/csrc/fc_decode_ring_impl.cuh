@@ -649,7 +649,7 @@ struct RingCall {
 
 template <bool TP>
 int launch_ring_impl(const RingCall* calls, int ncalls, int qtype, int G, unsigned flags, cudaStream_t s,
-                     const q4fc_tp_site* const* tp, void* ws, size_t ws_bytes) {
+                     const q4fc_tp_site* const* tp, void* ws, size_t ws_bytes, int* own_status = nullptr) {
     const DeviceInfo* di = device_info();
     if (!di) return Q4FC_ECUDA;
     RingParams p = {};
@@ -716,7 +716,7 @@ int launch_ring_impl(const RingCall* calls, int ncalls, int qtype, int G, unsign
         if (p.in[i].Kg > kg_max) kg_max = p.in[i].Kg;
     }
     p.rows_max = rows_max, p.rows_p = (rows_max + 1) / 2 * 2;
-    int* status = ws ? static_cast<int*>(ws) : ring_status_word();
+    int* status = own_status ? own_status : ws ? static_cast<int*>(ws) : ring_status_word();
     if (TP) {
         p.world = tp[0]->world, p.x_stamped = tp[0]->x_stamped, p.epoch = tp[0]->epoch;
         status = tp[0]->status;

@@ -1077,7 +1077,7 @@ size_t prefill_workspace_bytes(int64_t rows, int64_t K, int64_t N, int qtype, in
 
 int launch_fc_prefill(const float* x, int64_t rows, int64_t K, int64_t ldx, const uint8_t* wq, int64_t Ng,
                       int64_t Kg, int qtype, int G, int64_t N, float* y, int64_t ldy, void* ws, size_t ws_bytes,
-                      unsigned flags, cudaStream_t s) {
+                      unsigned flags, cudaStream_t s, int* status) {
     if (rows == 0 || N == 0) return Q4FC_OK;
     // A workspace without room for fp16 codes (of a size from when there were none, say) does for 64-row tiles.
     bool wide = may_be_wide(rows);
@@ -1089,7 +1089,7 @@ int launch_fc_prefill(const float* x, int64_t rows, int64_t K, int64_t ldx, cons
     }
     uint8_t* base = static_cast<uint8_t*>(ws);
     PrefillParams p = {};
-    p.wq = wq, p.y = y, p.status = reinterpret_cast<int*>(base);
+    p.wq = wq, p.y = y, p.status = status ? status : reinterpret_cast<int*>(base);
     p.N = N, p.ldy = ldy, p.Ng = (int)Ng, p.Kg = (int)Kg;
     const bool sgn = (flags & Q4FC_FLAG_NIBBLE_SIGNED) && qtype == 0;
     // the reference's 1/16 activation scale of Q4_0 pairs with its x16 nibble shift; neither is materialised

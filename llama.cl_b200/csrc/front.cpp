@@ -514,6 +514,79 @@ PyObject* fc_experts(PyObject*, PyObject* const* a, Py_ssize_t n) {
     FRONT_END
 }
 
+int adapter_dtype(const Tensor& t, PyObject* o) {
+    switch (t.scalar_type()) {
+        case at::kFloat: return Q4FC_F32;
+        case at::kHalf: return Q4FC_F16;
+        case at::kBFloat16: return Q4FC_BF16;
+        default: fail("lora_a: must be float32, float16 or bfloat16, got " + attr_str(o, "dtype"));
+    }
+}
+
+// lora(input, wei_quantized, N, lora_a, lora_b, ids, n_groups, plan, scales, nibble_signed, out): wei_quantized None: adds to
+// `out`, else fc_Q4A and the adapters on top
+PyObject* lora(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    if (!nargs_ok(n, 11)) return nullptr;
+    FRONT_BEGIN
+    const bool with_fc = a[1] != Py_None;
+    const char* who = with_fc ? "fc_Q4A_lora" : "lora_add";
+    const Tensor& x = tensor(a[0], "input", at::kFloat, 3);
+    for (int i = 3; i < 6; i++)
+        if (!THPVariable_Check(a[i]))
+            fail(std::string(i == 3 ? "lora_a" : i == 4 ? "lora_b" : "groups.ids") + ": expected a torch.Tensor, got " + Py_TYPE(a[i])->tp_name);
+    q4fc_lora_call c = {};
+    c.dtype = adapter_dtype(THPVariable_Unpack(a[3]), a[3]);
+    const at::ScalarType type = THPVariable_Unpack(a[3]).scalar_type();
+    const Tensor& la = tensor(a[3], "lora_a", type, 3);
+    const Tensor& lb = tensor(a[4], "lora_b", type, 3);
+    const Tensor& ids = THPVariable_Unpack(a[5]);
+    const int64_t B = x.size(0), M = x.size(1);
+    c.rows = B * M, c.K = c.ldx = x.size(2), c.adapters = la.size(0), c.rank = la.size(1), c.N = c.ldy = to_int(a[2]);
+    if (c.N < 0) fail(std::string(who) + ": negative N");
+    if (la.size(2) != c.K) fail("lora_a: expected [adapters, rank, " + std::to_string(c.K) + "], got " + shape_text(la.sizes()));
+    if (lb.size(0) != c.adapters || lb.size(1) != c.N || lb.size(2) != c.rank)
+        fail("lora_b: expected " + shape_text({c.adapters, c.N, c.rank}) + ", got " + shape_text(lb.sizes()));
+    if (ids.dim() != 2 || ids.size(0) != B || ids.size(1) != M)
+        fail("groups: ids of shape " + shape_text(ids.sizes()) + " do not fit the input " + shape_text(x.sizes()));
+    if (as_int(a[6]) != c.adapters)
+        fail("groups: a plan of " + std::to_string(as_int(a[6])) + " groups for " + std::to_string(c.adapters) + " adapters");
+    if (la.device() != x.device() || lb.device() != x.device()) fail("input and adapters live on different devices");
+    c10::cuda::CUDAGuard guard(x.device());
+    const int dev = x.device().index();
+    c.groups = plan_of(a[7], c.rows, c.adapters, x.device());
+    if (a[8] != Py_None) {
+        const Tensor& scales = tensor(a[8], "scales", at::kFloat, 1);
+        if (scales.size(0) != c.adapters) fail("scales: expected " + std::to_string(c.adapters) + " values, got " + std::to_string(scales.size(0)));
+        if (scales.device() != x.device()) fail("input and scales live on different devices");
+        c.scales = static_cast<const float*>(scales.data_ptr());
+    }
+    int64_t Ng = 0, Kg = 0;
+    int q = 0, G = 0;
+    const void* wp = nullptr;
+    if (with_fc) {
+        const Tensor& w = tensor(a[1], "wei_quantized", at::kChar, 3);
+        if (w.device() != x.device()) fail("input and wei_quantized live on different devices");
+        Ng = w.size(0), Kg = w.size(1), wp = w.data_ptr();
+        variant_of(w.size(2), &q, &G);
+    }
+    c.x = static_cast<const float*>(x.data_ptr()), c.lora_a = la.data_ptr(), c.lora_b = lb.data_ptr();
+    c.y = output(a[10], {B, M, c.N}, x.device(), &ret);
+    if (a[10] != Py_None && THPVariable_Unpack(a[10]).device() != x.device()) fail("input and out live on different devices");
+    const size_t need = with_fc ? q4fc_fc_lora_workspace_bytes(c.rows, c.rank, c.K, c.N, q, G) : q4fc_lora_workspace_bytes(c.rows, c.rank);
+    if (need == 0 && c.K > 0) fail(std::string(who) + ": rank " + std::to_string(c.rank) + " outside 1..256");
+    // scratch of this call's own, from torch's allocator: calls on several streams and captured graphs never share it
+    Tensor ws = at::detail::empty_cuda({(int64_t)need}, at::kByte, x.device(), std::nullopt);
+    void* sp = ws.data_ptr();
+    cudaStream_t stream = c10::cuda::getCurrentCUDAStream(dev).stream();
+    const unsigned flags = truth(a[9]) ? Q4FC_FLAG_NIBBLE_SIGNED : 0u;
+    if (with_fc) {
+        check(without_gil([&] { return q4fc_fc_lora(&c, wp, Ng, Kg, q, G, sp, need, flags, stream); }), who);
+    } else {
+        check(without_gil([&] { return q4fc_lora_add(&c, sp, need, stream); }), who);
+    }
+    FRONT_END
+}
+
 // ---- prepared argument blocks: fc_batch(address, n, qtype, group_k, flags, device), quant_batch(address, n, group_k,
 //      want_isum, flags, device) ------------------------------------------------------------------------------------------
 PyObject* fc_batch(PyObject*, PyObject* const* a, Py_ssize_t n) {
@@ -606,6 +679,7 @@ PyMethodDef methods[] = {
     {"group_rows", reinterpret_cast<PyCFunction>(group_rows), METH_FASTCALL, nullptr},
     {"route_top_k", reinterpret_cast<PyCFunction>(route_top_k), METH_FASTCALL, nullptr},
     {"fc_experts", reinterpret_cast<PyCFunction>(fc_experts), METH_FASTCALL, nullptr},
+    {"lora", reinterpret_cast<PyCFunction>(lora), METH_FASTCALL, nullptr},
     {"fc_batch", reinterpret_cast<PyCFunction>(fc_batch), METH_FASTCALL, nullptr},
     {"quant_batch", reinterpret_cast<PyCFunction>(quant_batch), METH_FASTCALL, nullptr},
     {"graph_step", reinterpret_cast<PyCFunction>(graph_step), METH_FASTCALL, nullptr},

@@ -90,4 +90,21 @@ int launch_experts_gemm(const ExpertsCall& c, GroupQuant q, cudaStream_t s);
 size_t experts_scratch_bytes(int64_t rows, int64_t K, int64_t N, int G, int64_t n, bool weighted);
 int launch_fc_experts(ExpertsCall c, const float* weights, int64_t top_k, cudaStream_t s);
 
+// lora.cu
+struct LoraCall {
+    const float* x;
+    int64_t rows, K, ldx;
+    const void *a, *b;   // [n][rank][K], [n][N][rank]
+    int dtype;
+    int64_t n, rank, N;
+    const float* scales;
+    GroupPlan plan;
+    float* y;
+    int64_t ldy;
+    void* scratch;
+};
+size_t lora_scratch_bytes(int64_t rows, int64_t rank);
+int launch_lora_shrink(const LoraCall& c, cudaStream_t s);  // the scratch holds A x for expand
+int launch_lora_expand(const LoraCall& c, cudaStream_t s);
+
 }  // namespace q4fc

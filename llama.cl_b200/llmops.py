@@ -25,7 +25,7 @@ from ._cabi import FLAG_NIBBLE_SIGNED, FLAG_PDL, FLAG_STREAMK, Q4_0, Q4_1
 __all__ = ["offline_FC_quant_Q4A", "offline_FC_dequant_Q4A", "fc_Q4A", "FC_dynamic_quantize_x",
            "fc_workspace", "Workspace", "fc_Q4A_multi", "FCBatch", "fc_Q4A_q8", "quantize_activations", "rmsnorm_quantize", "silu_mul_quantize",
            "QuantizedActivations", "QuantizeBatch", "FCChain", "FC_quant_Q8C", "FC_evaluate_Q8C", "embedding_q8c_quant_w", "embedding_q8c", "check_device_status",
-           "RowGroups", "group_rows", "route_top_k", "fc_Q4A_experts"]
+           "RowGroups", "group_rows", "route_top_k", "fc_Q4A_experts", "fc_Q4A_lora", "lora_add"]
 
 
 def _index(device: torch.device) -> int:
@@ -697,6 +697,27 @@ def fc_Q4A_experts(input: torch.Tensor, wei_quantized: torch.Tensor, N: int, gro
     reference, ops/op_misc.hpp:83-138)."""
     return _front().fc_experts(input, wei_quantized, N, groups.ids, groups.n_groups, groups.most_rows, groups.buf, weights,
                                silu_mul, nibble_signed, out)
+
+
+def fc_Q4A_lora(input: torch.Tensor, wei_quantized: torch.Tensor, N: int, lora_a: torch.Tensor, lora_b: torch.Tensor,
+                groups: RowGroups, *, scales: torch.Tensor | None = None, nibble_signed: bool = False,
+                out: torch.Tensor | None = None) -> torch.Tensor:
+    """``fc_Q4A`` with a low-rank adapter per row on top: ``y = fc_Q4A(x) + scales[i] * lora_b[i] @ (lora_a[i] @ x)``.
+
+    ``input`` fp32 ``[B, M, K]``; ``lora_a`` ``[adapters, rank, K]`` and ``lora_b`` ``[adapters, N, rank]``, both fp32, fp16 or
+    bf16, rank up to 256; ``groups``: of the adapters' ids ``[B, M]`` (``group_rows``; -1: none), made once for all
+    projections of a step; ``scales`` fp32 ``[adapters]`` (alpha / rank, say).  The adapters see the input as it is, not
+    quantized, and sum in fp32."""
+    return _front().lora(input, wei_quantized, N, lora_a, lora_b, groups.ids, groups.n_groups, groups.buf, scales, nibble_signed, out)
+
+
+def lora_add(output: torch.Tensor, input: torch.Tensor, lora_a: torch.Tensor, lora_b: torch.Tensor, groups: RowGroups, *,
+             scales: torch.Tensor | None = None) -> None:
+    """The adapters' part of ``fc_Q4A_lora`` added to ``output`` (fp32 ``[B, M, N]``) in place, for projections that other
+    calls compute (``fc_Q4A_multi``, ``FCBatch``, ...)."""
+    if not isinstance(output, torch.Tensor) or output.dim() != 3:
+        raise RuntimeError("output: expected an fp32 tensor [B, M, N]")
+    _front().lora(input, None, output.shape[2], lora_a, lora_b, groups.ids, groups.n_groups, groups.buf, scales, False, output)
 
 
 def check_device_status(device: torch.device | str | int | None = None) -> None:

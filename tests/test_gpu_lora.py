@@ -1,0 +1,213 @@
+"""Adapters beside a shared projection against 64 bits: every type and rank, odd sizes, rows without an adapter."""
+import numpy as np
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+TYPES = [torch.float32, torch.float16, torch.bfloat16]
+
+
+@pytest.fixture(scope="module")
+def pkg(lib_built):
+    assert torch.cuda.is_available()
+    import llama_cl_b200
+
+    return llama_cl_b200
+
+
+def inputs(rows, n, r, K, N, dtype, seed=0):
+    g = torch.Generator().manual_seed(seed + rows * 7 + r)
+    x = torch.randn(1, rows, K, generator=g)
+    a = (torch.randn(n, r, K, generator=g) / K ** 0.5).to(dtype)
+    b = (torch.randn(n, N, r, generator=g) * 0.05).to(dtype)
+    return x.cuda(), a.cuda(), b.cuda(), (torch.rand(n, generator=g) + 0.5).cuda()
+
+
+def added64(x, a, b, scales, ids):
+    """What is added to each row in 64 bits, and a bound of the kernel's error.
+
+    An operand of an MMA is cut to 11 bits and its rest to 11 more: a product of fp32 numbers is off by less than 2^-20 of
+    it (both rests' roundings and the product of the rests).  An MMA adds eight products to its sum with at most one unit in the last
+    place (2^-23) per addition, cut off or rounded: 2^-20 of the absolute terms; a chain has 3 MMAs (hi hi, hi lo, lo hi) for
+    eight of its terms, of which two are of rests, 2^-11 of it in size.  Partial sums of warps and slices add at most 24 more roundings."""
+    x, a, b = (v.double().cpu().numpy() for v in (x[0], a, b))
+    s = np.ones(len(a)) if scales is None else scales.double().cpu().numpy()
+    K, r = a.shape[2], a.shape[1]
+    want, bound = np.zeros((len(x), b.shape[1])), np.zeros((len(x), b.shape[1]))
+    for i in np.unique(ids[ids >= 0]):
+        m = ids == i
+        t, size = x[m] @ a[i].T, np.abs(x[m]) @ np.abs(a[i]).T
+        off = size * ((K // 8 + 4) * 2.0 ** -20 * 1.01 + 24 * 2.0 ** -24 + 2.0 ** -20) + np.abs(t) * 2.0 ** -23
+        want[m] = s[i] * (t @ b[i].T)
+        bound[m] = s[i] * (off @ np.abs(b[i]).T + (np.abs(t) @ np.abs(b[i]).T) * ((r // 8 + 3) * 2.0 ** -20 * 1.01 + 2.0 ** -20))
+    return want, bound + 1e-30
+
+
+def check(got, want, bound):
+    off = np.abs(got.double().cpu().numpy().reshape(want.shape) - want)
+    assert (off <= bound).all(), (off / bound).max()
+
+
+def groups_of(pkg, ids, n):
+    return pkg.llmops.group_rows(torch.from_numpy(ids).int().cuda()[None], n)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,n,r,K,N", [
+    (1, 1, 1, 1, 1), (1, 4, 16, 16, 128), (2, 2, 4, 24, 33), (8, 8, 16, 512, 256), (8, 3, 8, 1000, 130), (9, 2, 12, 77, 100), (40, 70, 64, 264, 96),
+    (61, 5, 65, 320, 129), (130, 2, 33, 100, 255), (256, 3, 32, 512, 200), (300, 7, 256, 96, 40), (700, 1, 100, 63, 17), (257, 400, 5, 129, 31)])
+def test_lora_add(pkg, rows, n, r, K, N, dtype):
+    x, a, b, scales = inputs(rows, n, r, K, N, dtype)
+    ids = np.random.default_rng(rows).integers(-1, n, rows)
+    if rows == 1:
+        ids[:] = n - 1
+    groups = groups_of(pkg, ids, n)
+    for s in (scales, None):
+        want, bound = added64(x, a, b, s, ids)
+        y = torch.zeros(1, rows, N, device="cuda")
+        pkg.llmops.lora_add(y, x, a, b, groups, scales=s)
+        check(y, want, bound)
+        # on top of what is there, one rounding more; rows without an adapter are left as they are
+        base = torch.randn(1, rows, N, generator=torch.Generator().manual_seed(1)).cuda()
+        y = base.clone()
+        pkg.llmops.lora_add(y, x, a, b, groups, scales=s)
+        there = base[0].double().cpu().numpy()
+        check(y, there + want, bound + (np.abs(there) + np.abs(want)) * 2.0 ** -23)
+        none = torch.from_numpy(ids < 0).cuda()
+        assert torch.equal(y[0, none], base[0, none])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows", [4, 300])
+def test_products_keep_22_bits(pkg, rows, dtype):
+    """One term a product: what a single tf32 operand would lose (2^-11) is not lost."""
+    n, K, N = 2, 8, 16
+    x, a, b, _ = inputs(rows, n, 1, K, N, dtype)
+    a[:, :, 1:] = 0
+    ids = np.arange(rows) % n
+    y = torch.zeros(1, rows, N, device="cuda")
+    pkg.llmops.lora_add(y, x, a, b, groups_of(pkg, ids, n))
+    want, _ = added64(x, a, b, None, ids)
+    # two products, each off by 2^-20 at most (see added64), nothing that cancels
+    assert (np.abs(y[0].double().cpu().numpy() - want) <= 2.0 ** -18 * np.abs(want) + 1e-30).all()
+
+
+@pytest.mark.parametrize("qtype,G", [("q4_0", 32), ("q4_1", 128)])
+@pytest.mark.parametrize("rows,K,N", [(1, 512, 96), (8, 4096, 300), (9, 260, 130), (61, 512, 257), (300, 384, 100)])
+def test_fc_lora_is_the_two_calls(pkg, rows, K, N, qtype, G):
+    ops = pkg.llmops
+    n = 3
+    x, a, b, scales = inputs(rows, n, 16, K, N, torch.bfloat16)
+    wq = ops.offline_FC_quant_Q4A((torch.randn(N, K, generator=torch.Generator().manual_seed(1)) * 0.02).cuda(), qtype=qtype, group_k=G)
+    groups = groups_of(pkg, np.arange(rows) % (n + 1) - 1, n)
+    for signed in (False, True):
+        want = ops.fc_Q4A(x, wq, N, nibble_signed=signed)
+        ops.lora_add(want, x, a, b, groups, scales=scales)
+        out = torch.full_like(want, float("nan"))
+        got = ops.fc_Q4A_lora(x, wq, N, a, b, groups, scales=scales, nibble_signed=signed, out=out)
+        assert got is out and torch.equal(got, want)
+    ops.check_device_status()
+
+
+@pytest.mark.parametrize("rows", [5, 280])
+def test_views_that_start_anywhere(pkg, rows):
+    """Contiguous tensors that start on no 16-byte boundary."""
+    n, r, K, N = 2, 16, 64, 64
+    x, a, b, scales = inputs(rows, n, r, K, N, torch.float16)
+    ids = np.arange(rows) % n
+    want, bound = added64(x, a, b, scales, ids)
+
+    def moved(t):
+        buf = torch.empty(t.numel() + 1, dtype=t.dtype, device="cuda")
+        v = buf[1:].view(t.shape)
+        v.copy_(t)
+        return v
+
+    groups = groups_of(pkg, ids, n)
+    for which in range(4):
+        args = [moved(t) if i == which else t for i, t in enumerate((torch.zeros(1, rows, N, device="cuda"), x, a, b))]
+        pkg.llmops.lora_add(*args, groups, scales=scales)
+        check(args[0], want, bound)
+
+
+@pytest.mark.parametrize("rows", [6, 300])
+def test_infinities_and_nan_stay_in_their_row(pkg, rows):
+    n, r, K, N = 2, 8, 40, 24
+    x, a, b, _ = inputs(rows, n, r, K, N, torch.bfloat16)
+    groups = groups_of(pkg, np.arange(rows) % n, n)
+    y = torch.zeros(1, rows, N, device="cuda")
+    pkg.llmops.lora_add(y, x, a, b, groups)
+    x[0, 1, 3], x[0, 4, 0] = float("inf"), float("nan")
+    again = torch.zeros(1, rows, N, device="cuda")
+    pkg.llmops.lora_add(again, x, a, b, groups)
+    others = torch.ones(rows, dtype=torch.bool)
+    others[[1, 4]] = False
+    assert torch.equal(again[0, others], y[0, others]) and again[0, 4].isnan().all() and not again[0, 1].isfinite().any()
+
+
+@pytest.mark.parametrize("rows", [3, 300])
+def test_captured_and_on_two_streams(pkg, rows):
+    """Two graphs captured on one stream and replayed on two do not share scratch; a replay follows its inputs."""
+    ops = pkg.llmops
+    n, K, N = 3, 4096, 256
+    x, a, b, scales = inputs(rows, n, 16, K, N, torch.bfloat16)
+    wq = ops.offline_FC_quant_Q4A((torch.randn(N, K) * 0.02).cuda())
+    ids = torch.zeros(1, rows, dtype=torch.int32, device="cuda")
+    xs = [x, torch.randn_like(x)]
+
+    def step(x):
+        return ops.fc_Q4A_lora(x, wq, N, a, b, ops.group_rows(ids, n), scales=scales)
+
+    step(x)
+    graphs, outs = [torch.cuda.CUDAGraph() for _ in xs], []
+    for graph, v in zip(graphs, xs):
+        with torch.cuda.graph(graph):
+            outs.append(step(v))
+    streams = [torch.cuda.Stream() for _ in xs]
+    for seed in (1, 2):
+        ids.copy_(torch.randint(-1, n, (1, rows), generator=torch.Generator().manual_seed(seed)).int())
+        want = [step(v) for v in xs]
+        torch.cuda.synchronize()
+        for _ in range(5):
+            for graph, stream in zip(graphs, streams):
+                with torch.cuda.stream(stream):
+                    graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(y, w) for y, w in zip(outs, want))
+
+
+def test_empty_sizes(pkg):
+    ops = pkg.llmops
+    a, b = torch.zeros(2, 4, 32, device="cuda"), torch.zeros(2, 0, 4, device="cuda")
+    x = torch.zeros(1, 3, 32, device="cuda")
+    wq = ops.offline_FC_quant_Q4A(torch.zeros(32, 32, device="cuda"))
+    groups = ops.group_rows(torch.zeros(1, 3, dtype=torch.int32, device="cuda"), 2)
+    assert ops.fc_Q4A_lora(x, wq, 0, a, b, groups).shape == (1, 3, 0)
+    none = ops.group_rows(torch.zeros(1, 0, dtype=torch.int32, device="cuda"), 2)
+    assert ops.fc_Q4A_lora(x[:, :0].contiguous(), wq, 32, a, torch.zeros(2, 32, 4, device="cuda"), none).shape == (1, 0, 32)
+
+
+def test_refusals(pkg):
+    ops = pkg.llmops
+    x, a, b, scales = inputs(3, 2, 4, 32, 32, torch.float16)
+    wq = ops.offline_FC_quant_Q4A(torch.zeros(32, 32, device="cuda"))
+    groups = ops.group_rows(torch.zeros(1, 3, dtype=torch.int32, device="cuda"), 2)
+    y = torch.zeros(1, 3, 32, device="cuda")
+    call, add = ops.fc_Q4A_lora, ops.lora_add
+    wide = torch.zeros(2, 257, 32, dtype=torch.half, device="cuda")
+    for bad, text in (
+            (lambda: call(x.half(), wq, 32, a, b, groups), "float32"), (lambda: call(x[0], wq, 32, a, b, groups), "rank 2"),
+            (lambda: call(x, wq, 32, a.double(), b, groups), "lora_a: must be"), (lambda: call(x, wq, 32, a, b.float(), groups), "lora_b"),
+            (lambda: call(x, wq, 32, a[..., :16].contiguous(), b, groups), "lora_a: expected"),
+            (lambda: call(x, wq, 31, a, b, groups), "lora_b: expected"), (lambda: call(x, wq, 32, a.transpose(1, 2), b, groups), "contiguous"),
+            (lambda: call(x, wq, 32, a[:1].contiguous(), b[:1].contiguous(), groups), "2 groups for 1 adapters"),
+            (lambda: call(x[:, :2].contiguous(), wq, 32, a, b, groups), "do not fit"),
+            (lambda: call(x, wq, 32, a, b, groups, scales=scales[:1]), "scales: expected 2"),
+            (lambda: call(x, wq, 32, a, b, groups, scales=scales.cpu()), "CUDA"), (lambda: call(x, wq, 32, a.cpu(), b, groups), "CUDA"),
+            (lambda: call(x, wq, 32, wide, wide.transpose(1, 2).contiguous()[:, :32], groups), "257"),
+            (lambda: call(x, wq[None], 32, a, b, groups), r"is<int8>\(3\)"), (lambda: call(x, wq, 32, a, b, groups, out=y[0]), "out"),
+            (lambda: add(y[0], x, a, b, groups), "output"), (lambda: add(y.half(), x, a, b, groups), "float32"),
+            (lambda: add(y[:, :2].contiguous(), x, a, b, groups), "out: expected")):
+        with pytest.raises(RuntimeError, match=text):
+            bad()
