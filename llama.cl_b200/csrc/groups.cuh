@@ -86,6 +86,10 @@ struct ExpertsCall {
 
 size_t experts_gemm_scratch(int64_t rows, int64_t Kg, int G, int64_t n);  // fc_prefill.cu
 int launch_experts_gemm(const ExpertsCall& c, GroupQuant q, cudaStream_t s);
+// fc_decode_ring_experts.cu: few rows; *done false: the shared memory does not hold the call
+bool experts_ring_serves(int64_t rows, int64_t n);
+size_t experts_ring_scratch(int64_t rows, int64_t Kg, int G, int64_t n);
+int launch_experts_ring(const ExpertsCall& c, GroupQuant q, cudaStream_t s, bool* done);
 // fc_experts.cu; with weights [rows / top_k][top_k] c.y is [rows / top_k][ldy]
 size_t experts_scratch_bytes(int64_t rows, int64_t K, int64_t N, int G, int64_t n, bool weighted);
 int launch_fc_experts(ExpertsCall c, const float* weights, int64_t top_k, cudaStream_t s);
