@@ -3,25 +3,29 @@
 // fp32, fp16 or bf16 as the adapter was trained.
 //
 // Two launches, around whatever computes y:
-//   shrink: t = A_i x, a CTA per tile of the plan's rows, slice of K and 64 ranks; slices are summed by expand, in order.
-//   expand: y += scale_i * B_i t, a CTA per tile and 128 columns.
+//   shrink: t = scale_i * A_i x, a cluster per tile of the plan's rows and 64 ranks; its CTAs divide K, and their sums meet in
+//           shared memory, in order.
+//   expand: y += B_i t.
 // Both on mma.sync.m16n8k8 (tf32 operands, fp32 sums), the adapter's rows on the 16-row side and the call's rows on the
 // 8-column side.  A tf32 operand keeps 11 bits: fp16 and bf16 weights are exact in one, an fp32 number is two (its first 11
-// bits and the rest, rounded), so that a product costs two MMAs, or three with fp32 weights, and is off by 2^-22.
+// bits and the next 11), so that a product costs two MMAs, or three with fp32 weights, and is off by 2^-20 at most.
 // The order of k in an MMA is free as long as both operands have the same: a lane takes consecutive k of a row (8 of a piece
-// of 32 in shrink, 4 of 16 in expand), so that fragments come straight from global memory in 16-byte loads.
+// of 32), so that fragments come straight from global memory in 16-byte loads.
+#include <cooperative_groups.h>
 #include <cuda_bf16.h>
 
 #include <cfloat>
 
 #include "groups.cuh"
 
+namespace cg = cooperative_groups;
+
 namespace q4fc {
 namespace {
 
 constexpr int kWarps = 8, kThreads = kWarps * 32;
 constexpr int kRankBlock = 64;   // ranks of a CTA in shrink
-constexpr int kColumns = 128;    // columns of a CTA in expand
+constexpr int kMostSlices = 8;   // CTAs of a cluster
 
 // D(16x8) += A(16x8) * B(8x8)
 __device__ __forceinline__ void mma_tf32(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -29,11 +33,10 @@ __device__ __forceinline__ void mma_tf32(float (&d)[4], const uint32_t (&a)[4], 
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// x = hi + lo: hi x's first 11 bits (cut off, which cannot overflow), lo the rest rounded to 11 bits
+// x = hi + lo, cut off to 11 bits each (which cannot overflow; an infinity leaves NaN)
 __device__ __forceinline__ void split(float x, uint32_t& hi, uint32_t& lo) {
     hi = __float_as_uint(x) & 0xffffe000u;
-    const float rest = fabsf(x) <= FLT_MAX ? x - __uint_as_float(hi) : 0.0f;  // (infinities and NaN are in hi)
-    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(lo) : "f"(rest));
+    lo = __float_as_uint(x - __uint_as_float(hi)) & 0xffffe000u;
 }
 __device__ __forceinline__ float number(float v) { return v; }
 __device__ __forceinline__ float number(__half v) { return __half2float(v); }
@@ -63,179 +66,286 @@ __device__ __forceinline__ void load_values(const T* p, int64_t valid, T (&v)[NV
     }
 }
 
+// four weights as the rows' operand, and what fp32 ones leave
+template <typename T>
+__device__ __forceinline__ void operand(T a, T b, T c, T d, uint32_t (&hi)[4], uint32_t (&lo)[4]) {
+    const float f[4] = {number(a), number(b), number(c), number(d)};
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+        if constexpr (sizeof(T) == 4) split(f[i], hi[i], lo[i]);
+        else hi[i] = __float_as_uint(f[i]), lo[i] = 0;
+}
+
 struct LoraArgs {
     const float* x;
     const void *a, *b;
     const float* scales;   // of the adapters, or null
     float* y;
-    float* part;           // [slice][row place][rank]
+    float* t;              // [place in the plan's order][rank]
     const int4* tiles;
     const int *tile_count, *order;
     int64_t rows, K, ldx, N, ldy, slice_k;
-    int rank, slices;
+    int rank;
 };
 
 // TILE rows: 64, eight warps with eight rows each, or 8, eight warps that divide the slice's K.  MB: 16-rank blocks in use.
 template <typename T, int TILE, int MB, bool VEC>
-__global__ void __launch_bounds__(kThreads) lora_shrink_kernel(const __grid_constant__ LoraArgs p) {
+__global__ void __launch_bounds__(kThreads, 2) lora_shrink_kernel(const __grid_constant__ LoraArgs p) {
     constexpr bool kByK = TILE == 8;
-    __shared__ float sums[kByK ? kWarps * MB * 16 * 8 : 1];
+    constexpr int kRanks = MB * 16;
+    __shared__ float sums[TILE * kRanks];                     // this CTA's [row][rank]
+    __shared__ float by_warp[kByK ? kWarps * TILE * kRanks : 1];
+    cg::cluster_group cluster = cg::this_cluster();
     pdl_wait_prior_grid();
     pdl_launch_dependents();
+    const int4 tile = __ldcg(p.tiles + blockIdx.y);  // (beyond the count: nothing that is used)
     if ((int)blockIdx.y >= __ldcg(p.tile_count)) return;
-    const int4 tile = __ldcg(p.tiles + blockIdx.y);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int row0 = kByK ? 0 : warp * 8;
-    if (!kByK && row0 >= tile.z) return;
     const int rank0 = blockIdx.z * kRankBlock;
     const int64_t k_begin = blockIdx.x * p.slice_k, k_end = min(p.K, k_begin + p.slice_k);
     const bool live = row0 + g < tile.z;
     const float* x = p.x + (live ? (int64_t)__ldcg(p.order + tile.y + row0 + g) * p.ldx : 0);
     const T* a = static_cast<const T*>(p.a) + ((int64_t)tile.x * p.rank + rank0) * p.K;
     float acc[MB][4] = {};
-    for (int64_t k0 = k_begin + (kByK ? warp * 32 : 0); k0 < k_end; k0 += kByK ? kWarps * 32 : 32) {
-        const int64_t k = k0 + 8 * t;
+    constexpr int64_t kStep = kByK ? kWarps * 32 : 32;
+    struct Piece {
         float v[8];
         T w[MB][2][8];
-        load_values<8, VEC>(x + k, live ? k_end - k : 0, v);
+    };
+    auto load = [&](int64_t k0, Piece& c) {
+        const int64_t k = k0 + 8 * t, valid = k_end - k;
+        load_values<8, VEC>(x + k, live ? valid : 0, c.v);
 #pragma unroll
         for (int m = 0; m < MB; m++)
 #pragma unroll
             for (int h = 0; h < 2; h++) {
                 const int r = m * 16 + h * 8 + g;
-                load_values<8, VEC>(a + (int64_t)r * p.K + k, rank0 + r < p.rank ? k_end - k : 0, w[m][h]);
+                load_values<8, VEC>(a + (int64_t)r * p.K + k, rank0 + r < p.rank ? valid : 0, c.w[m][h]);
             }
+    };
+    auto multiply = [&](const Piece& c) {
 #pragma unroll
         for (int j = 0; j < 4; j++) {
             uint32_t hi0, lo0, hi1, lo1;
-            split(v[2 * j], hi0, lo0), split(v[2 * j + 1], hi1, lo1);
+            split(c.v[2 * j], hi0, lo0), split(c.v[2 * j + 1], hi1, lo1);
 #pragma unroll
             for (int m = 0; m < MB; m++) {
-                const float f[4] = {number(w[m][0][2 * j]), number(w[m][1][2 * j]), number(w[m][0][2 * j + 1]), number(w[m][1][2 * j + 1])};
                 uint32_t wh[4], wl[4];
-                if constexpr (sizeof(T) == 4) {
-#pragma unroll
-                    for (int i = 0; i < 4; i++) split(f[i], wh[i], wl[i]);
-                    mma_tf32(acc[m], wl, hi0, hi1);
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 4; i++) wh[i] = __float_as_uint(f[i]);
-                }
+                operand(c.w[m][0][2 * j], c.w[m][1][2 * j], c.w[m][0][2 * j + 1], c.w[m][1][2 * j + 1], wh, wl);
+                if constexpr (sizeof(T) == 4) mma_tf32(acc[m], wl, hi0, hi1);
                 mma_tf32(acc[m], wh, lo0, lo1);
                 mma_tf32(acc[m], wh, hi0, hi1);
             }
         }
+    };
+    // pieces on their way while one is multiplied, as the registers allow
+    constexpr int kDepth = !VEC || MB * sizeof(T) > 8 ? 1 : MB * sizeof(T) > 4 ? 2 : 3;
+    Piece c[kDepth];
+    int64_t k0 = row0 < tile.z ? k_begin + (kByK ? warp * 32 : 0) : k_end;
+    if constexpr (kDepth > 1) {
+#pragma unroll
+        for (int d = 0; d + 1 < kDepth; d++)
+            if (k0 + d * kStep < k_end) load(k0 + d * kStep, c[d]);
+    }
+    while (k0 < k_end) {
+#pragma unroll
+        for (int d = 0; d < kDepth; d++) {
+            if (k0 >= k_end) break;
+            if (k0 + (kDepth - 1) * kStep < k_end) load(k0 + (kDepth - 1) * kStep, c[(d + kDepth - 1) % kDepth]);
+            multiply(c[d]);
+            k0 += kStep;
+        }
     }
     // acc[m][i]: rank m * 16 + 8 (i / 2) + g of row 2t + i % 2
-    float* part = p.part + ((int64_t)blockIdx.x * p.rows + tile.y) * p.rank + rank0;
+    float* mine = kByK ? by_warp + warp * TILE * kRanks : sums + row0 * kRanks;
+#pragma unroll
+    for (int m = 0; m < MB; m++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) mine[(2 * t + i % 2) * kRanks + m * 16 + 8 * (i / 2) + g] = acc[m][i];
     if constexpr (kByK) {
-#pragma unroll
-        for (int m = 0; m < MB; m++)
-#pragma unroll
-            for (int i = 0; i < 4; i++) sums[((warp * 8 + 2 * t + i % 2) * MB + m) * 16 + 8 * (i / 2) + g] = acc[m][i];
         __syncthreads();
-        for (int i = threadIdx.x; i < 8 * MB * 16; i += kThreads) {
-            const int row = i / (MB * 16), r = i % (MB * 16);
+        for (int i = threadIdx.x; i < TILE * kRanks; i += kThreads) {
             float sum = 0.0f;
 #pragma unroll
-            for (int w = 0; w < kWarps; w++) sum += sums[w * 8 * MB * 16 + i];
-            if (row < tile.z && rank0 + r < p.rank) part[(int64_t)row * p.rank + r] = sum;
+            for (int w = 0; w < kWarps; w++) sum += by_warp[w * TILE * kRanks + i];
+            sums[i] = sum;
         }
-    } else {
-#pragma unroll
-        for (int m = 0; m < MB; m++)
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const int row = row0 + 2 * t + i % 2, r = m * 16 + 8 * (i / 2) + g;
-                if (row < tile.z && rank0 + r < p.rank) part[(int64_t)row * p.rank + r] = acc[m][i];
-            }
     }
+    cluster.sync();
+    const float scale = p.scales ? p.scales[tile.x] : 1.0f;
+    const int slices = (int)gridDim.x, here = (int)blockIdx.x;
+    for (int i = here * kThreads + threadIdx.x; i < tile.z * kRanks; i += slices * kThreads) {
+        float sum = 0.0f;
+        for (int s = 0; s < slices; s++) sum += cluster.map_shared_rank(sums, s)[i];
+        const int row = i / kRanks, r = i % kRanks;
+        if (rank0 + r < p.rank) p.t[(int64_t)(tile.y + row) * p.rank + rank0 + r] = sum * scale;
+    }
+    cluster.sync();  // nobody leaves while its sums are being read
 }
 
-// VEC: 4 ranks of a row of B in one load, two columns of y in one
-template <typename T, int TILE, bool VEC>
-__global__ void __launch_bounds__(kThreads) lora_expand_kernel(const __grid_constant__ LoraArgs p) {
-    extern __shared__ float ts[];  // t of the tile: [TILE][pitch], scaled
-    const int ranks = (p.rank + 15) / 16 * 16, pitch = ranks + 8;  // (rows 8 words apart: a float2 a lane without conflicts)
+// y += B t.  The work is pieces of 32 rows of a tile and 64 columns, or of its eight rows and 128, the columns of a tile one behind
+// another; a CTA takes a contiguous share of what the plan has.  A warp takes 16 columns of 16 or 8 rows at a time; what the next piece
+// needs of y and of B's first ranks is on its way meanwhile.  t of a tile is in shared memory, as the MMAs want it: two ranks of a row in 16 bytes, {hi,
+// hi, lo, lo}, those that a lane reads in turn 64 bytes apart.
+// QUADS: fours of ranks that a lane takes of a piece of 16 ranks (1, for at most 16) or 32 (2); PIECES of these at a time.
+__host__ __device__ constexpr int expand_rows(int tile) { return tile < 32 ? tile : 32; }
+__host__ __device__ constexpr int expand_columns(int tile) { return tile < 32 ? 128 : 64; }
+__host__ __device__ constexpr int expand_pitch(int ranks) { return ranks * 8 / 128 * 128 + 64 + (ranks * 8 % 128 > 64 ? 128 : 0); }  // bytes
+template <typename T, int TILE, int QUADS, int PIECES, bool VEC>
+__global__ void __launch_bounds__(kThreads, 2) lora_expand_kernel(const __grid_constant__ LoraArgs p, const bool y_vec) {
+    constexpr int NV = 4 * QUADS, kPiece = 4 * NV, kChunk = kPiece * PIECES;  // values of a lane, ranks of a piece, ranks at a time
+    constexpr int kRows = expand_rows(TILE), kParts = TILE / kRows, NB = kRows > 8 ? 2 : 1;
+    constexpr int kAcross = expand_columns(TILE);
+    extern __shared__ uint4 ts[];  // [kRows][pitch]
+    const int chunks = (p.rank + kChunk - 1) / kChunk, pitch = expand_pitch(chunks * kChunk) / 16;
     pdl_wait_prior_grid();
     pdl_launch_dependents();
-    if ((int)blockIdx.y >= __ldcg(p.tile_count)) return;
-    const int4 tile = __ldcg(p.tiles + blockIdx.y);
-    const float scale = p.scales ? p.scales[tile.x] : 1.0f;
-    for (int i = threadIdx.x; i < TILE * ranks; i += kThreads) {
-        const int row = i / ranks, r = i - row * ranks;
-        float sum = 0.0f;
-        if (row < tile.z && r < p.rank) {
-            const float* src = p.part + ((int64_t)tile.y + row) * p.rank + r;
-#pragma unroll 4
-            for (int s = 0; s < p.slices; s++) sum += __ldcg(src + (int64_t)s * p.rows * p.rank);
-        }
-        ts[row * pitch + r] = sum * scale;
-    }
-    __syncthreads();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int64_t n = (int64_t)blockIdx.x * kColumns + warp * 16 + 2 * g;  // this lane's columns: n and n + 1
-    if (n - 2 * g >= p.N) return;
-    const T* b = static_cast<const T*>(p.b) + ((int64_t)tile.x * p.N + n) * p.rank;
-    constexpr int NB = TILE / 8;
-    const int blocks = (tile.z + 7) / 8;
-    float acc[NB][4] = {};
-    for (int r0 = 0; r0 < p.rank; r0 += 16) {
-        const int r = r0 + 4 * t;
-        T w[2][4];
+    const int64_t blocks = (p.N + kAcross - 1) / kAcross, total = (int64_t)__ldcg(p.tile_count) * kParts * blocks;
+    int64_t at = total * blockIdx.x / gridDim.x;
+    const int64_t end = total * (blockIdx.x + 1) / gridDim.x;
+    while (at < end) {
+        const int64_t part = at / blocks;  // of a tile
+        const int64_t first = at - part * blocks, last = min(blocks, first + end - at);
+        at += last - first;
+        int4 tile = __ldcg(p.tiles + part / kParts);
+        tile.y += kRows * (int)(part % kParts), tile.z -= kRows * (int)(part % kParts);  // this piece's rows of it
+        if (tile.z <= 0) continue;
+        const int rows = min(tile.z, kRows), row0 = warp * 16 / kAcross * 16, live = (rows - row0 + 7) / 8;  // (this warp's first row)
+        float* y_at[NB][2];  // row row0 + nb * 8 + 2t + i of the piece at this lane's columns n and n + 1; null: none
+        int64_t n = first * kAcross + warp * 16 % kAcross + 2 * g;
 #pragma unroll
-        for (int h = 0; h < 2; h++) load_values<4, VEC>(b + h * p.rank + r, n + h < p.N ? p.rank - r : 0, w[h]);
+        for (int nb = 0; nb < NB; nb++)
 #pragma unroll
-        for (int j = 0; j < 2; j++) {
-            const float f[4] = {number(w[0][2 * j]), number(w[1][2 * j]), number(w[0][2 * j + 1]), number(w[1][2 * j + 1])};
-            uint32_t wh[4], wl[4];
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-                if constexpr (sizeof(T) == 4) split(f[i], wh[i], wl[i]);
-                else wh[i] = __float_as_uint(f[i]);
-#pragma unroll
-            for (int nb = 0; nb < NB; nb++) {
-                if (nb >= blocks) break;
-                const float2 v = *reinterpret_cast<const float2*>(ts + (nb * 8 + g) * pitch + r + 2 * j);
-                uint32_t hi0, lo0, hi1, lo1;
-                split(v.x, hi0, lo0), split(v.y, hi1, lo1);
-                if constexpr (sizeof(T) == 4) mma_tf32(acc[nb], wl, hi0, hi1);
-                mma_tf32(acc[nb], wh, lo0, lo1);
-                mma_tf32(acc[nb], wh, hi0, hi1);
+            for (int i = 0; i < 2; i++) {
+                const int row = row0 + nb * 8 + 2 * t + i;
+                y_at[nb][i] = row < rows ? p.y + (int64_t)__ldcg(p.order + tile.y + row) * p.ldy + n : nullptr;
             }
+        const T* b = static_cast<const T*>(p.b) + ((int64_t)tile.x * p.N + n) * p.rank + NV * t;
+        auto load_b = [&](const T* b, int64_t n, int r0, T (&w)[PIECES][2][NV]) {
+#pragma unroll
+            for (int q = 0; q < PIECES; q++)
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    const int r = r0 + q * kPiece;
+                    load_values<NV, VEC>(b + h * p.rank + r, n + h < p.N ? p.rank - r - NV * t : 0, w[q][h]);
+                }
+        };
+        struct Next {
+            T w[PIECES][2][NV];
+            float2 y[NB][2];
+        };
+        auto load = [&](int ahead, Next& c) {  // `ahead` pieces further
+            load_b(b + ahead * kAcross * (int64_t)p.rank, n + ahead * kAcross, 0, c.w);
+            const int64_t m = n + ahead * kAcross;
+#pragma unroll
+            for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    const float* from = y_at[nb][i] + ahead * kAcross;
+                    float2 v = make_float2(0.0f, 0.0f);
+                    if (y_at[nb][i] != nullptr) {
+                        if (y_vec && m + 1 < p.N) {
+                            v = __ldcg(reinterpret_cast<const float2*>(from));
+                        } else {
+                            if (m < p.N) v.x = __ldcg(from);
+                            if (m + 1 < p.N) v.y = __ldcg(from + 1);
+                        }
+                    }
+                    c.y[nb][i] = v;
+                }
+        };
+        Next c[2];
+        load(0, c[0]);
+        __syncthreads();  // (nobody reads the piece in front any more)
+        for (int row = warp; row < kRows; row += kWarps)
+            for (int i = lane; i < chunks * kChunk / 2; i += 32) {  // pairs of ranks
+                float v[2] = {0.0f, 0.0f};
+                if (row < rows) {
+                    const float* from = p.t + (int64_t)(tile.y + row) * p.rank + 2 * i;
+                    if (2 * i < p.rank) v[0] = __ldcg(from);
+                    if (2 * i + 1 < p.rank) v[1] = __ldcg(from + 1);
+                }
+                uint4 u;
+                split(v[0], u.x, u.z), split(v[1], u.y, u.w);
+                // pair (NV / 2) t + j of a piece stands at place 4 j + t
+                constexpr int kPairs = kPiece / 2, kOf = NV / 2;
+                const int in = i % kPairs;
+                ts[row * pitch + i / kPairs * kPairs + in % kOf * 4 + in / kOf] = u;
+            }
+        __syncthreads();
+        float acc[NB][4];
+        auto multiply = [&](int chunk, const T (&w)[PIECES][2][NV]) {
+            const uint4* mine = ts + (row0 + g) * pitch + chunk * (kChunk / 2) + t;
+#pragma unroll
+            for (int q = 0; q < PIECES; q++)
+#pragma unroll
+                for (int j = 0; j < NV / 2; j++) {
+                    uint32_t wh[4], wl[4];
+                    operand(w[q][0][2 * j], w[q][1][2 * j], w[q][0][2 * j + 1], w[q][1][2 * j + 1], wh, wl);
+#pragma unroll
+                    for (int nb = 0; nb < NB; nb++) {
+                        if (nb >= live) break;
+                        const uint4 u = mine[nb * 8 * pitch + q * (kPiece / 2) + 4 * j];
+                        if constexpr (sizeof(T) == 4) mma_tf32(acc[nb], wl, u.x, u.y);
+                        mma_tf32(acc[nb], wh, u.z, u.w);
+                        mma_tf32(acc[nb], wh, u.x, u.y);
+                    }
+                }
+        };
+        auto finish = [&](Next& c) {
+#pragma unroll
+            for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+                for (int j = 0; j < 4; j++) acc[nb][j] = 0.0f;
+            multiply(0, c.w);
+#pragma unroll 1
+            for (int chunk = 1; chunk < chunks; chunk++) {
+                load_b(b, n, chunk * kChunk, c.w);
+                multiply(chunk, c.w);
+            }
+            // acc[nb][i]: column n + i / 2 of row row0 + nb * 8 + 2t + i % 2
+#pragma unroll
+            for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    if (y_at[nb][i] == nullptr) continue;
+                    const float2 v = make_float2(c.y[nb][i].x + acc[nb][i], c.y[nb][i].y + acc[nb][i + 2]);
+                    if (y_vec && n + 1 < p.N) {
+                        *reinterpret_cast<float2*>(y_at[nb][i]) = v;
+                    } else {
+                        if (n < p.N) y_at[nb][i][0] = v.x;
+                        if (n + 1 < p.N) y_at[nb][i][1] = v.y;
+                    }
+                    y_at[nb][i] += kAcross;
+                }
+            n += kAcross, b += kAcross * (int64_t)p.rank;
+        };
+#pragma unroll 1
+        for (int64_t k = first; k < last; k += 2) {
+            if (k + 1 < last) load(1, c[1]);
+            finish(c[0]);
+            if (k + 1 >= last) break;
+            if (k + 2 < last) load(1, c[0]);
+            finish(c[1]);
         }
     }
-    // acc[nb][i]: column n + i / 2 of row nb * 8 + 2t + i % 2
-#pragma unroll
-    for (int nb = 0; nb < NB; nb++)
-#pragma unroll
-        for (int i = 0; i < 2; i++) {
-            const int row = nb * 8 + 2 * t + i;
-            if (row >= tile.z) continue;
-            float* y = p.y + (int64_t)__ldcg(p.order + tile.y + row) * p.ldy + n;
-            if (VEC && n + 1 < p.N) {
-                float2 v = __ldcg(reinterpret_cast<const float2*>(y));
-                v.x += acc[nb][i], v.y += acc[nb][i + 2];
-                *reinterpret_cast<float2*>(y) = v;
-            } else {
-                if (n < p.N) y[0] = __ldcg(y) + acc[nb][i];
-                if (n + 1 < p.N) y[1] = __ldcg(y + 1) + acc[nb][i + 2];
-            }
-        }
 }
 
 struct LoraPlan {
     int which, slices;
-    int64_t slice_k;
+    int64_t slice_k, tiles;  // tiles that are likely in use
 };
 // Tiles of 64 rows from 256 rows on.  K in slices until the tiles that are likely in use fill the SMs twice, none below 256 k.
 LoraPlan lora_plan(int64_t rows, int64_t K, int64_t rank, int64_t n, int sms) {
     LoraPlan l;
     l.which = rows >= 256 ? kTiles64 : kTiles8;
-    const int64_t least = n < rows ? n : rows, tiles = rows / tile_rows(l.which) > least ? rows / tile_rows(l.which) : least;
-    const int64_t blocks = tiles * ((rank + kRankBlock - 1) / kRankBlock);
+    const int64_t filled = rows / tile_rows(l.which), used = (n < rows ? n : rows) * 2 / 3;
+    l.tiles = filled > used ? filled : used > 1 ? used : 1;
+    const int64_t blocks = l.tiles * ((rank + kRankBlock - 1) / kRankBlock);
     int64_t slices = (2 * sms + blocks - 1) / blocks;
-    const int64_t most = (K + 255) / 256 < 16 ? (K + 255) / 256 : 16;
+    const int64_t most = (K + 255) / 256 < kMostSlices ? (K + 255) / 256 : kMostSlices;
     if (slices > most) slices = most;
     l.slice_k = ((K + slices - 1) / slices + 31) / 32 * 32;
     l.slices = (int)((K + l.slice_k - 1) / l.slice_k);
@@ -245,30 +355,45 @@ LoraPlan lora_plan(int64_t rows, int64_t K, int64_t rank, int64_t n, int sms) {
 template <typename T, int TILE, int MB>
 int launch_shrink(const LoraArgs& p, bool vec, dim3 grid, cudaStream_t s) {
     DependentLaunch l(grid, kThreads, s);
+    cudaLaunchAttribute attrs[2] = {l.attr, {}};
+    attrs[1].id = cudaLaunchAttributeClusterDimension;
+    attrs[1].val.clusterDim.x = grid.x, attrs[1].val.clusterDim.y = attrs[1].val.clusterDim.z = 1;
+    l.cfg.attrs = attrs, l.cfg.numAttrs = 2;
     Q4FC_CUDA_OK(cudaLaunchKernelEx(&l.cfg, vec ? lora_shrink_kernel<T, TILE, MB, true> : lora_shrink_kernel<T, TILE, MB, false>, p));
     return Q4FC_OK;
 }
+template <typename T, int TILE, int QUADS, int PIECES>
+int launch_expand(const LoraCall& c, const LoraArgs& p, int64_t tiles, cudaStream_t s) {
+    const DeviceInfo* di = device_info();
+    if (!di) return Q4FC_ECUDA;
+    const bool vec = c.rank % (4 * QUADS) == 0 && (reinterpret_cast<uintptr_t>(c.b) & 15) == 0;
+    const bool y_vec = c.ldy % 2 == 0 && (reinterpret_cast<uintptr_t>(c.y) & 7) == 0;
+    constexpr int kChunk = 16 * QUADS * PIECES;
+    const int64_t pieces = tiles * (TILE / expand_rows(TILE)) * ((c.N + expand_columns(TILE) - 1) / expand_columns(TILE)), most = 2 * di->sm_count;
+    DependentLaunch l(dim3((unsigned)(pieces < most ? pieces : most)), kThreads, s);
+    auto* fn = vec ? lora_expand_kernel<T, TILE, QUADS, PIECES, true> : lora_expand_kernel<T, TILE, QUADS, PIECES, false>;
+    l.cfg.dynamicSmemBytes = expand_rows(TILE) * (size_t)expand_pitch((int)(c.rank + kChunk - 1) / kChunk * kChunk);
+    if (l.cfg.dynamicSmemBytes > 48 * 1024)
+        Q4FC_CUDA_OK(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)l.cfg.dynamicSmemBytes));
+    Q4FC_CUDA_OK(cudaLaunchKernelEx(&l.cfg, fn, p, y_vec));
+    return Q4FC_OK;
+}
 template <typename T, int TILE>
-int launch_lora_tile(const LoraCall& c, const LoraArgs& p, bool expand, int64_t tiles, cudaStream_t s) {
+int launch_lora_tile(const LoraCall& c, const LoraArgs& p, const LoraPlan& l, bool expand, int64_t tiles, cudaStream_t s) {
     if (!expand) {
         const bool vec = c.K % 8 == 0 && c.ldx % 4 == 0 && ((reinterpret_cast<uintptr_t>(c.x) | reinterpret_cast<uintptr_t>(c.a)) & 15) == 0;
-        const dim3 grid((unsigned)p.slices, (unsigned)tiles, (unsigned)((c.rank + kRankBlock - 1) / kRankBlock));
+        const dim3 grid((unsigned)l.slices, (unsigned)tiles, (unsigned)((c.rank + kRankBlock - 1) / kRankBlock));
         if (c.rank <= 16) return launch_shrink<T, TILE, 1>(p, vec, grid, s);
         if (c.rank <= 32) return launch_shrink<T, TILE, 2>(p, vec, grid, s);
         return launch_shrink<T, TILE, 4>(p, vec, grid, s);
     }
-    const bool vec = c.rank % 4 == 0 && c.ldy % 2 == 0 && (reinterpret_cast<uintptr_t>(c.y) & 7) == 0 && (reinterpret_cast<uintptr_t>(c.b) & 15) == 0;
-    DependentLaunch l(dim3((unsigned)((c.N + kColumns - 1) / kColumns), (unsigned)tiles), kThreads, s);
-    auto* fn = vec ? lora_expand_kernel<T, TILE, true> : lora_expand_kernel<T, TILE, false>;
-    l.cfg.dynamicSmemBytes = TILE * (size_t)((c.rank + 15) / 16 * 16 + 8) * 4;
-    if (l.cfg.dynamicSmemBytes > 48 * 1024)
-        Q4FC_CUDA_OK(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)l.cfg.dynamicSmemBytes));
-    Q4FC_CUDA_OK(cudaLaunchKernelEx(&l.cfg, fn, p));
-    return Q4FC_OK;
+    if (c.rank <= 16) return launch_expand<T, TILE, 1, 1>(c, p, tiles, s);
+    if (c.rank <= 32 || sizeof(T) == 4) return launch_expand<T, TILE, 2, 1>(c, p, tiles, s);
+    return launch_expand<T, TILE, 2, 2>(c, p, tiles, s);
 }
 template <typename T>
-int launch_lora_type(const LoraCall& c, const LoraArgs& p, int which, bool expand, int64_t tiles, cudaStream_t s) {
-    return which == kTiles8 ? launch_lora_tile<T, 8>(c, p, expand, tiles, s) : launch_lora_tile<T, 64>(c, p, expand, tiles, s);
+int launch_lora_type(const LoraCall& c, const LoraArgs& p, const LoraPlan& l, bool expand, int64_t tiles, cudaStream_t s) {
+    return l.which == kTiles8 ? launch_lora_tile<T, 8>(c, p, l, expand, tiles, s) : launch_lora_tile<T, 64>(c, p, l, expand, tiles, s);
 }
 int launch_lora(const LoraCall& c, bool expand, cudaStream_t s) {
     const DeviceInfo* di = device_info();
@@ -280,16 +405,15 @@ int launch_lora(const LoraCall& c, bool expand, cudaStream_t s) {
         return Q4FC_ELIMIT;
     }
     LoraArgs p = {c.x, c.a, c.b, c.scales, c.y, static_cast<float*>(c.scratch), c.plan.tiles[l.which], c.plan.counts + l.which, c.plan.order,
-                  c.rows, c.K, c.ldx, c.N, c.ldy, l.slice_k, (int)c.rank, l.slices};
-    if (c.dtype == Q4FC_F32) return launch_lora_type<float>(c, p, l.which, expand, tiles, s);
-    if (c.dtype == Q4FC_F16) return launch_lora_type<__half>(c, p, l.which, expand, tiles, s);
-    return launch_lora_type<__nv_bfloat16>(c, p, l.which, expand, tiles, s);
+                  c.rows, c.K, c.ldx, c.N, c.ldy, l.slice_k, (int)c.rank};
+    if (c.dtype == Q4FC_F32) return launch_lora_type<float>(c, p, l, expand, tiles, s);
+    if (c.dtype == Q4FC_F16) return launch_lora_type<__half>(c, p, l, expand, tiles, s);
+    return launch_lora_type<__nv_bfloat16>(c, p, l, expand, tiles, s);
 }
 
 }  // namespace
 
-// (slices do not depend on the card: at most 16)
-size_t lora_scratch_bytes(int64_t rows, int64_t rank) { return (size_t)(rows * rank) * 16 * 4; }
+size_t lora_scratch_bytes(int64_t rows, int64_t rank) { return (size_t)(rows * rank) * 4; }
 int launch_lora_shrink(const LoraCall& c, cudaStream_t s) { return launch_lora(c, false, s); }
 int launch_lora_expand(const LoraCall& c, cudaStream_t s) { return launch_lora(c, true, s); }
 
