@@ -8,10 +8,12 @@
 //
 // Route: a warp per token, a lane holds every 32nd logit.  A step of the choice is two warp reductions, of the largest key
 // and of the lowest index that has it; only the winner looks for its next.
-// Group: one cluster.  Each warp owns a contiguous piece of the rows and its own bins in shared memory, so that equal ids
-// need no atomics whose order would decide places: it counts its piece (lanes with equal ids find one another with
-// match.any, the first adds), the bins of all warps and CTAs are summed in order, and it walks its piece again with its
-// places.  The same from run to run.
+// Group, up to 256 rows: one CTA, a thread per row, that counts the rows in front of its own: those with a lower id and
+// those with the same that come earlier.  All else follows from these two numbers.
+// Group, more rows: one cluster.  Each warp owns a contiguous piece of the rows and its own bins in shared memory, so that
+// equal ids need no atomics whose order would decide places: it counts its piece (lanes with equal ids find one another with
+// ballots, the first adds) and notes each row's place among its own; the bins of all warps and CTAs are summed in order
+// and give the places in front.  The same from run to run.
 #include <cooperative_groups.h>
 
 #include <atomic>
@@ -117,85 +119,182 @@ struct GroupArgs {
     GroupPlan plan;
     int* status;
 };
-// ROUTE: the warps choose the experts of their own tokens first (NV logits a lane)
+__device__ __forceinline__ int bin_of(const GroupArgs& a, int64_t i) {
+    const int64_t id = a.i32 ? (int64_t)__ldcg(static_cast<const int*>(a.ids) + i) : (int64_t)__ldcg(static_cast<const long long*>(a.ids) + i);
+    if (id >= a.n) atomicOr(a.status, kStatusBadId);
+    return id >= 0 && id < a.n ? (int)id : a.n;
+}
+
+// Up to kFew rows.  NV > 0: the warps choose the experts of the tokens first (NV logits a lane).
+constexpr int kFew = 256;
+template <int NV>
+__global__ void __launch_bounds__(kFew) group_few_kernel(const GroupArgs a, const RouteArgs route) {
+    __shared__ __align__(16) int bins[kFew], sorted[kFew];
+    __shared__ int tiles_to[kTileSizes][kFew + 1];  // tiles that begin in front of a place
+    __shared__ int warp_tiles[kTileSizes][kFew / 32];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, me = threadIdx.x, rows = (int)a.rows;
+    pdl_wait_prior_grid();
+    pdl_launch_dependents();
+    if constexpr (NV > 0) {
+        for (int64_t t = warp; t < route.tokens; t += kFew / 32) route_token<NV>(route, t, lane);
+        __syncthreads();
+    }
+    const int b = me < rows ? bin_of(a, me) : a.n + 1;  // (behind all that are there)
+    bins[me] = b;
+    __syncthreads();
+    int less = 0, before = 0, equal = 0;
+    for (int i = 0; i < rows; i += 4) {
+        const int4 o = *reinterpret_cast<const int4*>(bins + i);
+        less += (o.x < b) + (o.y < b) + (o.z < b) + (o.w < b);
+        equal += (o.x == b) + (o.y == b) + (o.z == b) + (o.w == b);
+        before += (o.x == b && i < me) + (o.y == b && i + 1 < me) + (o.z == b && i + 2 < me) + (o.w == b && i + 3 < me);
+    }
+    const int place = me < rows ? less + before : me;
+    sorted[place] = b;
+    // a tile of a size begins at this row's place
+    for (int j = 0; j < kTileSizes; j++) tiles_to[j][place] = b < a.n && before % tile_rows(j) == 0;
+    if (me < rows) a.plan.order[place] = me, a.plan.group_of[place] = b;
+    __syncthreads();
+    // (place me) tiles in front
+    int begins[kTileSizes], in_warp[kTileSizes];
+#pragma unroll
+    for (int j = 0; j < kTileSizes; j++) {
+        begins[j] = tiles_to[j][me];
+        const uint32_t mask = __ballot_sync(0xffffffffu, begins[j]);
+        in_warp[j] = __popc(mask & ((1u << lane) - 1));
+        if (lane == 0) warp_tiles[j][warp] = __popc(mask);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < kTileSizes; j++) {
+        int front = in_warp[j], all = 0;
+#pragma unroll
+        for (int w = 0; w < kFew / 32; w++) {
+            const int c = warp_tiles[j][w];
+            if (w < warp) front += c;
+            all += c;
+        }
+        tiles_to[j][me] = front;
+        if (me == 0) tiles_to[j][kFew] = all;
+    }
+    if (me < 16) {
+        int all = 0;
+        if (me < kTileSizes)
+            for (int w = 0; w < kFew / 32; w++) all += warp_tiles[me][w];
+        a.plan.counts[me] = all;
+    }
+    __syncthreads();
+    if (b < a.n)
+        for (int j = 0; j < kTileSizes; j++)
+            if (before % tile_rows(j) == 0) a.plan.tiles[j][tiles_to[j][place]] = make_int4(b, place, min(tile_rows(j), equal - before), 0);
+    for (int e = me; e <= a.n; e += kFew) {  // the first place of a group
+        int lo = 0, hi = rows;
+        while (lo < hi) {
+            const int mid = (lo + hi) / 2;
+            if (sorted[mid] < e) lo = mid + 1; else hi = mid;
+        }
+        a.plan.offsets[e] = lo;
+        for (int j = 0; j < kTileSizes; j++) a.plan.tile0[j][e] = tiles_to[j][lo];
+    }
+}
+
+// More rows.  NV as above.
+constexpr int kHeld = 8;  // sets of 32 rows of a warp that stay in registers between its two walks
+constexpr int kStaged = kWarps * kHeld * 32;  // rows of a CTA that are sorted in shared memory on their way out
+constexpr int kScans = 5;
 template <int NV>
 __global__ void __launch_bounds__(kThreads, 1) group_kernel(const GroupArgs a, const RouteArgs route) {
     extern __shared__ uint32_t bins[];  // [warp][n + 1]
     __shared__ uint32_t sums[kMaxGroups + 1];             // this CTA's rows of each group
     __shared__ uint32_t first[kMaxGroups + 1];            // its first place of each group
     __shared__ uint32_t start[kMaxGroups + 1];            // the group's first place
+    __shared__ uint32_t here[kMaxGroups + 1];             // and the first among this CTA's rows
     __shared__ int tile0[kTileSizes][kMaxGroups + 1];     // first tile of each group
-    __shared__ uint32_t warp_sum[4][kWarps];
+    __shared__ uint32_t warp_sum[kScans][kWarps];
     cg::cluster_group cluster = cg::this_cluster();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int ctas = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
     const int nb = a.n + 1;  // bins; the last one is of rows without a group
     uint32_t* mine = bins + warp * nb;
-    for (int i = threadIdx.x; i < kWarps * nb; i += kThreads) bins[i] = 0;
+    for (int i = lane; i < nb; i += 32) mine[i] = 0;
     pdl_wait_prior_grid();
     pdl_launch_dependents();
-    __syncthreads();
     const int64_t begin = min(a.rows, ((int64_t)rank * kWarps + warp) * a.piece), end = min(a.rows, begin + a.piece);
-    if constexpr (NV > 0) {
+    if constexpr (NV > 0)
         for (int64_t t = begin / route.top_k; t < end / route.top_k; t++) route_token<NV>(route, t, lane);
-        __syncwarp();  // (a warp's own ids are what it sorts)
-    }
-    auto bin_of = [&](int64_t i) {
-        const int64_t id = a.i32 ? (int64_t)__ldcg(static_cast<const int*>(a.ids) + i)
-                                 : (int64_t)__ldcg(static_cast<const long long*>(a.ids) + i);
-        if (id >= a.n) atomicOr(a.status, kStatusBadId);
-        return id >= 0 && id < a.n ? (int)id : a.n;
-    };
-    for (int64_t i0 = begin; i0 < end; i0 += 32) {
-        const bool there = i0 + lane < end;
-        const int b = there ? bin_of(i0 + lane) : -1;
-        const uint32_t same = __match_any_sync(0xffffffffu, b);
-        if (there && (same & ((1u << lane) - 1)) == 0) mine[b] += __popc(same);
+    __syncwarp();  // (a warp's own ids are what it sorts)
+    // 32 rows: their bins, and the place of each among the warp's rows of its bin.  (Lanes with equal bins find one another bit by
+    // bit: a match.any takes the longer the more different ones there are.)
+    const int bits = 32 - __clz(a.n);
+    auto count = [&](int b, bool there) {
+        uint32_t same = __ballot_sync(0xffffffffu, there);
+        for (int i = 0; i < bits; i++) {
+            const uint32_t set = __ballot_sync(0xffffffffu, (b >> i) & 1);
+            same &= (b >> i) & 1 ? set : ~set;
+        }
+        const uint32_t below = same & ((1u << lane) - 1);
+        const uint32_t at = there ? mine[b] : 0;
         __syncwarp();
+        if (there && below == 0) mine[b] = at + __popc(same);
+        __syncwarp();
+        return at + __popc(below);
+    };
+    int held[kHeld];
+    uint32_t local[kHeld];
+#pragma unroll
+    for (int h = 0; h < kHeld; h++) held[h] = begin + 32 * h + lane < end ? bin_of(a, begin + 32 * h + lane) : -1;
+#pragma unroll
+    for (int h = 0; h < kHeld; h++)
+        if (begin + 32 * h < end) local[h] = count(held[h], held[h] >= 0);
+    for (int64_t i0 = begin + 32 * kHeld; i0 < end; i0 += 32) {
+        const bool there = i0 + lane < end;
+        count(there ? bin_of(a, i0 + lane) : -1, there);
     }
     __syncthreads();
     for (int b = threadIdx.x; b < nb; b += kThreads) {  // warps in order
-        uint32_t sum = 0;
-        for (int w = 0; w < kWarps; w++) {
-            const uint32_t c = bins[w * nb + b];
-            bins[w * nb + b] = sum;
-            sum += c;
-        }
+        uint32_t c[kWarps], sum = 0;
+#pragma unroll
+        for (int w = 0; w < kWarps; w++) c[w] = bins[w * nb + b];
+#pragma unroll
+        for (int w = 0; w < kWarps; w++) bins[w * nb + b] = sum, sum += c[w];
         sums[b] = sum;
     }
     cluster.sync();
     // group b = threadIdx.x (kMaxGroups = kThreads of them): its rows, those of the CTAs in front, its first place and tiles
     uint32_t all = 0, front = 0;
     if ((int)threadIdx.x < a.n)
-        for (int c = 0; c < ctas; c++) {
-            const uint32_t v = cluster.map_shared_rank(sums, c)[threadIdx.x];
+#pragma unroll
+        for (int c = 0; c < kCluster; c++) {
+            const uint32_t v = c < ctas ? cluster.map_shared_rank(sums, c)[threadIdx.x] : 0;
             all += v;
             if (c < rank) front += v;
         }
     uint32_t none_front = 0;  // of rows without a group
     if (threadIdx.x == 0)
         for (int c = 0; c < rank; c++) none_front += cluster.map_shared_rank(sums, c)[a.n];
-    uint32_t v[4] = {all, (all + 7) / 8, (all + 63) / 64, (all + 127) / 128};
-    uint32_t own[4] = {v[0], v[1], v[2], v[3]};
+    uint32_t v[kScans] = {all, (all + 7) / 8, (all + 63) / 64, (all + 127) / 128, (int)threadIdx.x < a.n ? sums[threadIdx.x] : 0};
+    uint32_t own[kScans];
+#pragma unroll
+    for (int j = 0; j < kScans; j++) own[j] = v[j];
 #pragma unroll
     for (int off = 1; off < 32; off <<= 1)
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
+        for (int j = 0; j < kScans; j++) {
             const uint32_t o = __shfl_up_sync(0xffffffffu, v[j], off);
             if (lane >= off) v[j] += o;
         }
     if (lane == 31)
-        for (int j = 0; j < 4; j++) warp_sum[j][warp] = v[j];
+        for (int j = 0; j < kScans; j++) warp_sum[j][warp] = v[j];
     __syncthreads();
-    uint32_t total[4];
+    uint32_t total[kScans];
 #pragma unroll
-    for (int j = 0; j < 4; j++) {
+    for (int j = 0; j < kScans; j++) {
         const uint32_t w = warp_sum[j][lane];  // (32 warps)
         total[j] = __reduce_add_sync(0xffffffffu, w);
         v[j] += __reduce_add_sync(0xffffffffu, lane < warp ? w : 0u) - own[j];  // in front of this group
     }
     if ((int)threadIdx.x < a.n) {
-        first[threadIdx.x] = v[0] + front, start[threadIdx.x] = v[0];
+        first[threadIdx.x] = v[0] + front, start[threadIdx.x] = v[0], here[threadIdx.x] = v[4];
         for (int j = 0; j < kTileSizes; j++) tile0[j][threadIdx.x] = (int)v[j + 1];
         if (rank == 0) {
             a.plan.offsets[threadIdx.x] = (int)v[0];
@@ -203,7 +302,7 @@ __global__ void __launch_bounds__(kThreads, 1) group_kernel(const GroupArgs a, c
         }
     }
     if (threadIdx.x == 0) {
-        first[a.n] = total[0] + none_front, start[a.n] = total[0];
+        first[a.n] = total[0] + none_front, start[a.n] = total[0], here[a.n] = total[4];
         for (int j = 0; j < kTileSizes; j++) tile0[j][a.n] = (int)total[j + 1];
         if (rank == 0) {
             a.plan.offsets[a.n] = (int)total[0];
@@ -212,19 +311,34 @@ __global__ void __launch_bounds__(kThreads, 1) group_kernel(const GroupArgs a, c
         }
     }
     __syncthreads();
-    // the rows' places
-    for (int64_t i0 = begin; i0 < end; i0 += 32) {
-        const bool there = i0 + lane < end;
-        const int b = there ? bin_of(i0 + lane) : -1;
-        const uint32_t same = __match_any_sync(0xffffffffu, b), below = same & ((1u << lane) - 1);
-        const uint32_t at = there ? mine[b] : 0;
-        __syncwarp();
-        if (there) {
-            const uint32_t place = first[b] + at + __popc(below);
-            a.plan.order[place] = (int)(i0 + lane), a.plan.group_of[place] = b;
-            if (below == 0) mine[b] = at + __popc(same);
+    // The rows' places.  A CTA's rows go through shared memory, in their order, if they fit: neighbours in it mostly are
+    // neighbours in the plan (stored one by one, 32768 rows take 8 us more: a sector each).
+    if (a.piece <= 32 * kHeld) {
+        uint32_t* row_of = bins + kWarps * nb;
+        uint16_t* bin_at = reinterpret_cast<uint16_t*>(row_of + kStaged);
+#pragma unroll
+        for (int h = 0; h < kHeld; h++)
+            if (held[h] >= 0) {
+                const uint32_t at = here[held[h]] + mine[held[h]] + local[h];
+                row_of[at] = (uint32_t)(begin + 32 * h + lane), bin_at[at] = (uint16_t)held[h];
+            }
+        __syncthreads();
+        const uint32_t there = here[a.n] + sums[a.n];
+        for (uint32_t i = threadIdx.x; i < there; i += kThreads) {
+            const int b = bin_at[i];
+            const uint32_t place = first[b] + i - here[b];
+            a.plan.order[place] = (int)row_of[i], a.plan.group_of[place] = b;
         }
-        __syncwarp();
+    } else {
+        for (int64_t i0 = begin; i0 < end; i0 += 32) {
+            const bool there = i0 + lane < end;
+            const int b = there ? bin_of(a, i0 + lane) : -1;
+            const uint32_t local = count(b, there);
+            if (there) {
+                const uint32_t place = first[b] + local;
+                a.plan.order[place] = (int)(i0 + lane), a.plan.group_of[place] = b;
+            }
+        }
     }
     // tiles: the group of tile i is the last whose first tile is not behind it
     for (int j = 0; j < kTileSizes; j++) {
@@ -243,10 +357,16 @@ __global__ void __launch_bounds__(kThreads, 1) group_kernel(const GroupArgs a, c
 }
 
 template <int NV>
+int launch_group_few(const GroupArgs& a, const RouteArgs& route, cudaStream_t s) {
+    DependentLaunch l(dim3(1), kFew, s);
+    Q4FC_CUDA_OK(cudaLaunchKernelEx(&l.cfg, group_few_kernel<NV>, a, route));
+    return Q4FC_OK;
+}
+template <int NV>
 int launch_group_variant(const GroupArgs& a, const RouteArgs& route, int ctas, cudaStream_t s) {
     static std::atomic<bool> attr_done[64] = {};  // set once per device; a second setter repeats the same call
     auto* fn = group_kernel<NV>;
-    const size_t most = kWarps * (kMaxGroups + 1) * sizeof(uint32_t);
+    const size_t most = kWarps * (kMaxGroups + 1) * sizeof(uint32_t) + kStaged * 6;
     int dev = 0;
     Q4FC_CUDA_OK(cudaGetDevice(&dev));
     if (dev >= 64 || !attr_done[dev]) {
@@ -258,7 +378,7 @@ int launch_group_variant(const GroupArgs& a, const RouteArgs& route, int ctas, c
     attrs[1].id = cudaLaunchAttributeClusterDimension;
     attrs[1].val.clusterDim.x = (unsigned)ctas, attrs[1].val.clusterDim.y = attrs[1].val.clusterDim.z = 1;
     l.cfg.attrs = attrs, l.cfg.numAttrs = 2;
-    l.cfg.dynamicSmemBytes = kWarps * (size_t)(a.n + 1) * sizeof(uint32_t);
+    l.cfg.dynamicSmemBytes = kWarps * (size_t)(a.n + 1) * sizeof(uint32_t) + kStaged * 6;
     Q4FC_CUDA_OK(cudaLaunchKernelEx(&l.cfg, fn, a, route));
     return Q4FC_OK;
 }
@@ -285,6 +405,7 @@ int launch_group_rows(const void* ids, int ids_are_i32, int64_t rows, int64_t n,
     GroupArgs a = {};
     const int ctas = rows > 2048 ? kCluster : 1;
     if (int rc = group_args(&a, ids, ids_are_i32, rows, n, groups, ctas, 1)) return rc;
+    if (rows <= kFew) return launch_group_few<0>(a, RouteArgs{}, s);
     return launch_group_variant<0>(a, RouteArgs{}, ctas, s);
 }
 
@@ -293,11 +414,12 @@ int launch_route_top_k(const float* logits, int64_t tokens, int64_t experts, int
     RouteArgs route = {logits, tokens, ld, (int)experts, (int)top_k, renormalize, weights, ids};
     GroupArgs a = {};
     const int64_t rows = tokens * top_k;
-    const bool inside = tokens <= 1024;
-    const int ctas = rows > 2048 || (inside && tokens > 64) ? kCluster : 1;
+    const bool inside = tokens <= 64;  // (17 tokens inside 8.5 us; 333 tokens, 1332 pairs 10.0, with a launch for the choice 9.1)
+    const int ctas = rows > 2048 ? kCluster : 1;
     if (int rc = group_args(&a, ids, 1, rows, experts, groups, ctas, top_k)) return rc;
     return with_lanes((int)experts, [&](auto nv) {
         constexpr int NV = decltype(nv)::value;
+        if (rows <= kFew && tokens <= 16) return launch_group_few<NV>(a, route, s);
         if (inside) return launch_group_variant<NV>(a, route, ctas, s);
         DependentLaunch l(dim3((unsigned)((tokens + 7) / 8)), 256, s);
         Q4FC_CUDA_OK(cudaLaunchKernelEx(&l.cfg, route_kernel<NV>, route));
