@@ -1,7 +1,6 @@
-// Decode FC (rows <= 8): the kernel behind q4fc_fc_decode / _q8 / _add / _multi, with TP = true behind
-// q4fc_fc_decode_tp, and with EXPERTS = true behind q4fc_fc_experts for few rows.  Included by fc_decode_ring.cu,
-// fc_decode_ring_tp.cu (TP = true) and fc_decode_ring_experts.cu (EXPERTS = true): translation units of their own, so that
-// the others' code paths cost an instantiation nothing.
+// Decode FC (rows <= 8): the kernel behind q4fc_fc_decode / _q8 / _add / _multi, and with TP = true behind
+// q4fc_fc_decode_tp.  Included by fc_decode_ring.cu (TP = false) and fc_decode_ring_tp.cu (TP = true): two
+// translation units, so that the multi-GPU code paths cost the single-GPU instantiations nothing.
 // Reference arithmetic: fc_Q4A, ops/op_fc.hpp:286-426 (shared pieces in decode_math.cuh).
 //
 // Work.  One CTA per SM.  A launch carries up to 16 "jobs" (weight tensors), each multiplying one of up to 16
@@ -41,7 +40,6 @@
 
 #include <cstdlib>
 #include <mutex>
-#include <type_traits>
 
 #include "common.cuh"
 #include "decode_math.cuh"
@@ -102,15 +100,6 @@ struct RingParams {
     int64_t col_off[kMaxTpJobs];
     unsigned long long* y_peer[kMaxTpJobs][8];
     const unsigned long long* epoch;
-};
-
-// EXPERTS: the jobs are tiles of up to 8 rows of a plan (groups.cuh), known on the device alone: job and input i are the plan's
-// tile i, all over weights of one shape.  What job[0] and in[0] say of y, N, K holds for all; the codes are in the plan's order.
-struct RingExpertParams : RingParams {
-    const int4* tiles;
-    const int *tile_count, *order;
-    int64_t group_bytes;  // of one expert's weights
-    int Ng, most_tiles, pairs, part_off;
 };
 
 __device__ __forceinline__ void cluster_arrive_release() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
@@ -234,10 +223,8 @@ __device__ __forceinline__ void quantize_slice(const RingParams& p, int warp, in
     }
 }
 
-template <int G, int QTYPE, bool SIGNED, int ROWS, bool TP, bool PREQ, bool EXPERTS = false>
-__global__ void __launch_bounds__(kRThreads, 1)
-    fc_decode_ring_kernel(const __grid_constant__ std::conditional_t<EXPERTS, RingExpertParams, RingParams> p) {
-    static_assert(!EXPERTS || (PREQ && !TP), "experts: quantized beforehand, on one GPU");
+template <int G, int QTYPE, bool SIGNED, int ROWS, bool TP, bool PREQ>
+__global__ void __launch_bounds__(kRThreads, 1) fc_decode_ring_kernel(const __grid_constant__ RingParams p) {
     using S = RingShape<G, QTYPE>;
     constexpr int BS = S::BS;
     constexpr int SETS = S::SETS;
@@ -246,7 +233,7 @@ __global__ void __launch_bounds__(kRThreads, 1)
 
     extern __shared__ __align__(128) uint8_t smem[];
     // [0,512): mbarriers full[kRingMax], empty[kRingMax], xbar; failure flag at 192; pfull[kPartBufs] at 256,
-    // pfree[kPartBufs] at 320; EXPERTS: the plan's tiles int4 [most_tiles] and order [pairs] at 512; then part [kPartBufs][kRW][rows_p*32] f32 | inbox [inbox_stripes][cs][rows_p*32] f32 (cs > 1) | sc [kc_max][16] f32
+    // pfree[kPartBufs] at 320; then part [kPartBufs][kRW][rows_p*32] f32 | inbox [inbox_stripes][cs][rows_p*32] f32 (cs > 1) | sc [kc_max][16] f32
     //      | codes [rows_max][code_stride] | ring [depth][slot_bytes]
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int g = lane >> 2, t = lane & 3;
@@ -254,23 +241,8 @@ __global__ void __launch_bounds__(kRThreads, 1)
     const int j = (int)(blockIdx.x & (cs - 1));   // K-split rank in the cluster (clusters are consecutive CTAs)
     const int jq = (int)(blockIdx.x & (bq - 1));  // rank among the CTAs that share the quantization
     const int unit = (int)(blockIdx.x >> p.log2cs);  // work unit: the cluster, or with cs == 1 the CTA
-    int s0, r;
-    [[maybe_unused]] int4* const tiles = reinterpret_cast<int4*>(smem + 512);
-    [[maybe_unused]] int* order = nullptr;
-    if constexpr (EXPERTS) {
-        // (behind the call's quantizer, which has let this launch begin only when the plan was complete)
-        order = reinterpret_cast<int*>(tiles + p.most_tiles);
-        for (int i = threadIdx.x; i < p.most_tiles; i += kRThreads) {
-            int4 tile = __ldcg(p.tiles + i);
-            tile.z = min(tile.z, p.rows_max);
-            tiles[i] = tile;
-        }
-        for (int i = threadIdx.x; i < p.pairs; i += kRThreads) order[i] = __ldcg(p.order + i);
-        const int total = __ldcg(p.tile_count) * p.Ng;  // < 2^31: the launcher's limit
-        s0 = (int)((int64_t)total * unit / p.nc), r = (int)((int64_t)total * (unit + 1) / p.nc) - s0;
-    } else {
-        s0 = p.unit_s0[unit], r = p.unit_s0[unit + 1] - s0;
-    }
+    const int s0 = p.unit_s0[unit];
+    const int r = p.unit_s0[unit + 1] - s0;
     const int slot_f = p.rows_p * 32;
 
     const uint32_t bar0 = smem_u32(smem);
@@ -280,9 +252,7 @@ __global__ void __launch_bounds__(kRThreads, 1)
     auto pfull_bar = [&](int b) { return bar0 + 256u + 8u * b; };
     auto pfree_bar = [&](int b) { return bar0 + 320u + 8u * b; };
     volatile int* fail = reinterpret_cast<volatile int*>(smem + 192);
-    float* part;
-    if constexpr (EXPERTS) part = reinterpret_cast<float*>(smem + p.part_off);
-    else part = reinterpret_cast<float*>(smem + 512);
+    float* part = reinterpret_cast<float*>(smem + 512);
     float* inbox = part + kPartBufs * kRW * slot_f;
     float* sc = inbox + (cs > 1 ? p.inbox_stripes * cs * slot_f : 0);
     uint8_t* codes = reinterpret_cast<uint8_t*>(sc + p.kc_max * 16);
@@ -312,7 +282,6 @@ __global__ void __launch_bounds__(kRThreads, 1)
     if (TP || p.weights_early) pdl_launch_dependents();
     // "this CTA runs": nobody may store into a CTA's shared memory before that CTA has started
     if (cs > 1 || bq > 1) cluster_arrive_release();
-    if constexpr (EXPERTS) __syncthreads();  // the plan is in shared memory
 
     // what this CTA has to do for global stripe sg: job, index inside the job, input, K slice, first byte
     struct Stripe {
@@ -321,26 +290,19 @@ __global__ void __launch_bounds__(kRThreads, 1)
     };
     auto describe = [&](int sg) {
         Stripe d;
-        int Kg;
-        if constexpr (EXPERTS) {
-            d.jb = d.in = sg / p.Ng, d.ls = sg - d.jb * p.Ng, Kg = p.in[0].Kg;
-        } else {
-            d.jb = 0;
-            while (d.jb + 1 < p.njobs && sg >= p.job[d.jb].s_end) d.jb++;
-            d.ls = sg - (d.jb ? p.job[d.jb - 1].s_end : 0);
-            d.in = p.job[d.jb].input;
-            Kg = p.in[d.in].Kg;
-        }
+        d.jb = 0;
+        while (d.jb + 1 < p.njobs && sg >= p.job[d.jb].s_end) d.jb++;
+        d.ls = sg - (d.jb ? p.job[d.jb - 1].s_end : 0);
+        d.in = p.job[d.jb].input;
+        const int Kg = p.in[d.in].Kg;
         d.k0 = cs > 1 ? j * p.kq + min(j, p.kr) : 0;
         d.Kc = cs > 1 ? p.kq + (j < p.kr ? 1 : 0) : Kg;  // >= 1: the launcher keeps cs <= Kg
-        if constexpr (EXPERTS) d.base = p.job[0].wq + tiles[d.jb].x * p.group_bytes + ((int64_t)d.ls * Kg + d.k0) * BS;
-        else d.base = p.job[d.jb].wq + ((int64_t)d.ls * Kg + d.k0) * BS;
+        d.base = p.job[d.jb].wq + ((int64_t)d.ls * Kg + d.k0) * BS;
         return d;
     };
     // bulk copies of one input's quantized activations (this CTA's K slice) into shared memory
     auto fetch_codes = [&](int in, int k0, int Kc) {
-        RingInputDev I = p.in[EXPERTS ? 0 : in];
-        if constexpr (EXPERTS) I.xq += tiles[in].y * I.xq_stride, I.xsc += (int64_t)in * I.Kg * 16, I.rows = tiles[in].z;
+        const RingInputDev& I = p.in[in];
         const uint32_t row_bytes = (uint32_t)(Kc * G);
         mbar_expect_tx(xbar, row_bytes * I.rows + (uint32_t)Kc * 64u);
         for (int m = 0; m < I.rows; m++)
@@ -409,13 +371,11 @@ __global__ void __launch_bounds__(kRThreads, 1)
 
     // the finished sum of (stripe, row m, column lane) leaves the CTA
     auto final_store = [&](const Stripe& d, int m, float sum) {
-        const RingJobDev& J = p.job[EXPERTS ? 0 : d.jb];
+        const RingJobDev& J = p.job[d.jb];
         const int64_t n = (int64_t)d.ls * 32 + lane;
         if (n < J.N) {
             if (J.addend != nullptr) sum = __fadd_rn(sum, J.addend[m * J.addend_ld + n]);
-            if constexpr (EXPERTS) {
-                J.y[order[tiles[d.jb].y + m] * J.ldy + n] = sum;
-            } else if constexpr (!TP) {
+            if constexpr (!TP) {
                 J.y[m * J.ldy + n] = sum;
             } else {
                 for (int rk = 0; rk < p.world; rk++)
@@ -464,9 +424,7 @@ __global__ void __launch_bounds__(kRThreads, 1)
                     cur_in = d.in;
                 }
             }
-            int rows;
-            if constexpr (EXPERTS) rows = tiles[d.in].z;
-            else rows = p.in[d.in].rows;
+            const int rows = p.in[d.in].rows;
             const bool row_live = g < rows;
             float acc[4][2];
 #pragma unroll
@@ -567,9 +525,7 @@ __global__ void __launch_bounds__(kRThreads, 1)
                 const float* src = inbox + ((li >> p.log2cs) << p.log2cs) * slot_f + warp * 32 + lane;
                 float sum = src[0];
                 for (int q = 1; q < cs; q++) sum += src[q * slot_f];
-                const Stripe d = describe(s0 + li);
-                if (EXPERTS && warp >= tiles[d.in].z) continue;
-                final_store(d, warp, sum);
+                final_store(describe(s0 + li), warp, sum);
             }
         }
         // no CTA touches another CTA's shared memory after the barrier above, so exiting is safe
@@ -589,10 +545,10 @@ struct RingVariant {
 };
 std::mutex g_setup_mutex;
 
-template <int G, int QTYPE, bool SIGNED, int ROWS, bool TP, bool PREQ, bool EXPERTS = false>
+template <int G, int QTYPE, bool SIGNED, int ROWS, bool TP, bool PREQ>
 RingVariant* ring_variant_of() {
     static RingVariant v = {
-        reinterpret_cast<const void*>(&fc_decode_ring_kernel<G, QTYPE, SIGNED, ROWS, TP, PREQ, EXPERTS>), {}, {}};
+        reinterpret_cast<const void*>(&fc_decode_ring_kernel<G, QTYPE, SIGNED, ROWS, TP, PREQ>), {}, {}};
     return &v;
 }
 

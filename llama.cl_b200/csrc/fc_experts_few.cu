@@ -1,0 +1,451 @@
+// FC by expert where experts have few rows: a weight-streaming kernel over the plan's tiles of up to 16 rows (groups.cuh).
+// Per pair the arithmetic is that of fc_Q4A (ops/op_fc.hpp:286-426): exact integer products per K group, scaled in fp32.
+//
+// Work.  One CTA per SM, 16 warps.  (tiles in use) x (stripes of 32 columns) are one list, known on the device alone; a CTA
+// takes a contiguous share of whole stripes, and its warps contiguous shares of the share's chunks (32 columns x 128 k, 2 to
+// 2.5 KB): a warp walks through the ends of stripes as they come.  It has a ring of its own in shared memory, which its first
+// lane fills with bulk copies, so no warp waits for another one until the end.  Sums of a stripe that one warp has walked
+// whole go straight to y; the others (at most two a warp) meet in shared memory behind the one barrier and are added in
+// warp order.  No atomics, the same from run to run.
+//
+// Why not the kernel of fc_decode_ring_impl.cuh, whose 16 warps share every stripe: a stripe of a narrow expert is one block for
+// each of them, and meeting over it costs more than the block (K = 2048, group 128: 367 instructions per block, here about 110).
+//
+// Arithmetic.  mma.sync.m16n8k32 (u8 x s8), weight columns on the 16-row side, activations on the 8 columns.  Experts of a small
+// batch mostly have one or two rows; eight columns for them would be scaled at the price of eight.  So the columns are shared by
+// rows and K groups: with at most 2 rows four K groups in turn have two columns each, with at most 4 two groups have four --
+// the codes of the other groups' columns are zeros -- and one pass of conversion and scaling, in which a lane has another
+// group's scales, serves all four (or two).  Up to 16 rows are two sets of eight columns on weights that are unpacked once.
+// Codes and scales come from global memory, through L1.
+#include "decode_math.cuh"
+#include "groups.cuh"
+#include "ring_ptx.cuh"
+
+#include <atomic>
+
+namespace q4fc {
+namespace {
+
+constexpr int kWarps = 16, kThreads = kWarps * 32;
+constexpr int kMaxDepth = 6;
+constexpr int kMostTiles = 1024;  // in shared memory
+constexpr int kPartRows = 16;
+
+struct FewParams {
+    const int8_t* codes;  // [place][row_bytes]
+    const float* sc;      // [tile][Kg][16 rows][scale, sum]
+    const uint8_t* wq;
+    float* y;
+    const int4* tiles;
+    const int *tile_count, *order;
+    int64_t row_bytes, N, ldy, group_bytes;
+    int Ng, Kg, chunks;  // chunks of a stripe
+    int most_tiles, depth, y_vec, part_off, ring_off;
+    int* status;
+};
+
+template <int G, int QTYPE>
+struct FewShape {
+    static constexpr int BS = block_bytes(QTYPE, G);
+    static constexpr int kBlocks = 128 / G;  // of a chunk
+    static constexpr int kSlot = kBlocks * BS;
+};
+
+// A warp's ring: what comes next into it, and what is read next.
+template <int G, int QTYPE>
+struct WarpRing {
+    using S = FewShape<G, QTYPE>;
+    const FewParams& p;
+    const int4* tiles;
+    uint8_t* slots;
+    uint32_t bars;
+    int s0;                 // first stripe of the CTA
+    int left;               // chunks that are not asked for yet
+    int stripe, kc;         // the next of them
+    const uint8_t* from;
+    int fill = 0, read = 0; // slots
+    uint32_t parity = 0;    // of the slot that is read next
+
+    __device__ __forceinline__ void seek() {
+        const int sg = s0 + stripe, tile = sg / p.Ng;
+        from = p.wq + tiles[tile].x * p.group_bytes + ((int64_t)(sg - tile * p.Ng) * p.Kg + kc * S::kBlocks) * S::BS;
+    }
+    // one lane
+    __device__ __forceinline__ void ask() {
+        const uint32_t bytes = (uint32_t)min(S::kBlocks, p.Kg - kc * S::kBlocks) * S::BS, bar = bars + 8 * fill;
+        mbar_expect_tx(bar, bytes);
+        bulk_g2s(smem_u32(slots + fill * S::kSlot), from, bytes, bar);
+    }
+    __device__ __forceinline__ void asked() {
+        left--;
+        if (++fill == p.depth) fill = 0;
+        from += S::kSlot;
+        if (++kc == p.chunks) {
+            kc = 0, stripe++;
+            if (left > 0) seek();
+        }
+    }
+    __device__ __forceinline__ const uint8_t* wait(volatile int* fail) {
+        mbar_wait(bars + 8 * read, parity, fail, p.status, 0x4658504Cu);  // 'FXPL'
+        return slots + read * S::kSlot;
+    }
+    // the slot has been read by all lanes
+    __device__ __forceinline__ void next(int lane) {
+        __syncwarp();
+        if (left > 0) {
+            if (lane == 0) ask();
+            asked();
+        }
+        if (++read == p.depth) read = 0, parity ^= 1;
+    }
+};
+
+// 32 columns x 32 k of a block: the words of block rows t, columns 4g .. 4g + 3, as the two MMAs want them.  (Block rows are 128 bytes
+// apart: two 64-bit loads whose halves swap with the parity of t, see fc_decode_ring_impl.cuh.)
+__device__ __forceinline__ uint4 load_words(const uint8_t* row, int t) {
+    const bool odd = t & 1;
+    const uint2 u = *reinterpret_cast<const uint2*>(row + (odd ? 8 : 0));
+    const uint2 v = *reinterpret_cast<const uint2*>(row + (odd ? 0 : 8));
+    return make_uint4(odd ? v.x : u.x, odd ? v.y : u.y, odd ? u.x : v.x, odd ? u.y : v.y);
+}
+
+// The sums of chunks [kc0, kc1) of a stripe.  SHARE: K groups that share the eight columns (4, 2 or 1); SETS: of eight columns.
+// acc[s][c][mi]: columns 4g + c; row of set s and lane t: SHARE 4: mi, K groups t mod 4; 2: 2 (t % 2) + mi, K groups t / 2 mod 2; 1: 2t + mi.
+template <int G, int QTYPE, bool SIGNED, int SHARE, int SETS>
+__device__ __forceinline__ void walk(const FewParams& p, WarpRing<G, QTYPE>& ring, volatile int* fail, int lane, int4 tile, int tile_index, int kc0,
+                                     int kc1, float (&acc)[SETS][4][2]) {
+    using S = FewShape<G, QTYPE>;
+    constexpr int BS = S::BS, kRows = 8 / SHARE;  // rows of a set
+    const int g = lane >> 2, t = lane & 3;
+    const int b_group = g / kRows, b_row = g % kRows;                              // what column g is of
+    const int d_group = t * SHARE / 4, d_row = 2 * (t % (4 / SHARE));              // what this lane's columns 2t, 2t + 1 are of
+    const int8_t* codes[SETS];
+    bool live[SETS];
+#pragma unroll
+    for (int s = 0; s < SETS; s++) {
+        live[s] = 8 * s + b_row < tile.z;
+        codes[s] = p.codes + (live[s] ? tile.y + 8 * s + b_row : tile.y) * p.row_bytes + 8 * t;
+    }
+    const float* sc = p.sc + (int64_t)tile_index * p.Kg * 32 + 2 * d_row;
+#pragma unroll
+    for (int s = 0; s < SETS; s++)
+#pragma unroll
+        for (int c = 0; c < 4; c++) acc[s][c][0] = acc[s][c][1] = 0.0f;
+    constexpr int kInts = G == 128 ? 16 : 8;
+    int I[SETS][kInts];      // [lower | upper nibbles][columns 4g, 4g + 1 | 4g + 2, 4g + 3][MMA's four]
+    uint2 wd, wm;
+    float4 x4[SETS];
+    auto begin = [&] {
+        wd = wm = make_uint2(0u, 0u);
+#pragma unroll
+        for (int s = 0; s < SETS; s++) {
+            x4[s] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int i = 0; i < kInts; i++) I[s][i] = 0;
+        }
+    };
+    // conversion and scaling of what the columns have gathered
+    auto finish = [&] {
+        const float2 wd01 = __half22float2(*reinterpret_cast<const __half2*>(&wd.x)), wd23 = __half22float2(*reinterpret_cast<const __half2*>(&wd.y));
+        const float2 wm01 = __half22float2(*reinterpret_cast<const __half2*>(&wm.x)), wm23 = __half22float2(*reinterpret_cast<const __half2*>(&wm.y));
+        const float wdf[4] = {wd01.x, wd01.y, wd23.x, wd23.y}, wmf[4] = {wm01.x, wm01.y, wm23.x, wm23.y};
+#pragma unroll
+        for (int s = 0; s < SETS; s++) {
+            const float xs[2] = {x4[s].x, x4[s].z}, gs[2] = {x4[s].y, x4[s].w};
+#pragma unroll
+            for (int c = 0; c < 4; c++)
+#pragma unroll
+                for (int mi = 0; mi < 2; mi++) {
+                    // MMA (c / 2): rows g and g + 8 are columns 4g + 2 (c / 2) and one more
+                    const int at = (c / 2) * 4 + (c % 2) * 2 + mi;
+                    int low = I[s][at];
+                    if (SIGNED) low -= __float_as_int(gs[mi]);
+                    float f = __int2float_rn(low);
+                    // (group 128: upper nibbles stay in place, 16 times their value; all of it is below 2^24 and exact)
+                    if constexpr (G == 128) f = fmaf(__int2float_rn(I[s][8 + at]), 0.0625f, f);
+                    acc[s][c][mi] = fmaf(__fmul_rn(wdf[c], xs[mi]), f, acc[s][c][mi]);
+                    if (QTYPE == 1) acc[s][c][mi] = fmaf(wmf[c], gs[mi], acc[s][c][mi]);
+                }
+        }
+    };
+    auto scales_of = [&](int kb) {
+#pragma unroll
+        for (int s = 0; s < SETS; s++) x4[s] = __ldca(reinterpret_cast<const float4*>(sc + (int64_t)kb * 32 + 16 * s));
+    };
+    auto mma = [&](int (&d)[kInts], int at, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+        int(&q)[4] = *reinterpret_cast<int(*)[4]>(&d[at]);
+        mma_u8s8(q, a0, a1, a2, a3, b0, b1);
+    };
+    if constexpr (G == 32) {
+#pragma unroll 1
+        for (int kc = kc0; kc < kc1; kc++) {
+            const int n = min(4, p.Kg - 4 * kc);
+            uint2 x[SETS][4 / SHARE];  // this lane's codes: of its own K groups b_group, b_group + SHARE, ...
+#pragma unroll
+            for (int s = 0; s < SETS; s++)
+#pragma unroll
+                for (int i = 0; i < 4 / SHARE; i++) {
+                    const int j = i * SHARE + b_group;
+                    x[s][i] = make_uint2(0u, 0u);
+                    if (live[s] && j < n) x[s][i] = __ldca(reinterpret_cast<const uint2*>(codes[s] + (kc * 4 + j) * 32));
+                }
+            const uint8_t* slot = ring.wait(fail);
+#pragma unroll
+            for (int i = 0; i < 4 / SHARE; i++) {
+                begin();
+                const int mine = i * SHARE + d_group;
+                if (mine < n) {
+                    scales_of(4 * kc + mine);
+                    const uint8_t* tail = slot + mine * BS + 16 * G + g * 8;
+                    wd = *reinterpret_cast<const uint2*>(tail);
+                    if (QTYPE == 1) wm = *reinterpret_cast<const uint2*>(tail + 64);
+                }
+#pragma unroll
+                for (int h = 0; h < SHARE; h++) {
+                    const int j = i * SHARE + h;
+                    if (j >= n) break;
+                    const uint4 q = load_words(slot + j * BS + t * 128 + g * 16, t);
+                    uint32_t l[4] = {q.x & kNibMask, q.y & kNibMask, q.z & kNibMask, q.w & kNibMask};
+                    uint32_t u[4] = {(q.x >> 4) & kNibMask, (q.y >> 4) & kNibMask, (q.z >> 4) & kNibMask, (q.w >> 4) & kNibMask};
+                    if (SIGNED)
+#pragma unroll
+                        for (int k = 0; k < 4; k++) l[k] ^= 0x08080808u, u[k] ^= 0x08080808u;
+#pragma unroll
+                    for (int s = 0; s < SETS; s++) {
+                        const uint2 b = SHARE == 1 || b_group == h ? x[s][i] : make_uint2(0u, 0u);
+                        mma(I[s], 0, l[0], l[1], u[0], u[1], b.x, b.y);
+                        mma(I[s], 4, l[2], l[3], u[2], u[3], b.x, b.y);
+                    }
+                }
+                finish();
+            }
+            ring.next(lane);
+        }
+    } else {
+        // one block a chunk: the groups that share columns are successive chunks
+#pragma unroll 1
+        for (int kc = kc0; kc < kc1;) {
+            begin();
+#pragma unroll
+            for (int h = 0; h < SHARE; h++) {
+                if (kc >= kc1) break;
+                uint2 x[SETS][4];
+#pragma unroll
+                for (int s = 0; s < SETS; s++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        x[s][i] = make_uint2(0u, 0u);
+                        if (live[s] && (SHARE == 1 || b_group == h)) x[s][i] = __ldca(reinterpret_cast<const uint2*>(codes[s] + kc * 128 + 32 * i));
+                    }
+                const bool mine = SHARE == 1 || d_group == h;
+                if (mine) scales_of(kc);
+                const uint8_t* slot = ring.wait(fail);
+                if (mine) {
+                    const uint8_t* tail = slot + 16 * G + g * 8;
+                    wd = *reinterpret_cast<const uint2*>(tail);
+                    if (QTYPE == 1) wm = *reinterpret_cast<const uint2*>(tail + 64);
+                }
+#pragma unroll
+                for (int pr = 0; pr < 2; pr++) {  // two sets of 32 k: lower nibbles in one MMA, upper ones, in place, in another
+                    const uint4 qa = load_words(slot + (8 * pr + t) * 128 + g * 16, t), qb = load_words(slot + (8 * pr + 4 + t) * 128 + g * 16, t);
+                    const uint32_t a[4] = {qa.x, qa.y, qa.z, qa.w}, b[4] = {qb.x, qb.y, qb.z, qb.w};
+                    constexpr uint32_t kFlip = SIGNED ? 0x88888888u : 0u;
+                    uint32_t la[4], lb[4], ua[4], ub[4];
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        la[k] = (a[k] ^ kFlip) & kNibMask, lb[k] = (b[k] ^ kFlip) & kNibMask;
+                        ua[k] = (a[k] ^ kFlip) & ~kNibMask, ub[k] = (b[k] ^ kFlip) & ~kNibMask;
+                    }
+#pragma unroll
+                    for (int s = 0; s < SETS; s++) {
+                        const uint2 xa = x[s][2 * pr], xb = x[s][2 * pr + 1];
+                        mma(I[s], 0, la[0], la[1], lb[0], lb[1], xa.x, xb.x);
+                        mma(I[s], 4, la[2], la[3], lb[2], lb[3], xa.x, xb.x);
+                        mma(I[s], 8, ua[0], ua[1], ub[0], ub[1], xa.y, xb.y);
+                        mma(I[s], 12, ua[2], ua[3], ub[2], ub[3], xa.y, xb.y);
+                    }
+                }
+                ring.next(lane);
+                kc++;
+            }
+            finish();
+        }
+    }
+}
+
+template <int G, int QTYPE, bool SIGNED>
+__global__ void __launch_bounds__(kThreads, 1) experts_few_kernel(const __grid_constant__ FewParams p) {
+    using S = FewShape<G, QTYPE>;
+    extern __shared__ __align__(128) uint8_t smem[];
+    // barriers [warp][kMaxDepth] | failure flag | tiles | partial sums [warp][2][rows][32] | rings [warp][depth]
+    constexpr int kFail = kWarps * kMaxDepth * 8;
+    int4* const tiles = reinterpret_cast<int4*>(smem + kFail + 16);
+    float* const part = reinterpret_cast<float*>(smem + p.part_off);
+    volatile int* fail = reinterpret_cast<volatile int*>(smem + kFail);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const uint32_t bars = smem_u32(smem) + warp * kMaxDepth * 8;
+    if (lane < p.depth) mbar_init(bars + 8 * lane, 1);
+    if (threadIdx.x == 0) *fail = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    // The plan, and then the weights: the quantizer in front has let this launch begin only when what is in front of it was complete.
+    for (int i = threadIdx.x; i < p.most_tiles; i += kThreads) {
+        int4 tile = __ldcg(p.tiles + i);
+        tile.z = min(tile.z, kPartRows);
+        tiles[i] = tile;
+    }
+    const int64_t stripes = (int64_t)__ldcg(p.tile_count) * p.Ng;
+    const int s0 = (int)(stripes * blockIdx.x / gridDim.x), r = (int)(stripes * (blockIdx.x + 1) / gridDim.x) - s0;
+    __syncthreads();
+    const int C = p.chunks;
+    auto share = [&](int w) { return (int)((int64_t)r * C * w / kWarps); };  // first chunk of a warp
+    const int begin = share(warp), end = share(warp + 1);
+    WarpRing<G, QTYPE> ring{p, tiles, smem + p.ring_off + warp * p.depth * S::kSlot, bars, s0, end - begin, 0, 0, nullptr};
+    if (end > begin) {
+        ring.stripe = begin / C, ring.kc = begin - ring.stripe * C;
+        ring.seek();
+        for (int i = 0; i < p.depth && ring.left > 0; i++) {
+            if (lane == 0) ring.ask();
+            ring.asked();
+        }
+    }
+    __syncwarp();
+    pdl_wait_prior_grid();
+    pdl_launch_dependents();
+
+    // four columns of a row to y
+    auto store = [&](int64_t n, int place, float4 v) {
+        float* y = p.y + (int64_t)__ldcg(p.order + place) * p.ldy + n;
+        if (p.y_vec && n + 4 <= p.N) {
+            *reinterpret_cast<float4*>(y) = v;
+        } else {
+            if (n < p.N) y[0] = v.x;
+            if (n + 1 < p.N) y[1] = v.y;
+            if (n + 2 < p.N) y[2] = v.z;
+            if (n + 3 < p.N) y[3] = v.w;
+        }
+    };
+    int slot = 0;
+#pragma unroll 1
+    for (int c = begin; c < end; slot = 1) {
+        const int li = c / C, kc0 = c - li * C, kc1 = min(C, kc0 + end - c);
+        c += kc1 - kc0;
+        const int sg = s0 + li, ti = sg / p.Ng;
+        const int4 tile = tiles[ti];
+        const int64_t n = (int64_t)(sg - ti * p.Ng) * 32 + 4 * g;
+        const bool whole = kc0 == 0 && kc1 == C;
+        // a row of the tile, all of the stripe or this warp's part of it
+        auto put = [&](int row, float4 v) {
+            if (row >= tile.z) return;
+            if (whole) store(n, tile.y + row, v);
+            else *reinterpret_cast<float4*>(part + ((warp * 2 + slot) * kPartRows + row) * 32 + 4 * g) = v;
+        };
+        if (tile.z <= 4) {
+            float acc[1][4][2];
+            if (tile.z <= 2) walk<G, QTYPE, SIGNED, 4, 1>(p, ring, fail, lane, tile, ti, kc0, kc1, acc);
+            else walk<G, QTYPE, SIGNED, 2, 1>(p, ring, fail, lane, tile, ti, kc0, kc1, acc);
+            const bool two = tile.z <= 2;
+#pragma unroll
+            for (int k = 0; k < 4; k++)
+#pragma unroll
+                for (int mi = 0; mi < 2; mi++) {  // the K groups of the other lanes
+                    float& v = acc[0][k][mi];
+                    v += __shfl_xor_sync(0xffffffffu, v, 2);
+                    const float o = __shfl_xor_sync(0xffffffffu, v, 1);
+                    if (two) v += o;
+                }
+            if (t < (two ? 1 : 2))
+#pragma unroll
+                for (int mi = 0; mi < 2; mi++) put(2 * t + mi, make_float4(acc[0][0][mi], acc[0][1][mi], acc[0][2][mi], acc[0][3][mi]));
+        } else if (tile.z <= 8) {
+            float acc[1][4][2];
+            walk<G, QTYPE, SIGNED, 1, 1>(p, ring, fail, lane, tile, ti, kc0, kc1, acc);
+#pragma unroll
+            for (int mi = 0; mi < 2; mi++) put(2 * t + mi, make_float4(acc[0][0][mi], acc[0][1][mi], acc[0][2][mi], acc[0][3][mi]));
+        } else {
+            float acc[2][4][2];
+            walk<G, QTYPE, SIGNED, 1, 2>(p, ring, fail, lane, tile, ti, kc0, kc1, acc);
+#pragma unroll
+            for (int s = 0; s < 2; s++)
+#pragma unroll
+                for (int mi = 0; mi < 2; mi++) put(8 * s + 2 * t + mi, make_float4(acc[s][0][mi], acc[s][1][mi], acc[s][2][mi], acc[s][3][mi]));
+        }
+    }
+    __syncthreads();
+    // stripes that several warps have walked, a warp each; lane w knows what warp w has walked
+    const int first = share(min(lane, kWarps)), last = lane < kWarps ? share(lane + 1) : first;
+    for (int li = warp; li < r; li += kWarps) {
+        const bool part_of = first < last && first < (li + 1) * C && last > li * C;
+        const uint32_t who = __ballot_sync(0xffffffffu, part_of), second = __ballot_sync(0xffffffffu, part_of && first / C != li);
+        if ((who & (who - 1)) == 0) continue;
+        const int sg = s0 + li, ti = sg / p.Ng;
+        const int4 tile = tiles[ti];
+        const int64_t n = (int64_t)(sg - ti * p.Ng) * 32 + lane;
+        for (int row = 0; row < tile.z; row++) {
+            float sum = 0.0f;
+            for (uint32_t left = who; left; left &= left - 1) {
+                const int w = __ffs(left) - 1;
+                sum += part[((w * 2 + (second >> w & 1)) * kPartRows + row) * 32 + lane];
+            }
+            if (n < p.N) p.y[(int64_t)__ldcg(p.order + tile.y + row) * p.ldy + n] = sum;
+        }
+    }
+    if (*fail != 0) {
+        // a wait ran out: copies that may still be in flight land before the shared memory is handed to another CTA
+        for (int i = 0; i < 64; i++) __nanosleep(32000);
+    }
+}
+
+template <int G, int QTYPE, bool SIGNED>
+int launch_few(FewParams p, const DeviceInfo* di, cudaStream_t s) {
+    using S = FewShape<G, QTYPE>;
+    static std::atomic<bool> attr_done[64] = {};  // set once per device; a second setter repeats the same call
+    auto* fn = experts_few_kernel<G, QTYPE, SIGNED>;
+    if (di->index >= 64 || !attr_done[di->index]) {
+        Q4FC_CUDA_OK(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, di->max_smem_optin));
+        if (di->index < 64) attr_done[di->index] = true;
+    }
+    p.part_off = (int)align_up(kWarps * kMaxDepth * 8 + 16 + (size_t)p.most_tiles * 16, 128);
+    p.ring_off = p.part_off + kWarps * 2 * kPartRows * 32 * 4;
+    int depth = (di->max_smem_optin - p.ring_off) / (kWarps * S::kSlot);
+    p.depth = depth < kMaxDepth ? depth : kMaxDepth;
+    DependentLaunch l(dim3((unsigned)di->sm_count), kThreads, s);
+    l.cfg.dynamicSmemBytes = (size_t)p.ring_off + (size_t)p.depth * kWarps * S::kSlot;
+    Q4FC_CUDA_OK(cudaLaunchKernelEx(&l.cfg, fn, p));
+    return Q4FC_OK;
+}
+
+}  // namespace
+
+bool experts_few_serves(int64_t rows, int64_t n) { return rows <= 32 * n && most_tiles(kTiles16, rows, n) <= kMostTiles; }
+
+size_t experts_few_scratch(int64_t rows, int64_t Kg, int G, int64_t n) {
+    return align_up((size_t)(rows * Kg * G), 256) + align_up((size_t)(most_tiles(kTiles16, rows, n) * Kg) * 128, 256);
+}
+
+int launch_experts_few(const ExpertsCall& c, GroupQuant q, cudaStream_t s) {
+    const DeviceInfo* di = device_info();
+    if (!di) return Q4FC_ECUDA;
+    const int64_t chunks = (c.Kg * c.G + 127) / 128, tiles = most_tiles(kTiles16, c.rows, c.n);
+    if (chunks * c.Ng > 0x7fffffffLL / tiles) {
+        set_error("fc_experts: %lld rows, K=%lld, N=%lld exceed the limit of a launch", (long long)c.rows, (long long)c.K, (long long)c.N);
+        return Q4FC_ELIMIT;
+    }
+    const bool sgn = (c.flags & Q4FC_FLAG_NIBBLE_SIGNED) && c.qtype == 0;
+    FewParams p = {};
+    p.status = ring_status_word();
+    if (!p.status) return Q4FC_ECUDA;
+    q.codes = reinterpret_cast<int8_t*>(c.scratch), q.sc = reinterpret_cast<float*>(c.scratch + align_up((size_t)(c.rows * c.Kg * c.G), 256));
+    q.tile0 = c.plan.tile0[kTiles16], q.log2tile = 4, q.sums = 1, q.isum = sgn;
+    if (int rc = launch_quant_x_group(q, c.G, false, s)) return rc;
+    p.codes = q.codes, p.sc = q.sc, p.wq = c.wq, p.y = c.y, p.N = c.N, p.ldy = c.ldy;
+    p.tiles = c.plan.tiles[kTiles16], p.tile_count = c.plan.counts + kTiles16, p.order = c.plan.order;
+    p.row_bytes = c.Kg * c.G, p.group_bytes = c.Ng * c.Kg * block_bytes(c.qtype, c.G);
+    p.Ng = (int)c.Ng, p.Kg = (int)c.Kg, p.chunks = (int)chunks, p.most_tiles = (int)tiles;
+    p.y_vec = c.ldy % 4 == 0 && (reinterpret_cast<uintptr_t>(c.y) & 15) == 0;
+    if (c.qtype == 1) return c.G == 32 ? launch_few<32, 1, false>(p, di, s) : launch_few<128, 1, false>(p, di, s);
+    if (!sgn) return c.G == 32 ? launch_few<32, 0, false>(p, di, s) : launch_few<128, 0, false>(p, di, s);
+    return c.G == 32 ? launch_few<32, 0, true>(p, di, s) : launch_few<128, 0, true>(p, di, s);
+}
+
+}  // namespace q4fc

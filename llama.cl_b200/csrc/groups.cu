@@ -201,7 +201,7 @@ __global__ void __launch_bounds__(kFew) group_few_kernel(const GroupArgs a, cons
 // More rows.  NV as above.
 constexpr int kHeld = 8;  // sets of 32 rows of a warp that stay in registers between its two walks
 constexpr int kStaged = kWarps * kHeld * 32;  // rows of a CTA that are sorted in shared memory on their way out
-constexpr int kScans = 5;
+constexpr int kScans = 2 + kTileSizes;  // rows of the groups, their tiles, this CTA's rows
 template <int NV>
 __global__ void __launch_bounds__(kThreads, 1) group_kernel(const GroupArgs a, const RouteArgs route) {
     extern __shared__ uint32_t bins[];  // [warp][n + 1]
@@ -272,7 +272,10 @@ __global__ void __launch_bounds__(kThreads, 1) group_kernel(const GroupArgs a, c
     uint32_t none_front = 0;  // of rows without a group
     if (threadIdx.x == 0)
         for (int c = 0; c < rank; c++) none_front += cluster.map_shared_rank(sums, c)[a.n];
-    uint32_t v[kScans] = {all, (all + 7) / 8, (all + 63) / 64, (all + 127) / 128, (int)threadIdx.x < a.n ? sums[threadIdx.x] : 0};
+    uint32_t v[kScans];
+    v[0] = all, v[1 + kTileSizes] = (int)threadIdx.x < a.n ? sums[threadIdx.x] : 0;
+#pragma unroll
+    for (int j = 0; j < kTileSizes; j++) v[1 + j] = (all + tile_rows(j) - 1) / tile_rows(j);
     uint32_t own[kScans];
 #pragma unroll
     for (int j = 0; j < kScans; j++) own[j] = v[j];
@@ -294,7 +297,7 @@ __global__ void __launch_bounds__(kThreads, 1) group_kernel(const GroupArgs a, c
         v[j] += __reduce_add_sync(0xffffffffu, lane < warp ? w : 0u) - own[j];  // in front of this group
     }
     if ((int)threadIdx.x < a.n) {
-        first[threadIdx.x] = v[0] + front, start[threadIdx.x] = v[0], here[threadIdx.x] = v[4];
+        first[threadIdx.x] = v[0] + front, start[threadIdx.x] = v[0], here[threadIdx.x] = v[1 + kTileSizes];
         for (int j = 0; j < kTileSizes; j++) tile0[j][threadIdx.x] = (int)v[j + 1];
         if (rank == 0) {
             a.plan.offsets[threadIdx.x] = (int)v[0];
@@ -302,7 +305,7 @@ __global__ void __launch_bounds__(kThreads, 1) group_kernel(const GroupArgs a, c
         }
     }
     if (threadIdx.x == 0) {
-        first[a.n] = total[0] + none_front, start[a.n] = total[0], here[a.n] = total[4];
+        first[a.n] = total[0] + none_front, start[a.n] = total[0], here[a.n] = total[1 + kTileSizes];
         for (int j = 0; j < kTileSizes; j++) tile0[j][a.n] = (int)total[j + 1];
         if (rank == 0) {
             a.plan.offsets[a.n] = (int)total[0];

@@ -1,11 +1,11 @@
 // Rows grouped by an id: what the kernels whose weights depend on the row (experts, adapters) read of a plan that
 // groups.cu makes.  A plan is one device buffer of int32:
-//   [0, 16)        tiles of 8, 64 and 128 rows in use; the others 0
+//   [0, 16)        tiles of 8, 16, 64 and 128 rows in use; the others 0
 //   offsets[n + 1] first place in `order` of each group; offsets[n]: of the rows without one
 //   order[rows]    row numbers, sorted by group and stable: the grouped ones, then those without a group
-//   tiles          of 8, of 64 and of 128 rows: {group, first place in order, rows, 0}; a tile's rows are of one group
+//   tiles          of 8, 16, 64 and 128 rows: {group, first place in order, rows, 0}; a tile's rows are of one group
 //   group_of[rows] the group of each place in order (n: none)
-//   tile0[n + 1]   of 8, of 64 and of 128 rows: the first tile of each group
+//   tile0[n + 1]   of 8, 16, 64 and 128 rows: the first tile of each group
 // Each part starts on 16 bytes.  No group has more tiles than its rows / size + 1, so rows / size + min(n, rows) places are enough.
 #pragma once
 #include "common.cuh"
@@ -14,9 +14,8 @@ namespace q4fc {
 
 constexpr int64_t kMaxGroups = 1024;       // bins of a warp in shared memory
 constexpr int64_t kMaxGroupRows = 1 << 23;
-constexpr int kTileSizes = 3;
-__host__ __device__ constexpr int tile_rows(int which) { return which == 0 ? 8 : which == 1 ? 64 : 128; }
-enum { kTiles8 = 0, kTiles64 = 1, kTiles128 = 2 };
+enum { kTiles8, kTiles16, kTiles64, kTiles128, kTileSizes };
+__host__ __device__ constexpr int tile_rows(int which) { return which == kTiles8 ? 8 : which == kTiles16 ? 16 : which == kTiles64 ? 64 : 128; }
 
 struct GroupPlan {
     int* counts;        // tiles in use, by size
@@ -86,10 +85,10 @@ struct ExpertsCall {
 
 size_t experts_gemm_scratch(int64_t rows, int64_t Kg, int G, int64_t n);  // fc_prefill.cu
 int launch_experts_gemm(const ExpertsCall& c, GroupQuant q, cudaStream_t s);
-// fc_decode_ring_experts.cu: few rows; *done false: the shared memory does not hold the call
-bool experts_ring_serves(int64_t rows, int64_t n);
-size_t experts_ring_scratch(int64_t rows, int64_t Kg, int G, int64_t n);
-int launch_experts_ring(const ExpertsCall& c, GroupQuant q, cudaStream_t s, bool* done);
+// fc_experts_few.cu: experts with few rows
+bool experts_few_serves(int64_t rows, int64_t n);
+size_t experts_few_scratch(int64_t rows, int64_t Kg, int G, int64_t n);
+int launch_experts_few(const ExpertsCall& c, GroupQuant q, cudaStream_t s);
 // fc_experts.cu; with weights [rows / top_k][top_k] c.y is [rows / top_k][ldy]
 size_t experts_scratch_bytes(int64_t rows, int64_t K, int64_t N, int G, int64_t n, bool weighted);
 int launch_fc_experts(ExpertsCall c, const float* weights, int64_t top_k, cudaStream_t s);

@@ -205,7 +205,7 @@ __global__ void __launch_bounds__(kQxWarps * 32) quant_x_tile_kernel(const float
 }
 
 // The quantizer of the experts' product: rows in the order of a plan (groups.cuh), codes in that order, scales by the
-// plan's tiles: for the decode kernel (tiles of 8 rows) as quant_x_pre_kernel has them, else as quant_x_tile_kernel.
+// plan's tiles: for experts with few rows (tiles of 16) [tile][Kg][row][scale, sum], else as quant_x_tile_kernel has them.
 // A row of x serves `per_row` (token, slot) pairs, or one; `gated`: the value is silu(x[k]) * x[K + k].  An output row
 // without an expert is zeroed here.
 template <int G, bool F16>
@@ -248,8 +248,8 @@ __global__ void __launch_bounds__(kQxWarps * 32) quant_x_group_kernel(const __gr
     }
     const int at = (int)place - first, tile = tile0 + (at >> a.log2tile), row = at & ((1 << a.log2tile) - 1);
     int8_t* codes = a.codes + place * (a.Kg * G) * (F16 ? 2 : 1);
-    if (a.log2tile == 3)
-        quantize_unit<G, F16>(v, c, lane, a.K, a.Kg, true, a.isum, codes, a.sc + (int64_t)tile * a.Kg * 16 + 2 * row, 16, 1);
+    if (a.log2tile == 4)
+        quantize_unit<G, F16>(v, c, lane, a.K, a.Kg, true, a.isum, codes, a.sc + (int64_t)tile * a.Kg * 32 + 2 * row, 32, 1);
     else {
         const int64_t size = (int64_t)1 << a.log2tile, per = size << a.sums;
         quantize_unit<G, F16>(v, c, lane, a.K, a.Kg, a.sums, false, codes, a.sc + (int64_t)tile * a.Kg * per + row, per, size);

@@ -24,7 +24,7 @@ def check_plan(groups, ids, n):
     # the tiles, as the kernels read them
     words = groups.buf.cpu().numpy()
     at = 16 + (n + 4) // 4 * 4 + (flat.size + 3) // 4 * 4
-    for i, size in enumerate((8, 64, 128)):
+    for i, size in enumerate((8, 16, 64, 128)):
         want = [(g, offsets[g] + k, min(size, offsets[g + 1] - offsets[g] - k), 0)
                 for g in range(n) for k in range(0, offsets[g + 1] - offsets[g], size)]
         assert words[i] == len(want)
@@ -32,10 +32,10 @@ def check_plan(groups, ids, n):
         at += 4 * (flat.size // size + min(n, flat.size))
     assert np.array_equal(words[at: at + flat.size], key[order])
     at += (flat.size + 3) // 4 * 4
-    for size in (8, 64, 128):
+    for size in (8, 16, 64, 128):
         assert np.array_equal(words[at: at + n + 1], np.cumsum(np.append(0, -(-np.diff(offsets) // size))))
         at += (n + 4) // 4 * 4
-    assert at == words.size and not words[3:16].any()
+    assert at == words.size and not words[4:16].any()
 
 
 @pytest.mark.parametrize("dtype", [torch.int32, torch.int64])
