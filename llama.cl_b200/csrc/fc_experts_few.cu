@@ -22,6 +22,7 @@
 #include "ring_ptx.cuh"
 
 #include <atomic>
+#include <type_traits>
 
 namespace q4fc {
 namespace {
@@ -33,7 +34,7 @@ constexpr int kPartRows = 16;
 
 struct FewParams {
     const int8_t* codes;  // [place][row_bytes]
-    const float* sc;      // [tile][Kg][16 rows][scale, sum]
+    const float* sc;      // [tile][K group, whole chunks][two rows of 16][their scales, sums]
     const uint8_t* wq;
     float* y;
     const int4* tiles;
@@ -109,102 +110,120 @@ __device__ __forceinline__ uint4 load_words(const uint8_t* row, int t) {
     return make_uint4(odd ? v.x : u.x, odd ? v.y : u.y, odd ? u.x : v.x, odd ? u.y : v.y);
 }
 
+// Integers without conversion: an MMA that starts from the bits of 1.5 x 2^23 leaves those of 1.5 x 2^23 + I (|I| < 2^22).
+constexpr int kIntBits = 0x4B400000;
+constexpr float kInt = 12582912.0f;
+// D(16x8, s32) = A(16x32, u8) * B(32x8, s8) + these bits, or + D
+template <bool FIRST>
+__device__ __forceinline__ void mma(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    if constexpr (FIRST)
+        asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+            : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(kIntBits));
+    else
+        mma_u8s8(d, a0, a1, a2, a3, b0, b1);
+}
+__device__ __forceinline__ uint64_t pair(float lo, float hi) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+__device__ __forceinline__ uint64_t pair(int lo, int hi) { return pair(__int_as_float(lo), __int_as_float(hi)); }
+__device__ __forceinline__ float2 unpair(uint64_t v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+
 // The sums of chunks [kc0, kc1) of a stripe.  SHARE: K groups that share the eight columns (4, 2 or 1); SETS: of eight columns.
-// acc[s][c][mi]: columns 4g + c; row of set s and lane t: SHARE 4: mi, K groups t mod 4; 2: 2 (t % 2) + mi, K groups t / 2 mod 2; 1: 2t + mi.
+// acc[s][c]: column 4g + c of two rows of set s; lane t: SHARE 4: rows 0, 1, K groups t mod 4; 2: rows 2 (t % 2) and one more, K
+// groups t / 2 mod 2; 1: rows 2t, 2t + 1.  What columns of rows beyond the tile's hold is not used.
 template <int G, int QTYPE, bool SIGNED, int SHARE, int SETS>
 __device__ __forceinline__ void walk(const FewParams& p, WarpRing<G, QTYPE>& ring, volatile int* fail, int lane, int4 tile, int tile_index, int kc0,
-                                     int kc1, float (&acc)[SETS][4][2]) {
+                                     int kc1, uint64_t (&acc)[SETS][4]) {
     using S = FewShape<G, QTYPE>;
     constexpr int BS = S::BS, kRows = 8 / SHARE;  // rows of a set
     const int g = lane >> 2, t = lane & 3;
     const int b_group = g / kRows, b_row = g % kRows;                              // what column g is of
     const int d_group = t * SHARE / 4, d_row = 2 * (t % (4 / SHARE));              // what this lane's columns 2t, 2t + 1 are of
     const int8_t* codes[SETS];
-    bool live[SETS];
 #pragma unroll
-    for (int s = 0; s < SETS; s++) {
-        live[s] = 8 * s + b_row < tile.z;
-        codes[s] = p.codes + (live[s] ? tile.y + 8 * s + b_row : tile.y) * p.row_bytes + 8 * t;
-    }
-    const float* sc = p.sc + (int64_t)tile_index * p.Kg * 32 + 2 * d_row;
+    for (int s = 0; s < SETS; s++) codes[s] = p.codes + (int64_t)(tile.y + min(8 * s + b_row, tile.z - 1)) * p.row_bytes + kc0 * 128 + 32 * t;
+    const float* sc = p.sc + ((int64_t)tile_index * p.chunks + kc0) * (S::kBlocks * 32) + 2 * d_row;
 #pragma unroll
     for (int s = 0; s < SETS; s++)
 #pragma unroll
-        for (int c = 0; c < 4; c++) acc[s][c][0] = acc[s][c][1] = 0.0f;
-    constexpr int kInts = G == 128 ? 16 : 8;
-    int I[SETS][kInts];      // [lower | upper nibbles][columns 4g, 4g + 1 | 4g + 2, 4g + 3][MMA's four]
-    uint2 wd, wm;
-    float4 x4[SETS];
-    auto begin = [&] {
-        wd = wm = make_uint2(0u, 0u);
-#pragma unroll
-        for (int s = 0; s < SETS; s++) {
-            x4[s] = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-            for (int i = 0; i < kInts; i++) I[s][i] = 0;
-        }
-    };
-    // conversion and scaling of what the columns have gathered
-    auto finish = [&] {
+        for (int c = 0; c < 4; c++) acc[s][c] = 0;
+    const uint64_t minus = pair(-kInt, -kInt);
+    uint2 wd = make_uint2(0u, 0u), wm = make_uint2(0u, 0u);
+    ulonglong2 x4[SETS];     // scales of the lane's two rows, their sums
+    // scaling of what the columns have gathered; low, up: [columns 4g, 4g + 1 | 4g + 2, 4g + 3][row of the MMA's half][rows]
+    auto finish = [&](const int (&low)[SETS][2][4], const int (&up)[SETS][2][4]) {
         const float2 wd01 = __half22float2(*reinterpret_cast<const __half2*>(&wd.x)), wd23 = __half22float2(*reinterpret_cast<const __half2*>(&wd.y));
         const float2 wm01 = __half22float2(*reinterpret_cast<const __half2*>(&wm.x)), wm23 = __half22float2(*reinterpret_cast<const __half2*>(&wm.y));
         const float wdf[4] = {wd01.x, wd01.y, wd23.x, wd23.y}, wmf[4] = {wm01.x, wm01.y, wm23.x, wm23.y};
 #pragma unroll
-        for (int s = 0; s < SETS; s++) {
-            const float xs[2] = {x4[s].x, x4[s].z}, gs[2] = {x4[s].y, x4[s].w};
+        for (int c = 0; c < 4; c++) {
+            const uint64_t wd2 = pair(wdf[c], wdf[c]), wm2 = pair(wmf[c], wmf[c]);
 #pragma unroll
-            for (int c = 0; c < 4; c++)
-#pragma unroll
-                for (int mi = 0; mi < 2; mi++) {
-                    // MMA (c / 2): rows g and g + 8 are columns 4g + 2 (c / 2) and one more
-                    const int at = (c / 2) * 4 + (c % 2) * 2 + mi;
-                    int low = I[s][at];
-                    if (SIGNED) low -= __float_as_int(gs[mi]);
-                    float f = __int2float_rn(low);
-                    // (group 128: upper nibbles stay in place, 16 times their value; all of it is below 2^24 and exact)
-                    if constexpr (G == 128) f = fmaf(__int2float_rn(I[s][8 + at]), 0.0625f, f);
-                    acc[s][c][mi] = fmaf(__fmul_rn(wdf[c], xs[mi]), f, acc[s][c][mi]);
-                    if (QTYPE == 1) acc[s][c][mi] = fmaf(wmf[c], gs[mi], acc[s][c][mi]);
+            for (int s = 0; s < SETS; s++) {
+                int l0 = low[s][c / 2][c % 2 * 2], l1 = low[s][c / 2][c % 2 * 2 + 1];
+                if (SIGNED) {
+                    const float2 eights = unpair(x4[s].y);
+                    l0 -= __float_as_int(eights.x), l1 -= __float_as_int(eights.y);
                 }
+                uint64_t f = add2(pair(l0, l1), minus);
+                // (group 128: upper nibbles stay in place, 16 times their value; all of it is below 2^24 and exact)
+                if constexpr (G == 128)
+                    f = fma2(add2(pair(up[s][c / 2][c % 2 * 2], up[s][c / 2][c % 2 * 2 + 1]), minus), pair(0.0625f, 0.0625f), f);
+                acc[s][c] = fma2(mul2(wd2, x4[s].x), f, acc[s][c]);
+                if (QTYPE == 1) acc[s][c] = fma2(wm2, x4[s].y, acc[s][c]);
+            }
         }
     };
-    auto scales_of = [&](int kb) {
+    auto scales_of = [&](int kb) {  // K group kb behind kc0
 #pragma unroll
-        for (int s = 0; s < SETS; s++) x4[s] = __ldca(reinterpret_cast<const float4*>(sc + (int64_t)kb * 32 + 16 * s));
-    };
-    auto mma = [&](int (&d)[kInts], int at, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-        int(&q)[4] = *reinterpret_cast<int(*)[4]>(&d[at]);
-        mma_u8s8(q, a0, a1, a2, a3, b0, b1);
+        for (int s = 0; s < SETS; s++) x4[s] = __ldca(reinterpret_cast<const ulonglong2*>(sc + kb * 32 + 16 * s));
     };
     if constexpr (G == 32) {
 #pragma unroll 1
         for (int kc = kc0; kc < kc1; kc++) {
-            const int n = min(4, p.Kg - 4 * kc);
-            uint2 x[SETS][4 / SHARE];  // this lane's codes: of its own K groups b_group, b_group + SHARE, ...
+            const int n = p.Kg - 4 * kc;  // blocks that are there; of others the codes and scales are zeros
+            uint4 x[SETS][2];             // this lane's codes of the four blocks
 #pragma unroll
-            for (int s = 0; s < SETS; s++)
-#pragma unroll
-                for (int i = 0; i < 4 / SHARE; i++) {
-                    const int j = i * SHARE + b_group;
-                    x[s][i] = make_uint2(0u, 0u);
-                    if (live[s] && j < n) x[s][i] = __ldca(reinterpret_cast<const uint2*>(codes[s] + (kc * 4 + j) * 32));
-                }
+            for (int s = 0; s < SETS; s++) {
+                x[s][0] = __ldca(reinterpret_cast<const uint4*>(codes[s])), x[s][1] = __ldca(reinterpret_cast<const uint4*>(codes[s]) + 1);
+                codes[s] += 128;
+            }
             const uint8_t* slot = ring.wait(fail);
+            const uint8_t* words = slot + t * 128 + g * 16;
 #pragma unroll
             for (int i = 0; i < 4 / SHARE; i++) {
-                begin();
                 const int mine = i * SHARE + d_group;
-                if (mine < n) {
-                    scales_of(4 * kc + mine);
-                    const uint8_t* tail = slot + mine * BS + 16 * G + g * 8;
-                    wd = *reinterpret_cast<const uint2*>(tail);
-                    if (QTYPE == 1) wm = *reinterpret_cast<const uint2*>(tail + 64);
-                }
+                scales_of(mine);
+                const uint8_t* tail = slot + mine * BS + 16 * G + g * 8;
+                wd = mine < n ? *reinterpret_cast<const uint2*>(tail) : make_uint2(0u, 0u);
+                if (QTYPE == 1) wm = mine < n ? *reinterpret_cast<const uint2*>(tail + 64) : make_uint2(0u, 0u);
+                int I[SETS][2][4];
 #pragma unroll
                 for (int h = 0; h < SHARE; h++) {
                     const int j = i * SHARE + h;
-                    if (j >= n) break;
-                    const uint4 q = load_words(slot + j * BS + t * 128 + g * 16, t);
+                    const uint4 q = load_words(words + j * BS, t);
                     uint32_t l[4] = {q.x & kNibMask, q.y & kNibMask, q.z & kNibMask, q.w & kNibMask};
                     uint32_t u[4] = {(q.x >> 4) & kNibMask, (q.y >> 4) & kNibMask, (q.z >> 4) & kNibMask, (q.w >> 4) & kNibMask};
                     if (SIGNED)
@@ -212,33 +231,40 @@ __device__ __forceinline__ void walk(const FewParams& p, WarpRing<G, QTYPE>& rin
                         for (int k = 0; k < 4; k++) l[k] ^= 0x08080808u, u[k] ^= 0x08080808u;
 #pragma unroll
                     for (int s = 0; s < SETS; s++) {
-                        const uint2 b = SHARE == 1 || b_group == h ? x[s][i] : make_uint2(0u, 0u);
-                        mma(I[s], 0, l[0], l[1], u[0], u[1], b.x, b.y);
-                        mma(I[s], 4, l[2], l[3], u[2], u[3], b.x, b.y);
+                        uint32_t b0 = j % 2 ? x[s][j / 2].z : x[s][j / 2].x, b1 = j % 2 ? x[s][j / 2].w : x[s][j / 2].y;
+                        if (SHARE > 1 && b_group != h) b0 = b1 = 0;
+                        if (h == 0) {
+                            mma<true>(I[s][0], l[0], l[1], u[0], u[1], b0, b1), mma<true>(I[s][1], l[2], l[3], u[2], u[3], b0, b1);
+                        } else {
+                            mma<false>(I[s][0], l[0], l[1], u[0], u[1], b0, b1), mma<false>(I[s][1], l[2], l[3], u[2], u[3], b0, b1);
+                        }
                     }
                 }
-                finish();
+                finish(I, I);
             }
+            sc += 4 * 32;
             ring.next(lane);
         }
     } else {
         // one block a chunk: the groups that share columns are successive chunks
 #pragma unroll 1
-        for (int kc = kc0; kc < kc1;) {
-            begin();
+        for (int kc = kc0; kc < kc1; kc += SHARE) {
+            int low[SETS][2][4], up[SETS][2][4];
+            if (SHARE > 1)
+#pragma unroll
+                for (int s = 0; s < SETS; s++) x4[s] = make_ulonglong2(0, 0);
 #pragma unroll
             for (int h = 0; h < SHARE; h++) {
-                if (kc >= kc1) break;
-                uint2 x[SETS][4];
-#pragma unroll
-                for (int s = 0; s < SETS; s++)
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        x[s][i] = make_uint2(0u, 0u);
-                        if (live[s] && (SHARE == 1 || b_group == h)) x[s][i] = __ldca(reinterpret_cast<const uint2*>(codes[s] + kc * 128 + 32 * i));
-                    }
+                if (h > 0 && kc + h >= kc1) break;
                 const bool mine = SHARE == 1 || d_group == h;
-                if (mine) scales_of(kc);
+                if (mine) scales_of(h);
+                uint4 x[SETS][2];
+#pragma unroll
+                for (int s = 0; s < SETS; s++) {
+                    x[s][0] = x[s][1] = make_uint4(0u, 0u, 0u, 0u);
+                    if (SHARE == 1 || b_group == h)
+                        x[s][0] = __ldca(reinterpret_cast<const uint4*>(codes[s] + 128 * h)), x[s][1] = __ldca(reinterpret_cast<const uint4*>(codes[s] + 128 * h) + 1);
+                }
                 const uint8_t* slot = ring.wait(fail);
                 if (mine) {
                     const uint8_t* tail = slot + 16 * G + g * 8;
@@ -258,17 +284,22 @@ __device__ __forceinline__ void walk(const FewParams& p, WarpRing<G, QTYPE>& rin
                     }
 #pragma unroll
                     for (int s = 0; s < SETS; s++) {
-                        const uint2 xa = x[s][2 * pr], xb = x[s][2 * pr + 1];
-                        mma(I[s], 0, la[0], la[1], lb[0], lb[1], xa.x, xb.x);
-                        mma(I[s], 4, la[2], la[3], lb[2], lb[3], xa.x, xb.x);
-                        mma(I[s], 8, ua[0], ua[1], ub[0], ub[1], xa.y, xb.y);
-                        mma(I[s], 12, ua[2], ua[3], ub[2], ub[3], xa.y, xb.y);
+                        const uint4 o = x[s][pr];
+                        auto all = [&](auto first) {
+                            constexpr bool F = decltype(first)::value;
+                            mma<F>(low[s][0], la[0], la[1], lb[0], lb[1], o.x, o.z), mma<F>(low[s][1], la[2], la[3], lb[2], lb[3], o.x, o.z);
+                            mma<F>(up[s][0], ua[0], ua[1], ub[0], ub[1], o.y, o.w), mma<F>(up[s][1], ua[2], ua[3], ub[2], ub[3], o.y, o.w);
+                        };
+                        if (h == 0 && pr == 0) all(std::true_type{});
+                        else all(std::false_type{});
                     }
                 }
                 ring.next(lane);
-                kc++;
             }
-            finish();
+#pragma unroll
+            for (int s = 0; s < SETS; s++) codes[s] += 128 * SHARE;
+            sc += 32 * SHARE;
+            finish(low, up);
         }
     }
 }
@@ -277,11 +308,12 @@ template <int G, int QTYPE, bool SIGNED>
 __global__ void __launch_bounds__(kThreads, 1) experts_few_kernel(const __grid_constant__ FewParams p) {
     using S = FewShape<G, QTYPE>;
     extern __shared__ __align__(128) uint8_t smem[];
-    // barriers [warp][kMaxDepth] | failure flag | tiles | partial sums [warp][2][rows][32] | rings [warp][depth]
+    // barriers [warp][kMaxDepth] | failure flag, weights | tiles | partial sums [warp][2][rows][32] | rings [warp][depth]
     constexpr int kFail = kWarps * kMaxDepth * 8;
     int4* const tiles = reinterpret_cast<int4*>(smem + kFail + 16);
     float* const part = reinterpret_cast<float*>(smem + p.part_off);
     volatile int* fail = reinterpret_cast<volatile int*>(smem + kFail);
+    int* const total = reinterpret_cast<int*>(smem + kFail + 4);  // the weights of all tiles
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const uint32_t bars = smem_u32(smem) + warp * kMaxDepth * 8;
     if (lane < p.depth) mbar_init(bars + 8 * lane, 1);
@@ -294,9 +326,45 @@ __global__ void __launch_bounds__(kThreads, 1) experts_few_kernel(const __grid_c
         tile.z = min(tile.z, kPartRows);
         tiles[i] = tile;
     }
-    const int64_t stripes = (int64_t)__ldcg(p.tile_count) * p.Ng;
-    const int s0 = (int)(stripes * blockIdx.x / gridDim.x), r = (int)(stripes * (blockIdx.x + 1) / gridDim.x) - s0;
+    const int count = __ldcg(p.tile_count);
     __syncthreads();
+    // The CTA's stripes: shares of the tiles' weights, each in front of its tile.
+    for (int i = threadIdx.x; i < count; i += kThreads) {
+        // (what a stripe costs the SM: its bytes, or with group 32 its arithmetic where there are more than four rows)
+        const int rows = tiles[i].z;
+        tiles[i].w = G == 128 || rows <= 4 ? 4 : rows <= 8 ? 5 : 7;
+    }
+    __syncthreads();
+    if (warp == 0) {
+        int sum = 0;
+        for (int i0 = 0; i0 < count; i0 += 32) {
+            const int w = i0 + lane < count ? tiles[i0 + lane].w : 0;
+            int v = w;
+#pragma unroll
+            for (int off = 1; off < 32; off <<= 1) {
+                const int o = __shfl_up_sync(0xffffffffu, v, off);
+                if (lane >= off) v += o;
+            }
+            if (i0 + lane < count) tiles[i0 + lane].w = sum + v - w;
+            sum += __shfl_sync(0xffffffffu, v, 31);
+        }
+        if (lane == 0) *total = sum;
+    }
+    __syncthreads();
+    auto stripe_at = [&](int part) {  // the first stripe of a CTA
+        const int all = *total;
+        if (part >= (int)gridDim.x || count == 0) return count * p.Ng;
+        const int64_t target = (int64_t)all * p.Ng * part / gridDim.x;
+        int lo = 0, hi = count;  // the last tile whose weights begin at or in front of it
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) / 2;
+            if ((int64_t)tiles[mid].w * p.Ng <= target) lo = mid; else hi = mid;
+        }
+        const int w = (lo + 1 < count ? tiles[lo + 1].w : all) - tiles[lo].w;
+        const int64_t in = (target - (int64_t)tiles[lo].w * p.Ng + w - 1) / w;
+        return lo * p.Ng + (int)min((int64_t)p.Ng, in);
+    };
+    const int s0 = stripe_at(blockIdx.x), r = stripe_at(blockIdx.x + 1) - s0;
     const int C = p.chunks;
     auto share = [&](int w) { return (int)((int64_t)r * C * w / kWarps); };  // first chunk of a warp
     const int begin = share(warp), end = share(warp + 1);
@@ -340,35 +408,32 @@ __global__ void __launch_bounds__(kThreads, 1) experts_few_kernel(const __grid_c
             if (whole) store(n, tile.y + row, v);
             else *reinterpret_cast<float4*>(part + ((warp * 2 + slot) * kPartRows + row) * 32 + 4 * g) = v;
         };
+        // rows row, row + 1 of this lane's four columns
+        auto put_two = [&](int row, const uint64_t (&acc)[4]) {
+            const float2 v[4] = {unpair(acc[0]), unpair(acc[1]), unpair(acc[2]), unpair(acc[3])};
+            put(row, make_float4(v[0].x, v[1].x, v[2].x, v[3].x));
+            put(row + 1, make_float4(v[0].y, v[1].y, v[2].y, v[3].y));
+        };
+        uint64_t acc[2][4];
+        uint64_t(&one)[1][4] = reinterpret_cast<uint64_t(&)[1][4]>(acc);
         if (tile.z <= 4) {
-            float acc[1][4][2];
-            if (tile.z <= 2) walk<G, QTYPE, SIGNED, 4, 1>(p, ring, fail, lane, tile, ti, kc0, kc1, acc);
-            else walk<G, QTYPE, SIGNED, 2, 1>(p, ring, fail, lane, tile, ti, kc0, kc1, acc);
             const bool two = tile.z <= 2;
+            if (two) walk<G, QTYPE, SIGNED, 4, 1>(p, ring, fail, lane, tile, ti, kc0, kc1, one);
+            else walk<G, QTYPE, SIGNED, 2, 1>(p, ring, fail, lane, tile, ti, kc0, kc1, one);
 #pragma unroll
-            for (int k = 0; k < 4; k++)
-#pragma unroll
-                for (int mi = 0; mi < 2; mi++) {  // the K groups of the other lanes
-                    float& v = acc[0][k][mi];
-                    v += __shfl_xor_sync(0xffffffffu, v, 2);
-                    const float o = __shfl_xor_sync(0xffffffffu, v, 1);
-                    if (two) v += o;
-                }
-            if (t < (two ? 1 : 2))
-#pragma unroll
-                for (int mi = 0; mi < 2; mi++) put(2 * t + mi, make_float4(acc[0][0][mi], acc[0][1][mi], acc[0][2][mi], acc[0][3][mi]));
+            for (int k = 0; k < 4; k++) {  // the K groups of the other lanes
+                acc[0][k] = add2(acc[0][k], __shfl_xor_sync(0xffffffffu, acc[0][k], 2));
+                const uint64_t o = __shfl_xor_sync(0xffffffffu, acc[0][k], 1);
+                if (two) acc[0][k] = add2(acc[0][k], o);
+            }
+            if (t < (two ? 1 : 2)) put_two(2 * t, acc[0]);
         } else if (tile.z <= 8) {
-            float acc[1][4][2];
-            walk<G, QTYPE, SIGNED, 1, 1>(p, ring, fail, lane, tile, ti, kc0, kc1, acc);
-#pragma unroll
-            for (int mi = 0; mi < 2; mi++) put(2 * t + mi, make_float4(acc[0][0][mi], acc[0][1][mi], acc[0][2][mi], acc[0][3][mi]));
+            walk<G, QTYPE, SIGNED, 1, 1>(p, ring, fail, lane, tile, ti, kc0, kc1, one);
+            put_two(2 * t, acc[0]);
         } else {
-            float acc[2][4][2];
             walk<G, QTYPE, SIGNED, 1, 2>(p, ring, fail, lane, tile, ti, kc0, kc1, acc);
-#pragma unroll
-            for (int s = 0; s < 2; s++)
-#pragma unroll
-                for (int mi = 0; mi < 2; mi++) put(8 * s + 2 * t + mi, make_float4(acc[s][0][mi], acc[s][1][mi], acc[s][2][mi], acc[s][3][mi]));
+            put_two(2 * t, acc[0]);
+            put_two(8 + 2 * t, acc[1]);
         }
     }
     __syncthreads();
@@ -420,14 +485,15 @@ int launch_few(FewParams p, const DeviceInfo* di, cudaStream_t s) {
 bool experts_few_serves(int64_t rows, int64_t n) { return rows <= 32 * n && most_tiles(kTiles16, rows, n) <= kMostTiles; }
 
 size_t experts_few_scratch(int64_t rows, int64_t Kg, int G, int64_t n) {
-    return align_up((size_t)(rows * Kg * G), 256) + align_up((size_t)(most_tiles(kTiles16, rows, n) * Kg) * 128, 256);
+    const int64_t chunks = (Kg * G + 127) / 128;
+    return align_up((size_t)(rows * chunks) * 128, 256) + align_up((size_t)(most_tiles(kTiles16, rows, n) * chunks * (128 / G)) * 128, 256);
 }
 
 int launch_experts_few(const ExpertsCall& c, GroupQuant q, cudaStream_t s) {
     const DeviceInfo* di = device_info();
     if (!di) return Q4FC_ECUDA;
     const int64_t chunks = (c.Kg * c.G + 127) / 128, tiles = most_tiles(kTiles16, c.rows, c.n);
-    if (chunks * c.Ng > 0x7fffffffLL / tiles) {
+    if (chunks * c.Ng > 0x7fffffffLL / 8 / tiles) {
         set_error("fc_experts: %lld rows, K=%lld, N=%lld exceed the limit of a launch", (long long)c.rows, (long long)c.K, (long long)c.N);
         return Q4FC_ELIMIT;
     }
@@ -435,12 +501,12 @@ int launch_experts_few(const ExpertsCall& c, GroupQuant q, cudaStream_t s) {
     FewParams p = {};
     p.status = ring_status_word();
     if (!p.status) return Q4FC_ECUDA;
-    q.codes = reinterpret_cast<int8_t*>(c.scratch), q.sc = reinterpret_cast<float*>(c.scratch + align_up((size_t)(c.rows * c.Kg * c.G), 256));
+    q.codes = reinterpret_cast<int8_t*>(c.scratch), q.sc = reinterpret_cast<float*>(c.scratch + align_up((size_t)(c.rows * chunks) * 128, 256));
     q.tile0 = c.plan.tile0[kTiles16], q.log2tile = 4, q.sums = 1, q.isum = sgn;
     if (int rc = launch_quant_x_group(q, c.G, false, s)) return rc;
     p.codes = q.codes, p.sc = q.sc, p.wq = c.wq, p.y = c.y, p.N = c.N, p.ldy = c.ldy;
     p.tiles = c.plan.tiles[kTiles16], p.tile_count = c.plan.counts + kTiles16, p.order = c.plan.order;
-    p.row_bytes = c.Kg * c.G, p.group_bytes = c.Ng * c.Kg * block_bytes(c.qtype, c.G);
+    p.row_bytes = chunks * 128, p.group_bytes = c.Ng * c.Kg * block_bytes(c.qtype, c.G);
     p.Ng = (int)c.Ng, p.Kg = (int)c.Kg, p.chunks = (int)chunks, p.most_tiles = (int)tiles;
     p.y_vec = c.ldy % 4 == 0 && (reinterpret_cast<uintptr_t>(c.y) & 15) == 0;
     if (c.qtype == 1) return c.G == 32 ? launch_few<32, 1, false>(p, di, s) : launch_few<128, 1, false>(p, di, s);

@@ -112,15 +112,14 @@ __global__ void __launch_bounds__(kQxWarps * 32) quant_x_kernel(const float* __r
 }
 
 // 128 k of a row, by one warp, in a form that the FC kernels read: lane l holds v[0..3] = x[k .. k + 3], 0 beyond K, of
-// k = 128 c + 4 l.  Codes and scales as in quant_x_kernel, group sums tree-ordered.  `codes`: the row's; `sc`: the row's
+// k = 128 c + 4 l.  Codes and scales as in quant_x_kernel, group sums tree-ordered.  `codes`: the lane's place; `sc`: the row's
 // place in the first K group, `per` floats from there to its place in the next, the sum `sum_at` behind the scale.
-// isum: instead of the sum, the bits of the integer 8 * sum of codes.
+// isum: instead of the sum, the bits of the integer 8 * sum of codes.  pad: the 128 k are written whole, zeros beyond the last group.
 template <int G, bool F16>
-__device__ __forceinline__ void quantize_unit(const float (&v)[4], int64_t c, int lane, int64_t K, int64_t Kg, bool sums, bool isum,
+__device__ __forceinline__ void quantize_unit(const float (&v)[4], int64_t c, int lane, int64_t K, int64_t Kg, bool sums, bool isum, bool pad,
                                               int8_t* __restrict__ codes, float* __restrict__ sc, int64_t per, int64_t sum_at) {
     constexpr int SEG = G / 4;    // lanes per group
     constexpr int GPC = 128 / G;  // groups per 128-k chunk
-    const int64_t k = c * 128 + lane * 4;
     const int64_t kb = c * GPC + lane / SEG;
     const bool exists = kb < Kg;
     const int len = exists ? (int)min((int64_t)G, K - kb * G) : 0;
@@ -159,11 +158,11 @@ __device__ __forceinline__ void quantize_unit(const float (&v)[4], int64_t c, in
         const uint32_t other = __shfl_xor_sync(0xffffffffu, (lane & 1) ? even : odd, 1);
         w[0] = (lane & 1) ? other : even, w[1] = (lane & 1) ? odd : other;
     }
-    if (exists) {
+    if (exists || pad) {
         if constexpr (F16)
-            *reinterpret_cast<uint2*>(codes + k * 2) = make_uint2(w[0], w[1]);
+            *reinterpret_cast<uint2*>(codes) = make_uint2(w[0], w[1]);
         else
-            *reinterpret_cast<uint32_t*>(codes + k) =
+            *reinterpret_cast<uint32_t*>(codes) =
                 (q[0] & 0xFF) | (q[1] & 0xFF) << 8 | (q[2] & 0xFF) << 16 | (uint32_t)(q[3] & 0xFF) << 24;
         if (e0 == 0) {
             float* dst = sc + kb * per;
@@ -200,12 +199,12 @@ __global__ void __launch_bounds__(kQxWarps * 32) quant_x_tile_kernel(const float
             if (k + j < K) v[j] = ld_after_wait(src + j);
     }
     const int64_t tile = (int64_t)1 << log2tile, per = tile << sums;
-    quantize_unit<G, F16>(v, c, lane, K, Kg, sums, false, codes + row * (Kg * G) * (F16 ? 2 : 1),
+    quantize_unit<G, F16>(v, c, lane, K, Kg, sums, false, false, codes + (row * (Kg * G) + k) * (F16 ? 2 : 1),
                           sc + (row >> log2tile) * Kg * per + (row & (tile - 1)), per, tile);
 }
 
 // The quantizer of the experts' product: rows in the order of a plan (groups.cuh), codes in that order, scales by the
-// plan's tiles: for experts with few rows (tiles of 16) [tile][Kg][row][scale, sum], else as quant_x_tile_kernel has them.
+// plan's tiles: for experts with few rows (tiles of 16) [tile][K group][two rows][scales, sums], else as quant_x_tile_kernel has them.
 // A row of x serves `per_row` (token, slot) pairs, or one; `gated`: the value is silu(x[k]) * x[K + k].  An output row
 // without an expert is zeroed here.
 template <int G, bool F16>
@@ -247,12 +246,15 @@ __global__ void __launch_bounds__(kQxWarps * 32) quant_x_group_kernel(const __gr
         for (int j = 0; j < 4; j++) v[j] = __fmul_rn(up[j], __fdiv_rn(v[j], __fadd_rn(1.0f, expf(-v[j]))));
     }
     const int at = (int)place - first, tile = tile0 + (at >> a.log2tile), row = at & ((1 << a.log2tile) - 1);
-    int8_t* codes = a.codes + place * (a.Kg * G) * (F16 ? 2 : 1);
-    if (a.log2tile == 4)
-        quantize_unit<G, F16>(v, c, lane, a.K, a.Kg, true, a.isum, codes, a.sc + (int64_t)tile * a.Kg * 32 + 2 * row, 32, 1);
-    else {
+    if (a.log2tile == 4) {
+        const int64_t chunks = (a.Kg * G + 127) / 128, groups = chunks * (128 / G);
+        // (what a lane of the FC kernel takes of 128 k -- eight of each 32 -- lies together; scales and sums of two rows do)
+        int8_t* codes = a.codes + (place * chunks + c) * 128 + (lane / 2 % 4) * 32 + (lane / 8) * 8 + (lane % 2) * 4;
+        quantize_unit<G, F16>(v, c, lane, a.K, a.Kg, true, a.isum, true, codes, a.sc + (int64_t)tile * groups * 32 + row / 2 * 4 + row % 2, 32, 2);
+    } else {
         const int64_t size = (int64_t)1 << a.log2tile, per = size << a.sums;
-        quantize_unit<G, F16>(v, c, lane, a.K, a.Kg, a.sums, false, codes, a.sc + (int64_t)tile * a.Kg * per + row, per, size);
+        quantize_unit<G, F16>(v, c, lane, a.K, a.Kg, a.sums, false, false, a.codes + (place * (a.Kg * G) + k) * (F16 ? 2 : 1),
+                              a.sc + (int64_t)tile * a.Kg * per + row, per, size);
     }
 }
 
