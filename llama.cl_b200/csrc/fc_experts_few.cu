@@ -41,9 +41,19 @@ struct FewParams {
     const int *tile_count, *order;
     int64_t row_bytes, N, ldy, group_bytes;
     int Ng, Kg, chunks;  // chunks of a stripe
-    int most_tiles, depth, y_vec, part_off, ring_off;
+    int most_tiles, depth, last_bytes, y_vec, weigh, part_off, ring_off;
     int* status;
 };
+
+__device__ __forceinline__ bool elect_lane() {  // one lane of a converged warp
+    uint32_t p;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "elect.sync _|p, 0xffffffff;\n\t"
+        "selp.b32 %0, 1, 0, p;\n\t}"
+        : "=r"(p));
+    return p != 0;
+}
 
 template <int G, int QTYPE>
 struct FewShape {
@@ -52,52 +62,53 @@ struct FewShape {
     static constexpr int kSlot = kBlocks * BS;
 };
 
-// A warp's ring: what comes next into it, and what is read next.
+__device__ __noinline__ void wait_longer(uint32_t bar, uint32_t parity, volatile int* fail, int* status) {
+    mbar_wait(bar, parity, fail, status, 0x4658504C);  // 'FXPL'
+}
+
+// A warp's ring.  A slot that has been read takes what comes next: of its stripes the weights follow one another in memory, up to the
+// end of an expert's.
 template <int G, int QTYPE>
 struct WarpRing {
     using S = FewShape<G, QTYPE>;
-    const FewParams& p;
-    const int4* tiles;
-    uint8_t* slots;
-    uint32_t bars;
-    int s0;                 // first stripe of the CTA
+    const uint8_t* slot;    // read next
+    uint32_t at, bar;       // its address and barrier
+    uint32_t parity;
+    int n;                  // its number
     int left;               // chunks that are not asked for yet
-    int stripe, kc;         // the next of them
-    const uint8_t* from;
-    int fill = 0, read = 0; // slots
-    uint32_t parity = 0;    // of the slot that is read next
+    int in_stripe, in_tile; // chunks to the end of the stripe and of the expert's weights, from the next one that is asked for on
+    int tile;
+    const uint8_t* from;    // where it is
 
-    __device__ __forceinline__ void seek() {
-        const int sg = s0 + stripe, tile = sg / p.Ng;
-        from = p.wq + tiles[tile].x * p.group_bytes + ((int64_t)(sg - tile * p.Ng) * p.Kg + kc * S::kBlocks) * S::BS;
-    }
-    // one lane
-    __device__ __forceinline__ void ask() {
-        const uint32_t bytes = (uint32_t)min(S::kBlocks, p.Kg - kc * S::kBlocks) * S::BS, bar = bars + 8 * fill;
-        mbar_expect_tx(bar, bytes);
-        bulk_g2s(smem_u32(slots + fill * S::kSlot), from, bytes, bar);
-    }
-    __device__ __forceinline__ void asked() {
-        left--;
-        if (++fill == p.depth) fill = 0;
-        from += S::kSlot;
-        if (++kc == p.chunks) {
-            kc = 0, stripe++;
-            if (left > 0) seek();
+    // the next chunk into a slot
+    __device__ __forceinline__ void ask(const FewParams& p, const int4* tiles) {
+        uint32_t bytes = S::kSlot;
+        if (--in_stripe == 0) in_stripe = p.chunks, bytes = p.last_bytes;
+        if (elect_lane()) {
+            mbar_expect_tx(bar, bytes);
+            bulk_g2s(at, from, bytes, bar);
+        }
+        from += bytes, left--;
+        if (--in_tile == 0 && left > 0) {
+            in_tile = p.chunks * p.Ng, tile++;
+            from = p.wq + tiles[tile].x * p.group_bytes;
         }
     }
-    __device__ __forceinline__ const uint8_t* wait(volatile int* fail) {
-        mbar_wait(bars + 8 * read, parity, fail, p.status, 0x4658504Cu);  // 'FXPL'
-        return slots + read * S::kSlot;
+    __device__ __forceinline__ void step(const FewParams& p) {
+        slot += S::kSlot, at += S::kSlot, bar += 8;
+        if (++n == p.depth) {
+            n = 0, parity ^= 1;
+            slot -= p.depth * S::kSlot, at -= p.depth * S::kSlot, bar -= 8 * p.depth;
+        }
+    }
+    __device__ __forceinline__ void wait(const FewParams& p, volatile int* fail) {
+        if (__builtin_expect(!mbar_try_wait(bar, parity), 0)) wait_longer(bar, parity, fail, p.status);
     }
     // the slot has been read by all lanes
-    __device__ __forceinline__ void next(int lane) {
+    __device__ __forceinline__ void next(const FewParams& p, const int4* tiles) {
         __syncwarp();
-        if (left > 0) {
-            if (lane == 0) ask();
-            asked();
-        }
-        if (++read == p.depth) read = 0, parity ^= 1;
+        if (left > 0) ask(p, tiles);
+        step(p);
     }
 };
 
@@ -113,15 +124,11 @@ __device__ __forceinline__ uint4 load_words(const uint8_t* row, int t) {
 // Integers without conversion: an MMA that starts from the bits of 1.5 x 2^23 leaves those of 1.5 x 2^23 + I (|I| < 2^22).
 constexpr int kIntBits = 0x4B400000;
 constexpr float kInt = 12582912.0f;
-// D(16x8, s32) = A(16x32, u8) * B(32x8, s8) + these bits, or + D
-template <bool FIRST>
-__device__ __forceinline__ void mma(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    if constexpr (FIRST)
-        asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
-            : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
-            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(kIntBits));
-    else
-        mma_u8s8(d, a0, a1, a2, a3, b0, b1);
+// D(16x8, s32) = A(16x32, u8) * B(32x8, s8) + C
+__device__ __forceinline__ void mma_from(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1, const int (&c)[4]) {
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+        : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(c[0]), "r"(c[1]), "r"(c[2]), "r"(c[3]));
 }
 __device__ __forceinline__ uint64_t pair(float lo, float hi) {
     uint64_t r;
@@ -154,8 +161,8 @@ __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
 // acc[s][c]: column 4g + c of two rows of set s; lane t: SHARE 4: rows 0, 1, K groups t mod 4; 2: rows 2 (t % 2) and one more, K
 // groups t / 2 mod 2; 1: rows 2t, 2t + 1.  What columns of rows beyond the tile's hold is not used.
 template <int G, int QTYPE, bool SIGNED, int SHARE, int SETS>
-__device__ __forceinline__ void walk(const FewParams& p, WarpRing<G, QTYPE>& ring, volatile int* fail, int lane, int4 tile, int tile_index, int kc0,
-                                     int kc1, uint64_t (&acc)[SETS][4]) {
+__device__ __forceinline__ void walk(const FewParams& p, const int4* tiles, WarpRing<G, QTYPE>& ring, volatile int* fail, int lane, int4 tile,
+                                     int tile_index, int kc0, int kc1, uint64_t (&acc)[SETS][4]) {
     using S = FewShape<G, QTYPE>;
     constexpr int BS = S::BS, kRows = 8 / SHARE;  // rows of a set
     const int g = lane >> 2, t = lane & 3;
@@ -169,11 +176,13 @@ __device__ __forceinline__ void walk(const FewParams& p, WarpRing<G, QTYPE>& rin
     for (int s = 0; s < SETS; s++)
 #pragma unroll
         for (int c = 0; c < 4; c++) acc[s][c] = 0;
+    int start[4];  // (kept: four registers that the first MMA of a round starts from)
+#pragma unroll
+    for (int i = 0; i < 4; i++) asm volatile("mov.b32 %0, %1;" : "=r"(start[i]) : "n"(kIntBits));
     const uint64_t minus = pair(-kInt, -kInt);
-    uint2 wd = make_uint2(0u, 0u), wm = make_uint2(0u, 0u);
-    ulonglong2 x4[SETS];     // scales of the lane's two rows, their sums
-    // scaling of what the columns have gathered; low, up: [columns 4g, 4g + 1 | 4g + 2, 4g + 3][row of the MMA's half][rows]
-    auto finish = [&](const int (&low)[SETS][2][4], const int (&up)[SETS][2][4]) {
+    // scaling of what the columns have gathered; low, up: [columns 4g, 4g + 1 | 4g + 2, 4g + 3][row of the MMA's half][rows]; x4: scales of
+    // the lane's two rows, their sums
+    auto finish = [&](const int (&low)[SETS][2][4], const int (&up)[SETS][2][4], uint2 wd, uint2 wm, const ulonglong2 (&x4)[SETS]) {
         const float2 wd01 = __half22float2(*reinterpret_cast<const __half2*>(&wd.x)), wd23 = __half22float2(*reinterpret_cast<const __half2*>(&wd.y));
         const float2 wm01 = __half22float2(*reinterpret_cast<const __half2*>(&wm.x)), wm23 = __half22float2(*reinterpret_cast<const __half2*>(&wm.y));
         const float wdf[4] = {wd01.x, wd01.y, wd23.x, wd23.y}, wmf[4] = {wm01.x, wm01.y, wm23.x, wm23.y};
@@ -196,29 +205,34 @@ __device__ __forceinline__ void walk(const FewParams& p, WarpRing<G, QTYPE>& rin
             }
         }
     };
-    auto scales_of = [&](int kb) {  // K group kb behind kc0
+    auto scales_of = [&](int kb, ulonglong2 (&x4)[SETS]) {  // K group kb behind kc0
 #pragma unroll
         for (int s = 0; s < SETS; s++) x4[s] = __ldca(reinterpret_cast<const ulonglong2*>(sc + kb * 32 + 16 * s));
+    };
+    auto codes_of = [&](int chunk, uint4 (&x)[SETS][2]) {  // this lane's of a chunk's four times 32 k
+#pragma unroll
+        for (int s = 0; s < SETS; s++) {
+            const uint4* from = reinterpret_cast<const uint4*>(codes[s] + 128 * chunk);
+            x[s][0] = __ldca(from), x[s][1] = __ldca(from + 1);
+        }
     };
     if constexpr (G == 32) {
 #pragma unroll 1
         for (int kc = kc0; kc < kc1; kc++) {
             const int n = p.Kg - 4 * kc;  // blocks that are there; of others the codes and scales are zeros
-            uint4 x[SETS][2];             // this lane's codes of the four blocks
-#pragma unroll
-            for (int s = 0; s < SETS; s++) {
-                x[s][0] = __ldca(reinterpret_cast<const uint4*>(codes[s])), x[s][1] = __ldca(reinterpret_cast<const uint4*>(codes[s]) + 1);
-                codes[s] += 128;
-            }
-            const uint8_t* slot = ring.wait(fail);
-            const uint8_t* words = slot + t * 128 + g * 16;
+            uint4 x[SETS][2];
+            codes_of(0, x);
+            ring.wait(p, fail);
+            const uint8_t* words = ring.slot + t * 128 + g * 16;
 #pragma unroll
             for (int i = 0; i < 4 / SHARE; i++) {
                 const int mine = i * SHARE + d_group;
-                scales_of(mine);
-                const uint8_t* tail = slot + mine * BS + 16 * G + g * 8;
-                wd = mine < n ? *reinterpret_cast<const uint2*>(tail) : make_uint2(0u, 0u);
-                if (QTYPE == 1) wm = mine < n ? *reinterpret_cast<const uint2*>(tail + 64) : make_uint2(0u, 0u);
+                ulonglong2 x4[SETS];
+                scales_of(mine, x4);
+                const uint8_t* tail = ring.slot + mine * BS + 16 * G + g * 8;
+                uint2 wd = *reinterpret_cast<const uint2*>(tail), wm = make_uint2(0u, 0u);
+                if (QTYPE == 1) wm = *reinterpret_cast<const uint2*>(tail + 64);
+                if (mine >= n) wd = wm = make_uint2(0u, 0u);  // (not what an earlier chunk has left there)
                 int I[SETS][2][4];
 #pragma unroll
                 for (int h = 0; h < SHARE; h++) {
@@ -234,46 +248,52 @@ __device__ __forceinline__ void walk(const FewParams& p, WarpRing<G, QTYPE>& rin
                         uint32_t b0 = j % 2 ? x[s][j / 2].z : x[s][j / 2].x, b1 = j % 2 ? x[s][j / 2].w : x[s][j / 2].y;
                         if (SHARE > 1 && b_group != h) b0 = b1 = 0;
                         if (h == 0) {
-                            mma<true>(I[s][0], l[0], l[1], u[0], u[1], b0, b1), mma<true>(I[s][1], l[2], l[3], u[2], u[3], b0, b1);
+                            mma_from(I[s][0], l[0], l[1], u[0], u[1], b0, b1, start), mma_from(I[s][1], l[2], l[3], u[2], u[3], b0, b1, start);
                         } else {
-                            mma<false>(I[s][0], l[0], l[1], u[0], u[1], b0, b1), mma<false>(I[s][1], l[2], l[3], u[2], u[3], b0, b1);
+                            mma_u8s8(I[s][0], l[0], l[1], u[0], u[1], b0, b1), mma_u8s8(I[s][1], l[2], l[3], u[2], u[3], b0, b1);
                         }
                     }
                 }
-                finish(I, I);
+                finish(I, I, wd, wm, x4);
             }
             sc += 4 * 32;
-            ring.next(lane);
+#pragma unroll
+            for (int s = 0; s < SETS; s++) codes[s] += 128;
+            ring.next(p, tiles);
         }
     } else {
-        // one block a chunk: the groups that share columns are successive chunks
-#pragma unroll 1
-        for (int kc = kc0; kc < kc1; kc += SHARE) {
+        // One block a chunk: the groups that share columns are successive chunks, `n` of them (all SHARE in the loop below).
+        auto round = [&](auto whole, int n) {
+            uint4 x[SETS][2];
+            ulonglong2 x4[SETS];
+            uint2 wd = make_uint2(0u, 0u), wm = make_uint2(0u, 0u);
             int low[SETS][2][4], up[SETS][2][4];
-            if (SHARE > 1)
+            constexpr bool kWhole = decltype(whole)::value;
+            if (kWhole || b_group < n) {
+                codes_of(b_group, x);
+            } else {
+#pragma unroll
+                for (int s = 0; s < SETS; s++) x[s][0] = x[s][1] = make_uint4(0u, 0u, 0u, 0u);
+            }
+            if (kWhole || d_group < n) {
+                scales_of(d_group, x4);
+            } else {
 #pragma unroll
                 for (int s = 0; s < SETS; s++) x4[s] = make_ulonglong2(0, 0);
+            }
 #pragma unroll
             for (int h = 0; h < SHARE; h++) {
-                if (h > 0 && kc + h >= kc1) break;
-                const bool mine = SHARE == 1 || d_group == h;
-                if (mine) scales_of(h);
-                uint4 x[SETS][2];
-#pragma unroll
-                for (int s = 0; s < SETS; s++) {
-                    x[s][0] = x[s][1] = make_uint4(0u, 0u, 0u, 0u);
-                    if (SHARE == 1 || b_group == h)
-                        x[s][0] = __ldca(reinterpret_cast<const uint4*>(codes[s] + 128 * h)), x[s][1] = __ldca(reinterpret_cast<const uint4*>(codes[s] + 128 * h) + 1);
-                }
-                const uint8_t* slot = ring.wait(fail);
-                if (mine) {
-                    const uint8_t* tail = slot + 16 * G + g * 8;
+                if (!kWhole && h >= n) break;
+                ring.wait(p, fail);
+                if (SHARE == 1 || d_group == h) {
+                    const uint8_t* tail = ring.slot + 16 * G + g * 8;
                     wd = *reinterpret_cast<const uint2*>(tail);
                     if (QTYPE == 1) wm = *reinterpret_cast<const uint2*>(tail + 64);
                 }
+                const uint8_t* words = ring.slot + t * 128 + g * 16;
 #pragma unroll
                 for (int pr = 0; pr < 2; pr++) {  // two sets of 32 k: lower nibbles in one MMA, upper ones, in place, in another
-                    const uint4 qa = load_words(slot + (8 * pr + t) * 128 + g * 16, t), qb = load_words(slot + (8 * pr + 4 + t) * 128 + g * 16, t);
+                    const uint4 qa = load_words(words + 1024 * pr, t), qb = load_words(words + 1024 * pr + 512, t);
                     const uint32_t a[4] = {qa.x, qa.y, qa.z, qa.w}, b[4] = {qb.x, qb.y, qb.z, qb.w};
                     constexpr uint32_t kFlip = SIGNED ? 0x88888888u : 0u;
                     uint32_t la[4], lb[4], ua[4], ub[4];
@@ -284,23 +304,30 @@ __device__ __forceinline__ void walk(const FewParams& p, WarpRing<G, QTYPE>& rin
                     }
 #pragma unroll
                     for (int s = 0; s < SETS; s++) {
-                        const uint4 o = x[s][pr];
-                        auto all = [&](auto first) {
-                            constexpr bool F = decltype(first)::value;
-                            mma<F>(low[s][0], la[0], la[1], lb[0], lb[1], o.x, o.z), mma<F>(low[s][1], la[2], la[3], lb[2], lb[3], o.x, o.z);
-                            mma<F>(up[s][0], ua[0], ua[1], ub[0], ub[1], o.y, o.w), mma<F>(up[s][1], ua[2], ua[3], ub[2], ub[3], o.y, o.w);
-                        };
-                        if (h == 0 && pr == 0) all(std::true_type{});
-                        else all(std::false_type{});
+                        uint4 o = x[s][pr];
+                        if (SHARE > 1 && b_group != h) o = make_uint4(0u, 0u, 0u, 0u);
+                        if (h == 0 && pr == 0) {
+                            mma_from(low[s][0], la[0], la[1], lb[0], lb[1], o.x, o.z, start), mma_from(low[s][1], la[2], la[3], lb[2], lb[3], o.x, o.z, start);
+                            mma_from(up[s][0], ua[0], ua[1], ub[0], ub[1], o.y, o.w, start), mma_from(up[s][1], ua[2], ua[3], ub[2], ub[3], o.y, o.w, start);
+                        } else {
+                            mma_u8s8(low[s][0], la[0], la[1], lb[0], lb[1], o.x, o.z), mma_u8s8(low[s][1], la[2], la[3], lb[2], lb[3], o.x, o.z);
+                            mma_u8s8(up[s][0], ua[0], ua[1], ub[0], ub[1], o.y, o.w), mma_u8s8(up[s][1], ua[2], ua[3], ub[2], ub[3], o.y, o.w);
+                        }
                     }
                 }
-                ring.next(lane);
+                ring.next(p, tiles);
             }
+            finish(low, up, wd, wm, x4);
+        };
+        int kc = kc0;
+#pragma unroll 1
+        for (; kc + SHARE <= kc1; kc += SHARE) {
+            round(std::true_type{}, SHARE);
 #pragma unroll
             for (int s = 0; s < SETS; s++) codes[s] += 128 * SHARE;
             sc += 32 * SHARE;
-            finish(low, up);
         }
+        if (SHARE > 1 && kc < kc1) round(std::false_type{}, kc1 - kc);
     }
 }
 
@@ -328,54 +355,59 @@ __global__ void __launch_bounds__(kThreads, 1) experts_few_kernel(const __grid_c
     }
     const int count = __ldcg(p.tile_count);
     __syncthreads();
-    // The CTA's stripes: shares of the tiles' weights, each in front of its tile.
-    for (int i = threadIdx.x; i < count; i += kThreads) {
-        // (what a stripe costs the SM: its bytes, or with group 32 its arithmetic where there are more than four rows)
-        const int rows = tiles[i].z;
-        tiles[i].w = G == 128 || rows <= 4 ? 4 : rows <= 8 ? 5 : 7;
-    }
-    __syncthreads();
-    if (warp == 0) {
-        int sum = 0;
-        for (int i0 = 0; i0 < count; i0 += 32) {
-            const int w = i0 + lane < count ? tiles[i0 + lane].w : 0;
-            int v = w;
+    // The CTA's stripes: equal shares, or where stripes may cost the SM more than their bytes shares of the tiles' weights.
+    int s0, r;
+    if (!p.weigh) {
+        const int64_t stripes = (int64_t)count * p.Ng;
+        s0 = (int)(stripes * blockIdx.x / gridDim.x), r = (int)(stripes * (blockIdx.x + 1) / gridDim.x) - s0;
+    } else {
+        if (warp == 0) {  // the weights in front of each tile
+            int sum = 0;
+            for (int i0 = 0; i0 < count; i0 += 32) {
+                const int rows = i0 + lane < count ? tiles[i0 + lane].z : 0;
+                const int w = i0 + lane < count ? rows <= 4 ? 4 : rows <= 8 ? 5 : 7 : 0;
+                int v = w;
 #pragma unroll
-            for (int off = 1; off < 32; off <<= 1) {
-                const int o = __shfl_up_sync(0xffffffffu, v, off);
-                if (lane >= off) v += o;
+                for (int off = 1; off < 32; off <<= 1) {
+                    const int o = __shfl_up_sync(0xffffffffu, v, off);
+                    if (lane >= off) v += o;
+                }
+                if (i0 + lane < count) tiles[i0 + lane].w = sum + v - w;
+                sum += __shfl_sync(0xffffffffu, v, 31);
             }
-            if (i0 + lane < count) tiles[i0 + lane].w = sum + v - w;
-            sum += __shfl_sync(0xffffffffu, v, 31);
+            if (lane == 0) *total = sum;
         }
-        if (lane == 0) *total = sum;
+        __syncthreads();
+        auto stripe_at = [&](int part) {  // the first stripe of a CTA
+            const int all = *total;
+            if (part >= (int)gridDim.x || count == 0) return count * p.Ng;
+            const int64_t target = (int64_t)all * p.Ng * part / gridDim.x;
+            int lo = 0, hi = count;  // the last tile whose weights begin at or in front of it
+            while (hi - lo > 1) {
+                const int mid = (lo + hi) / 2;
+                if ((int64_t)tiles[mid].w * p.Ng <= target) lo = mid; else hi = mid;
+            }
+            const int w = (lo + 1 < count ? tiles[lo + 1].w : all) - tiles[lo].w;
+            const int64_t in = (target - (int64_t)tiles[lo].w * p.Ng + w - 1) / w;
+            return lo * p.Ng + (int)min((int64_t)p.Ng, in);
+        };
+        s0 = stripe_at(blockIdx.x), r = stripe_at(blockIdx.x + 1) - s0;
     }
-    __syncthreads();
-    auto stripe_at = [&](int part) {  // the first stripe of a CTA
-        const int all = *total;
-        if (part >= (int)gridDim.x || count == 0) return count * p.Ng;
-        const int64_t target = (int64_t)all * p.Ng * part / gridDim.x;
-        int lo = 0, hi = count;  // the last tile whose weights begin at or in front of it
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) / 2;
-            if ((int64_t)tiles[mid].w * p.Ng <= target) lo = mid; else hi = mid;
-        }
-        const int w = (lo + 1 < count ? tiles[lo + 1].w : all) - tiles[lo].w;
-        const int64_t in = (target - (int64_t)tiles[lo].w * p.Ng + w - 1) / w;
-        return lo * p.Ng + (int)min((int64_t)p.Ng, in);
-    };
-    const int s0 = stripe_at(blockIdx.x), r = stripe_at(blockIdx.x + 1) - s0;
     const int C = p.chunks;
     auto share = [&](int w) { return (int)((int64_t)r * C * w / kWarps); };  // first chunk of a warp
     const int begin = share(warp), end = share(warp + 1);
-    WarpRing<G, QTYPE> ring{p, tiles, smem + p.ring_off + warp * p.depth * S::kSlot, bars, s0, end - begin, 0, 0, nullptr};
+    WarpRing<G, QTYPE> ring{};
     if (end > begin) {
-        ring.stripe = begin / C, ring.kc = begin - ring.stripe * C;
-        ring.seek();
-        for (int i = 0; i < p.depth && ring.left > 0; i++) {
-            if (lane == 0) ring.ask();
-            ring.asked();
+        uint8_t* slots = smem + p.ring_off + warp * p.depth * S::kSlot;
+        const int stripe = begin / C, kc = begin - stripe * C, sg = s0 + stripe, tile = sg / p.Ng, ls = sg - tile * p.Ng;
+        ring.slot = slots, ring.at = smem_u32(slots), ring.bar = bars, ring.left = end - begin, ring.tile = tile;
+        ring.in_stripe = C - kc, ring.in_tile = (p.Ng - ls) * C - kc;
+        ring.from = p.wq + tiles[tile].x * p.group_bytes + ((int64_t)ls * p.Kg + kc * S::kBlocks) * S::BS;
+        for (int i = 0; i < p.depth; i++) {
+            if (ring.left > 0) ring.ask(p, tiles);
+            ring.step(p);
         }
+        ring.parity = 0;
     }
     __syncwarp();
     pdl_wait_prior_grid();
@@ -418,8 +450,8 @@ __global__ void __launch_bounds__(kThreads, 1) experts_few_kernel(const __grid_c
         uint64_t(&one)[1][4] = reinterpret_cast<uint64_t(&)[1][4]>(acc);
         if (tile.z <= 4) {
             const bool two = tile.z <= 2;
-            if (two) walk<G, QTYPE, SIGNED, 4, 1>(p, ring, fail, lane, tile, ti, kc0, kc1, one);
-            else walk<G, QTYPE, SIGNED, 2, 1>(p, ring, fail, lane, tile, ti, kc0, kc1, one);
+            if (two) walk<G, QTYPE, SIGNED, 4, 1>(p, tiles, ring, fail, lane, tile, ti, kc0, kc1, one);
+            else walk<G, QTYPE, SIGNED, 2, 1>(p, tiles, ring, fail, lane, tile, ti, kc0, kc1, one);
 #pragma unroll
             for (int k = 0; k < 4; k++) {  // the K groups of the other lanes
                 acc[0][k] = add2(acc[0][k], __shfl_xor_sync(0xffffffffu, acc[0][k], 2));
@@ -428,10 +460,10 @@ __global__ void __launch_bounds__(kThreads, 1) experts_few_kernel(const __grid_c
             }
             if (t < (two ? 1 : 2)) put_two(2 * t, acc[0]);
         } else if (tile.z <= 8) {
-            walk<G, QTYPE, SIGNED, 1, 1>(p, ring, fail, lane, tile, ti, kc0, kc1, one);
+            walk<G, QTYPE, SIGNED, 1, 1>(p, tiles, ring, fail, lane, tile, ti, kc0, kc1, one);
             put_two(2 * t, acc[0]);
         } else {
-            walk<G, QTYPE, SIGNED, 1, 2>(p, ring, fail, lane, tile, ti, kc0, kc1, acc);
+            walk<G, QTYPE, SIGNED, 1, 2>(p, tiles, ring, fail, lane, tile, ti, kc0, kc1, acc);
             put_two(2 * t, acc[0]);
             put_two(8 + 2 * t, acc[1]);
         }
@@ -508,6 +540,9 @@ int launch_experts_few(const ExpertsCall& c, GroupQuant q, cudaStream_t s) {
     p.tiles = c.plan.tiles[kTiles16], p.tile_count = c.plan.counts + kTiles16, p.order = c.plan.order;
     p.row_bytes = chunks * 128, p.group_bytes = c.Ng * c.Kg * block_bytes(c.qtype, c.G);
     p.Ng = (int)c.Ng, p.Kg = (int)c.Kg, p.chunks = (int)chunks, p.most_tiles = (int)tiles;
+    p.last_bytes = (int)(c.Kg - (chunks - 1) * (128 / c.G)) * block_bytes(c.qtype, c.G);
+    // (group 32, more than four rows: its arithmetic takes longer than its bytes)
+    p.weigh = c.G == 32 && c.most_rows > 4;
     p.y_vec = c.ldy % 4 == 0 && (reinterpret_cast<uintptr_t>(c.y) & 15) == 0;
     if (c.qtype == 1) return c.G == 32 ? launch_few<32, 1, false>(p, di, s) : launch_few<128, 1, false>(p, di, s);
     if (!sgn) return c.G == 32 ? launch_few<32, 0, false>(p, di, s) : launch_few<128, 0, false>(p, di, s);
