@@ -18,6 +18,8 @@
 // fused copy of this arithmetic (tree-ordered sums), the prefill path its own
 // kernel below; this one serves callers that want the quantized activations
 // themselves and the per-channel int8 FC on mma.sync (q8c.cu).
+#include <type_traits>
+
 #include "groups.cuh"
 
 namespace q4fc {
@@ -111,24 +113,22 @@ __global__ void __launch_bounds__(kQxWarps * 32) quant_x_kernel(const float* __r
     }
 }
 
-// 128 k of a row, by one warp, in a form that the FC kernels read: lane l holds v[0..3] = x[k .. k + 3], 0 beyond K, of
-// k = 128 c + 4 l.  Codes and scales as in quant_x_kernel, group sums tree-ordered.  `codes`: the lane's place; `sc`: the row's
-// place in the first K group, `per` floats from there to its place in the next, the sum `sum_at` behind the scale.
-// isum: instead of the sum, the bits of the integer 8 * sum of codes.  pad: the 128 k are written whole, zeros beyond the last group.
+// 128 k of a row, by one warp, in a form that the FC kernels read: lane l holds v[0..3] = x[k .. k + 3], k = 4 l behind the first one; 0
+// beyond K, which is `left` behind it.  Codes and scales as in quant_x_kernel, group sums tree-ordered.  `codes`: the lane's place;
+// `sc`: the row's place in the first of the 128 k's groups, `per` floats from there to its place in the next, the sum `sum_at` behind
+// the scale.  isum: instead of the sum, the bits of the integer 8 * sum of codes.  pad: the 128 k are written whole, zeros beyond the
+// last group.
 template <int G, bool F16>
-__device__ __forceinline__ void quantize_unit(const float (&v)[4], int64_t c, int lane, int64_t K, int64_t Kg, bool sums, bool isum, bool pad,
-                                              int8_t* __restrict__ codes, float* __restrict__ sc, int64_t per, int64_t sum_at) {
+__device__ __forceinline__ void quantize_unit(const float (&v)[4], int lane, int left, bool sums, bool isum, bool pad, int8_t* __restrict__ codes,
+                                              float* __restrict__ sc, int64_t per, int64_t sum_at) {
     constexpr int SEG = G / 4;    // lanes per group
-    constexpr int GPC = 128 / G;  // groups per 128-k chunk
-    const int64_t kb = c * GPC + lane / SEG;
-    const bool exists = kb < Kg;
-    const int len = exists ? (int)min((int64_t)G, K - kb * G) : 0;
+    const int before = lane / SEG * G;  // k in front of this lane's group
+    const bool exists = before < left;
+    const int len = min(G, max(0, left - before));
     const int body = len & ~7;
     const int e0 = (lane % SEG) * 4;
-    float amax = 0.0f, sum = (v[0] + v[1]) + (v[2] + v[3]);
-#pragma unroll
-    for (int j = 0; j < 4; j++)
-        if (e0 + j < len) amax = fmaxf(amax, fabsf(v[j]));
+    float amax = fmaxf(fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3]))), 0.0f);  // (0 of missing values alone)
+    float sum = (v[0] + v[1]) + (v[2] + v[3]);
 #pragma unroll
     for (int off = SEG / 2; off > 0; off >>= 1) {
         amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, off));
@@ -136,46 +136,93 @@ __device__ __forceinline__ void quantize_unit(const float (&v)[4], int64_t c, in
     }
     const float d = div_const_rn(amax, 127.0f, 1.0f / 127.0f);
     const float id = inv_or_zero(d);
-    int q[4] = {};
-#pragma unroll
-    for (int j = 0; j < 4; j++)
-        if (e0 + j < len) {
-            const float t = __fmul_rn(v[j], id);
-            q[j] = sat8(e0 + j < body ? __float2int_rn(t) : round_half_away(t));
-        }
-    if (isum) {
-        int s = q[0] + q[1] + q[2] + q[3];
-#pragma unroll
-        for (int off = SEG / 2; off > 0; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
-        sum = __int_as_float(8 * s);
-    }
     uint32_t w[2];  // F16: four codes, as two lanes hold eight k: the even one takes k = 0,2,4,6 (see launch_quant_x_tile)
-    if constexpr (F16) {
-        uint32_t h[4];
+    // Ordinary groups, whole: |v x id| < 128, and t + 1.5 x 2^23 rounds t to the nearest integer, half to even, and has it in its low bits.
+    // (Missing values: fmaxf does not see them, the sum does.)
+    const bool ordinary = (amax == 0.0f || (amax >= 0x1p-100f && amax <= 0x1p100f)) && sum == sum;
+    if (left >= 128 && __all_sync(0xffffffffu, ordinary)) {
+        float t[4];
 #pragma unroll
-        for (int j = 0; j < 4; j++) h[j] = __half_as_ushort(__int2half_rn(q[j] * ((lane & 1) ? 16 : 256)));
-        const uint32_t even = h[0] | h[2] << 16, odd = h[1] | h[3] << 16;
-        const uint32_t other = __shfl_xor_sync(0xffffffffu, (lane & 1) ? even : odd, 1);
-        w[0] = (lane & 1) ? other : even, w[1] = (lane & 1) ? odd : other;
+        for (int j = 0; j < 4; j++) t[j] = __fadd_rn(__fmul_rn(v[j], id), 12582912.0f);
+        const uint32_t lo = __byte_perm(__float_as_uint(t[0]), __float_as_uint(t[1]), 0x0040), hi = __byte_perm(__float_as_uint(t[2]), __float_as_uint(t[3]), 0x0040);
+        w[0] = __byte_perm(lo, hi, 0x5410);
+        if constexpr (F16) {
+            const float up = (lane & 1) ? 16.0f : 256.0f;
+#pragma unroll
+            for (int j = 0; j < 4; j++) t[j] = __fmul_rn(__fadd_rn(t[j], -12582912.0f), up);
+            const __half2 even2 = __floats2half2_rn(t[0], t[2]), odd2 = __floats2half2_rn(t[1], t[3]);
+            const uint32_t even = *reinterpret_cast<const uint32_t*>(&even2), odd = *reinterpret_cast<const uint32_t*>(&odd2);
+            const uint32_t other = __shfl_xor_sync(0xffffffffu, (lane & 1) ? even : odd, 1);
+            w[0] = (lane & 1) ? other : even, w[1] = (lane & 1) ? odd : other;
+        } else if (isum) {
+            int s = __dp4a((int)w[0], 0x01010101, 0);
+#pragma unroll
+            for (int off = SEG / 2; off > 0; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
+            sum = __int_as_float(8 * s);
+        }
+    } else {
+        int q[4] = {};
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+            if (e0 + j < len) {
+                const float t = __fmul_rn(v[j], id);
+                q[j] = sat8(e0 + j < body ? __float2int_rn(t) : round_half_away(t));
+            }
+        if (isum) {
+            int s = q[0] + q[1] + q[2] + q[3];
+#pragma unroll
+            for (int off = SEG / 2; off > 0; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
+            sum = __int_as_float(8 * s);
+        }
+        w[0] = (q[0] & 0xFF) | (q[1] & 0xFF) << 8 | (q[2] & 0xFF) << 16 | (uint32_t)(q[3] & 0xFF) << 24;
+        if constexpr (F16) {
+            uint32_t h[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) h[j] = __half_as_ushort(__int2half_rn(q[j] * ((lane & 1) ? 16 : 256)));
+            const uint32_t even = h[0] | h[2] << 16, odd = h[1] | h[3] << 16;
+            const uint32_t other = __shfl_xor_sync(0xffffffffu, (lane & 1) ? even : odd, 1);
+            w[0] = (lane & 1) ? other : even, w[1] = (lane & 1) ? odd : other;
+        }
     }
     if (exists || pad) {
         if constexpr (F16)
             *reinterpret_cast<uint2*>(codes) = make_uint2(w[0], w[1]);
         else
-            *reinterpret_cast<uint32_t*>(codes) =
-                (q[0] & 0xFF) | (q[1] & 0xFF) << 8 | (q[2] & 0xFF) << 16 | (uint32_t)(q[3] & 0xFF) << 24;
+            *reinterpret_cast<uint32_t*>(codes) = w[0];
         if (e0 == 0) {
-            float* dst = sc + kb * per;
+            float* dst = sc + lane / SEG * per;
             dst[0] = F16 ? __fmul_rn(d, 64.0f) : d;
             if (sums) dst[sum_at] = sum;
         }
     }
 }
 
+// The lane's values of `CHUNKS` times 128 k from chunk c on, all asked for at once; 0 beyond K.
+template <int CHUNKS>
+__device__ __forceinline__ void load_chunks(const float* __restrict__ row, int64_t c, int lane, int64_t K, int vec_ok, float (&v)[CHUNKS][4]) {
+#pragma unroll
+    for (int i = 0; i < CHUNKS; i++) {
+        const int64_t k = (c + i) * 128 + lane * 4;
+        v[i][0] = v[i][1] = v[i][2] = v[i][3] = 0.0f;
+        if (vec_ok && k + 4 <= K) {
+            const float4 a = ld_after_wait(reinterpret_cast<const float4*>(row + k));
+            v[i][0] = a.x, v[i][1] = a.y, v[i][2] = a.z, v[i][3] = a.w;
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                if (k + j < K) v[i][j] = ld_after_wait(row + k + j);
+        }
+    }
+}
+// Chunks of a warp: many rows are quantized four at a time, so that a warp starts, and finds its row, a quarter as often (2048 x 4096
+// XX -> XX us); few rows one at a time, for the shortest way through.
+constexpr int kManyChunks = 4;
+constexpr int64_t kManyUnits = 16384;  // rows x chunks
+
 // The prefill GEMM's quantizer: the codes and scales of quant_x_kernel, scales (and, `sums`, group sums, tree-ordered)
 // in the layout in which the GEMM's tiles of 2^log2tile rows read them: [row tile][Kg][scale | sum][row in tile].
-// The eight warps of a CTA take the same 128 k of eight neighbouring rows, whose scales share a 32-byte sector.
-template <int G, bool F16>
+// The eight warps of a CTA take the same k of eight neighbouring rows, whose scales share a 32-byte sector.
+template <int G, bool F16, int CHUNKS>
 __global__ void __launch_bounds__(kQxWarps * 32) quant_x_tile_kernel(const float* __restrict__ x, int64_t rows, int64_t K,
                                                                      int64_t ldx, int64_t Kg, int vec_ok, int sums,
                                                                      int log2tile, int8_t* __restrict__ codes,
@@ -184,38 +231,34 @@ __global__ void __launch_bounds__(kQxWarps * 32) quant_x_tile_kernel(const float
     pdl_launch_dependents();      // the GEMM's weight copies run beside this launch
     const int lane = threadIdx.x & 31;
     const int64_t row_sets = (rows + kQxWarps - 1) / kQxWarps;
-    const int64_t c = blockIdx.x / row_sets;
-    const int64_t row = (blockIdx.x - c * row_sets) * kQxWarps + (threadIdx.x >> 5);
+    const int64_t set = blockIdx.x / row_sets, c = set * CHUNKS;
+    const int64_t row = (blockIdx.x - set * row_sets) * kQxWarps + (threadIdx.x >> 5);
     if (row >= rows) return;
-    const int64_t k = c * 128 + lane * 4;
-    const float* src = x + row * ldx + k;
-    float v[4] = {0.f, 0.f, 0.f, 0.f};
-    if (vec_ok && k + 4 <= K) {
-        const float4 a = ld_after_wait(reinterpret_cast<const float4*>(src));
-        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
-    } else {
-#pragma unroll
-        for (int j = 0; j < 4; j++)
-            if (k + j < K) v[j] = ld_after_wait(src + j);
-    }
+    float v[CHUNKS][4];
+    load_chunks<CHUNKS>(x + row * ldx, c, lane, K, vec_ok, v);
     const int64_t tile = (int64_t)1 << log2tile, per = tile << sums;
-    quantize_unit<G, F16>(v, c, lane, K, Kg, sums, false, false, codes + (row * (Kg * G) + k) * (F16 ? 2 : 1),
-                          sc + (row >> log2tile) * Kg * per + (row & (tile - 1)), per, tile);
+    float* dst = sc + ((row >> log2tile) * Kg + c * (128 / G)) * per + (row & (tile - 1));
+    int8_t* to = codes + (row * (Kg * G) + c * 128 + lane * 4) * (F16 ? 2 : 1);
+    const int left = (int)min((int64_t)CHUNKS * 128, K - c * 128);
+#pragma unroll
+    for (int i = 0; i < CHUNKS; i++)
+        if (CHUNKS == 1 || 128 * i < left)
+            quantize_unit<G, F16>(v[i], lane, left - 128 * i, sums, false, false, to + 128 * i * (F16 ? 2 : 1), dst + i * (128 / G) * per, per, tile);
 }
 
 // The quantizer of the experts' product: rows in the order of a plan (groups.cuh), codes in that order, scales by the
 // plan's tiles: for experts with few rows (tiles of 16) [tile][K group][two rows][scales, sums], else as quant_x_tile_kernel has them.
 // A row of x serves `per_row` (token, slot) pairs, or one; `gated`: the value is silu(x[k]) * x[K + k].  An output row
 // without an expert is zeroed here.
-template <int G, bool F16>
+template <int G, bool F16, int CHUNKS>
 __global__ void __launch_bounds__(kQxWarps * 32) quant_x_group_kernel(const __grid_constant__ GroupQuant a) {
     pdl_wait_prior_grid();
     __threadfence();              // what is behind this launch reads the plan, too, before this launch has ended
     pdl_launch_dependents();
     const int lane = threadIdx.x & 31;
     const int64_t row_sets = (a.rows + kQxWarps - 1) / kQxWarps;
-    const int64_t c = blockIdx.x / row_sets;
-    const int64_t place = (blockIdx.x - c * row_sets) * kQxWarps + (threadIdx.x >> 5);
+    const int64_t set = blockIdx.x / row_sets, c = set * CHUNKS;
+    const int64_t place = (blockIdx.x - set * row_sets) * kQxWarps + (threadIdx.x >> 5);
     if (place >= a.rows) return;
     const int group = __ldcg(a.group_of + place);
     const int64_t pair = __ldcg(a.order + place);
@@ -225,36 +268,36 @@ __global__ void __launch_bounds__(kQxWarps * 32) quant_x_group_kernel(const __gr
         return;
     }
     const int first = __ldcg(a.offsets + group), tile0 = __ldcg(a.tile0 + group);
-    const int64_t k = c * 128 + lane * 4;
-    const float* src = a.x + (a.per_row > 1 ? pair / a.per_row : pair) * a.ldx + k;
-    float v[4] = {0.f, 0.f, 0.f, 0.f};
-    auto load = [&](const float* src, float (&v)[4]) {
-        if (a.vec_ok && k + 4 <= a.K) {
-            const float4 b = ld_after_wait(reinterpret_cast<const float4*>(src));
-            v[0] = b.x, v[1] = b.y, v[2] = b.z, v[3] = b.w;
-        } else {
-#pragma unroll
-            for (int j = 0; j < 4; j++)
-                if (k + j < a.K) v[j] = ld_after_wait(src + j);
-        }
-    };
-    load(src, v);
+    const float* src = a.x + (a.per_row > 1 ? (int64_t)((uint32_t)pair / (uint32_t)a.per_row) : pair) * a.ldx;
+    float v[CHUNKS][4];
+    load_chunks<CHUNKS>(src, c, lane, a.K, a.vec_ok, v);
     if (a.gated) {
-        float up[4] = {0.f, 0.f, 0.f, 0.f};
-        load(src + a.K, up);
+        float up[CHUNKS][4];
+        load_chunks<CHUNKS>(src + a.K, c, lane, a.K, a.vec_ok, up);
 #pragma unroll
-        for (int j = 0; j < 4; j++) v[j] = __fmul_rn(up[j], __fdiv_rn(v[j], __fadd_rn(1.0f, expf(-v[j]))));
+        for (int i = 0; i < CHUNKS; i++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) v[i][j] = __fmul_rn(up[i][j], __fdiv_rn(v[i][j], __fadd_rn(1.0f, expf(-v[i][j]))));
     }
+    const int left = (int)min((int64_t)CHUNKS * 128, a.K - c * 128);
     const int at = (int)place - first, tile = tile0 + (at >> a.log2tile), row = at & ((1 << a.log2tile) - 1);
     if (a.log2tile == 4) {
         const int64_t chunks = (a.Kg * G + 127) / 128, groups = chunks * (128 / G);
         // (what a lane of the FC kernel takes of 128 k -- eight of each 32 -- lies together; scales and sums of two rows do)
         int8_t* codes = a.codes + (place * chunks + c) * 128 + (lane / 2 % 4) * 32 + (lane / 8) * 8 + (lane % 2) * 4;
-        quantize_unit<G, F16>(v, c, lane, a.K, a.Kg, true, a.isum, true, codes, a.sc + (int64_t)tile * groups * 32 + row / 2 * 4 + row % 2, 32, 2);
+        float* sc = a.sc + ((int64_t)tile * groups + c * (128 / G)) * 32 + row / 2 * 4 + row % 2;
+#pragma unroll
+        for (int i = 0; i < CHUNKS; i++)
+            if (CHUNKS == 1 || 128 * i < left)
+                quantize_unit<G, F16>(v[i], lane, left - 128 * i, true, a.isum, true, codes + 128 * i, sc + i * (128 / G) * 32, 32, 2);
     } else {
         const int64_t size = (int64_t)1 << a.log2tile, per = size << a.sums;
-        quantize_unit<G, F16>(v, c, lane, a.K, a.Kg, a.sums, false, false, a.codes + (place * (a.Kg * G) + k) * (F16 ? 2 : 1),
-                              a.sc + (int64_t)tile * a.Kg * per + row, per, size);
+        int8_t* codes = a.codes + (place * (a.Kg * G) + c * 128 + lane * 4) * (F16 ? 2 : 1);
+        float* sc = a.sc + ((int64_t)tile * a.Kg + c * (128 / G)) * per + row;
+#pragma unroll
+        for (int i = 0; i < CHUNKS; i++)
+            if (CHUNKS == 1 || 128 * i < left)
+                quantize_unit<G, F16>(v[i], lane, left - 128 * i, a.sums, false, false, codes + 128 * i * (F16 ? 2 : 1), sc + i * (128 / G) * per, per, size);
     }
 }
 
@@ -499,30 +542,42 @@ int launch_quant_x_tile(const float* x, int64_t rows, int64_t K, int64_t ldx, in
                         int8_t* codes, float* sc, cudaStream_t s) {
     const int64_t Kg = (K + G - 1) / G;
     if (rows == 0 || Kg == 0) return Q4FC_OK;
-    const int64_t grid = (rows + kQxWarps - 1) / kQxWarps * ((Kg * G + 127) / 128);
+    const int64_t chunks = (Kg * G + 127) / 128;
+    const bool many = rows * chunks >= kManyUnits;
+    const int64_t grid = (rows + kQxWarps - 1) / kQxWarps * (many ? (chunks + kManyChunks - 1) / kManyChunks : chunks);
     if (grid > 0x7fffffffLL) {
         set_error("quant_x: %lld x %lld exceeds the grid limit", (long long)rows, (long long)K);
         return Q4FC_ELIMIT;
     }
     const int vec_ok = (K % 4 == 0) && (ldx % 4 == 0) && ((reinterpret_cast<uintptr_t>(x) & 15) == 0);
     const int l2 = tile == 128 ? 7 : 6;
-    auto* kernel = G == 128 ? quant_x_tile_kernel<128, false> : f16 ? quant_x_tile_kernel<32, true> : quant_x_tile_kernel<32, false>;
     DependentLaunch l(dim3((unsigned)grid), kQxWarps * 32, s);
-    Q4FC_CUDA_OK(cudaLaunchKernelEx(&l.cfg, kernel, x, rows, K, ldx, Kg, vec_ok, (int)sums, l2, codes, sc));
-    return Q4FC_OK;
+    auto launch = [&](auto n) -> int {
+        constexpr int N = decltype(n)::value;
+        auto* kernel = G == 128 ? quant_x_tile_kernel<128, false, N> : f16 ? quant_x_tile_kernel<32, true, N> : quant_x_tile_kernel<32, false, N>;
+        Q4FC_CUDA_OK(cudaLaunchKernelEx(&l.cfg, kernel, x, rows, K, ldx, Kg, vec_ok, (int)sums, l2, codes, sc));
+        return Q4FC_OK;
+    };
+    return many ? launch(std::integral_constant<int, kManyChunks>{}) : launch(std::integral_constant<int, 1>{});
 }
 
 int launch_quant_x_group(const GroupQuant& q, int G, bool f16, cudaStream_t s) {
     if (q.rows == 0) return Q4FC_OK;
-    const int64_t grid = (q.rows + kQxWarps - 1) / kQxWarps * ((q.Kg * G + 127) / 128);
+    const int64_t chunks = (q.Kg * G + 127) / 128;
+    const bool many = q.rows * chunks >= kManyUnits;
+    const int64_t grid = (q.rows + kQxWarps - 1) / kQxWarps * (many ? (chunks + kManyChunks - 1) / kManyChunks : chunks);
     if (grid > 0x7fffffffLL) {
         set_error("quant_x: %lld x %lld exceeds the grid limit", (long long)q.rows, (long long)q.K);
         return Q4FC_ELIMIT;
     }
-    auto* kernel = G == 128 ? quant_x_group_kernel<128, false> : f16 ? quant_x_group_kernel<32, true> : quant_x_group_kernel<32, false>;
     DependentLaunch l(dim3((unsigned)grid), kQxWarps * 32, s);
-    Q4FC_CUDA_OK(cudaLaunchKernelEx(&l.cfg, kernel, q));
-    return Q4FC_OK;
+    auto launch = [&](auto n) -> int {
+        constexpr int N = decltype(n)::value;
+        auto* kernel = G == 128 ? quant_x_group_kernel<128, false, N> : f16 ? quant_x_group_kernel<32, true, N> : quant_x_group_kernel<32, false, N>;
+        Q4FC_CUDA_OK(cudaLaunchKernelEx(&l.cfg, kernel, q));
+        return Q4FC_OK;
+    };
+    return many ? launch(std::integral_constant<int, kManyChunks>{}) : launch(std::integral_constant<int, 1>{});
 }
 
 int launch_quant_x(const float* x, int64_t rows, int64_t K, int64_t ldx, int G, float scale, int8_t* codes,
