@@ -72,7 +72,7 @@ int launch_fc_experts(ExpertsCall c, const float* weights, int64_t top_k, cudaSt
     }
     GroupQuant q = {};
     q.x = c.x, q.rows = c.rows, q.K = c.K, q.Kg = c.Kg, q.ldx = c.ldx, q.per_row = c.per_row, q.gated = c.gated;
-    q.order = c.plan.order, q.group_of = c.plan.group_of, q.offsets = c.plan.offsets, q.n = (int)c.n;
+    q.group_of = c.plan.group_of, q.place_of = c.plan.place_of, q.offsets = c.plan.offsets, q.n = (int)c.n;
     q.vec_ok = c.K % 4 == 0 && c.ldx % 4 == 0 && (reinterpret_cast<uintptr_t>(c.x) & 15) == 0;
     q.y = c.y, q.N = c.N, q.ldy = c.ldy;
     if (int rc = experts_few_serves(c.rows, c.n) ? launch_experts_few(c, q, s) : launch_experts_gemm(c, q, s)) return rc;

@@ -153,7 +153,7 @@ __global__ void __launch_bounds__(kFew) group_few_kernel(const GroupArgs a, cons
     sorted[place] = b;
     // a tile of a size begins at this row's place
     for (int j = 0; j < kTileSizes; j++) tiles_to[j][place] = b < a.n && before % tile_rows(j) == 0;
-    if (me < rows) a.plan.order[place] = me, a.plan.group_of[place] = b;
+    if (me < rows) a.plan.order[place] = me, a.plan.group_of[me] = b, a.plan.place_of[me] = place;
     __syncthreads();
     // (place me) tiles in front
     int begins[kTileSizes], in_warp[kTileSizes];
@@ -323,14 +323,16 @@ __global__ void __launch_bounds__(kThreads, 1) group_kernel(const GroupArgs a, c
         for (int h = 0; h < kHeld; h++)
             if (held[h] >= 0) {
                 const uint32_t at = here[held[h]] + mine[held[h]] + local[h];
-                row_of[at] = (uint32_t)(begin + 32 * h + lane), bin_at[at] = (uint16_t)held[h];
+                const int64_t i = begin + 32 * h + lane;
+                row_of[at] = (uint32_t)i, bin_at[at] = (uint16_t)held[h];
+                a.plan.group_of[i] = held[h], a.plan.place_of[i] = (int)(first[held[h]] + at - here[held[h]]);
             }
         __syncthreads();
         const uint32_t there = here[a.n] + sums[a.n];
         for (uint32_t i = threadIdx.x; i < there; i += kThreads) {
             const int b = bin_at[i];
             const uint32_t place = first[b] + i - here[b];
-            a.plan.order[place] = (int)row_of[i], a.plan.group_of[place] = b;
+            a.plan.order[place] = (int)row_of[i];
         }
     } else {
         for (int64_t i0 = begin; i0 < end; i0 += 32) {
@@ -339,7 +341,7 @@ __global__ void __launch_bounds__(kThreads, 1) group_kernel(const GroupArgs a, c
             const uint32_t local = count(b, there);
             if (there) {
                 const uint32_t place = first[b] + local;
-                a.plan.order[place] = (int)(i0 + lane), a.plan.group_of[place] = b;
+                a.plan.order[place] = (int)(i0 + lane), a.plan.group_of[i0 + lane] = b, a.plan.place_of[i0 + lane] = (int)place;
             }
         }
     }

@@ -4,7 +4,8 @@
 //   offsets[n + 1] first place in `order` of each group; offsets[n]: of the rows without one
 //   order[rows]    row numbers, sorted by group and stable: the grouped ones, then those without a group
 //   tiles          of 8, 16, 64 and 128 rows: {group, first place in order, rows, 0}; a tile's rows are of one group
-//   group_of[rows] the group of each place in order (n: none)
+//   group_of[rows] the group of each row (n: none)
+//   place_of[rows] the place of each row in order
 //   tile0[n + 1]   of 8, 16, 64 and 128 rows: the first tile of each group
 // Each part starts on 16 bytes.  No group has more tiles than its rows / size + 1, so rows / size + min(n, rows) places are enough.
 #pragma once
@@ -22,7 +23,7 @@ struct GroupPlan {
     int* offsets;
     int* order;
     int4* tiles[kTileSizes];
-    int* group_of;
+    int *group_of, *place_of;
     int* tile0[kTileSizes];
     int64_t bytes;
 };
@@ -43,6 +44,7 @@ inline GroupPlan group_plan(void* buffer, int64_t rows, int64_t n) {
     p.order = reinterpret_cast<int*>(take(rows * 4));
     for (int w = 0; w < kTileSizes; w++) p.tiles[w] = reinterpret_cast<int4*>(take(most_tiles(w, rows, n) * 16));
     p.group_of = reinterpret_cast<int*>(take(rows * 4));
+    p.place_of = reinterpret_cast<int*>(take(rows * 4));
     for (int w = 0; w < kTileSizes; w++) p.tile0[w] = reinterpret_cast<int*>(take((n + 1) * 4));
     p.bytes = at;
     return p;
@@ -58,7 +60,7 @@ struct GroupQuant {  // quant_x.cu
     const float* x;
     int64_t rows, K, Kg, ldx;  // rows: pairs of the plan
     int64_t per_row;           // pairs that share a row of x
-    const int *order, *group_of, *offsets, *tile0;
+    const int *group_of, *place_of, *offsets, *tile0;
     int n, log2tile, vec_ok, gated, sums, isum;
     int8_t* codes;
     float* sc;

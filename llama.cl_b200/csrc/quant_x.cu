@@ -113,18 +113,17 @@ __global__ void __launch_bounds__(kQxWarps * 32) quant_x_kernel(const float* __r
     }
 }
 
-// 128 k of a row, by one warp, in a form that the FC kernels read: lane l holds v[0..3] = x[k .. k + 3], k = 4 l behind the first one; 0
-// beyond K, which is `left` behind it.  Codes and scales as in quant_x_kernel, group sums tree-ordered.  `codes`: the lane's place;
-// `sc`: the row's place in the first of the 128 k's groups, `per` floats from there to its place in the next, the sum `sum_at` behind
-// the scale.  isum: instead of the sum, the bits of the integer 8 * sum of codes.  pad: the 128 k are written whole, zeros beyond the
-// last group.
+// 128 k of a row, by one warp, as the FC kernels read them: lane l holds v[0..3] = x[k .. k + 3], k = 4 l behind the first one; 0
+// beyond K, which is `left` behind it.  Codes and scales as in quant_x_kernel, group sums tree-ordered.  isum: instead of the sum, the
+// bits of the integer 8 * sum of codes.
+struct QuantizedUnit {
+    uint32_t w[2];  // the lane's codes: four bytes, or four fp16 (see launch_quant_x_tile)
+    float scale, sum;
+};
 template <int G, bool F16>
-__device__ __forceinline__ void quantize_unit(const float (&v)[4], int lane, int left, bool sums, bool isum, bool pad, int8_t* __restrict__ codes,
-                                              float* __restrict__ sc, int64_t per, int64_t sum_at) {
+__device__ __forceinline__ QuantizedUnit quantize_unit(const float (&v)[4], int lane, int left, bool isum) {
     constexpr int SEG = G / 4;    // lanes per group
-    const int before = lane / SEG * G;  // k in front of this lane's group
-    const bool exists = before < left;
-    const int len = min(G, max(0, left - before));
+    const int len = min(G, max(0, left - lane / SEG * G));  // of this lane's group
     const int body = len & ~7;
     const int e0 = (lane % SEG) * 4;
     float amax = fmaxf(fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3]))), 0.0f);  // (0 of missing values alone)
@@ -136,7 +135,7 @@ __device__ __forceinline__ void quantize_unit(const float (&v)[4], int lane, int
     }
     const float d = div_const_rn(amax, 127.0f, 1.0f / 127.0f);
     const float id = inv_or_zero(d);
-    uint32_t w[2];  // F16: four codes, as two lanes hold eight k: the even one takes k = 0,2,4,6 (see launch_quant_x_tile)
+    uint32_t w[2] = {};  // F16: four codes, as two lanes hold eight k: the even one takes k = 0,2,4,6
     // Ordinary groups, whole: |v x id| < 128, and t + 1.5 x 2^23 rounds t to the nearest integer, half to even, and has it in its low bits.
     // (Missing values: fmaxf does not see them, the sum does.)
     const bool ordinary = (amax == 0.0f || (amax >= 0x1p-100f && amax <= 0x1p100f)) && sum == sum;
@@ -184,16 +183,22 @@ __device__ __forceinline__ void quantize_unit(const float (&v)[4], int lane, int
             w[0] = (lane & 1) ? other : even, w[1] = (lane & 1) ? odd : other;
         }
     }
-    if (exists || pad) {
-        if constexpr (F16)
-            *reinterpret_cast<uint2*>(codes) = make_uint2(w[0], w[1]);
-        else
-            *reinterpret_cast<uint32_t*>(codes) = w[0];
-        if (e0 == 0) {
-            float* dst = sc + lane / SEG * per;
-            dst[0] = F16 ? __fmul_rn(d, 64.0f) : d;
-            if (sums) dst[sum_at] = sum;
-        }
+    return {{w[0], w[1]}, F16 ? __fmul_rn(d, 64.0f) : d, sum};
+}
+// `codes`: the lane's place; `sc`: the row's place in the first of the 128 k's groups, `per` floats from there to its place in the next, the
+// sum `sum_at` behind the scale.  groups: of the 128 k that are written.
+template <int G, bool F16>
+__device__ __forceinline__ void store_unit(const QuantizedUnit& q, int lane, int groups, bool sums, int8_t* codes, float* sc, int64_t per, int64_t sum_at) {
+    constexpr int SEG = G / 4;
+    if (lane / SEG >= groups) return;
+    if constexpr (F16)
+        *reinterpret_cast<uint2*>(codes) = make_uint2(q.w[0], q.w[1]);
+    else
+        *reinterpret_cast<uint32_t*>(codes) = q.w[0];
+    if (lane % SEG == 0) {
+        float* dst = sc + lane / SEG * per;
+        dst[0] = q.scale;
+        if (sums) dst[sum_at] = q.sum;
     }
 }
 
@@ -215,7 +220,7 @@ __device__ __forceinline__ void load_chunks(const float* __restrict__ row, int64
     }
 }
 // Chunks of a warp: many rows are quantized four at a time, so that a warp starts, and finds its row, a quarter as often (2048 x 4096
-// XX -> XX us); few rows one at a time, for the shortest way through.
+// 20 -> 18 us); few rows one at a time, for the shortest way through.
 constexpr int kManyChunks = 4;
 constexpr int64_t kManyUnits = 16384;  // rows x chunks
 
@@ -243,61 +248,69 @@ __global__ void __launch_bounds__(kQxWarps * 32) quant_x_tile_kernel(const float
 #pragma unroll
     for (int i = 0; i < CHUNKS; i++)
         if (CHUNKS == 1 || 128 * i < left)
-            quantize_unit<G, F16>(v[i], lane, left - 128 * i, sums, false, false, to + 128 * i * (F16 ? 2 : 1), dst + i * (128 / G) * per, per, tile);
+            store_unit<G, F16>(quantize_unit<G, F16>(v[i], lane, left - 128 * i, false), lane, (left - 128 * i + G - 1) / G, sums,
+                               to + 128 * i * (F16 ? 2 : 1), dst + i * (128 / G) * per, per, tile);
 }
 
-// The quantizer of the experts' product: rows in the order of a plan (groups.cuh), codes in that order, scales by the
-// plan's tiles: for experts with few rows (tiles of 16) [tile][K group][two rows][scales, sums], else as quant_x_tile_kernel has them.
-// A row of x serves `per_row` (token, slot) pairs, or one; `gated`: the value is silu(x[k]) * x[K + k].  An output row
-// without an expert is zeroed here.
+// The quantizer of the experts' product: a row of x for each of its `per_row` (token, slot) pairs, or one; codes in the order of the
+// plan (groups.cuh), scales by its tiles: for experts with few rows (tiles of 16) [tile][K group][two rows][scales, sums], else
+// as quant_x_tile_kernel has them.  `gated`: the value is silu(x[k]) * x[K + k].  An output row without an expert is zeroed here.
 template <int G, bool F16, int CHUNKS>
 __global__ void __launch_bounds__(kQxWarps * 32) quant_x_group_kernel(const __grid_constant__ GroupQuant a) {
     pdl_wait_prior_grid();
     __threadfence();              // what is behind this launch reads the plan, too, before this launch has ended
     pdl_launch_dependents();
     const int lane = threadIdx.x & 31;
-    const int64_t row_sets = (a.rows + kQxWarps - 1) / kQxWarps;
+    const int64_t x_rows = a.rows / a.per_row, row_sets = (x_rows + kQxWarps - 1) / kQxWarps;
     const int64_t set = blockIdx.x / row_sets, c = set * CHUNKS;
-    const int64_t place = (blockIdx.x - set * row_sets) * kQxWarps + (threadIdx.x >> 5);
-    if (place >= a.rows) return;
-    const int group = __ldcg(a.group_of + place);
-    const int64_t pair = __ldcg(a.order + place);
-    if (group >= a.n) {
-        if (c == 0)
-            for (int64_t n = lane; n < a.N; n += 32) a.y[pair * a.ldy + n] = 0.0f;
-        return;
-    }
-    const int first = __ldcg(a.offsets + group), tile0 = __ldcg(a.tile0 + group);
-    const float* src = a.x + (a.per_row > 1 ? (int64_t)((uint32_t)pair / (uint32_t)a.per_row) : pair) * a.ldx;
+    const int64_t row = (blockIdx.x - set * row_sets) * kQxWarps + (threadIdx.x >> 5);
+    if (row >= x_rows) return;
     float v[CHUNKS][4];
-    load_chunks<CHUNKS>(src, c, lane, a.K, a.vec_ok, v);
+    load_chunks<CHUNKS>(a.x + row * a.ldx, c, lane, a.K, a.vec_ok, v);
+    // lane s: where the codes and scales of slot s go; -1: nowhere
+    const bool few = a.log2tile == 4;
+    const int64_t chunks = (a.Kg * G + 127) / 128, size = (int64_t)1 << a.log2tile, per = few ? 32 : size << a.sums, sum_at = few ? 2 : size;
+    int64_t code_at = -1, sc_at = 0;
+    int group = a.n;
+    if (lane < a.per_row) {
+        const int64_t pair = row * a.per_row + lane;
+        group = __ldcg(a.group_of + pair);
+        const int64_t place = __ldcg(a.place_of + pair);
+        if (group < a.n) {
+            const int at = (int)place - __ldcg(a.offsets + group), in = at & ((1 << a.log2tile) - 1);
+            const int64_t tile = __ldcg(a.tile0 + group) + (at >> a.log2tile);
+            code_at = few ? (place * chunks + c) * 128 : (place * (a.Kg * G) + c * 128) * (F16 ? 2 : 1);
+            sc_at = (tile * (few ? chunks * (128 / G) : a.Kg) + c * (128 / G)) * per + (few ? in / 2 * 4 + in % 2 : in);
+        }
+    }
+    const uint32_t none = __ballot_sync(0xffffffffu, lane < a.per_row && group >= a.n);
+    if (c == 0)
+        for (uint32_t left = none; left; left &= left - 1)
+            for (int64_t n = lane; n < a.N; n += 32) a.y[(row * a.per_row + __ffs(left) - 1) * a.ldy + n] = 0.0f;
     if (a.gated) {
         float up[CHUNKS][4];
-        load_chunks<CHUNKS>(src + a.K, c, lane, a.K, a.vec_ok, up);
+        load_chunks<CHUNKS>(a.x + row * a.ldx + a.K, c, lane, a.K, a.vec_ok, up);
 #pragma unroll
         for (int i = 0; i < CHUNKS; i++)
 #pragma unroll
             for (int j = 0; j < 4; j++) v[i][j] = __fmul_rn(up[i][j], __fdiv_rn(v[i][j], __fadd_rn(1.0f, expf(-v[i][j]))));
     }
     const int left = (int)min((int64_t)CHUNKS * 128, a.K - c * 128);
-    const int at = (int)place - first, tile = tile0 + (at >> a.log2tile), row = at & ((1 << a.log2tile) - 1);
-    if (a.log2tile == 4) {
-        const int64_t chunks = (a.Kg * G + 127) / 128, groups = chunks * (128 / G);
-        // (what a lane of the FC kernel takes of 128 k -- eight of each 32 -- lies together; scales and sums of two rows do)
-        int8_t* codes = a.codes + (place * chunks + c) * 128 + (lane / 2 % 4) * 32 + (lane / 8) * 8 + (lane % 2) * 4;
-        float* sc = a.sc + ((int64_t)tile * groups + c * (128 / G)) * 32 + row / 2 * 4 + row % 2;
+    QuantizedUnit q[CHUNKS];
+#pragma unroll
+    for (int i = 0; i < CHUNKS; i++)
+        if (CHUNKS == 1 || 128 * i < left) q[i] = quantize_unit<G, F16>(v[i], lane, left - 128 * i, a.isum);
+    // (what a lane of the FC kernel for few rows takes of 128 k -- eight of each 32 -- lies together; scales and sums of two rows do)
+    const int mine = few ? (lane / 2 % 4) * 32 + (lane / 8) * 8 + (lane % 2) * 4 : lane * 4 * (F16 ? 2 : 1);
+#pragma unroll 1
+    for (int s = 0; s < a.per_row; s++) {
+        const int64_t to = __shfl_sync(0xffffffffu, code_at, s), sc = __shfl_sync(0xffffffffu, sc_at, s);
+        if (to < 0) continue;
 #pragma unroll
         for (int i = 0; i < CHUNKS; i++)
             if (CHUNKS == 1 || 128 * i < left)
-                quantize_unit<G, F16>(v[i], lane, left - 128 * i, true, a.isum, true, codes + 128 * i, sc + i * (128 / G) * 32, 32, 2);
-    } else {
-        const int64_t size = (int64_t)1 << a.log2tile, per = size << a.sums;
-        int8_t* codes = a.codes + (place * (a.Kg * G) + c * 128 + lane * 4) * (F16 ? 2 : 1);
-        float* sc = a.sc + ((int64_t)tile * a.Kg + c * (128 / G)) * per + row;
-#pragma unroll
-        for (int i = 0; i < CHUNKS; i++)
-            if (CHUNKS == 1 || 128 * i < left)
-                quantize_unit<G, F16>(v[i], lane, left - 128 * i, a.sums, false, false, codes + 128 * i * (F16 ? 2 : 1), sc + i * (128 / G) * per, per, size);
+                store_unit<G, F16>(q[i], lane, few ? 128 / G : (left - 128 * i + G - 1) / G, few || a.sums,
+                                   a.codes + to + mine + 128 * i * (F16 ? 2 : 1), a.sc + sc + i * (128 / G) * per, per, sum_at);
     }
 }
 
@@ -564,8 +577,9 @@ int launch_quant_x_tile(const float* x, int64_t rows, int64_t K, int64_t ldx, in
 int launch_quant_x_group(const GroupQuant& q, int G, bool f16, cudaStream_t s) {
     if (q.rows == 0) return Q4FC_OK;
     const int64_t chunks = (q.Kg * G + 127) / 128;
-    const bool many = q.rows * chunks >= kManyUnits;
-    const int64_t grid = (q.rows + kQxWarps - 1) / kQxWarps * (many ? (chunks + kManyChunks - 1) / kManyChunks : chunks);
+    const int64_t x_rows = q.rows / q.per_row;
+    const bool many = x_rows * chunks >= kManyUnits;
+    const int64_t grid = (x_rows + kQxWarps - 1) / kQxWarps * (many ? (chunks + kManyChunks - 1) / kManyChunks : chunks);
     if (grid > 0x7fffffffLL) {
         set_error("quant_x: %lld x %lld exceeds the grid limit", (long long)q.rows, (long long)q.K);
         return Q4FC_ELIMIT;

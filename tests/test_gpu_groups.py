@@ -30,8 +30,9 @@ def check_plan(groups, ids, n):
         assert words[i] == len(want)
         assert np.array_equal(words[at: at + 4 * len(want)].reshape(-1, 4), np.array(want, np.int64).reshape(-1, 4))
         at += 4 * (flat.size // size + min(n, flat.size))
-    assert np.array_equal(words[at: at + flat.size], key[order])
-    at += (flat.size + 3) // 4 * 4
+    for want in (key, np.argsort(order)):  # the group and the place of each row
+        assert np.array_equal(words[at: at + flat.size], want)
+        at += (flat.size + 3) // 4 * 4
     for size in (8, 16, 64, 128):
         assert np.array_equal(words[at: at + n + 1], np.cumsum(np.append(0, -(-np.diff(offsets) // size))))
         at += (n + 4) // 4 * 4
