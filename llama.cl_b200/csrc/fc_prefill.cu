@@ -348,11 +348,11 @@ __global__ void __launch_bounds__(PrefillShape<FMT, G, TM, FOLD>::kThreads, TM =
     int n_tile = (int)(blockIdx.x / cs) + p.n_off, m_tile = (int)blockIdx.y + p.m_off;
     if (n_tile >= p.n_tiles) n_tile -= p.n_tiles, m_tile++;
     if (m_tile > p.m_end || (m_tile == p.m_end && n_tile >= p.n_end)) return;  // (the whole cluster)
-    if (GROUPED && m_tile >= __ldcg(p.tile_count)) {
+    const RowTile tile = row_tile<GROUPED, TM>(p, m_tile);
+    if (GROUPED && tile.live == 0) {
         if (m_tile == 0) pdl_wait_prior_grid();  // no tile at all: this launch's end still stands for the quantizer's
         return;
     }
-    const RowTile tile = row_tile<GROUPED, TM>(p, m_tile);
     const int64_t n0 = (int64_t)n_tile * kTileN, m0 = tile.m0;
     const int live = tile.live;  // rows of this tile that exist
     const int nstage = (p.Kg + GPS - 1) / GPS;
@@ -401,6 +401,7 @@ __global__ void __launch_bounds__(PrefillShape<FMT, G, TM, FOLD>::kThreads, TM =
         if (iters == 0) pdl_wait_prior_grid();  // no K group: nothing else orders the stores behind earlier work
         // chunks of 16 rows are dealt out to the warps of a quarter in turn, so that few rows still occupy all of them
         const bool live0 = cgrp * 16 < live, live1 = (cgrp + CGN) * 16 < live;
+        [[maybe_unused]] const int rows_y[2] = {y_rows<GROUPED>(p, tile, cgrp * 16, 1), y_rows<GROUPED>(p, tile, (cgrp + CGN) * 16, 1)};
 #pragma unroll
         for (int i = 0; i < 8; i++) acc[0][i] = acc[1][i] = 0ull;
         const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16) + cgrp * 16;
@@ -493,7 +494,7 @@ __global__ void __launch_bounds__(PrefillShape<FMT, G, TM, FOLD>::kThreads, TM =
         }
         if (cs == 1) {
             const int64_t n = n0 + nrow;
-            if (n < p.N && !*abort_flag) {
+            if (GROUPED ? !*abort_flag : n < p.N && !*abort_flag) {  // (GROUPED: the lanes tell one another their rows)
                 const float ws = FMT == kQ8C ? __ldg(p.wscales + n) : 1.0f;
 #pragma unroll
                 for (int h = 0; h < 2; h++) {
@@ -504,8 +505,9 @@ __global__ void __launch_bounds__(PrefillShape<FMT, G, TM, FOLD>::kThreads, TM =
                         float lo, hi;
                         unpack2(acc[h][j], lo, hi);
                         if (GROUPED) {
-                            if (mc + 2 * j < live) y_row<GROUPED>(p, m0 + mc + 2 * j)[n] = lo;
-                            if (mc + 2 * j + 1 < live) y_row<GROUPED>(p, m0 + mc + 2 * j + 1)[n] = hi;
+                            const int64_t y0 = __shfl_sync(0xffffffffu, rows_y[h], 2 * j), y1 = __shfl_sync(0xffffffffu, rows_y[h], 2 * j + 1);
+                            if (n < p.N && mc + 2 * j < live) p.y[y0 * p.ldy + n] = lo;
+                            if (n < p.N && mc + 2 * j + 1 < live) p.y[y1 * p.ldy + n] = hi;
                             continue;
                         }
                         if (FMT == kQ8C) lo = __fmul_rn(ws, lo), hi = __fmul_rn(ws, hi);
@@ -695,8 +697,10 @@ __global__ void __launch_bounds__(PrefillShape<FMT, G, TM, FOLD>::kThreads, TM =
         if (warp < kUnpackWarp && !*abort_flag) {
             // rows rank, rank + cs, ... of the tile: the partial sums of all ranks in rank order
             const float* red = reinterpret_cast<const float*>(smem);
+            [[maybe_unused]] const int rows_y = y_rows<GROUPED>(p, tile, rank + cs * warp, cs * S::kEpiWarps);
 #pragma unroll 1
-            for (int m = rank + cs * warp; m < live; m += cs * S::kEpiWarps) {
+            for (int m = rank + cs * warp, i = 0; m < live; m += cs * S::kEpiWarps, i++) {
+                const int64_t row = GROUPED ? __shfl_sync(0xffffffffu, rows_y, i) : m0 + m;
                 uint64_t sum[2] = {}, rest[2] = {};  // columns lane, lane + 32 and lane + 64, lane + 96
 #pragma unroll 1
                 for (int q = 0; q < cs; q++) {
@@ -721,7 +725,7 @@ __global__ void __launch_bounds__(PrefillShape<FMT, G, TM, FOLD>::kThreads, TM =
                 for (int c = 0; c < 4; c++) {
                     const int64_t n = n0 + lane + 32 * c;
                     if (n < p.N)
-                        y_row<GROUPED>(p, m0 + m)[n] = FMT == kQ8C ? __fmul_rn(__ldg(p.wscales + n), out[c]) : out[c];
+                        p.y[row * p.ldy + n] = FMT == kQ8C ? __fmul_rn(__ldg(p.wscales + n), out[c]) : out[c];
                 }
             }
         }

@@ -211,11 +211,11 @@ __global__ void __launch_bounds__(kThreads, 1) fc_prefill_wide_kernel(const Pref
     int n_tile = (int)(blockIdx.x / cs) + p.n_off, m_tile = (int)blockIdx.y + p.m_off;
     if (n_tile >= p.n_tiles) n_tile -= p.n_tiles, m_tile++;
     if (m_tile > p.m_end || (m_tile == p.m_end && n_tile >= p.n_end)) return;  // (the whole cluster)
-    if (GROUPED && m_tile >= __ldcg(p.tile_count)) {
+    const RowTile tile = row_tile<GROUPED, TM>(p, m_tile);
+    if (GROUPED && tile.live == 0) {
         if (m_tile == 0) pdl_wait_prior_grid();  // no tile at all: this launch's end still stands for the quantizer's
         return;
     }
-    const RowTile tile = row_tile<GROUPED, TM>(p, m_tile);
     const int64_t n0 = (int64_t)n_tile * kTileN, m0 = tile.m0;
     const int live = tile.live;  // rows of this tile that exist
     const int nstage = (p.Kg + GPS - 1) / GPS;
@@ -274,6 +274,10 @@ __global__ void __launch_bounds__(kThreads, 1) fc_prefill_wide_kernel(const Pref
         if (iters == 0) pdl_wait_prior_grid();  // no K group: nothing else orders the stores behind earlier work
         // chunks are dealt out to the two warps of a quarter in turn, so that few rows still occupy both
         const int mine = min(kChunks, max(0, (live + W - 1) / W - half + 1) / 2);
+        [[maybe_unused]] int rows_y[kChunks];
+        if constexpr (GROUPED)
+#pragma unroll
+            for (int c = 0; c < kChunks; c++) rows_y[c] = y_rows<GROUPED>(p, tile, (half + 2 * c) * W, 1);
 #pragma unroll
         for (int c = 0; c < kChunks; c++)
 #pragma unroll
@@ -424,7 +428,7 @@ __global__ void __launch_bounds__(kThreads, 1) fc_prefill_wide_kernel(const Pref
             if (iters > p.fold * kPerFold) sums([](ulonglong2& s, uint64_t& a, uint64_t& b) { a = fadd2(s.x, a), b = fadd2(s.y, b); });
         if (cs == 1) {
             const int64_t n = n0 + nrow;
-            if (n < p.N && !*aborted) {
+            if (GROUPED ? !*aborted : n < p.N && !*aborted) {  // (GROUPED: the lanes tell one another their rows)
 #pragma unroll
                 for (int h = 0; h < kChunks; h++) {
                     const int mc = (half + 2 * h) * W;
@@ -434,8 +438,9 @@ __global__ void __launch_bounds__(kThreads, 1) fc_prefill_wide_kernel(const Pref
                         float lo, hi;
                         unpack2(acc[h][j], lo, hi);
                         if (GROUPED) {
-                            if (mc + 2 * j < live) y_row<GROUPED>(p, m0 + mc + 2 * j)[n] = lo;
-                            if (mc + 2 * j + 1 < live) y_row<GROUPED>(p, m0 + mc + 2 * j + 1)[n] = hi;
+                            const int64_t y0 = __shfl_sync(0xffffffffu, rows_y[h], 2 * j), y1 = __shfl_sync(0xffffffffu, rows_y[h], 2 * j + 1);
+                            if (n < p.N && mc + 2 * j < live) p.y[y0 * p.ldy + n] = lo;
+                            if (n < p.N && mc + 2 * j + 1 < live) p.y[y1 * p.ldy + n] = hi;
                             continue;
                         }
                         if (mc + 2 * j < live) *dst = lo;
@@ -577,8 +582,10 @@ __global__ void __launch_bounds__(kThreads, 1) fc_prefill_wide_kernel(const Pref
         if (warp < kEpiWarps && !*aborted) {
             // rows rank, rank + cs, ... of the tile: the partial sums of all ranks in rank order
             const float* red = reinterpret_cast<const float*>(smem);
+            [[maybe_unused]] const int rows_y = y_rows<GROUPED>(p, tile, rank + cs * warp, cs * kEpiWarps);
 #pragma unroll 1
-            for (int m = rank + cs * warp; m < live; m += cs * kEpiWarps) {
+            for (int m = rank + cs * warp, i = 0; m < live; m += cs * kEpiWarps, i++) {
+                const int64_t row = GROUPED ? __shfl_sync(0xffffffffu, rows_y, i) : m0 + m;
                 uint64_t sum[2] = {};  // columns lane, lane + 32 and lane + 64, lane + 96
 #pragma unroll 1
                 for (int q = 0; q < cs; q++) {
@@ -594,7 +601,7 @@ __global__ void __launch_bounds__(kThreads, 1) fc_prefill_wide_kernel(const Pref
 #pragma unroll
                 for (int c = 0; c < 4; c++) {
                     const int64_t n = n0 + lane + 32 * c;
-                    if (n < p.N) y_row<GROUPED>(p, m0 + m)[n] = out[c];
+                    if (n < p.N) p.y[row * p.ldy + n] = out[c];
                 }
             }
         }

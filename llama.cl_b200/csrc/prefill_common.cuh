@@ -44,21 +44,25 @@ struct RowTile {
     int64_t m0;
     int live;
 };
+// GROUPED: none (live 0) where the plan has fewer tiles.
 template <bool GROUPED, int TM>
 __device__ __forceinline__ RowTile row_tile(const PrefillParams& p, int m_tile) {
     if constexpr (GROUPED) {
-        const int4 t = __ldcg(p.tiles + m_tile);
-        return {p.wq + t.x * p.group_bytes, t.y, t.z};
+        const int4 t = __ldcg(p.tiles + m_tile);  // (beyond the count: nothing that is used)
+        return {p.wq + t.x * p.group_bytes, t.y, m_tile < __ldcg(p.tile_count) ? t.z : 0};
     } else {
         const int64_t m0 = (int64_t)m_tile * TM;
         return {p.wq, m0, (int)min((int64_t)TM, p.rows - m0)};
     }
 }
-// row m of the codes in y
+// GROUPED: the rows of y that a thread's stores go to, asked for by the lanes of its warp long before: lane i knows that of row `first` +
+// step * i of the tile.  (Asked for store by store, each takes its way to L2 and back: 2 x 512 rows x 4096 x 22016 402 us, so XX.)
 template <bool GROUPED>
-__device__ __forceinline__ float* y_row(const PrefillParams& p, int64_t m) {
-    return p.y + (GROUPED ? (int64_t)__ldcg(p.order + m) : m) * p.ldy;
+__device__ __forceinline__ int y_rows(const PrefillParams& p, const RowTile& tile, int first, int step) {
+    const int row = first + step * (int)(threadIdx.x & 31);
+    return GROUPED && row < tile.live ? __ldcg(p.order + tile.m0 + row) : 0;
 }
+
 // one lane of a converged warp.  (The compiler knows that exactly one lane runs the branch and keeps descriptors in
 // uniform registers; behind `lane == 0` it cannot, and issuing an MMA takes about a third longer.)
 __device__ __forceinline__ bool elect_one() {
