@@ -514,7 +514,10 @@ int launch_few(FewParams p, const DeviceInfo* di, cudaStream_t s) {
 
 }  // namespace
 
-bool experts_few_serves(int64_t rows, int64_t n) { return rows <= 32 * n && most_tiles(kTiles16, rows, n) <= kMostTiles; }
+// Up to 48 rows an expert in the mean with group 32, up to 14 with group 128, whose 64-row tiles on tcgen05 have a quarter of the groups to
+// scale.  This kernel and those tiles, us, whole call, 32 experts x 2048 x 2048: group 32, 16 rows 49 and 72, 32 rows 80 and 94, 48
+// rows 111 and 108; group 128, 12 rows 32 and 38, 16 rows 45 and 39; 8 x 4096 x 8192, 48 rows 184 and 186; 12 rows 47 and 62, 16 rows 66 and 64.
+bool experts_few_serves(int64_t rows, int G, int64_t n) { return rows <= (G == 32 ? 48 : 14) * n && most_tiles(kTiles16, rows, n) <= kMostTiles; }
 
 size_t experts_few_scratch(int64_t rows, int64_t Kg, int G, int64_t n) {
     const int64_t chunks = (Kg * G + 127) / 128;
