@@ -465,7 +465,7 @@ void* plan_of(PyObject* o, int64_t rows, int64_t n_groups, const at::Device& dev
     return t.data_ptr();
 }
 
-// fc_experts(input, wei_quantized, N, ids, n_groups, most_rows, plan, weights, silu_mul, nibble_signed, out)
+// fc_experts(input, wei_quantized, N, ids, n_groups, distinct, plan, weights, silu_mul, nibble_signed, out)
 PyObject* fc_experts(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (!nargs_ok(n, 11)) return nullptr;
     FRONT_BEGIN
@@ -489,7 +489,7 @@ PyObject* fc_experts(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (as_int(a[4]) != c.experts)
         fail("groups: a plan of " + std::to_string(as_int(a[4])) + " groups for " + std::to_string(c.experts) + " experts");
     if (c.top_k < 1) fail("groups: ids without a slot");
-    c.most_rows = as_int(a[5]);
+    c.most_rows = truth(a[5]) ? c.tokens : 0;
     c10::cuda::CUDAGuard guard(x.device());
     c.groups = plan_of(a[6], c.tokens * c.top_k, c.experts, x.device());
     at::DimVector shape(ids.sizes().begin(), ids.sizes().end());

@@ -109,7 +109,12 @@ struct LoraCall {
     void* scratch;
 };
 size_t lora_scratch_bytes(int64_t rows, int64_t rank);
-int launch_lora_shrink(const LoraCall& c, cudaStream_t s);  // the scratch holds A x for expand
-int launch_lora_expand(const LoraCall& c, cudaStream_t s);
+struct QuantPre;  // quant_pre.cuh
+int launch_lora_add(const LoraCall& c, cudaStream_t s);
+// around a decode FC (rows <= 8): in front of it, y of the adapters alone and the FC's quantized input
+int launch_lora_first(const LoraCall& c, const QuantPre& q, cudaStream_t s);
+// around a launch that computes y from x, between them: y is complete where what is in front of that launch is
+int launch_lora_before(const LoraCall& c, cudaStream_t s);
+int launch_lora_behind(const LoraCall& c, cudaStream_t s);
 
 }  // namespace q4fc

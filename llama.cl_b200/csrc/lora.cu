@@ -2,10 +2,10 @@
 // call in groups (groups.cuh).  No counterpart in the reference.  x is not quantized; A_i [rank][K] and B_i [N][rank] are
 // fp32, fp16 or bf16 as the adapter was trained.
 //
-// Two launches, around whatever computes y:
 //   shrink: t = scale_i * A_i x, a cluster per tile of the plan's rows and 64 ranks; its CTAs divide K, and their sums meet in
 //           shared memory, in order.
 //   expand: y += B_i t.
+// With few rows one launch does both; with many, shrink is a launch in front of the projection and expand one behind it.
 // Both on mma.sync.m16n8k8 (tf32 operands, fp32 sums), the adapter's rows on the 16-row side and the call's rows on the
 // 8-column side.  A tf32 operand keeps 11 bits: fp16 and bf16 weights are exact in one, an fp32 number is two (its first 11
 // bits and the next 11), so that a product costs two MMAs, or three with fp32 weights, and is off by 2^-20 at most.
@@ -17,6 +17,7 @@
 #include <cfloat>
 
 #include "groups.cuh"
+#include "quant_pre.cuh"
 
 namespace cg = cooperative_groups;
 
@@ -85,30 +86,16 @@ struct LoraArgs {
     const int4* tiles;
     const int *tile_count, *order;
     int64_t rows, K, ldx, N, ldy, slice_k;
-    int rank;
+    int rank, n;
+    const int* offsets;
 };
 
-// TILE rows: 64, eight warps with eight rows each, or 8, eight warps that divide the slice's K.  MB: 16-rank blocks in use.
-template <typename T, int TILE, int MB, bool VEC>
-__global__ void __launch_bounds__(kThreads, 2) lora_shrink_kernel(const __grid_constant__ LoraArgs p) {
-    constexpr bool kByK = TILE == 8;
-    constexpr int kRanks = MB * 16;
-    __shared__ float sums[TILE * kRanks];                     // this CTA's [row][rank]
-    __shared__ float by_warp[kByK ? kWarps * TILE * kRanks : 1];
-    cg::cluster_group cluster = cg::this_cluster();
-    pdl_wait_prior_grid();
-    pdl_launch_dependents();
-    const int4 tile = __ldcg(p.tiles + blockIdx.y);  // (beyond the count: nothing that is used)
-    if ((int)blockIdx.y >= __ldcg(p.tile_count)) return;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int row0 = kByK ? 0 : warp * 8;
-    const int rank0 = blockIdx.z * kRankBlock;
-    const int64_t k_begin = blockIdx.x * p.slice_k, k_end = min(p.K, k_begin + p.slice_k);
-    const bool live = row0 + g < tile.z;
-    const float* x = p.x + (live ? (int64_t)__ldcg(p.order + tile.y + row0 + g) * p.ldx : 0);
-    const T* a = static_cast<const T*>(p.a) + ((int64_t)tile.x * p.rank + rank0) * p.K;
-    float acc[MB][4] = {};
-    constexpr int64_t kStep = kByK ? kWarps * 32 : 32;
+// A_i x of eight rows and MB times 16 ranks, by one warp: pieces of 32 k from k0 on, `step` apart, up to k_end.  `x`: the row of lane (g, t)'s
+// g, if `live`; `ranks`: of A that are there.  acc[m][i]: rank m * 16 + 8 (i / 2) + g of row 2t + i % 2.
+template <typename T, int MB, bool VEC>
+__device__ __forceinline__ void shrink_rows(const float* x, bool live, const T* a, int ranks, int64_t K, int64_t k0, int64_t k_end, int64_t step,
+                                            float (&acc)[MB][4]) {
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     struct Piece {
         float v[8];
         T w[MB][2][8];
@@ -121,7 +108,7 @@ __global__ void __launch_bounds__(kThreads, 2) lora_shrink_kernel(const __grid_c
 #pragma unroll
             for (int h = 0; h < 2; h++) {
                 const int r = m * 16 + h * 8 + g;
-                load_values<8, VEC>(a + (int64_t)r * p.K + k, rank0 + r < p.rank ? valid : 0, c.w[m][h]);
+                load_values<8, VEC>(a + (int64_t)r * K + k, r < ranks ? valid : 0, c.w[m][h]);
             }
     };
     auto multiply = [&](const Piece& c) {
@@ -142,22 +129,249 @@ __global__ void __launch_bounds__(kThreads, 2) lora_shrink_kernel(const __grid_c
     // pieces on their way while one is multiplied, as the registers allow
     constexpr int kDepth = !VEC || MB * sizeof(T) > 8 ? 1 : MB * sizeof(T) > 4 ? 2 : 3;
     Piece c[kDepth];
-    int64_t k0 = row0 < tile.z ? k_begin + (kByK ? warp * 32 : 0) : k_end;
     if constexpr (kDepth > 1) {
 #pragma unroll
         for (int d = 0; d + 1 < kDepth; d++)
-            if (k0 + d * kStep < k_end) load(k0 + d * kStep, c[d]);
+            if (k0 + d * step < k_end) load(k0 + d * step, c[d]);
     }
     while (k0 < k_end) {
 #pragma unroll
         for (int d = 0; d < kDepth; d++) {
             if (k0 >= k_end) break;
-            if (k0 + (kDepth - 1) * kStep < k_end) load(k0 + (kDepth - 1) * kStep, c[(d + kDepth - 1) % kDepth]);
+            if (k0 + (kDepth - 1) * step < k_end) load(k0 + (kDepth - 1) * step, c[(d + kDepth - 1) % kDepth]);
             multiply(c[d]);
-            k0 += kStep;
+            k0 += step;
         }
     }
-    // acc[m][i]: rank m * 16 + 8 (i / 2) + g of row 2t + i % 2
+}
+
+// y += B t, or without `onto` y = B t, by one warp: 16 columns of NB times eight rows at a time, the next kAcross further; what the next
+// ones need of y and of B's first ranks is on its way meanwhile.  t is in shared memory, as the MMAs want it: two ranks of a row in 16
+// bytes, {hi, hi, lo, lo}, those that a lane reads in turn 64 bytes apart, rows `pitch` apart.
+// QUADS: fours of ranks that a lane takes of a piece of 16 ranks (1, for at most 16) or 32 (2); PIECES of these at a time.
+__host__ __device__ constexpr int expand_pitch(int ranks) { return ranks * 8 / 128 * 128 + 64 + (ranks * 8 % 128 > 64 ? 128 : 0); }  // bytes
+template <typename T, int QUADS, int PIECES, int NB, int kAcross, bool VEC>
+struct Columns {
+    static constexpr int NV = 4 * QUADS, kPiece = 4 * NV, kChunk = kPiece * PIECES;  // values of a lane, ranks of a piece, ranks at a time
+    struct Next {
+        T w[PIECES][2][NV];
+        float2 y[NB][2];
+    };
+    const T* b;        // of this lane's first column
+    float* y_at[NB][2];  // row nb * 8 + 2t + i at the lane's columns n and n + 1; null: none
+    int64_t n, N;
+    int rank, live;    // live: blocks of eight rows that have any
+    bool y_vec, onto;
+    Next c[2];
+
+    // where pair i of a row's ranks stands in it
+    static __device__ __forceinline__ int place(int i) {
+        constexpr int kPairs = kPiece / 2, kOf = NV / 2;  // pair (NV / 2) t + j of a piece: at 4 j + t
+        const int in = i % kPairs;
+        return i / kPairs * kPairs + in % kOf * 4 + in / kOf;
+    }
+    // rows of the tile from `row0` of its place on, columns from n0 on
+    __device__ __forceinline__ void begin(const LoraArgs& p, int4 tile, int rows, int row0, int64_t n0, bool vec, bool add) {
+        const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+        n = n0 + 2 * g, N = p.N, rank = p.rank, live = (rows - row0 + 7) / 8, y_vec = vec, onto = add;
+#pragma unroll
+        for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                const int row = row0 + nb * 8 + 2 * t + i;
+                y_at[nb][i] = row < rows ? p.y + (int64_t)__ldcg(p.order + tile.y + row) * p.ldy + n : nullptr;
+            }
+        b = static_cast<const T*>(p.b) + ((int64_t)tile.x * p.N + n) * p.rank + NV * t;
+    }
+    __device__ __forceinline__ void load_b(int ahead, int r0, T (&w)[PIECES][2][NV]) {
+        const T* from = b + ahead * kAcross * (int64_t)rank;
+        const int t = threadIdx.x & 3;
+#pragma unroll
+        for (int q = 0; q < PIECES; q++)
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const int r = r0 + q * kPiece;
+                load_values<NV, VEC>(from + h * rank + r, n + ahead * kAcross + h < N ? rank - r - NV * t : 0, w[q][h]);
+            }
+    }
+    __device__ __forceinline__ void load_y(int ahead, Next& c) {
+        const int64_t m = n + ahead * kAcross;
+#pragma unroll
+        for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                const float* from = y_at[nb][i] + ahead * kAcross;
+                float2 v = make_float2(0.0f, 0.0f);
+                if (onto && y_at[nb][i] != nullptr) {
+                    if (y_vec && m + 1 < N) {
+                        v = __ldcg(reinterpret_cast<const float2*>(from));
+                    } else {
+                        if (m < N) v.x = __ldcg(from);
+                        if (m + 1 < N) v.y = __ldcg(from + 1);
+                    }
+                }
+                c.y[nb][i] = v;
+            }
+    }
+    __device__ __forceinline__ void finish(Next& c, const uint4* ts, int pitch) {
+        float acc[NB][4];
+#pragma unroll
+        for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) acc[nb][j] = 0.0f;
+        const int lane = threadIdx.x & 31;
+#pragma unroll 1
+        for (int r0 = 0; r0 < rank; r0 += kChunk) {
+            if (r0 > 0) load_b(0, r0, c.w);
+            const uint4* mine = ts + (lane >> 2) * pitch + r0 / 2 + (lane & 3);
+#pragma unroll
+            for (int q = 0; q < PIECES; q++)
+#pragma unroll
+                for (int j = 0; j < NV / 2; j++) {
+                    uint32_t wh[4], wl[4];
+                    operand(c.w[q][0][2 * j], c.w[q][1][2 * j], c.w[q][0][2 * j + 1], c.w[q][1][2 * j + 1], wh, wl);
+#pragma unroll
+                    for (int nb = 0; nb < NB; nb++) {
+                        if (nb >= live) break;
+                        const uint4 u = mine[nb * 8 * pitch + q * (kPiece / 2) + 4 * j];
+                        if constexpr (sizeof(T) == 4) mma_tf32(acc[nb], wl, u.x, u.y);
+                        mma_tf32(acc[nb], wh, u.z, u.w);
+                        mma_tf32(acc[nb], wh, u.x, u.y);
+                    }
+                }
+        }
+        // acc[nb][i]: column n + i / 2 of row nb * 8 + 2t + i % 2
+#pragma unroll
+        for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                if (y_at[nb][i] == nullptr) continue;
+                const float2 v = make_float2(c.y[nb][i].x + acc[nb][i], c.y[nb][i].y + acc[nb][i + 2]);
+                if (y_vec && n + 1 < N) {
+                    *reinterpret_cast<float2*>(y_at[nb][i]) = v;
+                } else {
+                    if (n < N) y_at[nb][i][0] = v.x;
+                    if (n + 1 < N) y_at[nb][i][1] = v.y;
+                }
+                y_at[nb][i] += kAcross;
+            }
+        n += kAcross, b += kAcross * (int64_t)rank;
+    }
+    // `times` of them; the first one's B and y have been asked for into c[0]
+    __device__ __forceinline__ void run(int64_t times, const uint4* ts, int pitch) {
+#pragma unroll 1
+        for (int64_t k = 0; k < times; k += 2) {
+            if (k + 1 < times) load_b(1, 0, c[1].w), load_y(1, c[1]);
+            finish(c[0], ts, pitch);
+            if (k + 1 >= times) break;
+            if (k + 2 < times) load_b(1, 0, c[0].w), load_y(1, c[0]);
+            finish(c[1], ts, pitch);
+        }
+    }
+};
+// rows without an adapter, from the first-th on
+__device__ __forceinline__ void zero_rows(const LoraArgs& p, int64_t first, int64_t step, int64_t n_begin, int64_t n_end) {
+    for (int64_t i = __ldcg(p.offsets + p.n) + first; i < p.rows; i += step) {
+        float* y = p.y + (int64_t)__ldcg(p.order + i) * p.ldy;
+        for (int64_t n = n_begin + threadIdx.x; n < n_end; n += kThreads) y[n] = 0.0f;
+    }
+}
+
+// ---- few rows and up to 64 ranks: both products in one launch ---------------------------------------------------------------------------
+// A cluster per tile of eight rows: its CTAs divide K (and their warps that again), their sums meet in every one of them, and then they
+// divide the columns.  With `early` the launch in front computes y alone: all else is complete, and the first product does not wait
+// for it.  CTAs behind those of the tiles quantize x for the decode FC (quant_pre.cuh), which has to be done in front of it anyway.
+template <typename T, int MB, bool VEC>
+__global__ void __launch_bounds__(kThreads, 2) lora_few_kernel(const __grid_constant__ LoraArgs p, const __grid_constant__ QuantPre q, const bool y_vec,
+                                                               const bool onto, const bool early) {
+    constexpr int kRanks = MB * 16, QUADS = MB == 1 ? 1 : 2, PIECES = MB == 4 && sizeof(T) < 4 ? 2 : 1, kAcross = kWarps * 16;
+    using C = Columns<T, QUADS, PIECES, 1, kAcross, VEC>;
+    constexpr int kPitch = expand_pitch((kRanks + C::kChunk - 1) / C::kChunk * C::kChunk) / 16;
+    __shared__ float sums[8 * kRanks];                 // this CTA's [row][rank]
+    __shared__ float by_warp[kWarps * 8 * kRanks];
+    __shared__ uint4 ts[8 * kPitch];
+    cg::cluster_group cluster = cg::this_cluster();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int slices = (int)gridDim.x, here = (int)blockIdx.x;
+    auto others_done = [&] {
+        pdl_wait_prior_grid();
+        pdl_launch_dependents();
+    };
+    if (!early) others_done();
+    if ((int)blockIdx.y >= q.first_block) {
+        quant_pre_block(q, ((int64_t)(blockIdx.y - q.first_block) * slices + here) * kWarps + warp);
+        return;
+    }
+    const int64_t blocks = (p.N + kAcross - 1) / kAcross;
+    const int64_t first = blocks * here / slices, times = blocks * (here + 1) / slices - first;
+    const int4 tile = __ldcg(p.tiles + blockIdx.y);  // (beyond the count: nothing that is used)
+    if ((int)blockIdx.y < __ldcg(p.tile_count)) {
+        const int64_t k_begin = here * p.slice_k, k_end = min(p.K, k_begin + p.slice_k);
+        const bool live = g < tile.z;
+        const float* x = p.x + (live ? (int64_t)__ldcg(p.order + tile.y + g) * p.ldx : 0);
+        float acc[MB][4] = {};
+        shrink_rows<T, MB, VEC>(x, live, static_cast<const T*>(p.a) + (int64_t)tile.x * p.rank * p.K, p.rank, p.K, k_begin + warp * 32, k_end, kWarps * 32, acc);
+        float* mine = by_warp + warp * 8 * kRanks;
+#pragma unroll
+        for (int m = 0; m < MB; m++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) mine[(2 * t + i % 2) * kRanks + m * 16 + 8 * (i / 2) + g] = acc[m][i];
+        __syncthreads();
+        for (int i = threadIdx.x; i < 8 * kRanks; i += kThreads) {
+            float sum = 0.0f;
+#pragma unroll
+            for (int w = 0; w < kWarps; w++) sum += by_warp[w * 8 * kRanks + i];
+            sums[i] = sum;
+        }
+        if (early) others_done();
+        C cols;
+        cols.begin(p, tile, tile.z, 0, (first * kWarps + warp) * 16, y_vec, onto);
+        if (times > 0) cols.load_b(0, 0, cols.c[0].w), cols.load_y(0, cols.c[0]);
+        cluster.sync();
+        const float scale = p.scales ? p.scales[tile.x] : 1.0f;
+        for (int i = threadIdx.x; i < 8 * kRanks / 2; i += kThreads) {
+            const int row = i / (kRanks / 2), r = i % (kRanks / 2) * 2;
+            float v[2] = {0.0f, 0.0f};
+            for (int s = 0; s < slices; s++) {
+                const float2 o = *reinterpret_cast<const float2*>(cluster.map_shared_rank(sums, s) + row * kRanks + r);
+                v[0] += o.x, v[1] += o.y;
+            }
+            uint4 u;
+            split(v[0] * scale, u.x, u.z), split(v[1] * scale, u.y, u.w);
+            ts[row * kPitch + C::place(r / 2)] = u;
+        }
+        __syncthreads();
+        cols.run(times, ts, kPitch);
+        cluster.sync();  // nobody leaves while its sums are being read
+    } else if (early) {
+        others_done();
+    }
+    if (!onto) zero_rows(p, blockIdx.y, q.first_block, first * kAcross, min(p.N, (first + times) * kAcross));
+}
+
+// ---- more rows, or more ranks: two launches ---------------------------------------------------------------------------------------------
+// TILE rows: 64, eight warps with eight rows each, or 8, eight warps that divide the slice's K.  MB: 16-rank blocks in use.
+template <typename T, int TILE, int MB, bool VEC>
+__global__ void __launch_bounds__(kThreads, 2) lora_shrink_kernel(const __grid_constant__ LoraArgs p) {
+    constexpr bool kByK = TILE == 8;
+    constexpr int kRanks = MB * 16;
+    __shared__ float sums[TILE * kRanks];                     // this CTA's [row][rank]
+    __shared__ float by_warp[kByK ? kWarps * TILE * kRanks : 1];
+    cg::cluster_group cluster = cg::this_cluster();
+    pdl_wait_prior_grid();
+    pdl_launch_dependents();
+    const int4 tile = __ldcg(p.tiles + blockIdx.y);  // (beyond the count: nothing that is used)
+    if ((int)blockIdx.y >= __ldcg(p.tile_count)) return;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int row0 = kByK ? 0 : warp * 8;
+    const int rank0 = blockIdx.z * kRankBlock;
+    const int64_t k_begin = blockIdx.x * p.slice_k, k_end = min(p.K, k_begin + p.slice_k);
+    const bool live = row0 + g < tile.z;
+    const float* x = p.x + (live ? (int64_t)__ldcg(p.order + tile.y + row0 + g) * p.ldx : 0);
+    float acc[MB][4] = {};
+    if (row0 < tile.z)
+        shrink_rows<T, MB, VEC>(x, live, static_cast<const T*>(p.a) + ((int64_t)tile.x * p.rank + rank0) * p.K, p.rank - rank0, p.K,
+                                k_begin + (kByK ? warp * 32 : 0), k_end, kByK ? kWarps * 32 : 32, acc);
     float* mine = kByK ? by_warp + warp * TILE * kRanks : sums + row0 * kRanks;
 #pragma unroll
     for (int m = 0; m < MB; m++)
@@ -184,24 +398,27 @@ __global__ void __launch_bounds__(kThreads, 2) lora_shrink_kernel(const __grid_c
     cluster.sync();  // nobody leaves while its sums are being read
 }
 
-// y += B t.  The work is pieces of 32 rows of a tile and 64 columns, or of its eight rows and 128, the columns of a tile one behind
-// another; a CTA takes a contiguous share of what the plan has.  A warp takes 16 columns of 16 or 8 rows at a time; what the next piece
-// needs of y and of B's first ranks is on its way meanwhile.  t of a tile is in shared memory, as the MMAs want it: two ranks of a row in 16 bytes, {hi,
-// hi, lo, lo}, those that a lane reads in turn 64 bytes apart.
-// QUADS: fours of ranks that a lane takes of a piece of 16 ranks (1, for at most 16) or 32 (2); PIECES of these at a time.
+// The work is pieces of 32 rows of a tile and 64 columns, or of its eight rows and 128, the columns of a tile one behind another; a CTA
+// takes a contiguous share of what the plan has.
 __host__ __device__ constexpr int expand_rows(int tile) { return tile < 32 ? tile : 32; }
 __host__ __device__ constexpr int expand_columns(int tile) { return tile < 32 ? 128 : 64; }
-__host__ __device__ constexpr int expand_pitch(int ranks) { return ranks * 8 / 128 * 128 + 64 + (ranks * 8 % 128 > 64 ? 128 : 0); }  // bytes
 template <typename T, int TILE, int QUADS, int PIECES, bool VEC>
-__global__ void __launch_bounds__(kThreads, 2) lora_expand_kernel(const __grid_constant__ LoraArgs p, const bool y_vec) {
-    constexpr int NV = 4 * QUADS, kPiece = 4 * NV, kChunk = kPiece * PIECES;  // values of a lane, ranks of a piece, ranks at a time
-    constexpr int kRows = expand_rows(TILE), kParts = TILE / kRows, NB = kRows > 8 ? 2 : 1;
-    constexpr int kAcross = expand_columns(TILE);
+__global__ void __launch_bounds__(kThreads, 2) lora_expand_kernel(const __grid_constant__ LoraArgs p, const bool y_vec, const bool onto) {
+    constexpr int kRows = expand_rows(TILE), kParts = TILE / kRows, NB = kRows > 8 ? 2 : 1, kAcross = expand_columns(TILE);
+    using C = Columns<T, QUADS, PIECES, NB, kAcross, VEC>;
     extern __shared__ uint4 ts[];  // [kRows][pitch]
-    const int chunks = (p.rank + kChunk - 1) / kChunk, pitch = expand_pitch(chunks * kChunk) / 16;
-    pdl_wait_prior_grid();
-    pdl_launch_dependents();
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int pairs = (p.rank + C::kChunk - 1) / C::kChunk * C::kChunk / 2, pitch = expand_pitch(2 * pairs) / 16;
+    // The launches in front, from shrink on, write t and y.  All else was complete when shrink had waited, and this launch begins only
+    // after that: the plan and B need not wait.
+    bool waited = false;
+    auto others_done = [&] {
+        if (!waited) {
+            pdl_wait_prior_grid();
+            pdl_launch_dependents();
+        }
+        waited = true;
+    };
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int64_t blocks = (p.N + kAcross - 1) / kAcross, total = (int64_t)__ldcg(p.tile_count) * kParts * blocks;
     int64_t at = total * blockIdx.x / gridDim.x;
     const int64_t end = total * (blockIdx.x + 1) / gridDim.x;
@@ -212,55 +429,15 @@ __global__ void __launch_bounds__(kThreads, 2) lora_expand_kernel(const __grid_c
         int4 tile = __ldcg(p.tiles + part / kParts);
         tile.y += kRows * (int)(part % kParts), tile.z -= kRows * (int)(part % kParts);  // this piece's rows of it
         if (tile.z <= 0) continue;
-        const int rows = min(tile.z, kRows), row0 = warp * 16 / kAcross * 16, live = (rows - row0 + 7) / 8;  // (this warp's first row)
-        float* y_at[NB][2];  // row row0 + nb * 8 + 2t + i of the piece at this lane's columns n and n + 1; null: none
-        int64_t n = first * kAcross + warp * 16 % kAcross + 2 * g;
-#pragma unroll
-        for (int nb = 0; nb < NB; nb++)
-#pragma unroll
-            for (int i = 0; i < 2; i++) {
-                const int row = row0 + nb * 8 + 2 * t + i;
-                y_at[nb][i] = row < rows ? p.y + (int64_t)__ldcg(p.order + tile.y + row) * p.ldy + n : nullptr;
-            }
-        const T* b = static_cast<const T*>(p.b) + ((int64_t)tile.x * p.N + n) * p.rank + NV * t;
-        auto load_b = [&](const T* b, int64_t n, int r0, T (&w)[PIECES][2][NV]) {
-#pragma unroll
-            for (int q = 0; q < PIECES; q++)
-#pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    const int r = r0 + q * kPiece;
-                    load_values<NV, VEC>(b + h * p.rank + r, n + h < p.N ? p.rank - r - NV * t : 0, w[q][h]);
-                }
-        };
-        struct Next {
-            T w[PIECES][2][NV];
-            float2 y[NB][2];
-        };
-        auto load = [&](int ahead, Next& c) {  // `ahead` pieces further
-            load_b(b + ahead * kAcross * (int64_t)p.rank, n + ahead * kAcross, 0, c.w);
-            const int64_t m = n + ahead * kAcross;
-#pragma unroll
-            for (int nb = 0; nb < NB; nb++)
-#pragma unroll
-                for (int i = 0; i < 2; i++) {
-                    const float* from = y_at[nb][i] + ahead * kAcross;
-                    float2 v = make_float2(0.0f, 0.0f);
-                    if (y_at[nb][i] != nullptr) {
-                        if (y_vec && m + 1 < p.N) {
-                            v = __ldcg(reinterpret_cast<const float2*>(from));
-                        } else {
-                            if (m < p.N) v.x = __ldcg(from);
-                            if (m + 1 < p.N) v.y = __ldcg(from + 1);
-                        }
-                    }
-                    c.y[nb][i] = v;
-                }
-        };
-        Next c[2];
-        load(0, c[0]);
+        const int rows = min(tile.z, kRows), row0 = warp * 16 / kAcross * 16;  // (this warp's first row)
+        C cols;
+        cols.begin(p, tile, rows, row0, first * kAcross + warp * 16 % kAcross, y_vec, onto);
+        cols.load_b(0, 0, cols.c[0].w);
+        others_done();
+        cols.load_y(0, cols.c[0]);
         __syncthreads();  // (nobody reads the piece in front any more)
         for (int row = warp; row < kRows; row += kWarps)
-            for (int i = lane; i < chunks * kChunk / 2; i += 32) {  // pairs of ranks
+            for (int i = lane; i < pairs; i += 32) {
                 float v[2] = {0.0f, 0.0f};
                 if (row < rows) {
                     const float* from = p.t + (int64_t)(tile.y + row) * p.rank + 2 * i;
@@ -269,70 +446,16 @@ __global__ void __launch_bounds__(kThreads, 2) lora_expand_kernel(const __grid_c
                 }
                 uint4 u;
                 split(v[0], u.x, u.z), split(v[1], u.y, u.w);
-                // pair (NV / 2) t + j of a piece stands at place 4 j + t
-                constexpr int kPairs = kPiece / 2, kOf = NV / 2;
-                const int in = i % kPairs;
-                ts[row * pitch + i / kPairs * kPairs + in % kOf * 4 + in / kOf] = u;
+                ts[row * pitch + C::place(i)] = u;
             }
         __syncthreads();
-        float acc[NB][4];
-        auto multiply = [&](int chunk, const T (&w)[PIECES][2][NV]) {
-            const uint4* mine = ts + (row0 + g) * pitch + chunk * (kChunk / 2) + t;
-#pragma unroll
-            for (int q = 0; q < PIECES; q++)
-#pragma unroll
-                for (int j = 0; j < NV / 2; j++) {
-                    uint32_t wh[4], wl[4];
-                    operand(w[q][0][2 * j], w[q][1][2 * j], w[q][0][2 * j + 1], w[q][1][2 * j + 1], wh, wl);
-#pragma unroll
-                    for (int nb = 0; nb < NB; nb++) {
-                        if (nb >= live) break;
-                        const uint4 u = mine[nb * 8 * pitch + q * (kPiece / 2) + 4 * j];
-                        if constexpr (sizeof(T) == 4) mma_tf32(acc[nb], wl, u.x, u.y);
-                        mma_tf32(acc[nb], wh, u.z, u.w);
-                        mma_tf32(acc[nb], wh, u.x, u.y);
-                    }
-                }
-        };
-        auto finish = [&](Next& c) {
-#pragma unroll
-            for (int nb = 0; nb < NB; nb++)
-#pragma unroll
-                for (int j = 0; j < 4; j++) acc[nb][j] = 0.0f;
-            multiply(0, c.w);
-#pragma unroll 1
-            for (int chunk = 1; chunk < chunks; chunk++) {
-                load_b(b, n, chunk * kChunk, c.w);
-                multiply(chunk, c.w);
-            }
-            // acc[nb][i]: column n + i / 2 of row row0 + nb * 8 + 2t + i % 2
-#pragma unroll
-            for (int nb = 0; nb < NB; nb++)
-#pragma unroll
-                for (int i = 0; i < 2; i++) {
-                    if (y_at[nb][i] == nullptr) continue;
-                    const float2 v = make_float2(c.y[nb][i].x + acc[nb][i], c.y[nb][i].y + acc[nb][i + 2]);
-                    if (y_vec && n + 1 < p.N) {
-                        *reinterpret_cast<float2*>(y_at[nb][i]) = v;
-                    } else {
-                        if (n < p.N) y_at[nb][i][0] = v.x;
-                        if (n + 1 < p.N) y_at[nb][i][1] = v.y;
-                    }
-                    y_at[nb][i] += kAcross;
-                }
-            n += kAcross, b += kAcross * (int64_t)p.rank;
-        };
-#pragma unroll 1
-        for (int64_t k = first; k < last; k += 2) {
-            if (k + 1 < last) load(1, c[1]);
-            finish(c[0]);
-            if (k + 1 >= last) break;
-            if (k + 2 < last) load(1, c[0]);
-            finish(c[1]);
-        }
+        cols.run(last - first, ts + row0 * pitch, pitch);
     }
+    others_done();
+    if (!onto) zero_rows(p, blockIdx.x, gridDim.x, 0, p.N);
 }
 
+enum Step { kShrink, kExpand, kExpandOnto };
 struct LoraPlan {
     int which, slices;
     int64_t slice_k, tiles;  // tiles that are likely in use
@@ -352,22 +475,38 @@ LoraPlan lora_plan(int64_t rows, int64_t K, int64_t rank, int64_t n, int sms) {
     return l;
 }
 
+bool shrink_vec(const LoraCall& c) {
+    return c.K % 8 == 0 && c.ldx % 4 == 0 && ((reinterpret_cast<uintptr_t>(c.x) | reinterpret_cast<uintptr_t>(c.a)) & 15) == 0;
+}
+bool expand_vec(const LoraCall& c, int values) { return c.rank % values == 0 && (reinterpret_cast<uintptr_t>(c.b) & 15) == 0; }
+bool rows_vec(const LoraCall& c) { return c.ldy % 2 == 0 && (reinterpret_cast<uintptr_t>(c.y) & 7) == 0; }
+// clusters along x
+struct ClusterLaunch : DependentLaunch {
+    cudaLaunchAttribute attrs[2];
+    ClusterLaunch(dim3 grid, cudaStream_t s) : DependentLaunch(grid, kThreads, s), attrs{attr, {}} {
+        attrs[1].id = cudaLaunchAttributeClusterDimension;
+        attrs[1].val.clusterDim.x = grid.x, attrs[1].val.clusterDim.y = attrs[1].val.clusterDim.z = 1;
+        cfg.attrs = attrs, cfg.numAttrs = 2;
+    }
+};
+template <typename T, int MB>
+int launch_few(const LoraCall& c, const LoraArgs& p, const QuantPre& q, bool onto, bool early, dim3 grid, cudaStream_t s) {
+    ClusterLaunch l(grid, s);
+    auto* fn = shrink_vec(c) && expand_vec(c, MB == 1 ? 4 : 8) ? lora_few_kernel<T, MB, true> : lora_few_kernel<T, MB, false>;
+    Q4FC_CUDA_OK(cudaLaunchKernelEx(&l.cfg, fn, p, q, rows_vec(c), onto, early));
+    return Q4FC_OK;
+}
 template <typename T, int TILE, int MB>
 int launch_shrink(const LoraArgs& p, bool vec, dim3 grid, cudaStream_t s) {
-    DependentLaunch l(grid, kThreads, s);
-    cudaLaunchAttribute attrs[2] = {l.attr, {}};
-    attrs[1].id = cudaLaunchAttributeClusterDimension;
-    attrs[1].val.clusterDim.x = grid.x, attrs[1].val.clusterDim.y = attrs[1].val.clusterDim.z = 1;
-    l.cfg.attrs = attrs, l.cfg.numAttrs = 2;
+    ClusterLaunch l(grid, s);
     Q4FC_CUDA_OK(cudaLaunchKernelEx(&l.cfg, vec ? lora_shrink_kernel<T, TILE, MB, true> : lora_shrink_kernel<T, TILE, MB, false>, p));
     return Q4FC_OK;
 }
 template <typename T, int TILE, int QUADS, int PIECES>
-int launch_expand(const LoraCall& c, const LoraArgs& p, int64_t tiles, cudaStream_t s) {
+int launch_expand(const LoraCall& c, const LoraArgs& p, bool onto, int64_t tiles, cudaStream_t s) {
     const DeviceInfo* di = device_info();
     if (!di) return Q4FC_ECUDA;
-    const bool vec = c.rank % (4 * QUADS) == 0 && (reinterpret_cast<uintptr_t>(c.b) & 15) == 0;
-    const bool y_vec = c.ldy % 2 == 0 && (reinterpret_cast<uintptr_t>(c.y) & 7) == 0;
+    const bool vec = expand_vec(c, 4 * QUADS), y_vec = rows_vec(c);
     constexpr int kChunk = 16 * QUADS * PIECES;
     const int64_t pieces = tiles * (TILE / expand_rows(TILE)) * ((c.N + expand_columns(TILE) - 1) / expand_columns(TILE)), most = 2 * di->sm_count;
     DependentLaunch l(dim3((unsigned)(pieces < most ? pieces : most)), kThreads, s);
@@ -375,46 +514,94 @@ int launch_expand(const LoraCall& c, const LoraArgs& p, int64_t tiles, cudaStrea
     l.cfg.dynamicSmemBytes = expand_rows(TILE) * (size_t)expand_pitch((int)(c.rank + kChunk - 1) / kChunk * kChunk);
     if (l.cfg.dynamicSmemBytes > 48 * 1024)
         Q4FC_CUDA_OK(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)l.cfg.dynamicSmemBytes));
-    Q4FC_CUDA_OK(cudaLaunchKernelEx(&l.cfg, fn, p, y_vec));
+    Q4FC_CUDA_OK(cudaLaunchKernelEx(&l.cfg, fn, p, y_vec, onto));
     return Q4FC_OK;
 }
 template <typename T, int TILE>
-int launch_lora_tile(const LoraCall& c, const LoraArgs& p, const LoraPlan& l, bool expand, int64_t tiles, cudaStream_t s) {
-    if (!expand) {
-        const bool vec = c.K % 8 == 0 && c.ldx % 4 == 0 && ((reinterpret_cast<uintptr_t>(c.x) | reinterpret_cast<uintptr_t>(c.a)) & 15) == 0;
+int launch_lora_tile(const LoraCall& c, const LoraArgs& p, const LoraPlan& l, Step step, int64_t tiles, cudaStream_t s) {
+    if (step == kShrink) {
+        const bool vec = shrink_vec(c);
         const dim3 grid((unsigned)l.slices, (unsigned)tiles, (unsigned)((c.rank + kRankBlock - 1) / kRankBlock));
         if (c.rank <= 16) return launch_shrink<T, TILE, 1>(p, vec, grid, s);
         if (c.rank <= 32) return launch_shrink<T, TILE, 2>(p, vec, grid, s);
         return launch_shrink<T, TILE, 4>(p, vec, grid, s);
     }
-    if (c.rank <= 16) return launch_expand<T, TILE, 1, 1>(c, p, tiles, s);
-    if (c.rank <= 32 || sizeof(T) == 4) return launch_expand<T, TILE, 2, 1>(c, p, tiles, s);
-    return launch_expand<T, TILE, 2, 2>(c, p, tiles, s);
+    if (c.rank <= 16) return launch_expand<T, TILE, 1, 1>(c, p, step == kExpandOnto, tiles, s);
+    if (c.rank <= 32 || sizeof(T) == 4) return launch_expand<T, TILE, 2, 1>(c, p, step == kExpandOnto, tiles, s);
+    return launch_expand<T, TILE, 2, 2>(c, p, step == kExpandOnto, tiles, s);
 }
 template <typename T>
-int launch_lora_type(const LoraCall& c, const LoraArgs& p, const LoraPlan& l, bool expand, int64_t tiles, cudaStream_t s) {
-    return l.which == kTiles8 ? launch_lora_tile<T, 8>(c, p, l, expand, tiles, s) : launch_lora_tile<T, 64>(c, p, l, expand, tiles, s);
+int launch_lora_type(const LoraCall& c, const LoraArgs& p, const LoraPlan& l, Step step, int64_t tiles, cudaStream_t s) {
+    return l.which == kTiles8 ? launch_lora_tile<T, 8>(c, p, l, step, tiles, s) : launch_lora_tile<T, 64>(c, p, l, step, tiles, s);
 }
-int launch_lora(const LoraCall& c, bool expand, cudaStream_t s) {
+int lora_args(const LoraCall& c, LoraPlan* l, LoraArgs* p, int64_t* tiles) {
     const DeviceInfo* di = device_info();
     if (!di) return Q4FC_ECUDA;
-    const LoraPlan l = lora_plan(c.rows, c.K, c.rank, c.n, di->sm_count);
-    const int64_t tiles = most_tiles(l.which, c.rows, c.n);
-    if (tiles > 65535) {
+    *l = lora_plan(c.rows, c.K, c.rank, c.n, di->sm_count);
+    *tiles = most_tiles(l->which, c.rows, c.n);
+    if (*tiles > 65535 / 2) {
         set_error("lora: %lld rows exceed the grid limit", (long long)c.rows);
         return Q4FC_ELIMIT;
     }
-    LoraArgs p = {c.x, c.a, c.b, c.scales, c.y, static_cast<float*>(c.scratch), c.plan.tiles[l.which], c.plan.counts + l.which, c.plan.order,
-                  c.rows, c.K, c.ldx, c.N, c.ldy, l.slice_k, (int)c.rank};
-    if (c.dtype == Q4FC_F32) return launch_lora_type<float>(c, p, l, expand, tiles, s);
-    if (c.dtype == Q4FC_F16) return launch_lora_type<__half>(c, p, l, expand, tiles, s);
-    return launch_lora_type<__nv_bfloat16>(c, p, l, expand, tiles, s);
+    *p = LoraArgs{c.x, c.a, c.b, c.scales, c.y, static_cast<float*>(c.scratch), c.plan.tiles[l->which], c.plan.counts + l->which, c.plan.order,
+                  c.rows, c.K, c.ldx, c.N, c.ldy, l->slice_k, (int)c.rank, (int)c.n, c.plan.offsets};
+    return Q4FC_OK;
+}
+int launch_lora(const LoraCall& c, Step step, cudaStream_t s) {
+    LoraPlan l;
+    LoraArgs p;
+    int64_t tiles;
+    if (int rc = lora_args(c, &l, &p, &tiles)) return rc;
+    if (c.dtype == Q4FC_F32) return launch_lora_type<float>(c, p, l, step, tiles, s);
+    if (c.dtype == Q4FC_F16) return launch_lora_type<__half>(c, p, l, step, tiles, s);
+    return launch_lora_type<__nv_bfloat16>(c, p, l, step, tiles, s);
+}
+// Both products in one launch where each CTA of the second would have few of the columns anyway: 133 rows x 1001 x 2999, fp32, rank 12, with
+// the FC 23.4 and 21.5 us, 8 rows x 4096 x 4096, rank 16, 13.7 and 12.9; but 61 rows x 4096 x 11008, rank 64, 45 and 49.
+bool few(const LoraCall& c) {
+    if (c.rows >= 256 || c.rank > kRankBlock) return false;
+    const DeviceInfo* di = device_info();
+    return di && lora_plan(c.rows, c.K, c.rank, c.n, di->sm_count).tiles * ((c.N + expand_columns(8) - 1) / expand_columns(8)) <= 4 * di->sm_count;
+}
+int launch_lora_few(const LoraCall& c, QuantPre q, bool onto, bool early, cudaStream_t s) {
+    LoraPlan l;
+    LoraArgs p;
+    int64_t tiles;
+    if (int rc = lora_args(c, &l, &p, &tiles)) return rc;
+    q.first_block = (int)tiles;
+    const int64_t warps = (int64_t)l.slices * kWarps, quant = (q.units() + warps - 1) / warps;
+    const dim3 grid((unsigned)l.slices, (unsigned)(tiles + quant));
+    auto with = [&](auto type) {
+        using T = decltype(type);
+        if (c.rank <= 16) return launch_few<T, 1>(c, p, q, onto, early, grid, s);
+        if (c.rank <= 32) return launch_few<T, 2>(c, p, q, onto, early, grid, s);
+        return launch_few<T, 4>(c, p, q, onto, early, grid, s);
+    };
+    if (c.dtype == Q4FC_F32) return with(float{});
+    if (c.dtype == Q4FC_F16) return with(__half{});
+    return with(__nv_bfloat16{});
 }
 
 }  // namespace
 
 size_t lora_scratch_bytes(int64_t rows, int64_t rank) { return (size_t)(rows * rank) * 4; }
-int launch_lora_shrink(const LoraCall& c, cudaStream_t s) { return launch_lora(c, false, s); }
-int launch_lora_expand(const LoraCall& c, cudaStream_t s) { return launch_lora(c, true, s); }
+
+int launch_lora_add(const LoraCall& c, cudaStream_t s) {
+    if (few(c)) return launch_lora_few(c, QuantPre{}, true, false, s);
+    if (int rc = launch_lora(c, kShrink, s)) return rc;
+    return launch_lora(c, kExpandOnto, s);
+}
+
+int launch_lora_first(const LoraCall& c, const QuantPre& q, cudaStream_t s) {
+    if (few(c)) return launch_lora_few(c, q, false, false, s);
+    if (int rc = launch_quant_x_pre(q.x, q.rows, q.K, q.ldx, q.G, q.want_isum, q.codes, q.sc, false, s)) return rc;
+    if (int rc = launch_lora(c, kShrink, s)) return rc;
+    return launch_lora(c, kExpand, s);
+}
+
+int launch_lora_before(const LoraCall& c, cudaStream_t s) { return few(c) ? Q4FC_OK : launch_lora(c, kShrink, s); }
+int launch_lora_behind(const LoraCall& c, cudaStream_t s) {
+    return few(c) ? launch_lora_few(c, QuantPre{}, true, true, s) : launch_lora(c, kExpandOnto, s);
+}
 
 }  // namespace q4fc

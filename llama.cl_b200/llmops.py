@@ -645,12 +645,13 @@ class RowGroups:
     """The rows of a call sorted by the id of the weights they take (``q4fc_groups_*`` format): made by ``group_rows`` or
     ``route_top_k``, and read by every call of a step that shares the choice.
 
-    ``ids``: the ids as given, int32 or int64 of any shape; ``n_groups``; ``most_rows``: no group has more rows."""
+    ``ids``: the ids as given, int32 or int64 of any shape; ``n_groups``; ``distinct``: no two ids of the last dimension are
+    equal (as a router chooses them), so that no group has more rows than the other dimensions."""
 
-    __slots__ = ("ids", "n_groups", "most_rows", "buf")
+    __slots__ = ("ids", "n_groups", "distinct", "buf")
 
-    def __init__(self, ids: torch.Tensor, n_groups: int, most_rows: int, buf: torch.Tensor) -> None:
-        self.ids, self.n_groups, self.most_rows, self.buf = ids, n_groups, most_rows, buf
+    def __init__(self, ids: torch.Tensor, n_groups: int, distinct: bool, buf: torch.Tensor) -> None:
+        self.ids, self.n_groups, self.distinct, self.buf = ids, n_groups, distinct, buf
 
     @property
     def offsets(self) -> torch.Tensor:
@@ -667,8 +668,7 @@ class RowGroups:
 def group_rows(ids: torch.Tensor, n_groups: int) -> RowGroups:
     """Sorts rows by id.  ``ids``: int32 or int64 of any shape, ``0 <= id < n_groups``; a negative id stands for no
     group, one beyond the last too and makes ``check_device_status`` raise.  At most 1024 groups."""
-    buf = _front().group_rows(ids, n_groups)
-    return RowGroups(ids, n_groups, ids.numel(), buf)
+    return RowGroups(ids, n_groups, False, _front().group_rows(ids, n_groups))
 
 
 def route_top_k(logits: torch.Tensor, top_k: int, *, renormalize: bool = True) -> tuple[torch.Tensor, RowGroups]:
@@ -679,7 +679,7 @@ def route_top_k(logits: torch.Tensor, top_k: int, *, renormalize: bool = True) -
     ``ids`` are int32 ``[..., top_k]``.  Equal logits: the lower index first.  An expert whose logit is -inf is closed; where too
     few are open the remaining slots have id -1 and weight 0.  A NaN makes the token's weights NaN."""
     weights, ids, buf = _front().route_top_k(logits, top_k, renormalize)
-    return weights, RowGroups(ids, logits.shape[-1], ids.numel() // top_k, buf)
+    return weights, RowGroups(ids, logits.shape[-1], True, buf)
 
 
 def fc_Q4A_experts(input: torch.Tensor, wei_quantized: torch.Tensor, N: int, groups: RowGroups, *,
@@ -695,7 +695,7 @@ def fc_Q4A_experts(input: torch.Tensor, wei_quantized: torch.Tensor, N: int, gro
     ``silu_mul``: a row of ``input`` is gate, then up, as one product with both projections packed as one tensor of
     ``2 K`` columns leaves them, and ``silu(gate) * up`` is multiplied (``llmops.itrans`` and ``imul`` of the
     reference, ops/op_misc.hpp:83-138)."""
-    return _front().fc_experts(input, wei_quantized, N, groups.ids, groups.n_groups, groups.most_rows, groups.buf, weights,
+    return _front().fc_experts(input, wei_quantized, N, groups.ids, groups.n_groups, groups.distinct, groups.buf, weights,
                                silu_mul, nibble_signed, out)
 
 

@@ -42,14 +42,13 @@ def check(got, want, bound):
     assert (off <= bound).all(), f"{(off / np.maximum(bound, 1e-300)).max()} of the bound at {np.argmax(off - bound)}"
 
 
-def call_and_check(pkg, ids, n, K, N, qtype, G, per_slot=False, weighted=False, seed=0, signed=False, most_rows=None):
+def call_and_check(pkg, ids, n, K, N, qtype, G, per_slot=False, weighted=False, seed=0, signed=False, distinct=False):
     tokens, top_k = ids.shape
     g = torch.Generator().manual_seed(seed + 1)
     x = torch.randn(1, tokens, *((top_k,) if per_slot else ()), K, generator=g)
     wq = pack(pkg, n, N, K, qtype, G, seed)
     groups = pkg.llmops.group_rows(torch.from_numpy(ids).int().cuda()[None], n)
-    if most_rows is not None:
-        groups.most_rows = most_rows
+    groups.distinct = distinct
     weights = torch.rand(1, tokens, top_k, generator=g) if weighted else None
     want, bound = want64(x[0].numpy(), ids, wq.cpu().numpy(), N, qtype, G, signed)
     out = torch.full((1, tokens, N) if weighted else (1, tokens, top_k, N), float("nan"), device="cuda")
@@ -80,6 +79,7 @@ def choose(rng, tokens, n, top_k, skew=0.0, none=0.0):
 def test_products(pkg, tokens, n, top_k, K, N, qtype, G):
     ids = choose(np.random.default_rng(tokens + K), tokens, n, top_k)
     call_and_check(pkg, ids, n, K, N, qtype, G, seed=tokens)
+    call_and_check(pkg, ids, n, K, N, qtype, G, seed=tokens, distinct=True)  # a token's experts are different ones
 
 
 @pytest.mark.parametrize("qtype,G", BLOCKS)
