@@ -14,8 +14,6 @@
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 
-#include <cfloat>
-
 #include "groups.cuh"
 #include "quant_pre.cuh"
 
@@ -157,11 +155,11 @@ struct Columns {
         T w[PIECES][2][NV];
         float2 y[NB][2];
     };
-    const T* b;        // of this lane's first column
-    float* y_at[NB][2];  // row nb * 8 + 2t + i at the lane's columns n and n + 1; null: none
-    int64_t n, N;
-    int rank, live;    // live: blocks of eight rows that have any
-    bool y_vec, onto;
+    const T* b;          // of the lane's first values of column 0
+    float* y_at[NB][2];  // row nb * 8 + 2t + i at column 0; where there is none, another's
+    int64_t n, N;        // the lane's columns: n and n + 1
+    int rank, rows, live;  // rows from this warp's first on, blocks of eight that have any
+    bool onto;
     Next c[2];
 
     // where pair i of a row's ranks stands in it
@@ -171,27 +169,32 @@ struct Columns {
         return i / kPairs * kPairs + in % kOf * 4 + in / kOf;
     }
     // rows of the tile from `row0` of its place on, columns from n0 on
-    __device__ __forceinline__ void begin(const LoraArgs& p, int4 tile, int rows, int row0, int64_t n0, bool vec, bool add) {
+    __device__ __forceinline__ void begin(const LoraArgs& p, int4 tile, int tile_rows, int row0, int64_t n0, bool add) {
         const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-        n = n0 + 2 * g, N = p.N, rank = p.rank, live = (rows - row0 + 7) / 8, y_vec = vec, onto = add;
+        n = n0 + 2 * g, N = p.N, rank = p.rank, rows = tile_rows - row0, live = (rows + 7) / 8, onto = add;
 #pragma unroll
         for (int nb = 0; nb < NB; nb++)
 #pragma unroll
             for (int i = 0; i < 2; i++) {
-                const int row = row0 + nb * 8 + 2 * t + i;
-                y_at[nb][i] = row < rows ? p.y + (int64_t)__ldcg(p.order + tile.y + row) * p.ldy + n : nullptr;
+                const int row = nb * 8 + 2 * t + i;
+                y_at[nb][i] = p.y + (int64_t)__ldcg(p.order + tile.y + (row < rows ? row0 + row : 0)) * p.ldy;
             }
-        b = static_cast<const T*>(p.b) + ((int64_t)tile.x * p.N + n) * p.rank + NV * t;
+        b = static_cast<const T*>(p.b) + (int64_t)tile.x * p.N * p.rank + NV * t;
     }
+    // VEC: no branch and no predicate stands between these loads and what comes behind them, or the next piece would be waited for where it
+    // is asked for.  So columns and ranks that do not exist read others': nothing of the former is stored, the latter are zeros in finish().
     __device__ __forceinline__ void load_b(int ahead, int r0, T (&w)[PIECES][2][NV]) {
-        const T* from = b + ahead * kAcross * (int64_t)rank;
         const int t = threadIdx.x & 3;
 #pragma unroll
         for (int q = 0; q < PIECES; q++)
 #pragma unroll
             for (int h = 0; h < 2; h++) {
                 const int r = r0 + q * kPiece;
-                load_values<NV, VEC>(from + h * rank + r, n + ahead * kAcross + h < N ? rank - r - NV * t : 0, w[q][h]);
+                const int64_t m = n + ahead * kAcross + h;
+                if constexpr (VEC)
+                    load_values<NV, VEC>(b + min(m, N - 1) * rank + (r + NV * t < rank ? r : -NV * t), 1, w[q][h]);
+                else
+                    load_values<NV, VEC>(b + m * rank + r, m < N ? rank - r - NV * t : 0, w[q][h]);
             }
     }
     __device__ __forceinline__ void load_y(int ahead, Next& c) {
@@ -200,17 +203,12 @@ struct Columns {
         for (int nb = 0; nb < NB; nb++)
 #pragma unroll
             for (int i = 0; i < 2; i++) {
-                const float* from = y_at[nb][i] + ahead * kAcross;
-                float2 v = make_float2(0.0f, 0.0f);
-                if (onto && y_at[nb][i] != nullptr) {
-                    if (y_vec && m + 1 < N) {
-                        v = __ldcg(reinterpret_cast<const float2*>(from));
-                    } else {
-                        if (m < N) v.x = __ldcg(from);
-                        if (m + 1 < N) v.y = __ldcg(from + 1);
-                    }
+                if constexpr (VEC) {
+                    c.y[nb][i] = __ldcg(reinterpret_cast<const float2*>(y_at[nb][i] + min(m, N - 2)));
+                } else {
+                    c.y[nb][i].x = m < N ? __ldcg(y_at[nb][i] + m) : 0.0f;
+                    c.y[nb][i].y = m + 1 < N ? __ldcg(y_at[nb][i] + m + 1) : 0.0f;
                 }
-                c.y[nb][i] = v;
             }
     }
     __device__ __forceinline__ void finish(Next& c, const uint4* ts, int pitch) {
@@ -222,10 +220,14 @@ struct Columns {
         const int lane = threadIdx.x & 31;
 #pragma unroll 1
         for (int r0 = 0; r0 < rank; r0 += kChunk) {
-            if (r0 > 0) load_b(0, r0, c.w);
+            if (r0 > 0) load_b(0, r0, c.w);  // (more ranks than are held)
             const uint4* mine = ts + (lane >> 2) * pitch + r0 / 2 + (lane & 3);
 #pragma unroll
-            for (int q = 0; q < PIECES; q++)
+            for (int q = 0; q < PIECES; q++) {
+                if (VEC && r0 + q * kPiece + NV * (lane & 3) >= rank) {
+#pragma unroll
+                    for (int v = 0; v < NV; v++) c.w[q][0][v] = T(0.0f), c.w[q][1][v] = T(0.0f);
+                }
 #pragma unroll
                 for (int j = 0; j < NV / 2; j++) {
                     uint32_t wh[4], wl[4];
@@ -239,23 +241,25 @@ struct Columns {
                         mma_tf32(acc[nb], wh, u.x, u.y);
                     }
                 }
+            }
         }
         // acc[nb][i]: column n + i / 2 of row nb * 8 + 2t + i % 2
 #pragma unroll
         for (int nb = 0; nb < NB; nb++)
 #pragma unroll
             for (int i = 0; i < 2; i++) {
-                if (y_at[nb][i] == nullptr) continue;
-                const float2 v = make_float2(c.y[nb][i].x + acc[nb][i], c.y[nb][i].y + acc[nb][i + 2]);
-                if (y_vec && n + 1 < N) {
-                    *reinterpret_cast<float2*>(y_at[nb][i]) = v;
-                } else {
-                    if (n < N) y_at[nb][i][0] = v.x;
-                    if (n + 1 < N) y_at[nb][i][1] = v.y;
+                if (nb * 8 + 2 * (lane & 3) + i >= rows) continue;
+                const float2 on = onto ? c.y[nb][i] : make_float2(0.0f, 0.0f);
+                const float2 v = make_float2(on.x + acc[nb][i], on.y + acc[nb][i + 2]);
+                float* y = y_at[nb][i] + n;
+                if (VEC && n < N) {
+                    *reinterpret_cast<float2*>(y) = v;
+                } else if (!VEC) {
+                    if (n < N) y[0] = v.x;
+                    if (n + 1 < N) y[1] = v.y;
                 }
-                y_at[nb][i] += kAcross;
             }
-        n += kAcross, b += kAcross * (int64_t)rank;
+        n += kAcross;
     }
     // `times` of them; the first one's B and y have been asked for into c[0]
     __device__ __forceinline__ void run(int64_t times, const uint4* ts, int pitch) {
@@ -282,8 +286,8 @@ __device__ __forceinline__ void zero_rows(const LoraArgs& p, int64_t first, int6
 // divide the columns.  With `early` the launch in front computes y alone: all else is complete, and the first product does not wait
 // for it.  CTAs behind those of the tiles quantize x for the decode FC (quant_pre.cuh), which has to be done in front of it anyway.
 template <typename T, int MB, bool VEC>
-__global__ void __launch_bounds__(kThreads, 2) lora_few_kernel(const __grid_constant__ LoraArgs p, const __grid_constant__ QuantPre q, const bool y_vec,
-                                                               const bool onto, const bool early) {
+__global__ void __launch_bounds__(kThreads, 2) lora_few_kernel(const __grid_constant__ LoraArgs p, const __grid_constant__ QuantPre q, const bool onto,
+                                                               const bool early) {
     constexpr int kRanks = MB * 16, QUADS = MB == 1 ? 1 : 2, PIECES = MB == 4 && sizeof(T) < 4 ? 2 : 1, kAcross = kWarps * 16;
     using C = Columns<T, QUADS, PIECES, 1, kAcross, VEC>;
     constexpr int kPitch = expand_pitch((kRanks + C::kChunk - 1) / C::kChunk * C::kChunk) / 16;
@@ -325,7 +329,7 @@ __global__ void __launch_bounds__(kThreads, 2) lora_few_kernel(const __grid_cons
         }
         if (early) others_done();
         C cols;
-        cols.begin(p, tile, tile.z, 0, (first * kWarps + warp) * 16, y_vec, onto);
+        cols.begin(p, tile, tile.z, 0, (first * kWarps + warp) * 16, onto);
         if (times > 0) cols.load_b(0, 0, cols.c[0].w), cols.load_y(0, cols.c[0]);
         cluster.sync();
         const float scale = p.scales ? p.scales[tile.x] : 1.0f;
@@ -399,11 +403,13 @@ __global__ void __launch_bounds__(kThreads, 2) lora_shrink_kernel(const __grid_c
 }
 
 // The work is pieces of 32 rows of a tile and 64 columns, or of its eight rows and 128, the columns of a tile one behind another; a CTA
-// takes a contiguous share of what the plan has.
+// takes a contiguous share of what the plan has.  (Both launches of lora_add with two and with three CTAs an SM: 61 rows x 4096 x
+// 11008, 40 fp16 adapters of rank 64, 23.8 and 21.9 us; tiles of 64, 2048 rows x 4096 x 4096, 4 bf16 adapters of rank 32, 45.7 and 47.8.)
 __host__ __device__ constexpr int expand_rows(int tile) { return tile < 32 ? tile : 32; }
 __host__ __device__ constexpr int expand_columns(int tile) { return tile < 32 ? 128 : 64; }
+__host__ __device__ constexpr int expand_ctas(int tile) { return tile < 32 ? 3 : 2; }  // an SM
 template <typename T, int TILE, int QUADS, int PIECES, bool VEC>
-__global__ void __launch_bounds__(kThreads, 2) lora_expand_kernel(const __grid_constant__ LoraArgs p, const bool y_vec, const bool onto) {
+__global__ void __launch_bounds__(kThreads, expand_ctas(TILE)) lora_expand_kernel(const __grid_constant__ LoraArgs p, const bool onto) {
     constexpr int kRows = expand_rows(TILE), kParts = TILE / kRows, NB = kRows > 8 ? 2 : 1, kAcross = expand_columns(TILE);
     using C = Columns<T, QUADS, PIECES, NB, kAcross, VEC>;
     extern __shared__ uint4 ts[];  // [kRows][pitch]
@@ -431,7 +437,7 @@ __global__ void __launch_bounds__(kThreads, 2) lora_expand_kernel(const __grid_c
         if (tile.z <= 0) continue;
         const int rows = min(tile.z, kRows), row0 = warp * 16 / kAcross * 16;  // (this warp's first row)
         C cols;
-        cols.begin(p, tile, rows, row0, first * kAcross + warp * 16 % kAcross, y_vec, onto);
+        cols.begin(p, tile, rows, row0, first * kAcross + warp * 16 % kAcross, onto);
         cols.load_b(0, 0, cols.c[0].w);
         others_done();
         cols.load_y(0, cols.c[0]);
@@ -478,8 +484,10 @@ LoraPlan lora_plan(int64_t rows, int64_t K, int64_t rank, int64_t n, int sms) {
 bool shrink_vec(const LoraCall& c) {
     return c.K % 8 == 0 && c.ldx % 4 == 0 && ((reinterpret_cast<uintptr_t>(c.x) | reinterpret_cast<uintptr_t>(c.a)) & 15) == 0;
 }
-bool expand_vec(const LoraCall& c, int values) { return c.rank % values == 0 && (reinterpret_cast<uintptr_t>(c.b) & 15) == 0; }
-bool rows_vec(const LoraCall& c) { return c.ldy % 2 == 0 && (reinterpret_cast<uintptr_t>(c.y) & 7) == 0; }
+bool expand_vec(const LoraCall& c, int values) {
+    return c.rank % values == 0 && (reinterpret_cast<uintptr_t>(c.b) & 15) == 0 && c.N % 2 == 0 && c.ldy % 2 == 0 &&
+           (reinterpret_cast<uintptr_t>(c.y) & 7) == 0;
+}
 // clusters along x
 struct ClusterLaunch : DependentLaunch {
     cudaLaunchAttribute attrs[2];
@@ -493,7 +501,7 @@ template <typename T, int MB>
 int launch_few(const LoraCall& c, const LoraArgs& p, const QuantPre& q, bool onto, bool early, dim3 grid, cudaStream_t s) {
     ClusterLaunch l(grid, s);
     auto* fn = shrink_vec(c) && expand_vec(c, MB == 1 ? 4 : 8) ? lora_few_kernel<T, MB, true> : lora_few_kernel<T, MB, false>;
-    Q4FC_CUDA_OK(cudaLaunchKernelEx(&l.cfg, fn, p, q, rows_vec(c), onto, early));
+    Q4FC_CUDA_OK(cudaLaunchKernelEx(&l.cfg, fn, p, q, onto, early));
     return Q4FC_OK;
 }
 template <typename T, int TILE, int MB>
@@ -506,15 +514,15 @@ template <typename T, int TILE, int QUADS, int PIECES>
 int launch_expand(const LoraCall& c, const LoraArgs& p, bool onto, int64_t tiles, cudaStream_t s) {
     const DeviceInfo* di = device_info();
     if (!di) return Q4FC_ECUDA;
-    const bool vec = expand_vec(c, 4 * QUADS), y_vec = rows_vec(c);
+    const bool vec = expand_vec(c, 4 * QUADS);
     constexpr int kChunk = 16 * QUADS * PIECES;
-    const int64_t pieces = tiles * (TILE / expand_rows(TILE)) * ((c.N + expand_columns(TILE) - 1) / expand_columns(TILE)), most = 2 * di->sm_count;
+    const int64_t pieces = tiles * (TILE / expand_rows(TILE)) * ((c.N + expand_columns(TILE) - 1) / expand_columns(TILE)), most = expand_ctas(TILE) * di->sm_count;
     DependentLaunch l(dim3((unsigned)(pieces < most ? pieces : most)), kThreads, s);
     auto* fn = vec ? lora_expand_kernel<T, TILE, QUADS, PIECES, true> : lora_expand_kernel<T, TILE, QUADS, PIECES, false>;
     l.cfg.dynamicSmemBytes = expand_rows(TILE) * (size_t)expand_pitch((int)(c.rank + kChunk - 1) / kChunk * kChunk);
     if (l.cfg.dynamicSmemBytes > 48 * 1024)
         Q4FC_CUDA_OK(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)l.cfg.dynamicSmemBytes));
-    Q4FC_CUDA_OK(cudaLaunchKernelEx(&l.cfg, fn, p, y_vec, onto));
+    Q4FC_CUDA_OK(cudaLaunchKernelEx(&l.cfg, fn, p, onto));
     return Q4FC_OK;
 }
 template <typename T, int TILE>
