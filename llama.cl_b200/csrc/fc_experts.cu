@@ -61,7 +61,9 @@ size_t hidden_bytes(int64_t rows, int64_t N, bool weighted) { return weighted ? 
 
 size_t experts_scratch_bytes(int64_t rows, int64_t K, int64_t N, int G, int64_t n, bool weighted) {
     const int64_t Kg = (K + G - 1) / G;
-    return hidden_bytes(rows, N, weighted) + (experts_few_serves(rows, G, n) ? experts_few_scratch(rows, Kg, G, n) : experts_gemm_scratch(rows, Kg, G, n));
+    // (what serves a call depends on its packed tensor's columns too, which may be more than N)
+    const size_t gemm = experts_gemm_scratch(rows, Kg, G, n), few = experts_few_serves(rows, Kg, 1, G, n) ? experts_few_scratch(rows, Kg, G, n) : 0;
+    return hidden_bytes(rows, N, weighted) + (few > gemm ? few : gemm);
 }
 
 int launch_fc_experts(ExpertsCall c, const float* weights, int64_t top_k, cudaStream_t s) {
@@ -75,7 +77,7 @@ int launch_fc_experts(ExpertsCall c, const float* weights, int64_t top_k, cudaSt
     q.group_of = c.plan.group_of, q.place_of = c.plan.place_of, q.offsets = c.plan.offsets, q.n = (int)c.n;
     q.vec_ok = c.K % 4 == 0 && c.ldx % 4 == 0 && (reinterpret_cast<uintptr_t>(c.x) & 15) == 0;
     q.y = c.y, q.N = c.N, q.ldy = c.ldy;
-    if (int rc = experts_few_serves(c.rows, c.G, c.n) ? launch_experts_few(c, q, s) : launch_experts_gemm(c, q, s)) return rc;
+    if (int rc = experts_few_serves(c.rows, c.Kg, c.Ng, c.G, c.n) ? launch_experts_few(c, q, s) : launch_experts_gemm(c, q, s)) return rc;
     return weights ? launch_combine(sum, s) : Q4FC_OK;
 }
 

@@ -28,9 +28,9 @@ namespace q4fc {
 namespace {
 
 constexpr int kWarps = 16, kThreads = kWarps * 32;
-constexpr int kMaxDepth = 6;
+constexpr int kMaxDepth = 3;
 constexpr int kMostTiles = 1024;  // in shared memory
-constexpr int kPartRows = 16;
+constexpr int kTileRows = 16;
 
 struct FewParams {
     const int8_t* codes;  // [place][row_bytes]
@@ -41,7 +41,7 @@ struct FewParams {
     const int *tile_count, *order;
     int64_t row_bytes, N, ldy, group_bytes;
     int Ng, Kg, chunks;  // chunks of a stripe
-    int most_tiles, depth, last_bytes, y_vec, weigh, part_off, ring_off;
+    int most_tiles, part_rows, depth, last_bytes, y_vec, weigh, part_off, ring_off;
     int* status;
 };
 
@@ -54,6 +54,10 @@ __device__ __forceinline__ bool elect_lane() {  // one lane of a converged warp
         : "=r"(p));
     return p != 0;
 }
+
+// What a chunk costs in a tile of at most 2, 4, 8 and 16 rows.  (64 experts x 1408 x 2048, group 32, all with as many rows: 28, 32, 36 and
+// 54 us, of which other launches take 6 to 10.  170 tokens to 6 of them each: equal shares of the stripes 65.3 us, these costs 60.1.)
+__device__ constexpr int kCosts[4] = {5, 6, 7, 10};
 
 template <int G, int QTYPE>
 struct FewShape {
@@ -335,12 +339,15 @@ template <int G, int QTYPE, bool SIGNED>
 __global__ void __launch_bounds__(kThreads, 1) experts_few_kernel(const __grid_constant__ FewParams p) {
     using S = FewShape<G, QTYPE>;
     extern __shared__ __align__(128) uint8_t smem[];
-    // barriers [warp][kMaxDepth] | failure flag, weights | tiles | partial sums [warp][2][rows][32] | rings [warp][depth]
+    // barriers [warp][kMaxDepth] | failure flag, costs | tiles | partial sums of each warp's first stripe [warp][rows][32] | rings
+    // [warp][depth].  Those of its last stripe go where its ring was.
     constexpr int kFail = kWarps * kMaxDepth * 8;
     int4* const tiles = reinterpret_cast<int4*>(smem + kFail + 16);
-    float* const part = reinterpret_cast<float*>(smem + p.part_off);
+    auto part = [&](int w, bool last) {
+        return reinterpret_cast<float*>(smem + (last ? p.ring_off + w * p.depth * S::kSlot : p.part_off + w * p.part_rows * 128));
+    };
     volatile int* fail = reinterpret_cast<volatile int*>(smem + kFail);
-    int* const total = reinterpret_cast<int*>(smem + kFail + 4);  // the weights of all tiles
+    int* const total = reinterpret_cast<int*>(smem + kFail + 4);  // the costs of all tiles
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const uint32_t bars = smem_u32(smem) + warp * kMaxDepth * 8;
     if (lane < p.depth) mbar_init(bars + 8 * lane, 1);
@@ -350,52 +357,67 @@ __global__ void __launch_bounds__(kThreads, 1) experts_few_kernel(const __grid_c
     // The plan, and then the weights: the quantizer in front has let this launch begin only when what is in front of it was complete.
     for (int i = threadIdx.x; i < p.most_tiles; i += kThreads) {
         int4 tile = __ldcg(p.tiles + i);
-        tile.z = min(tile.z, kPartRows);
+        tile.z = min(tile.z, p.part_rows);
         tiles[i] = tile;
     }
     const int count = __ldcg(p.tile_count);
     __syncthreads();
-    // The CTA's stripes: equal shares, or where stripes may cost the SM more than their bytes shares of the tiles' weights.
+    // The CTA's stripes and its warps' chunks: equal shares of the chunks, or where tiles cost the SM more than their bytes, of the
+    // tiles' costs.
+    const int C = p.chunks;
     int s0, r;
+    auto share = [&](int w) { return (int)((int64_t)r * C * w / kWarps); };  // first chunk of a warp
+    int mine;  // that of warp `lane`
     if (!p.weigh) {
         const int64_t stripes = (int64_t)count * p.Ng;
         s0 = (int)(stripes * blockIdx.x / gridDim.x), r = (int)(stripes * (blockIdx.x + 1) / gridDim.x) - s0;
+        mine = share(min(lane, kWarps));
     } else {
-        if (warp == 0) {  // the weights in front of each tile
+        auto cost = [&](int rows) { return rows <= 2 ? kCosts[0] : rows <= 4 ? kCosts[1] : rows <= 8 ? kCosts[2] : kCosts[3]; };
+        if (warp == 0) {  // the costs in front of each tile, of a chunk each
             int sum = 0;
             for (int i0 = 0; i0 < count; i0 += 32) {
-                const int rows = i0 + lane < count ? tiles[i0 + lane].z : 0;
-                const int w = i0 + lane < count ? rows <= 4 ? 4 : rows <= 8 ? 5 : 7 : 0;
-                int v = w;
+                const int c = i0 + lane < count ? cost(tiles[i0 + lane].z) : 0;
+                int v = c;
 #pragma unroll
                 for (int off = 1; off < 32; off <<= 1) {
                     const int o = __shfl_up_sync(0xffffffffu, v, off);
                     if (lane >= off) v += o;
                 }
-                if (i0 + lane < count) tiles[i0 + lane].w = sum + v - w;
+                if (i0 + lane < count) tiles[i0 + lane].w = sum + v - c;
                 sum += __shfl_sync(0xffffffffu, v, 31);
             }
             if (lane == 0) *total = sum;
         }
         __syncthreads();
-        auto stripe_at = [&](int part) {  // the first stripe of a CTA
-            const int all = *total;
-            if (part >= (int)gridDim.x || count == 0) return count * p.Ng;
-            const int64_t target = (int64_t)all * p.Ng * part / gridDim.x;
-            int lo = 0, hi = count;  // the last tile whose weights begin at or in front of it
+        const int all = *total;
+        // of all pieces, `per_tile` a tile, the first one that begins at or behind a cost (in units of a piece's)
+        auto piece_at = [&](int64_t target, int64_t per_tile) {
+            int lo = 0, hi = count;  // the last tile whose costs begin at or in front of it
             while (hi - lo > 1) {
                 const int mid = (lo + hi) / 2;
-                if ((int64_t)tiles[mid].w * p.Ng <= target) lo = mid; else hi = mid;
+                if (tiles[mid].w * per_tile <= target) lo = mid; else hi = mid;
             }
-            const int w = (lo + 1 < count ? tiles[lo + 1].w : all) - tiles[lo].w;
-            const int64_t in = (target - (int64_t)tiles[lo].w * p.Ng + w - 1) / w;
-            return lo * p.Ng + (int)min((int64_t)p.Ng, in);
+            const int c = cost(tiles[lo].z);
+            return lo * per_tile + min(per_tile, (target - tiles[lo].w * per_tile + c - 1) / c);
         };
-        s0 = stripe_at(blockIdx.x), r = stripe_at(blockIdx.x + 1) - s0;
+        auto stripe_at = [&](int part) {  // the first stripe of a CTA
+            return count == 0 ? 0 : part >= (int)gridDim.x ? count * p.Ng : (int)piece_at((int64_t)all * p.Ng * part / gridDim.x, p.Ng);
+        };
+        const int edge = stripe_at(blockIdx.x + min(lane, 1));
+        s0 = __shfl_sync(0xffffffffu, edge, 0), r = __shfl_sync(0xffffffffu, edge, 1) - s0;
+        mine = 0;
+        if (r > 0) {
+            const int64_t per_tile = (int64_t)p.Ng * C;
+            auto cost_at = [&](int stripe) {  // the costs in front of it
+                const int tile = min(stripe / p.Ng, count - 1);
+                return tiles[tile].w * per_tile + (int64_t)(stripe - tile * p.Ng) * C * cost(tiles[tile].z);
+            };
+            const int64_t from = cost_at(s0), to = cost_at(s0 + r);
+            mine = lane >= kWarps ? r * C : (int)(piece_at(from + (to - from) * lane / kWarps, per_tile) - (int64_t)s0 * C);
+        }
     }
-    const int C = p.chunks;
-    auto share = [&](int w) { return (int)((int64_t)r * C * w / kWarps); };  // first chunk of a warp
-    const int begin = share(warp), end = share(warp + 1);
+    const int begin = __shfl_sync(0xffffffffu, mine, warp), end = __shfl_sync(0xffffffffu, mine, warp + 1);
     WarpRing<G, QTYPE> ring{};
     if (end > begin) {
         uint8_t* slots = smem + p.ring_off + warp * p.depth * S::kSlot;
@@ -425,9 +447,8 @@ __global__ void __launch_bounds__(kThreads, 1) experts_few_kernel(const __grid_c
             if (n + 3 < p.N) y[3] = v.w;
         }
     };
-    int slot = 0;
 #pragma unroll 1
-    for (int c = begin; c < end; slot = 1) {
+    for (int c = begin; c < end;) {
         const int li = c / C, kc0 = c - li * C, kc1 = min(C, kc0 + end - c);
         c += kc1 - kc0;
         const int sg = s0 + li, ti = sg / p.Ng;
@@ -438,7 +459,7 @@ __global__ void __launch_bounds__(kThreads, 1) experts_few_kernel(const __grid_c
         auto put = [&](int row, float4 v) {
             if (row >= tile.z) return;
             if (whole) store(n, tile.y + row, v);
-            else *reinterpret_cast<float4*>(part + ((warp * 2 + slot) * kPartRows + row) * 32 + 4 * g) = v;
+            else *reinterpret_cast<float4*>(part(warp, c == end) + row * 32 + 4 * g) = v;
         };
         // rows row, row + 1 of this lane's four columns
         auto put_two = [&](int row, const uint64_t (&acc)[4]) {
@@ -470,10 +491,10 @@ __global__ void __launch_bounds__(kThreads, 1) experts_few_kernel(const __grid_c
     }
     __syncthreads();
     // stripes that several warps have walked, a warp each; lane w knows what warp w has walked
-    const int first = share(min(lane, kWarps)), last = lane < kWarps ? share(lane + 1) : first;
+    const int first = mine, after = __shfl_down_sync(0xffffffffu, mine, 1), last = lane < kWarps ? after : first;
     for (int li = warp; li < r; li += kWarps) {
         const bool part_of = first < last && first < (li + 1) * C && last > li * C;
-        const uint32_t who = __ballot_sync(0xffffffffu, part_of), second = __ballot_sync(0xffffffffu, part_of && first / C != li);
+        const uint32_t who = __ballot_sync(0xffffffffu, part_of), ends = __ballot_sync(0xffffffffu, part_of && last <= (li + 1) * C);
         if ((who & (who - 1)) == 0) continue;
         const int sg = s0 + li, ti = sg / p.Ng;
         const int4 tile = tiles[ti];
@@ -482,7 +503,7 @@ __global__ void __launch_bounds__(kThreads, 1) experts_few_kernel(const __grid_c
             float sum = 0.0f;
             for (uint32_t left = who; left; left &= left - 1) {
                 const int w = __ffs(left) - 1;
-                sum += part[((w * 2 + (second >> w & 1)) * kPartRows + row) * 32 + lane];
+                sum += part(w, ends >> w & 1)[row * 32 + lane];
             }
             if (n < p.N) p.y[(int64_t)__ldcg(p.order + tile.y + row) * p.ldy + n] = sum;
         }
@@ -503,9 +524,10 @@ int launch_few(FewParams p, const DeviceInfo* di, cudaStream_t s) {
         if (di->index < 64) attr_done[di->index] = true;
     }
     p.part_off = (int)align_up(kWarps * kMaxDepth * 8 + 16 + (size_t)p.most_tiles * 16, 128);
-    p.ring_off = p.part_off + kWarps * 2 * kPartRows * 32 * 4;
-    int depth = (di->max_smem_optin - p.ring_off) / (kWarps * S::kSlot);
-    p.depth = depth < kMaxDepth ? depth : kMaxDepth;
+    p.ring_off = p.part_off + kWarps * p.part_rows * 128;
+    // What the rings leave of the SM's memory is L1, and codes and scales come through it: 64 experts x 1408 x 2048, group 32, with rings
+    // of 2, 3 and 4 chunks a warp 16 rows each 54.4, 55.2 and 57.9 us, one row 27.6, 27.3 and 27.7; 8 x 4096 x 22016, 2 rows 23.5, 23.3 and 23.8.
+    p.depth = p.weigh ? 2 : kMaxDepth;
     DependentLaunch l(dim3((unsigned)di->sm_count), kThreads, s);
     l.cfg.dynamicSmemBytes = (size_t)p.ring_off + (size_t)p.depth * kWarps * S::kSlot;
     Q4FC_CUDA_OK(cudaLaunchKernelEx(&l.cfg, fn, p));
@@ -514,10 +536,14 @@ int launch_few(FewParams p, const DeviceInfo* di, cudaStream_t s) {
 
 }  // namespace
 
-// Up to 48 rows an expert in the mean with group 32, up to 14 with group 128, whose 64-row tiles on tcgen05 have a quarter of the groups to
-// scale.  This kernel and those tiles, us, whole call, 32 experts x 2048 x 2048: group 32, 16 rows 49 and 72, 32 rows 80 and 94, 48
-// rows 111 and 108; group 128, 12 rows 32 and 38, 16 rows 45 and 39; 8 x 4096 x 8192, 48 rows 184 and 186; 12 rows 47 and 62, 16 rows 66 and 64.
-bool experts_few_serves(int64_t rows, int G, int64_t n) { return rows <= (G == 32 ? 48 : 14) * n && most_tiles(kTiles16, rows, n) <= kMostTiles; }
+// Up to 80 rows an expert in the mean with group 32, up to 16 with group 128, whose 64-row tiles on tcgen05 have a quarter of the groups to
+// scale.  This kernel and those tiles, us, whole call, 32 experts x 2048 x 2048: group 32, 16 rows 45 and 72, 64 rows 115 and 142, 96
+// rows 174 and 193; group 128, 12 rows 34 and 38, 16 rows 38 and 39, 20 rows 48 and 40; 8 x 4096 x 8192: group 32, 64 rows 227 and 271, 96
+// rows 328 and 348; group 128, 16 rows 59 and 63, 20 rows 68 and 65.  (Its list of stripes is counted in 32 bits.)
+bool experts_few_serves(int64_t rows, int64_t Kg, int64_t Ng, int G, int64_t n) {
+    const int64_t tiles = most_tiles(kTiles16, rows, n);
+    return rows <= (G == 32 ? 80 : 16) * n && tiles <= kMostTiles && (Kg * G + 127) / 128 * Ng * tiles <= 0x7fffffffLL / 8;
+}
 
 size_t experts_few_scratch(int64_t rows, int64_t Kg, int G, int64_t n) {
     const int64_t chunks = (Kg * G + 127) / 128;
@@ -528,10 +554,6 @@ int launch_experts_few(const ExpertsCall& c, GroupQuant q, cudaStream_t s) {
     const DeviceInfo* di = device_info();
     if (!di) return Q4FC_ECUDA;
     const int64_t chunks = (c.Kg * c.G + 127) / 128, tiles = most_tiles(kTiles16, c.rows, c.n);
-    if (chunks * c.Ng > 0x7fffffffLL / 8 / tiles) {
-        set_error("fc_experts: %lld rows, K=%lld, N=%lld exceed the limit of a launch", (long long)c.rows, (long long)c.K, (long long)c.N);
-        return Q4FC_ELIMIT;
-    }
     const bool sgn = (c.flags & Q4FC_FLAG_NIBBLE_SIGNED) && c.qtype == 0;
     FewParams p = {};
     p.status = ring_status_word();
@@ -542,10 +564,10 @@ int launch_experts_few(const ExpertsCall& c, GroupQuant q, cudaStream_t s) {
     p.codes = q.codes, p.sc = q.sc, p.wq = c.wq, p.y = c.y, p.N = c.N, p.ldy = c.ldy;
     p.tiles = c.plan.tiles[kTiles16], p.tile_count = c.plan.counts + kTiles16, p.order = c.plan.order;
     p.row_bytes = chunks * 128, p.group_bytes = c.Ng * c.Kg * block_bytes(c.qtype, c.G);
-    p.Ng = (int)c.Ng, p.Kg = (int)c.Kg, p.chunks = (int)chunks, p.most_tiles = (int)tiles;
+    p.Ng = (int)c.Ng, p.Kg = (int)c.Kg, p.chunks = (int)chunks, p.most_tiles = (int)tiles, p.part_rows = (int)(c.most_rows < kTileRows ? c.most_rows : kTileRows);
     p.last_bytes = (int)(c.Kg - (chunks - 1) * (128 / c.G)) * block_bytes(c.qtype, c.G);
-    // (group 32, more than four rows: its arithmetic takes longer than its bytes)
-    p.weigh = c.G == 32 && c.most_rows > 4;
+    // (beyond two rows the arithmetic takes longer than the bytes)
+    p.weigh = c.most_rows > 2;
     p.y_vec = c.ldy % 4 == 0 && (reinterpret_cast<uintptr_t>(c.y) & 15) == 0;
     if (c.qtype == 1) return c.G == 32 ? launch_few<32, 1, false>(p, di, s) : launch_few<128, 1, false>(p, di, s);
     if (!sgn) return c.G == 32 ? launch_few<32, 0, false>(p, di, s) : launch_few<128, 0, false>(p, di, s);

@@ -88,7 +88,7 @@ struct ExpertsCall {
 size_t experts_gemm_scratch(int64_t rows, int64_t Kg, int G, int64_t n);  // fc_prefill.cu
 int launch_experts_gemm(const ExpertsCall& c, GroupQuant q, cudaStream_t s);
 // fc_experts_few.cu: experts with few rows
-bool experts_few_serves(int64_t rows, int G, int64_t n);
+bool experts_few_serves(int64_t rows, int64_t Kg, int64_t Ng, int G, int64_t n);
 size_t experts_few_scratch(int64_t rows, int64_t Kg, int G, int64_t n);
 int launch_experts_few(const ExpertsCall& c, GroupQuant q, cudaStream_t s);
 // fc_experts.cu; with weights [rows / top_k][top_k] c.y is [rows / top_k][ldy]
