@@ -75,6 +75,11 @@ __device__ __forceinline__ void operand(T a, T b, T c, T d, uint32_t (&hi)[4], u
         else hi[i] = __float_as_uint(f[i]), lo[i] = 0;
 }
 
+// *y += (a, b): nothing comes back, L2 adds.  (One addition for each element: no order to depend on.)
+__device__ __forceinline__ void add_to(float* y, float a, float b) {
+    asm volatile("red.global.add.v2.f32 [%0], {%1, %2};" ::"l"(y), "f"(a), "f"(b) : "memory");
+}
+
 struct LoraArgs {
     const float* x;
     const void *a, *b;
@@ -143,8 +148,9 @@ __device__ __forceinline__ void shrink_rows(const float* x, bool live, const T* 
     }
 }
 
-// y += B t, or without `onto` y = B t, by one warp: 16 columns of NB times eight rows at a time, the next kAcross further; what the next
-// ones need of y and of B's first ranks is on its way meanwhile.  t is in shared memory, as the MMAs want it: two ranks of a row in 16
+// y += B t, or without `onto` y = B t, by one warp: 16 columns of NB times eight rows at a time, the next kAcross further; the next
+// ones' first ranks of B are on their way meanwhile, and y is added to where it is (read and written back, its latency in each step:
+// lora_add, 2048 rows x 4096 x 4096, 4 adapters of rank 32, 41.9 us, so 36.4).  t is in shared memory, as the MMAs want it: two ranks of a row in 16
 // bytes, {hi, hi, lo, lo}, those that a lane reads in turn 64 bytes apart, rows `pitch` apart.
 // QUADS: fours of ranks that a lane takes of a piece of 16 ranks (1, for at most 16) or 32 (2); PIECES of these at a time.
 __host__ __device__ constexpr int expand_pitch(int ranks) { return ranks * 8 / 128 * 128 + 64 + (ranks * 8 % 128 > 64 ? 128 : 0); }  // bytes
@@ -153,7 +159,6 @@ struct Columns {
     static constexpr int NV = 4 * QUADS, kPiece = 4 * NV, kChunk = kPiece * PIECES;  // values of a lane, ranks of a piece, ranks at a time
     struct Next {
         T w[PIECES][2][NV];
-        float2 y[NB][2];
     };
     const T* b;          // of the lane's first values of column 0
     float* y_at[NB][2];  // row nb * 8 + 2t + i at column 0; where there is none, another's
@@ -197,20 +202,6 @@ struct Columns {
                     load_values<NV, VEC>(b + m * rank + r, m < N ? rank - r - NV * t : 0, w[q][h]);
             }
     }
-    __device__ __forceinline__ void load_y(int ahead, Next& c) {
-        const int64_t m = n + ahead * kAcross;
-#pragma unroll
-        for (int nb = 0; nb < NB; nb++)
-#pragma unroll
-            for (int i = 0; i < 2; i++) {
-                if constexpr (VEC) {
-                    c.y[nb][i] = __ldcg(reinterpret_cast<const float2*>(y_at[nb][i] + min(m, N - 2)));
-                } else {
-                    c.y[nb][i].x = m < N ? __ldcg(y_at[nb][i] + m) : 0.0f;
-                    c.y[nb][i].y = m + 1 < N ? __ldcg(y_at[nb][i] + m + 1) : 0.0f;
-                }
-            }
-    }
     __device__ __forceinline__ void finish(Next& c, const uint4* ts, int pitch) {
         float acc[NB][4];
 #pragma unroll
@@ -249,14 +240,15 @@ struct Columns {
 #pragma unroll
             for (int i = 0; i < 2; i++) {
                 if (nb * 8 + 2 * (lane & 3) + i >= rows) continue;
-                const float2 on = onto ? c.y[nb][i] : make_float2(0.0f, 0.0f);
-                const float2 v = make_float2(on.x + acc[nb][i], on.y + acc[nb][i + 2]);
                 float* y = y_at[nb][i] + n;
-                if (VEC && n < N) {
-                    *reinterpret_cast<float2*>(y) = v;
-                } else if (!VEC) {
-                    if (n < N) y[0] = v.x;
-                    if (n + 1 < N) y[1] = v.y;
+                if (onto) {
+                    if (VEC && n < N) add_to(y, acc[nb][i], acc[nb][i + 2]);
+                    if (!VEC && n < N) atomicAdd(y, acc[nb][i]);
+                    if (!VEC && n + 1 < N) atomicAdd(y + 1, acc[nb][i + 2]);
+                } else {
+                    if (VEC && n < N) *reinterpret_cast<float2*>(y) = make_float2(acc[nb][i], acc[nb][i + 2]);
+                    if (!VEC && n < N) y[0] = acc[nb][i];
+                    if (!VEC && n + 1 < N) y[1] = acc[nb][i + 2];
                 }
             }
         n += kAcross;
@@ -265,10 +257,10 @@ struct Columns {
     __device__ __forceinline__ void run(int64_t times, const uint4* ts, int pitch) {
 #pragma unroll 1
         for (int64_t k = 0; k < times; k += 2) {
-            if (k + 1 < times) load_b(1, 0, c[1].w), load_y(1, c[1]);
+            if (k + 1 < times) load_b(1, 0, c[1].w);
             finish(c[0], ts, pitch);
             if (k + 1 >= times) break;
-            if (k + 2 < times) load_b(1, 0, c[0].w), load_y(1, c[0]);
+            if (k + 2 < times) load_b(1, 0, c[0].w);
             finish(c[1], ts, pitch);
         }
     }
@@ -330,7 +322,7 @@ __global__ void __launch_bounds__(kThreads, 2) lora_few_kernel(const __grid_cons
         if (early) others_done();
         C cols;
         cols.begin(p, tile, tile.z, 0, (first * kWarps + warp) * 16, onto);
-        if (times > 0) cols.load_b(0, 0, cols.c[0].w), cols.load_y(0, cols.c[0]);
+        if (times > 0) cols.load_b(0, 0, cols.c[0].w);
         cluster.sync();
         const float scale = p.scales ? p.scales[tile.x] : 1.0f;
         for (int i = threadIdx.x; i < 8 * kRanks / 2; i += kThreads) {
@@ -403,13 +395,14 @@ __global__ void __launch_bounds__(kThreads, 2) lora_shrink_kernel(const __grid_c
 }
 
 // The work is pieces of 32 rows of a tile and 64 columns, or of its eight rows and 128, the columns of a tile one behind another; a CTA
-// takes a contiguous share of what the plan has.  (Both launches of lora_add with two and with three CTAs an SM: 61 rows x 4096 x
-// 11008, 40 fp16 adapters of rank 64, 23.8 and 21.9 us; tiles of 64, 2048 rows x 4096 x 4096, 4 bf16 adapters of rank 32, 45.7 and 47.8.)
+// takes a contiguous share of what the plan has.  (Both launches of lora_add with 2, 3 and 4 CTAs an SM: tiles of 64 rows, 2048 rows x
+// 4096 x 4096, 4 bf16 adapters of rank 32, 37.3, 36.4 and 38.0 us; of eight, 61 rows x 4096 x 11008, 40 fp16 ones of rank 64, with 3 and
+// 4 22.3 and 23.0.  Four times eight rows a warp instead of two: the same.)
 __host__ __device__ constexpr int expand_rows(int tile) { return tile < 32 ? tile : 32; }
 __host__ __device__ constexpr int expand_columns(int tile) { return tile < 32 ? 128 : 64; }
-__host__ __device__ constexpr int expand_ctas(int tile) { return tile < 32 ? 3 : 2; }  // an SM
+constexpr int kExpandCtas = 3;  // an SM
 template <typename T, int TILE, int QUADS, int PIECES, bool VEC>
-__global__ void __launch_bounds__(kThreads, expand_ctas(TILE)) lora_expand_kernel(const __grid_constant__ LoraArgs p, const bool onto) {
+__global__ void __launch_bounds__(kThreads, kExpandCtas) lora_expand_kernel(const __grid_constant__ LoraArgs p, const bool onto) {
     constexpr int kRows = expand_rows(TILE), kParts = TILE / kRows, NB = kRows > 8 ? 2 : 1, kAcross = expand_columns(TILE);
     using C = Columns<T, QUADS, PIECES, NB, kAcross, VEC>;
     extern __shared__ uint4 ts[];  // [kRows][pitch]
@@ -440,7 +433,6 @@ __global__ void __launch_bounds__(kThreads, expand_ctas(TILE)) lora_expand_kerne
         cols.begin(p, tile, rows, row0, first * kAcross + warp * 16 % kAcross, onto);
         cols.load_b(0, 0, cols.c[0].w);
         others_done();
-        cols.load_y(0, cols.c[0]);
         __syncthreads();  // (nobody reads the piece in front any more)
         for (int row = warp; row < kRows; row += kWarps)
             for (int i = lane; i < pairs; i += 32) {
@@ -516,7 +508,7 @@ int launch_expand(const LoraCall& c, const LoraArgs& p, bool onto, int64_t tiles
     if (!di) return Q4FC_ECUDA;
     const bool vec = expand_vec(c, 4 * QUADS);
     constexpr int kChunk = 16 * QUADS * PIECES;
-    const int64_t pieces = tiles * (TILE / expand_rows(TILE)) * ((c.N + expand_columns(TILE) - 1) / expand_columns(TILE)), most = expand_ctas(TILE) * di->sm_count;
+    const int64_t pieces = tiles * (TILE / expand_rows(TILE)) * ((c.N + expand_columns(TILE) - 1) / expand_columns(TILE)), most = kExpandCtas * di->sm_count;
     DependentLaunch l(dim3((unsigned)(pieces < most ? pieces : most)), kThreads, s);
     auto* fn = vec ? lora_expand_kernel<T, TILE, QUADS, PIECES, true> : lora_expand_kernel<T, TILE, QUADS, PIECES, false>;
     l.cfg.dynamicSmemBytes = expand_rows(TILE) * (size_t)expand_pitch((int)(c.rank + kChunk - 1) / kChunk * kChunk);
