@@ -14,6 +14,9 @@
 // equal ids need no atomics whose order would decide places: it counts its piece (lanes with equal ids find one another with
 // ballots, the first adds) and notes each row's place among its own; the bins of all warps and CTAs are summed in order
 // and give the places in front.  The same from run to run.
+//
+// Bound by the latencies of one CTA's (or cluster's) steps, not by bytes.  Measured, one call behind another: route, 1 token of 8 experts
+// 2.4 us, 8 of 64 3.8, 170 of 64 10.0 (two launches), 4096 of 128, 8 each, 15.5; group, 61 rows 2.6, 2048 rows 7.4.
 #include <cooperative_groups.h>
 
 #include <atomic>

@@ -11,6 +11,10 @@
 // bits and the next 11), so that a product costs two MMAs, or three with fp32 weights, and is off by 2^-20 at most.
 // The order of k in an MMA is free as long as both operands have the same: a lane takes consecutive k of a row (8 of a piece
 // of 32), so that fragments come straight from global memory in 16-byte loads.
+//
+// Bound by the bytes of x, A, B and y where there are many, and in front of that by dependent steps: plan, rows, K, the sums' meeting, columns.
+// Measured, both products: 8 rows x 4096 x 4096, 8 bf16 adapters of rank 16 (2 MB) 6.1 us, 61 rows x 4096 x 11008, 40 fp16 ones of rank 64
+// (65 MB) 22.4, 2048 rows x 4096 x 4096, 4 bf16 ones of rank 32 (34 MB of x, 67 of y) 36.4; shrink alone 7.1 of the second, 15.4 of the third.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 
@@ -150,8 +154,8 @@ __device__ __forceinline__ void shrink_rows(const float* x, bool live, const T* 
 
 // y += B t, or without `onto` y = B t, by one warp: 16 columns of NB times eight rows at a time, the next kAcross further; the next
 // ones' first ranks of B are on their way meanwhile, and y is added to where it is (read and written back, its latency in each step:
-// lora_add, 2048 rows x 4096 x 4096, 4 adapters of rank 32, 41.9 us, so 36.4).  t is in shared memory, as the MMAs want it: two ranks of a row in 16
-// bytes, {hi, hi, lo, lo}, those that a lane reads in turn 64 bytes apart, rows `pitch` apart.
+// lora_add, 2048 rows x 4096 x 4096, 4 adapters of rank 32, 41.9 us, so 36.4).  t is in shared memory, as the MMAs want it: two ranks of a
+// row in 16 bytes, {hi, hi, lo, lo}, those that a lane reads in turn 64 bytes apart, rows `pitch` apart.
 // QUADS: fours of ranks that a lane takes of a piece of 16 ranks (1, for at most 16) or 32 (2); PIECES of these at a time.
 __host__ __device__ constexpr int expand_pitch(int ranks) { return ranks * 8 / 128 * 128 + 64 + (ranks * 8 % 128 > 64 ? 128 : 0); }  // bytes
 template <typename T, int QUADS, int PIECES, int NB, int kAcross, bool VEC>

@@ -56,7 +56,7 @@ __device__ __forceinline__ RowTile row_tile(const PrefillParams& p, int m_tile) 
     }
 }
 // GROUPED: the rows of y that a thread's stores go to, asked for by the lanes of its warp long before: lane i knows that of row `first` +
-// step * i of the tile.  (Asked for store by store, each takes its way to L2 and back: 2 x 512 rows x 4096 x 22016 402 us, so XX.)
+// step * i of the tile.  (Asked for store by store, each takes its way to L2 and back: 2 x 512 rows x 4096 x 22016 402 us, so 304.)
 template <bool GROUPED>
 __device__ __forceinline__ int y_rows(const PrefillParams& p, const RowTile& tile, int first, int step) {
     const int row = first + step * (int)(threadIdx.x & 31);
