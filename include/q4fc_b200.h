@@ -445,7 +445,7 @@ int q4fc_route_top_k(const float* logits, int64_t tokens, int64_t experts, int64
  * says beyond it is an error of the caller's that leaves outputs unwritten.
  * ws: q4fc_experts_workspace_bytes bytes of scratch, 256-byte aligned; nothing is kept in it between calls, calls that may
  * overlap need separate ones.  Sums have a fixed order that depends on the sizes, the counts of rows per expert and the card.
- * flags: Q4FC_FLAG_NIBBLE_SIGNED. */
+ * flags: Q4FC_FLAG_NIBBLE_SIGNED.  Limit (Q4FC_ELIMIT): tokens * top_k / 128 + experts at most 65535. */
 typedef struct q4fc_experts_call {
     const float* x;      /* fp32 [tokens][ldx], or with x_per_slot [tokens * top_k][ldx] */
     int64_t tokens, top_k, K, ldx;

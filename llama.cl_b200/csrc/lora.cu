@@ -360,12 +360,13 @@ __global__ void __launch_bounds__(kThreads, 2) lora_shrink_kernel(const __grid_c
     cg::cluster_group cluster = cg::this_cluster();
     pdl_wait_prior_grid();
     pdl_launch_dependents();
-    const int4 tile = __ldcg(p.tiles + blockIdx.y);  // (beyond the count: nothing that is used)
-    if ((int)blockIdx.y >= __ldcg(p.tile_count)) return;
+    const int slices = (int)cluster.num_blocks(), here = (int)cluster.block_rank(), at = (int)blockIdx.x / slices;  // (clusters lie along x)
+    const int4 tile = __ldcg(p.tiles + at);  // (beyond the count: nothing that is used)
+    if (at >= __ldcg(p.tile_count)) return;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int row0 = kByK ? 0 : warp * 8;
     const int rank0 = blockIdx.z * kRankBlock;
-    const int64_t k_begin = blockIdx.x * p.slice_k, k_end = min(p.K, k_begin + p.slice_k);
+    const int64_t k_begin = here * p.slice_k, k_end = min(p.K, k_begin + p.slice_k);
     const bool live = row0 + g < tile.z;
     const float* x = p.x + (live ? (int64_t)__ldcg(p.order + tile.y + row0 + g) * p.ldx : 0);
     float acc[MB][4] = {};
@@ -388,7 +389,6 @@ __global__ void __launch_bounds__(kThreads, 2) lora_shrink_kernel(const __grid_c
     }
     cluster.sync();
     const float scale = p.scales ? p.scales[tile.x] : 1.0f;
-    const int slices = (int)gridDim.x, here = (int)blockIdx.x;
     for (int i = here * kThreads + threadIdx.x; i < tile.z * kRanks; i += slices * kThreads) {
         float sum = 0.0f;
         for (int s = 0; s < slices; s++) sum += cluster.map_shared_rank(sums, s)[i];
@@ -484,25 +484,25 @@ bool expand_vec(const LoraCall& c, int values) {
     return c.rank % values == 0 && (reinterpret_cast<uintptr_t>(c.b) & 15) == 0 && c.N % 2 == 0 && c.ldy % 2 == 0 &&
            (reinterpret_cast<uintptr_t>(c.y) & 7) == 0;
 }
-// clusters along x
+// clusters of `ctas` along x
 struct ClusterLaunch : DependentLaunch {
     cudaLaunchAttribute attrs[2];
-    ClusterLaunch(dim3 grid, cudaStream_t s) : DependentLaunch(grid, kThreads, s), attrs{attr, {}} {
+    ClusterLaunch(dim3 grid, int ctas, cudaStream_t s) : DependentLaunch(grid, kThreads, s), attrs{attr, {}} {
         attrs[1].id = cudaLaunchAttributeClusterDimension;
-        attrs[1].val.clusterDim.x = grid.x, attrs[1].val.clusterDim.y = attrs[1].val.clusterDim.z = 1;
+        attrs[1].val.clusterDim.x = (unsigned)ctas, attrs[1].val.clusterDim.y = attrs[1].val.clusterDim.z = 1;
         cfg.attrs = attrs, cfg.numAttrs = 2;
     }
 };
 template <typename T, int MB>
 int launch_few(const LoraCall& c, const LoraArgs& p, const QuantPre& q, bool onto, bool early, dim3 grid, cudaStream_t s) {
-    ClusterLaunch l(grid, s);
+    ClusterLaunch l(grid, (int)grid.x, s);
     auto* fn = shrink_vec(c) && expand_vec(c, MB == 1 ? 4 : 8) ? lora_few_kernel<T, MB, true> : lora_few_kernel<T, MB, false>;
     Q4FC_CUDA_OK(cudaLaunchKernelEx(&l.cfg, fn, p, q, onto, early));
     return Q4FC_OK;
 }
 template <typename T, int TILE, int MB>
-int launch_shrink(const LoraArgs& p, bool vec, dim3 grid, cudaStream_t s) {
-    ClusterLaunch l(grid, s);
+int launch_shrink(const LoraArgs& p, bool vec, dim3 grid, int slices, cudaStream_t s) {
+    ClusterLaunch l(grid, slices, s);
     Q4FC_CUDA_OK(cudaLaunchKernelEx(&l.cfg, vec ? lora_shrink_kernel<T, TILE, MB, true> : lora_shrink_kernel<T, TILE, MB, false>, p));
     return Q4FC_OK;
 }
@@ -525,10 +525,10 @@ template <typename T, int TILE>
 int launch_lora_tile(const LoraCall& c, const LoraArgs& p, const LoraPlan& l, Step step, int64_t tiles, cudaStream_t s) {
     if (step == kShrink) {
         const bool vec = shrink_vec(c);
-        const dim3 grid((unsigned)l.slices, (unsigned)tiles, (unsigned)((c.rank + kRankBlock - 1) / kRankBlock));
-        if (c.rank <= 16) return launch_shrink<T, TILE, 1>(p, vec, grid, s);
-        if (c.rank <= 32) return launch_shrink<T, TILE, 2>(p, vec, grid, s);
-        return launch_shrink<T, TILE, 4>(p, vec, grid, s);
+        const dim3 grid((unsigned)(l.slices * tiles), 1, (unsigned)((c.rank + kRankBlock - 1) / kRankBlock));
+        if (c.rank <= 16) return launch_shrink<T, TILE, 1>(p, vec, grid, l.slices, s);
+        if (c.rank <= 32) return launch_shrink<T, TILE, 2>(p, vec, grid, l.slices, s);
+        return launch_shrink<T, TILE, 4>(p, vec, grid, l.slices, s);
     }
     if (c.rank <= 16) return launch_expand<T, TILE, 1, 1>(c, p, step == kExpandOnto, tiles, s);
     if (c.rank <= 32 || sizeof(T) == 4) return launch_expand<T, TILE, 2, 1>(c, p, step == kExpandOnto, tiles, s);
@@ -543,10 +543,6 @@ int lora_args(const LoraCall& c, LoraPlan* l, LoraArgs* p, int64_t* tiles) {
     if (!di) return Q4FC_ECUDA;
     *l = lora_plan(c.rows, c.K, c.rank, c.n, di->sm_count);
     *tiles = most_tiles(l->which, c.rows, c.n);
-    if (*tiles > 65535 / 2) {
-        set_error("lora: %lld rows exceed the grid limit", (long long)c.rows);
-        return Q4FC_ELIMIT;
-    }
     *p = LoraArgs{c.x, c.a, c.b, c.scales, c.y, static_cast<float*>(c.scratch), c.plan.tiles[l->which], c.plan.counts + l->which, c.plan.order,
                   c.rows, c.K, c.ldx, c.N, c.ldy, l->slice_k, (int)c.rank, (int)c.n, c.plan.offsets};
     return Q4FC_OK;

@@ -303,3 +303,19 @@ def test_adapters_beyond_32_bit_offsets(pkg, rows):
     want, bound = added64(x, a[-1:], b[-1:, -40:], None, np.zeros(rows, np.int64))
     check(y[..., -40:].contiguous(), want, bound)
     assert not y[..., :-40].any()
+
+
+def test_adapters_of_as_many_rows_as_a_plan_holds(pkg):
+    """2^23 rows, few columns."""
+    rows, n, K, N = 1 << 23, 3, 8, 4
+    g = torch.Generator(device="cuda").manual_seed(1)
+    x = torch.randn(1, rows, K, device="cuda", generator=g)
+    a, b = torch.randn(n, 2, K, device="cuda", generator=g), torch.randn(n, N, 2, device="cuda", generator=g)
+    ids = torch.randint(-1, n, (1, rows), device="cuda", generator=g, dtype=torch.int32)
+    groups = pkg.llmops.group_rows(ids, n)
+    y = torch.zeros(1, rows, N, device="cuda")
+    pkg.llmops.lora_add(y, x, a, b, groups)
+    some = torch.cat([torch.arange(200), torch.randint(0, rows, (200,), generator=torch.Generator().manual_seed(2)), torch.arange(rows - 200, rows)])
+    want, bound = added64(x[:, some.cuda()], a, b, None, ids[0, some.cuda()].cpu().numpy())
+    check(y[0, some.cuda()], want, bound)
+    assert not y[0, ids[0] < 0].any()
