@@ -16,7 +16,7 @@
 // and give the places in front.  The same from run to run.
 //
 // Bound by the latencies of one CTA's (or cluster's) steps, not by bytes.  Measured, one call behind another: route, 1 token of 8 experts
-// 2.4 us, 8 of 64 3.8, 170 of 64 10.0 (two launches), 4096 of 128, 8 each, 15.5; group, 61 rows 2.6, 2048 rows 7.4.
+// 2.5 us, 8 of 64 3.6, 333 of 64 7.8 (two launches), 4096 of 128, 8 each, 15.2; group, 48 rows 2.5, 2048 rows 6.5 (by one CTA 7.7).
 #include <cooperative_groups.h>
 
 #include <atomic>
@@ -201,12 +201,11 @@ __global__ void __launch_bounds__(kFew) group_few_kernel(const GroupArgs a, cons
     }
 }
 
-// More rows.  NV as above.
+// More rows.
 constexpr int kHeld = 8;  // sets of 32 rows of a warp that stay in registers between its two walks
 constexpr int kStaged = kWarps * kHeld * 32;  // rows of a CTA that are sorted in shared memory on their way out
 constexpr int kScans = 2 + kTileSizes;  // rows of the groups, their tiles, this CTA's rows
-template <int NV>
-__global__ void __launch_bounds__(kThreads, 1) group_kernel(const GroupArgs a, const RouteArgs route) {
+__global__ void __launch_bounds__(kThreads, 1) group_kernel(const GroupArgs a) {
     extern __shared__ uint32_t bins[];  // [warp][n + 1]
     __shared__ uint32_t sums[kMaxGroups + 1];             // this CTA's rows of each group
     __shared__ uint32_t first[kMaxGroups + 1];            // its first place of each group
@@ -216,16 +215,14 @@ __global__ void __launch_bounds__(kThreads, 1) group_kernel(const GroupArgs a, c
     __shared__ uint32_t warp_sum[kScans][kWarps];
     cg::cluster_group cluster = cg::this_cluster();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int ctas = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+    const int rank = (int)cluster.block_rank();
     const int nb = a.n + 1;  // bins; the last one is of rows without a group
     uint32_t* mine = bins + warp * nb;
     for (int i = lane; i < nb; i += 32) mine[i] = 0;
     pdl_wait_prior_grid();
     pdl_launch_dependents();
     const int64_t begin = min(a.rows, ((int64_t)rank * kWarps + warp) * a.piece), end = min(a.rows, begin + a.piece);
-    if constexpr (NV > 0)
-        for (int64_t t = begin / route.top_k; t < end / route.top_k; t++) route_token<NV>(route, t, lane);
-    __syncwarp();  // (a warp's own ids are what it sorts)
+    __syncwarp();
     // 32 rows: their bins, and the place of each among the warp's rows of its bin.  (Lanes with equal bins find one another bit by
     // bit: a match.any takes the longer the more different ones there are.)
     const int bits = 32 - __clz(a.n);
@@ -263,57 +260,66 @@ __global__ void __launch_bounds__(kThreads, 1) group_kernel(const GroupArgs a, c
         sums[b] = sum;
     }
     cluster.sync();
-    // group b = threadIdx.x (kMaxGroups = kThreads of them): its rows, those of the CTAs in front, its first place and tiles
+    // group b = threadIdx.x (kMaxGroups = kThreads of them): its rows, those of the CTAs in front, its first place and tiles; by the warps
+    // that have any
+    const int group_warps = (a.n + 31) / 32;
     uint32_t all = 0, front = 0;
-    if ((int)threadIdx.x < a.n)
+    uint32_t v[kScans], own[kScans];
+    if (warp < group_warps) {
+        if ((int)threadIdx.x < a.n)
+            for (int c = 0; c < kCluster; c++) {
+                const uint32_t v = cluster.map_shared_rank(sums, c)[threadIdx.x];
+                all += v;
+                if (c < rank) front += v;
+            }
+        v[0] = all, v[1 + kTileSizes] = (int)threadIdx.x < a.n ? sums[threadIdx.x] : 0;
 #pragma unroll
-        for (int c = 0; c < kCluster; c++) {
-            const uint32_t v = c < ctas ? cluster.map_shared_rank(sums, c)[threadIdx.x] : 0;
-            all += v;
-            if (c < rank) front += v;
-        }
-    uint32_t none_front = 0;  // of rows without a group
-    if (threadIdx.x == 0)
-        for (int c = 0; c < rank; c++) none_front += cluster.map_shared_rank(sums, c)[a.n];
-    uint32_t v[kScans];
-    v[0] = all, v[1 + kTileSizes] = (int)threadIdx.x < a.n ? sums[threadIdx.x] : 0;
+        for (int j = 0; j < kTileSizes; j++) v[1 + j] = (all + tile_rows(j) - 1) / tile_rows(j);
 #pragma unroll
-    for (int j = 0; j < kTileSizes; j++) v[1 + j] = (all + tile_rows(j) - 1) / tile_rows(j);
-    uint32_t own[kScans];
+        for (int j = 0; j < kScans; j++) own[j] = v[j];
+#pragma unroll 1
+        for (int off = 1; off < 32; off <<= 1)
 #pragma unroll
-    for (int j = 0; j < kScans; j++) own[j] = v[j];
+            for (int j = 0; j < kScans; j++) {
+                const uint32_t o = __shfl_up_sync(0xffffffffu, v[j], off);
+                if (lane >= off) v[j] += o;
+            }
+        if (lane == 31)
 #pragma unroll
-    for (int off = 1; off < 32; off <<= 1)
+            for (int j = 0; j < kScans; j++) warp_sum[j][warp] = v[j];
+    }
+    __syncthreads();
+    if (warp < group_warps) {
+        uint32_t total[kScans];
 #pragma unroll
         for (int j = 0; j < kScans; j++) {
-            const uint32_t o = __shfl_up_sync(0xffffffffu, v[j], off);
-            if (lane >= off) v[j] += o;
+            const uint32_t w = lane < group_warps ? warp_sum[j][lane] : 0;
+            total[j] = __reduce_add_sync(0xffffffffu, w);
+            v[j] += __reduce_add_sync(0xffffffffu, lane < warp ? w : 0u) - own[j];  // in front of this group
         }
-    if (lane == 31)
-        for (int j = 0; j < kScans; j++) warp_sum[j][warp] = v[j];
-    __syncthreads();
-    uint32_t total[kScans];
+        if ((int)threadIdx.x < a.n) {
+            first[threadIdx.x] = v[0] + front, start[threadIdx.x] = v[0], here[threadIdx.x] = v[1 + kTileSizes];
 #pragma unroll
-    for (int j = 0; j < kScans; j++) {
-        const uint32_t w = warp_sum[j][lane];  // (32 warps)
-        total[j] = __reduce_add_sync(0xffffffffu, w);
-        v[j] += __reduce_add_sync(0xffffffffu, lane < warp ? w : 0u) - own[j];  // in front of this group
-    }
-    if ((int)threadIdx.x < a.n) {
-        first[threadIdx.x] = v[0] + front, start[threadIdx.x] = v[0], here[threadIdx.x] = v[1 + kTileSizes];
-        for (int j = 0; j < kTileSizes; j++) tile0[j][threadIdx.x] = (int)v[j + 1];
-        if (rank == 0) {
-            a.plan.offsets[threadIdx.x] = (int)v[0];
-            for (int j = 0; j < kTileSizes; j++) a.plan.tile0[j][threadIdx.x] = (int)v[j + 1];
+            for (int j = 0; j < kTileSizes; j++) tile0[j][threadIdx.x] = (int)v[j + 1];
+            if (rank == 0) {
+                a.plan.offsets[threadIdx.x] = (int)v[0];
+#pragma unroll
+                for (int j = 0; j < kTileSizes; j++) a.plan.tile0[j][threadIdx.x] = (int)v[j + 1];
+            }
         }
-    }
-    if (threadIdx.x == 0) {
-        first[a.n] = total[0] + none_front, start[a.n] = total[0], here[a.n] = total[1 + kTileSizes];
-        for (int j = 0; j < kTileSizes; j++) tile0[j][a.n] = (int)total[j + 1];
-        if (rank == 0) {
-            a.plan.offsets[a.n] = (int)total[0];
-            for (int j = 0; j < kTileSizes; j++) a.plan.tile0[j][a.n] = (int)total[j + 1];
-            for (int j = 0; j < 16; j++) a.plan.counts[j] = j < kTileSizes ? (int)total[j + 1] : 0;
+        if (threadIdx.x == 0) {
+            uint32_t none_front = 0;  // of rows without a group
+            for (int c = 0; c < rank; c++) none_front += cluster.map_shared_rank(sums, c)[a.n];
+            first[a.n] = total[0] + none_front, start[a.n] = total[0], here[a.n] = total[1 + kTileSizes];
+#pragma unroll
+            for (int j = 0; j < kTileSizes; j++) tile0[j][a.n] = (int)total[j + 1];
+            if (rank == 0) {
+                a.plan.offsets[a.n] = (int)total[0];
+#pragma unroll
+                for (int j = 0; j < kTileSizes; j++) a.plan.tile0[j][a.n] = (int)total[j + 1];
+#pragma unroll
+                for (int j = 0; j < 16; j++) a.plan.counts[j] = j < kTileSizes ? (int)total[j + 1] : 0;
+            }
         }
     }
     __syncthreads();
@@ -348,18 +354,22 @@ __global__ void __launch_bounds__(kThreads, 1) group_kernel(const GroupArgs a, c
             }
         }
     }
-    // tiles: the group of tile i is the last whose first tile is not behind it
-    for (int j = 0; j < kTileSizes; j++) {
-        const int size = tile_rows(j);
-        for (int i = rank * kThreads + threadIdx.x; i < (int)total[j + 1]; i += ctas * kThreads) {
-            int lo = 0, hi = a.n;  // tile0[lo] <= i < tile0[hi]
-            while (hi - lo > 1) {
-                const int mid = (lo + hi) / 2;
-                if (tile0[j][mid] <= i) lo = mid; else hi = mid;
-            }
-            const int at = (i - tile0[j][lo]) * size;
-            a.plan.tiles[j][i] = make_int4(lo, (int)start[lo] + at, min(size, (int)(start[lo + 1] - start[lo]) - at), 0);
+    // tiles of all sizes, one list: the group of tile i of a size is the last whose first tile is not behind it
+    int ends[kTileSizes];
+#pragma unroll
+    for (int j = 0; j < kTileSizes; j++) ends[j] = (j > 0 ? ends[j - 1] : 0) + tile0[j][a.n];
+    for (int at = rank * kThreads + threadIdx.x; at < ends[kTileSizes - 1]; at += kCluster * kThreads) {
+        int j = 0, i = at;
+#pragma unroll
+        for (int k = 0; k + 1 < kTileSizes; k++)
+            if (at >= ends[k]) j = k + 1, i = at - ends[k];
+        int lo = 0, hi = a.n;  // tile0[lo] <= i < tile0[hi]
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) / 2;
+            if (tile0[j][mid] <= i) lo = mid; else hi = mid;
         }
+        const int size = tile_rows(j), in = (i - tile0[j][lo]) * size;
+        a.plan.tiles[j][i] = make_int4(lo, (int)start[lo] + in, min(size, (int)(start[lo + 1] - start[lo]) - in), 0);
     }
     cluster.sync();  // nobody leaves while its sums are being read
 }
@@ -370,10 +380,9 @@ int launch_group_few(const GroupArgs& a, const RouteArgs& route, cudaStream_t s)
     Q4FC_CUDA_OK(cudaLaunchKernelEx(&l.cfg, group_few_kernel<NV>, a, route));
     return Q4FC_OK;
 }
-template <int NV>
-int launch_group_variant(const GroupArgs& a, const RouteArgs& route, int ctas, cudaStream_t s) {
+int launch_group(const GroupArgs& a, cudaStream_t s) {
     static std::atomic<bool> attr_done[64] = {};  // set once per device; a second setter repeats the same call
-    auto* fn = group_kernel<NV>;
+    auto* fn = group_kernel;
     const size_t most = kWarps * (kMaxGroups + 1) * sizeof(uint32_t) + kStaged * 6;
     int dev = 0;
     Q4FC_CUDA_OK(cudaGetDevice(&dev));
@@ -381,13 +390,13 @@ int launch_group_variant(const GroupArgs& a, const RouteArgs& route, int ctas, c
         Q4FC_CUDA_OK(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most));
         if (dev < 64) attr_done[dev] = true;
     }
-    DependentLaunch l(dim3((unsigned)ctas), kThreads, s);
+    DependentLaunch l(dim3(kCluster), kThreads, s);
     cudaLaunchAttribute attrs[2] = {l.attr, {}};
     attrs[1].id = cudaLaunchAttributeClusterDimension;
-    attrs[1].val.clusterDim.x = (unsigned)ctas, attrs[1].val.clusterDim.y = attrs[1].val.clusterDim.z = 1;
+    attrs[1].val.clusterDim.x = kCluster, attrs[1].val.clusterDim.y = attrs[1].val.clusterDim.z = 1;
     l.cfg.attrs = attrs, l.cfg.numAttrs = 2;
     l.cfg.dynamicSmemBytes = kWarps * (size_t)(a.n + 1) * sizeof(uint32_t) + kStaged * 6;
-    Q4FC_CUDA_OK(cudaLaunchKernelEx(&l.cfg, fn, a, route));
+    Q4FC_CUDA_OK(cudaLaunchKernelEx(&l.cfg, fn, a));
     return Q4FC_OK;
 }
 // NV: logits a lane holds, for as many experts
@@ -399,10 +408,10 @@ int with_lanes(int experts, F f) {
     if (experts <= 256) return f(std::integral_constant<int, 8>{});
     return f(std::integral_constant<int, 32>{});
 }
-int group_args(GroupArgs* a, const void* ids, int i32, int64_t rows, int64_t n, void* groups, int ctas, int64_t together) {
+int group_args(GroupArgs* a, const void* ids, int i32, int64_t rows, int64_t n, void* groups) {
     a->ids = ids, a->i32 = i32, a->rows = rows, a->n = (int)n, a->plan = group_plan(groups, rows, n);
-    const int64_t warps = (int64_t)ctas * kWarps;
-    a->piece = (rows / together + warps - 1) / warps * together;
+    constexpr int64_t warps = (int64_t)kCluster * kWarps;
+    a->piece = (rows + warps - 1) / warps;
     a->status = ring_status_word();
     return a->status ? Q4FC_OK : Q4FC_ECUDA;
 }
@@ -411,10 +420,9 @@ int group_args(GroupArgs* a, const void* ids, int i32, int64_t rows, int64_t n, 
 
 int launch_group_rows(const void* ids, int ids_are_i32, int64_t rows, int64_t n, void* groups, cudaStream_t s) {
     GroupArgs a = {};
-    const int ctas = rows > 2048 ? kCluster : 1;
-    if (int rc = group_args(&a, ids, ids_are_i32, rows, n, groups, ctas, 1)) return rc;
+    if (int rc = group_args(&a, ids, ids_are_i32, rows, n, groups)) return rc;
     if (rows <= kFew) return launch_group_few<0>(a, RouteArgs{}, s);
-    return launch_group_variant<0>(a, RouteArgs{}, ctas, s);
+    return launch_group(a, s);
 }
 
 int launch_route_top_k(const float* logits, int64_t tokens, int64_t experts, int64_t ld, int64_t top_k, int renormalize,
@@ -422,16 +430,14 @@ int launch_route_top_k(const float* logits, int64_t tokens, int64_t experts, int
     RouteArgs route = {logits, tokens, ld, (int)experts, (int)top_k, renormalize, weights, ids};
     GroupArgs a = {};
     const int64_t rows = tokens * top_k;
-    const bool inside = tokens <= 64;  // (17 tokens inside 8.5 us; 333 tokens, 1332 pairs 10.0, with a launch for the choice 9.1)
-    const int ctas = rows > 2048 ? kCluster : 1;
-    if (int rc = group_args(&a, ids, 1, rows, experts, groups, ctas, top_k)) return rc;
+    if (int rc = group_args(&a, ids, 1, rows, experts, groups)) return rc;
     return with_lanes((int)experts, [&](auto nv) {
         constexpr int NV = decltype(nv)::value;
-        if (rows <= kFew && tokens <= 16) return launch_group_few<NV>(a, route, s);
-        if (inside) return launch_group_variant<NV>(a, route, ctas, s);
+        // (a token for each warp of the plan's launch: 8 of 64 experts, 6 each, 3.6 us; 16 of them, 8 each, 6.2 so and 5.4 in two launches)
+        if (rows <= kFew && tokens <= kFew / 32) return launch_group_few<NV>(a, route, s);
         DependentLaunch l(dim3((unsigned)((tokens + 7) / 8)), 256, s);
         Q4FC_CUDA_OK(cudaLaunchKernelEx(&l.cfg, route_kernel<NV>, route));
-        return launch_group_variant<0>(a, RouteArgs{}, ctas, s);
+        return rows <= kFew ? launch_group_few<0>(a, RouteArgs{}, s) : launch_group(a, s);
     });
 }
 
