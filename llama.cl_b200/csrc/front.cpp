@@ -457,6 +457,20 @@ PyObject* route_top_k(PyObject*, PyObject* const* a, Py_ssize_t n) {
     FRONT_END
 }
 
+// plan_part(plan, first, count) -> a view of its words (torch's own slices of both parts take the host 2.7 us, these 0.5)
+PyObject* plan_part(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    if (!nargs_ok(n, 3)) return nullptr;
+    FRONT_BEGIN
+    const Tensor& t = tensor(a[0], "groups.buf", at::kInt, 1);
+    const int64_t first = as_int(a[1]), count = as_int(a[2]);
+    if (first < 0 || count < 0 || first > t.numel() || count > t.numel() - first) fail("groups: not a plan of these ids");
+    Tensor part = at::detail::make_tensor<c10::TensorImpl>(c10::TensorImpl::VIEW, c10::Storage(t.storage()), t.key_set(), t.dtype());
+    part.unsafeGetTensorImpl()->set_storage_offset(t.storage_offset() + first);
+    part.unsafeGetTensorImpl()->set_sizes_contiguous({count});
+    ret = wrap(std::move(part));
+    FRONT_END
+}
+
 // a plan as made here for these ids
 void* plan_of(PyObject* o, int64_t rows, int64_t n_groups, const at::Device& dev) {
     const Tensor& t = tensor(o, "groups.buf", at::kInt, 1);
@@ -677,6 +691,7 @@ PyMethodDef methods[] = {
     {"q8c_fc", reinterpret_cast<PyCFunction>(q8c_fc), METH_FASTCALL, nullptr},
     {"embedding", reinterpret_cast<PyCFunction>(embedding), METH_FASTCALL, nullptr},
     {"group_rows", reinterpret_cast<PyCFunction>(group_rows), METH_FASTCALL, nullptr},
+    {"plan_part", reinterpret_cast<PyCFunction>(plan_part), METH_FASTCALL, nullptr},
     {"route_top_k", reinterpret_cast<PyCFunction>(route_top_k), METH_FASTCALL, nullptr},
     {"fc_experts", reinterpret_cast<PyCFunction>(fc_experts), METH_FASTCALL, nullptr},
     {"lora", reinterpret_cast<PyCFunction>(lora), METH_FASTCALL, nullptr},

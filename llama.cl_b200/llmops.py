@@ -656,13 +656,12 @@ class RowGroups:
     @property
     def offsets(self) -> torch.Tensor:
         """int32 ``[n_groups + 1]``: the first place in ``order`` of each group, and of the rows without one."""
-        return self.buf[16: 17 + self.n_groups]
+        return _front().plan_part(self.buf, 16, self.n_groups + 1)
 
     @property
     def order(self) -> torch.Tensor:
         """int32 ``[rows]``: row numbers sorted by group, stable; those without a group last."""
-        first = 16 + (self.n_groups + 4) // 4 * 4
-        return self.buf[first: first + self.ids.numel()]
+        return _front().plan_part(self.buf, 16 + (self.n_groups + 4) // 4 * 4, self.ids.numel())
 
 
 def group_rows(ids: torch.Tensor, n_groups: int) -> RowGroups:
