@@ -368,15 +368,15 @@ __global__ void __launch_bounds__(kThreads, 1) experts_few_kernel(const __grid_c
     const int count = __ldcg(p.tile_count);
     __syncthreads();
     // The CTA's stripes and its warps' chunks: equal shares of the chunks, or where tiles cost the SM more than their bytes, of the
-    // tiles' costs.
+    // tiles' costs.  (Places in the list of costs are floats: all CTAs and warps round them alike, and upwards with the place.  With the
+    // divisions of 64-bit integers this took 4 us.)
     const int C = p.chunks;
     int s0, r;
-    auto share = [&](int w) { return (int)((int64_t)r * C * w / kWarps); };  // first chunk of a warp
-    int mine;  // that of warp `lane`
+    int mine;  // first chunk of warp `lane`
     if (!p.weigh) {
-        const int64_t stripes = (int64_t)count * p.Ng;
-        s0 = (int)(stripes * blockIdx.x / gridDim.x), r = (int)(stripes * (blockIdx.x + 1) / gridDim.x) - s0;
-        mine = share(min(lane, kWarps));
+        const int stripes = count * p.Ng, each = stripes / (int)gridDim.x, more = stripes - each * (int)gridDim.x, b = (int)blockIdx.x;
+        s0 = each * b + min(b, more), r = each + (b < more);
+        mine = (int)((int64_t)r * C * min(lane, kWarps) / kWarps);
     } else {
         auto cost = [&](int rows) { return rows <= 2 ? kCosts[0] : rows <= 4 ? kCosts[1] : rows <= 8 ? kCosts[2] : kCosts[3]; };
         if (warp == 0) {  // the costs in front of each tile, of a chunk each
@@ -389,37 +389,34 @@ __global__ void __launch_bounds__(kThreads, 1) experts_few_kernel(const __grid_c
                     const int o = __shfl_up_sync(0xffffffffu, v, off);
                     if (lane >= off) v += o;
                 }
-                if (i0 + lane < count) tiles[i0 + lane].w = sum + v - c;
+                if (i0 + lane < count) tiles[i0 + lane].w = __float_as_int((float)(sum + v - c));
                 sum += __shfl_sync(0xffffffffu, v, 31);
             }
             if (lane == 0) *total = sum;
         }
         __syncthreads();
-        const int all = *total;
-        // of all pieces, `per_tile` a tile, the first one that begins at or behind a cost (in units of a piece's)
-        auto piece_at = [&](int64_t target, int64_t per_tile) {
+        const float all = (float)*total;
+        // of all pieces, `per_tile` a tile, the first one that begins at or behind a place
+        auto piece_at = [&](float place, int per_tile) {
             int lo = 0, hi = count;  // the last tile whose costs begin at or in front of it
             while (hi - lo > 1) {
                 const int mid = (lo + hi) / 2;
-                if (tiles[mid].w * per_tile <= target) lo = mid; else hi = mid;
+                if (__int_as_float(tiles[mid].w) <= place) lo = mid; else hi = mid;
             }
-            const int c = cost(tiles[lo].z);
-            return lo * per_tile + min(per_tile, (target - tiles[lo].w * per_tile + c - 1) / c);
+            const float in = (place - __int_as_float(tiles[lo].w)) * (1.0f / cost(tiles[lo].z));
+            return lo * per_tile + min(per_tile, (int)ceilf(in * per_tile));
         };
-        auto stripe_at = [&](int part) {  // the first stripe of a CTA
-            return count == 0 ? 0 : part >= (int)gridDim.x ? count * p.Ng : (int)piece_at((int64_t)all * p.Ng * part / gridDim.x, p.Ng);
-        };
-        const int edge = stripe_at(blockIdx.x + min(lane, 1));
+        const int part = (int)blockIdx.x + min(lane, 1), parts = (int)gridDim.x;
+        const int edge = count == 0 || part == 0 ? 0 : part == parts ? count * p.Ng : piece_at(all * part / parts, p.Ng);
         s0 = __shfl_sync(0xffffffffu, edge, 0), r = __shfl_sync(0xffffffffu, edge, 1) - s0;
-        mine = 0;
+        mine = lane == 0 ? 0 : r * C;
         if (r > 0) {
-            const int64_t per_tile = (int64_t)p.Ng * C;
-            auto cost_at = [&](int stripe) {  // the costs in front of it
+            auto place_of = [&](int stripe) {
                 const int tile = min(stripe / p.Ng, count - 1);
-                return tiles[tile].w * per_tile + (int64_t)(stripe - tile * p.Ng) * C * cost(tiles[tile].z);
+                return __int_as_float(tiles[tile].w) + (float)(stripe - tile * p.Ng) / p.Ng * cost(tiles[tile].z);
             };
-            const int64_t from = cost_at(s0), to = cost_at(s0 + r);
-            mine = lane >= kWarps ? r * C : (int)(piece_at(from + (to - from) * lane / kWarps, per_tile) - (int64_t)s0 * C);
+            const float from = place_of(s0), to = place_of(s0 + r);
+            if (lane > 0 && lane < kWarps) mine = max(0, min(r * C, piece_at(from + (to - from) * (lane * (1.0f / kWarps)), p.Ng * C) - s0 * C));
         }
     }
     const int begin = __shfl_sync(0xffffffffu, mine, warp), end = __shfl_sync(0xffffffffu, mine, warp + 1);
@@ -494,10 +491,19 @@ __global__ void __launch_bounds__(kThreads, 1) experts_few_kernel(const __grid_c
             put_two(8 + 2 * t, acc[1]);
         }
     }
+    // Stripes that several warps have walked, a warp each; lane w knows what warp w has walked.  (Lane i asks for row i of a stripe's tile
+    // ahead: row by row, each in its turn, these loads took 6 us with 16 rows.)
+    auto rows_of = [&](int li) {
+        if (li >= r) return 0;
+        const int4 tile = tiles[(s0 + li) / p.Ng];
+        return lane < tile.z ? __ldcg(p.order + tile.y + lane) : 0;
+    };
+    int next = rows_of(warp);
     __syncthreads();
-    // stripes that several warps have walked, a warp each; lane w knows what warp w has walked
     const int first = mine, after = __shfl_down_sync(0xffffffffu, mine, 1), last = lane < kWarps ? after : first;
     for (int li = warp; li < r; li += kWarps) {
+        const int at = next;
+        next = rows_of(li + kWarps);
         const bool part_of = first < last && first < (li + 1) * C && last > li * C;
         const uint32_t who = __ballot_sync(0xffffffffu, part_of), ends = __ballot_sync(0xffffffffu, part_of && last <= (li + 1) * C);
         if ((who & (who - 1)) == 0) continue;
@@ -510,7 +516,8 @@ __global__ void __launch_bounds__(kThreads, 1) experts_few_kernel(const __grid_c
                 const int w = __ffs(left) - 1;
                 sum += part(w, ends >> w & 1)[row * 32 + lane];
             }
-            if (n < p.N) p.y[(int64_t)__ldcg(p.order + tile.y + row) * p.ldy + n] = sum;
+            float* y = p.y + (int64_t)__shfl_sync(0xffffffffu, at, row) * p.ldy + n;
+            if (n < p.N) *y = sum;
         }
     }
     if (*fail != 0) {
