@@ -34,7 +34,7 @@ namespace {
 
 constexpr int kWarps = 16, kThreads = kWarps * 32;
 constexpr int kMaxDepth = 3;
-constexpr int kMostTiles = 1024;  // in shared memory
+constexpr int kMostTiles = 2 * kThreads;  // in shared memory
 constexpr int kTileRows = 16;
 
 struct FewParams {
@@ -344,15 +344,15 @@ template <int G, int QTYPE, bool SIGNED>
 __global__ void __launch_bounds__(kThreads, 1) experts_few_kernel(const __grid_constant__ FewParams p) {
     using S = FewShape<G, QTYPE>;
     extern __shared__ __align__(128) uint8_t smem[];
-    // barriers [warp][kMaxDepth] | failure flag, costs | tiles | partial sums of each warp's first stripe [warp][rows][32] | rings
+    // barriers [warp][kMaxDepth] | failure flag, costs by warp | tiles | partial sums of each warp's first stripe [warp][rows][32] | rings
     // [warp][depth].  Those of its last stripe go where its ring was.
     constexpr int kFail = kWarps * kMaxDepth * 8;
-    int4* const tiles = reinterpret_cast<int4*>(smem + kFail + 16);
+    int4* const tiles = reinterpret_cast<int4*>(smem + kFail + 16 + kWarps * 4);
     auto part = [&](int w, bool last) {
         return reinterpret_cast<float*>(smem + (last ? p.ring_off + w * p.depth * S::kSlot : p.part_off + w * p.part_rows * 128));
     };
     volatile int* fail = reinterpret_cast<volatile int*>(smem + kFail);
-    int* const total = reinterpret_cast<int*>(smem + kFail + 4);  // the costs of all tiles
+    int* const by_warp = reinterpret_cast<int*>(smem + kFail + 16);  // costs of the tiles that a warp has loaded
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const uint32_t bars = smem_u32(smem) + warp * kMaxDepth * 8;
     if (lane < p.depth) mbar_init(bars + 8 * lane, 1);
@@ -360,16 +360,42 @@ __global__ void __launch_bounds__(kThreads, 1) experts_few_kernel(const __grid_c
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     // The plan, and then the weights: the quantizer in front has let this launch begin only when what is in front of it was complete.
-    for (int i = threadIdx.x; i < p.most_tiles; i += kThreads) {
-        int4 tile = __ldcg(p.tiles + i);
-        tile.z = min(tile.z, p.part_rows);
-        tiles[i] = tile;
-    }
     const int count = __ldcg(p.tile_count);
+    auto cost = [&](int rows) { return rows <= 2 ? kCosts[0] : rows <= 4 ? kCosts[1] : rows <= 8 ? kCosts[2] : kCosts[3]; };
+    int4 two[2];  // of the tiles, this thread's (kMostTiles)
+    int costs[2] = {0, 0}, all = 0;
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+        const int i = 2 * threadIdx.x + k;
+        two[k] = i < p.most_tiles ? __ldcg(p.tiles + i) : make_int4(0, 0, 0, 0);
+        two[k].z = min(two[k].z, p.part_rows);
+        if (i < count) costs[k] = cost(two[k].z);
+    }
+    if (p.weigh) {  // the costs in front of each tile, of a chunk each
+        int v = costs[0] + costs[1];
+#pragma unroll
+        for (int off = 1; off < 32; off <<= 1) {
+            const int o = __shfl_up_sync(0xffffffffu, v, off);
+            if (lane >= off) v += o;
+        }
+        if (lane == 31) by_warp[warp] = v;
+        __syncthreads();
+        v -= costs[0] + costs[1];
+#pragma unroll
+        for (int w = 0; w < kWarps; w++) {
+            const int c = by_warp[w];
+            all += c;
+            if (w < warp) v += c;
+        }
+        two[0].w = __float_as_int((float)v), two[1].w = __float_as_int((float)(v + costs[0]));
+    }
+#pragma unroll
+    for (int k = 0; k < 2; k++)
+        if (2 * (int)threadIdx.x + k < p.most_tiles) tiles[2 * threadIdx.x + k] = two[k];
     __syncthreads();
     // The CTA's stripes and its warps' chunks: equal shares of the chunks, or where tiles cost the SM more than their bytes, of the
     // tiles' costs.  (Places in the list of costs are floats: all CTAs and warps round them alike, and upwards with the place.  With the
-    // divisions of 64-bit integers this took 4 us.)
+    // divisions of 64-bit integers, and the costs summed by one warp, this took 4 us.)
     const int C = p.chunks;
     int s0, r;
     int mine;  // first chunk of warp `lane`
@@ -378,45 +404,34 @@ __global__ void __launch_bounds__(kThreads, 1) experts_few_kernel(const __grid_c
         s0 = each * b + min(b, more), r = each + (b < more);
         mine = (int)((int64_t)r * C * min(lane, kWarps) / kWarps);
     } else {
-        auto cost = [&](int rows) { return rows <= 2 ? kCosts[0] : rows <= 4 ? kCosts[1] : rows <= 8 ? kCosts[2] : kCosts[3]; };
-        if (warp == 0) {  // the costs in front of each tile, of a chunk each
-            int sum = 0;
-            for (int i0 = 0; i0 < count; i0 += 32) {
-                const int c = i0 + lane < count ? cost(tiles[i0 + lane].z) : 0;
-                int v = c;
-#pragma unroll
-                for (int off = 1; off < 32; off <<= 1) {
-                    const int o = __shfl_up_sync(0xffffffffu, v, off);
-                    if (lane >= off) v += o;
-                }
-                if (i0 + lane < count) tiles[i0 + lane].w = __float_as_int((float)(sum + v - c));
-                sum += __shfl_sync(0xffffffffu, v, 31);
-            }
-            if (lane == 0) *total = sum;
-        }
-        __syncthreads();
-        const float all = (float)*total;
-        // of all pieces, `per_tile` a tile, the first one that begins at or behind a place
-        auto piece_at = [&](float place, int per_tile) {
-            int lo = 0, hi = count;  // the last tile whose costs begin at or in front of it
+        auto front = [&](int tile) { return __int_as_float(tiles[tile].w); };
+        auto tile_at = [&](float place, int lo, int hi) {  // of tiles [lo, hi) the last whose costs begin at or in front of a place
             while (hi - lo > 1) {
                 const int mid = (lo + hi) / 2;
-                if (__int_as_float(tiles[mid].w) <= place) lo = mid; else hi = mid;
+                if (front(mid) <= place) lo = mid; else hi = mid;
             }
-            const float in = (place - __int_as_float(tiles[lo].w)) * (1.0f / cost(tiles[lo].z));
-            return lo * per_tile + min(per_tile, (int)ceilf(in * per_tile));
+            return lo;
         };
-        const int part = (int)blockIdx.x + min(lane, 1), parts = (int)gridDim.x;
-        const int edge = count == 0 || part == 0 ? 0 : part == parts ? count * p.Ng : piece_at(all * part / parts, p.Ng);
-        s0 = __shfl_sync(0xffffffffu, edge, 0), r = __shfl_sync(0xffffffffu, edge, 1) - s0;
+        // of a tile's pieces the first one that begins at or behind a place
+        auto piece_at = [&](float place, int tile, int pieces) {
+            return min(pieces, (int)ceilf((place - front(tile)) * (1.0f / cost(tiles[tile].z)) * pieces));
+        };
+        const int part = (int)blockIdx.x + min(lane, 1), parts = (int)gridDim.x;  // lane 0: where the CTA begins, 1: where it ends
+        int tile = 0, in = 0;
+        float place = 0.0f;
+        if (count > 0) {
+            place = (float)(all * part) / parts, tile = tile_at(place, 0, count);
+            in = part == 0 ? 0 : part == parts ? p.Ng : piece_at(place, tile, p.Ng);
+            place = front(tile) + (float)in / p.Ng * cost(tiles[tile].z);
+        }
+        const int first_tile = __shfl_sync(0xffffffffu, tile, 0), last_tile = __shfl_sync(0xffffffffu, tile, 1);
+        const float from = __shfl_sync(0xffffffffu, place, 0), to = __shfl_sync(0xffffffffu, place, 1);
+        const int stripe = tile * p.Ng + in;
+        s0 = __shfl_sync(0xffffffffu, stripe, 0), r = __shfl_sync(0xffffffffu, stripe, 1) - s0;
         mine = lane == 0 ? 0 : r * C;
-        if (r > 0) {
-            auto place_of = [&](int stripe) {
-                const int tile = min(stripe / p.Ng, count - 1);
-                return __int_as_float(tiles[tile].w) + (float)(stripe - tile * p.Ng) / p.Ng * cost(tiles[tile].z);
-            };
-            const float from = place_of(s0), to = place_of(s0 + r);
-            if (lane > 0 && lane < kWarps) mine = max(0, min(r * C, piece_at(from + (to - from) * (lane * (1.0f / kWarps)), p.Ng * C) - s0 * C));
+        if (r > 0 && lane > 0 && lane < kWarps) {
+            place = from + (to - from) * (lane * (1.0f / kWarps)), tile = tile_at(place, first_tile, last_tile + 1);
+            mine = max(0, min(r * C, tile * p.Ng * C + piece_at(place, tile, p.Ng * C) - s0 * C));
         }
     }
     const int begin = __shfl_sync(0xffffffffu, mine, warp), end = __shfl_sync(0xffffffffu, mine, warp + 1);
@@ -510,14 +525,20 @@ __global__ void __launch_bounds__(kThreads, 1) experts_few_kernel(const __grid_c
         const int sg = s0 + li, ti = sg / p.Ng;
         const int4 tile = tiles[ti];
         const int64_t n = (int64_t)(sg - ti * p.Ng) * 32 + lane;
-        for (int row = 0; row < tile.z; row++) {
-            float sum = 0.0f;
+        for (int row0 = 0; row0 < tile.z; row0 += 4) {
+            float sum[4] = {};
             for (uint32_t left = who; left; left &= left - 1) {
                 const int w = __ffs(left) - 1;
-                sum += part(w, ends >> w & 1)[row * 32 + lane];
+                const float* from = part(w, ends >> w & 1) + row0 * 32 + lane;
+#pragma unroll
+                for (int k = 0; k < 4; k++)
+                    if (row0 + k < tile.z) sum[k] += from[k * 32];
             }
-            float* y = p.y + (int64_t)__shfl_sync(0xffffffffu, at, row) * p.ldy + n;
-            if (n < p.N) *y = sum;
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                float* y = p.y + (int64_t)__shfl_sync(0xffffffffu, at, row0 + k) * p.ldy + n;
+                if (row0 + k < tile.z && n < p.N) *y = sum[k];
+            }
         }
     }
     if (*fail != 0) {
@@ -535,7 +556,7 @@ int launch_few(FewParams p, const DeviceInfo* di, cudaStream_t s) {
         Q4FC_CUDA_OK(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, di->max_smem_optin));
         if (di->index < 64) attr_done[di->index] = true;
     }
-    p.part_off = (int)align_up(kWarps * kMaxDepth * 8 + 16 + (size_t)p.most_tiles * 16, 128);
+    p.part_off = (int)align_up(kWarps * kMaxDepth * 8 + 16 + kWarps * 4 + (size_t)p.most_tiles * 16, 128);
     p.ring_off = p.part_off + kWarps * p.part_rows * 128;
     // What the rings leave of the SM's memory is L1, and codes and scales come through it: 64 experts x 1408 x 2048, group
     // 32, with rings of 2, 3 and 4 chunks a warp 16 rows each 54.4, 55.2 and 57.9 us, one row 27.6, 27.3 and 27.7; 8 x 4096 x
