@@ -18,10 +18,10 @@
 // group's scales, serves all four (or two).  Up to 16 rows are two sets of eight columns on weights that are unpacked once.
 // Codes and scales come from global memory, through L1.
 //
-// Measured, with the quantizer in front: one token to two of 8 experts, 4096 x 22016, Q4_1 group 32: 113 MB in 23.3 us, 4.8 TB/s (the same
-// copies without the arithmetic 23.2 when the whole took 27.5: start, ramp and the last stripes' meeting are the rest); 8 tokens to 6 of 64, 2048 x
-// 2816, group 128: 29.0; 170 tokens to 6 of 64, 1408 x 2048, group 32: 60.3.  There the scaling, in fp32 for every row, column and K group,
-// is the work: 0.45 instructions a cycle and scheduler, fixed latencies first among the waits (fewer instructions alone changed nothing).
+// Measured, with the quantizer in front: one token to two of 8 experts, 4096 x 22016, Q4_1 group 32: 113 MB in 22.4 to 23.3 us, 5 TB/s; 8 tokens
+// to 6 of 64, 2048 x 2816, group 128: 28.2; 170 tokens to 6 of 64, 1408 x 2048, group 32: 48.4.  There the scaling, in fp32 for every row,
+// column and K group, is the work: half an instruction a cycle and scheduler, fixed latencies first among the waits (fewer instructions alone
+// changed nothing).
 #include "decode_math.cuh"
 #include "groups.cuh"
 #include "ring_ptx.cuh"
@@ -60,9 +60,9 @@ __device__ __forceinline__ bool elect_lane() {  // one lane of a converged warp
     return p != 0;
 }
 
-// What a chunk costs in a tile of at most 2, 4, 8 and 16 rows.  (64 experts x 1408 x 2048, group 32, all with as many rows: 28, 32, 36 and
-// 54 us, of which other launches take 6 to 10.  170 tokens to 6 of them each: equal shares of the stripes 65.3 us, these costs 60.1.)
-__device__ constexpr int kCosts[4] = {5, 6, 7, 10};
+// What a chunk costs in a tile of at most 2, 4, 8 and 16 rows.  (64 experts x 1408 x 2048, group 32, all with as many rows: 28, 29, 30 and
+// 42 us, of which other launches take 6 to 10.  170 tokens to 6 of them each: equal shares of the stripes 5 us more.)
+__device__ constexpr int kCosts[4] = {6, 6, 7, 10};
 
 template <int G, int QTYPE>
 struct FewShape {
@@ -559,8 +559,7 @@ int launch_few(FewParams p, const DeviceInfo* di, cudaStream_t s) {
     p.part_off = (int)align_up(kWarps * kMaxDepth * 8 + 16 + kWarps * 4 + (size_t)p.most_tiles * 16, 128);
     p.ring_off = p.part_off + kWarps * p.part_rows * 128;
     // What the rings leave of the SM's memory is L1, and codes and scales come through it: 64 experts x 1408 x 2048, group
-    // 32, with rings of 2, 3 and 4 chunks a warp 16 rows each 54.4, 55.2 and 57.9 us, one row 27.6, 27.3 and 27.7; 8 x 4096 x
-    // 22016, 2 rows 23.5, 23.3 and 23.8.
+    // 32, with rings of 2 and 3 chunks a warp 16 rows each 42.6 and 43.6 us (of 4, before, 3 more), one row 27.2 and 27.1.
     p.depth = p.weigh ? 2 : kMaxDepth;
     DependentLaunch l(dim3((unsigned)di->sm_count), kThreads, s);
     l.cfg.dynamicSmemBytes = (size_t)p.ring_off + (size_t)p.depth * kWarps * S::kSlot;
@@ -570,13 +569,13 @@ int launch_few(FewParams p, const DeviceInfo* di, cudaStream_t s) {
 
 }  // namespace
 
-// Up to 80 rows an expert in the mean with group 32, up to 16 with group 128, whose 64-row tiles on tcgen05 have a quarter of the groups to
-// scale.  This kernel and those tiles, us, whole call, 32 experts x 2048 x 2048: group 32, 16 rows 45 and 72, 64 rows 115 and 142, 96
-// rows 174 and 193; group 128, 12 rows 34 and 38, 16 rows 38 and 39, 20 rows 48 and 40; 8 x 4096 x 8192: group 32, 64 rows 227 and 271, 96
-// rows 328 and 348; group 128, 16 rows 59 and 63, 20 rows 68 and 65.  (Its list of stripes is counted in 32 bits.)
+// Up to 96 rows an expert in the mean with group 32, up to 20 with group 128, whose 64-row tiles on tcgen05 have a quarter of the groups to
+// scale.  This kernel and those tiles, us, whole call, 32 experts x 2048 x 2048: group 32, 16 rows 38 and 72, 64 rows 105 and 142, 96
+// rows 165 and 193; group 128, 16 rows 33 and 39, 20 rows 39 and 40, 32 rows 53 and 44; 8 x 4096 x 8192: group 32, 64 rows 219 and 272, 96
+// rows 301 and 348; group 128, 20 rows 64 and 65, 24 rows 71 and 65.  (Its list of stripes is counted in 32 bits.)
 bool experts_few_serves(int64_t rows, int64_t Kg, int64_t Ng, int G, int64_t n) {
     const int64_t tiles = most_tiles(kTiles16, rows, n);
-    return rows <= (G == 32 ? 80 : 16) * n && tiles <= kMostTiles && (Kg * G + 127) / 128 * Ng * tiles <= 0x7fffffffLL / 8;
+    return rows <= (G == 32 ? 96 : 20) * n && tiles <= kMostTiles && (Kg * G + 127) / 128 * Ng * tiles <= 0x7fffffffLL / 8;
 }
 
 size_t experts_few_scratch(int64_t rows, int64_t Kg, int G, int64_t n) {
