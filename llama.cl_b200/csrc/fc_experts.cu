@@ -14,15 +14,15 @@ struct Combine {
     const float *h, *weights;  // [tokens * top_k][ldh]
     float* y;
     int64_t tokens, N, ldh, ldy;
+    unsigned per;  // CTAs of a token
     int top_k;
 };
-// V columns a thread
+// V columns a thread.  Bound by h and y at many tokens: 4096 of them, 8 slots, 4096 columns, 604 MB in 96 us; 2048, 2 slots, 22016, 541 MB in 118.
 template <int V>
 __global__ void __launch_bounds__(256) combine_kernel(const Combine a) {
     pdl_wait_prior_grid();
     pdl_launch_dependents();
-    const int64_t per = (a.N + 256 * V - 1) / (256 * V), t = blockIdx.x / per;
-    const int64_t n = ((blockIdx.x - t * per) * 256 + threadIdx.x) * V;
+    const int64_t t = blockIdx.x / a.per, n = ((int64_t)(blockIdx.x % a.per) * 256 + threadIdx.x) * V;
     if (n >= a.N) return;
     float sum[V] = {};
 #pragma unroll 4
@@ -43,13 +43,14 @@ __global__ void __launch_bounds__(256) combine_kernel(const Combine a) {
         *y = sum[0];
 }
 
-int launch_combine(const Combine& c, cudaStream_t s) {
+int launch_combine(Combine c, cudaStream_t s) {
     const bool vec = c.N % 4 == 0 && c.ldy % 4 == 0 && (reinterpret_cast<uintptr_t>(c.y) & 15) == 0;
-    const int64_t grid = c.tokens * ((c.N + (vec ? 1023 : 255)) / (vec ? 1024 : 256));
+    const int64_t per = (c.N + (vec ? 1023 : 255)) / (vec ? 1024 : 256), grid = c.tokens * per;
     if (grid > 0x7fffffffLL) {
         set_error("fc_experts: %lld tokens x %lld exceeds the grid limit", (long long)c.tokens, (long long)c.N);
         return Q4FC_ELIMIT;
     }
+    c.per = (unsigned)per;
     DependentLaunch l(dim3((unsigned)grid), 256, s);
     Q4FC_CUDA_OK(cudaLaunchKernelEx(&l.cfg, vec ? combine_kernel<4> : combine_kernel<1>, c));
     return Q4FC_OK;
@@ -67,7 +68,7 @@ size_t experts_scratch_bytes(int64_t rows, int64_t K, int64_t N, int G, int64_t 
 }
 
 int launch_fc_experts(ExpertsCall c, const float* weights, int64_t top_k, cudaStream_t s) {
-    const Combine sum = {reinterpret_cast<const float*>(c.scratch), weights, c.y, c.rows / top_k, c.N, c.N, c.ldy, (int)top_k};
+    const Combine sum = {reinterpret_cast<const float*>(c.scratch), weights, c.y, c.rows / top_k, c.N, c.N, c.ldy, 0, (int)top_k};
     if (weights) {
         c.y = reinterpret_cast<float*>(c.scratch), c.ldy = c.N;
         c.scratch += hidden_bytes(c.rows, c.N, true);
