@@ -263,6 +263,22 @@ def test_an_infinite_weight_reaches_its_column_alone(pkg, rank, rows, dtype):
     assert torch.equal(got[0][~hit], want[0][~hit]) and not got[0][hit].isfinite().any()
 
 
+@pytest.mark.parametrize("G", [32, 128])
+@pytest.mark.parametrize("tokens,n,top_k", [(700, 1000, 1), (2000, 1000, 2), (300, 1024, 32), (60, 1024, 4)])
+def test_hundreds_of_experts(pkg, tokens, n, top_k, G):
+    """As many tiles as the kernel for few rows lists, more than that, and most experts without a row."""
+    K, N = 100, 40
+    rng = np.random.default_rng(tokens)
+    ids = np.stack([rng.choice(n, top_k, replace=False) for _ in range(tokens)])
+    ids[: tokens // 8, 0] = n - 1  # one expert with many
+    some = pack(pkg, 7, N, K, 1, G, 3)
+    wq = some[torch.arange(n, device="cuda") % 7].contiguous()
+    g = torch.Generator().manual_seed(1)
+    x = torch.randn(1, tokens, K, generator=g)
+    got = pkg.llmops.fc_Q4A_experts(x.cuda(), wq, N, groups_of(pkg, ids, n))
+    check(got, *want64(x[0].numpy(), ids % 7, some.cpu().numpy(), N, 1, G))
+
+
 def test_experts_beyond_32_bit_offsets(pkg):
     """5 GB of experts, the last one chosen; then 9.6 GB of outputs."""
     ops, n, K, N = pkg.llmops, 1024, 4096, 2048
