@@ -14,7 +14,7 @@
 //
 // Bound by the bytes of x, A, B and y where there are many, and in front of that by dependent steps: plan, rows, K, the sums' meeting, columns.
 // Measured, both products: 8 rows x 4096 x 4096, 8 bf16 adapters of rank 16 (2 MB) 6.1 us, 61 rows x 4096 x 11008, 40 fp16 ones of rank 64
-// (65 MB) 22.4, 2048 rows x 4096 x 4096, 4 bf16 ones of rank 32 (34 MB of x, 67 of y) 36.4; shrink alone 7.1 of the second, 15.4 of the third.
+// (65 MB) 22.4, 2048 rows x 4096 x 4096, 4 bf16 ones of rank 32 (34 MB of x, 67 of y) 37.4; shrink alone 7.1 of the second, 16.5 of the third.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 
@@ -99,7 +99,7 @@ struct LoraArgs {
 
 // A_i x of eight rows and MB times 16 ranks, by one warp: pieces of 32 k from k0 on, `step` apart, up to k_end.  `x`: the row of lane (g, t)'s
 // g, if `live`; `ranks`: of A that are there.  acc[m][i]: rank m * 16 + 8 (i / 2) + g of row 2t + i % 2.
-template <typename T, int MB, bool VEC>
+template <typename T, int MB, bool VEC, bool LONG>
 __device__ __forceinline__ void shrink_rows(const float* x, bool live, const T* a, int ranks, int64_t K, int64_t k0, int64_t k_end, int64_t step,
                                             float (&acc)[MB][4]) {
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -118,6 +118,22 @@ __device__ __forceinline__ void shrink_rows(const float* x, bool live, const T* 
                 load_values<8, VEC>(a + (int64_t)r * K + k, r < ranks ? valid : 0, c.w[m][h]);
             }
     };
+    // An MMA cuts its sum off, always towards zero, so that a long chain of them shrinks.  LONG: after eight or nine pieces the sums move to
+    // where additions round (1270 rows x 2011, fp32: 1.6e-5 of the outputs, so 4e-6; 1 us of 36 at 2048 rows x 4096 x 4096).  Where warps and
+    // CTAs divide K, chains are short.
+    float moved[MB][4];
+    float(&part)[MB][4] = LONG ? moved : acc;
+    auto move = [&] {
+#pragma unroll
+        for (int m = 0; m < MB; m++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) acc[m][i] += moved[m][i], moved[m][i] = 0.0f;
+    };
+    if constexpr (LONG)
+#pragma unroll
+        for (int m = 0; m < MB; m++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) moved[m][i] = 0.0f;
     auto multiply = [&](const Piece& c) {
 #pragma unroll
         for (int j = 0; j < 4; j++) {
@@ -127,9 +143,9 @@ __device__ __forceinline__ void shrink_rows(const float* x, bool live, const T* 
             for (int m = 0; m < MB; m++) {
                 uint32_t wh[4], wl[4];
                 operand(c.w[m][0][2 * j], c.w[m][1][2 * j], c.w[m][0][2 * j + 1], c.w[m][1][2 * j + 1], wh, wl);
-                if constexpr (sizeof(T) == 4) mma_tf32(acc[m], wl, hi0, hi1);
-                mma_tf32(acc[m], wh, lo0, lo1);
-                mma_tf32(acc[m], wh, hi0, hi1);
+                if constexpr (sizeof(T) == 4) mma_tf32(part[m], wl, hi0, hi1);
+                mma_tf32(part[m], wh, lo0, lo1);
+                mma_tf32(part[m], wh, hi0, hi1);
             }
         }
     };
@@ -141,6 +157,8 @@ __device__ __forceinline__ void shrink_rows(const float* x, bool live, const T* 
         for (int d = 0; d + 1 < kDepth; d++)
             if (k0 + d * step < k_end) load(k0 + d * step, c[d]);
     }
+    constexpr int kMoves = kDepth == 3 ? 3 : 8 / kDepth;
+    int left = kMoves;
     while (k0 < k_end) {
 #pragma unroll
         for (int d = 0; d < kDepth; d++) {
@@ -149,7 +167,9 @@ __device__ __forceinline__ void shrink_rows(const float* x, bool live, const T* 
             multiply(c[d]);
             k0 += step;
         }
+        if (LONG && --left == 0) move(), left = kMoves;
     }
+    if constexpr (LONG) move();
 }
 
 // y += B t, or without `onto` y = B t, by one warp: 16 columns of NB times eight rows at a time, the next kAcross further; the next
@@ -310,7 +330,8 @@ __global__ void __launch_bounds__(kThreads, 2) lora_few_kernel(const __grid_cons
         const bool live = g < tile.z;
         const float* x = p.x + (live ? (int64_t)__ldcg(p.order + tile.y + g) * p.ldx : 0);
         float acc[MB][4] = {};
-        shrink_rows<T, MB, VEC>(x, live, static_cast<const T*>(p.a) + (int64_t)tile.x * p.rank * p.K, p.rank, p.K, k_begin + warp * 32, k_end, kWarps * 32, acc);
+        shrink_rows<T, MB, VEC, false>(x, live, static_cast<const T*>(p.a) + (int64_t)tile.x * p.rank * p.K, p.rank, p.K, k_begin + warp * 32, k_end,
+                                       kWarps * 32, acc);
         float* mine = by_warp + warp * 8 * kRanks;
 #pragma unroll
         for (int m = 0; m < MB; m++)
@@ -371,7 +392,7 @@ __global__ void __launch_bounds__(kThreads, 2) lora_shrink_kernel(const __grid_c
     const float* x = p.x + (live ? (int64_t)__ldcg(p.order + tile.y + row0 + g) * p.ldx : 0);
     float acc[MB][4] = {};
     if (row0 < tile.z)
-        shrink_rows<T, MB, VEC>(x, live, static_cast<const T*>(p.a) + ((int64_t)tile.x * p.rank + rank0) * p.K, p.rank - rank0, p.K,
+        shrink_rows<T, MB, VEC, !kByK>(x, live, static_cast<const T*>(p.a) + ((int64_t)tile.x * p.rank + rank0) * p.K, p.rank - rank0, p.K,
                                 k_begin + (kByK ? warp * 32 : 0), k_end, kByK ? kWarps * 32 : 32, acc);
     float* mine = kByK ? by_warp + warp * TILE * kRanks : sums + row0 * kRanks;
 #pragma unroll
