@@ -18,6 +18,8 @@
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 
+#include <atomic>
+
 #include "groups.cuh"
 #include "quant_pre.cuh"
 
@@ -29,6 +31,7 @@ namespace {
 constexpr int kWarps = 8, kThreads = kWarps * 32;
 constexpr int kRankBlock = 64;   // ranks of a CTA in shrink
 constexpr int kMostSlices = 8;   // CTAs of a cluster
+constexpr int kMostRanks = 256;
 
 // D(16x8) += A(16x8) * B(8x8)
 __device__ __forceinline__ void mma_tf32(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -537,8 +540,15 @@ int launch_expand(const LoraCall& c, const LoraArgs& p, bool onto, int64_t tiles
     DependentLaunch l(dim3((unsigned)(pieces < most ? pieces : most)), kThreads, s);
     auto* fn = vec ? lora_expand_kernel<T, TILE, QUADS, PIECES, true> : lora_expand_kernel<T, TILE, QUADS, PIECES, false>;
     l.cfg.dynamicSmemBytes = expand_rows(TILE) * (size_t)expand_pitch((int)(c.rank + kChunk - 1) / kChunk * kChunk);
-    if (l.cfg.dynamicSmemBytes > 48 * 1024)
-        Q4FC_CUDA_OK(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)l.cfg.dynamicSmemBytes));
+    // (what the highest rank needs, whatever this call's: a limit of its own would be another host thread's between that one's launch and its own)
+    constexpr int kMost = expand_rows(TILE) * expand_pitch(kMostRanks);
+    if constexpr (kMost > 48 * 1024) {
+        static std::atomic<bool> attr_done[2][64] = {};  // set once per device; a second setter repeats the same call
+        if (di->index >= 64 || !attr_done[vec][di->index]) {
+            Q4FC_CUDA_OK(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, kMost));
+            if (di->index < 64) attr_done[vec][di->index] = true;
+        }
+    }
     Q4FC_CUDA_OK(cudaLaunchKernelEx(&l.cfg, fn, p, onto));
     return Q4FC_OK;
 }

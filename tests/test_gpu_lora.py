@@ -211,3 +211,36 @@ def test_refusals(pkg):
             (lambda: add(y[:, :2].contiguous(), x, a, b, groups), "out: expected")):
         with pytest.raises(RuntimeError, match=text):
             bad()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_ranks_of_several_host_threads(pkg, dtype):
+    """Ranks that need different amounts of shared memory of one kernel, called at once, each on a stream of its own."""
+    import threading
+
+    n, rows, K, N = 2, 256, 64, 64
+    failed, sums = [], {}
+
+    def work(rank):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                x, a, b, _ = inputs(rows, n, rank, K, N, dtype)
+                groups = groups_of(pkg, np.arange(rows) % n, n)
+                y = torch.zeros(1, rows, N, device="cuda")
+                for _ in range(2000):
+                    pkg.llmops.lora_add(y, x, a, b, groups)
+                one = torch.zeros(1, rows, N, device="cuda")
+                pkg.llmops.lora_add(one, x, a, b, groups)
+                torch.cuda.current_stream().synchronize()
+                sums[rank] = (one.cpu(), x, a, b)
+        except Exception as e:  # (a thread's error would go nowhere)
+            failed.append((rank, str(e)))
+
+    threads = [threading.Thread(target=work, args=(rank,)) for rank in (160, 256, 144, 224)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed
+    for one, x, a, b in sums.values():
+        check(one, *added64(x, a, b, None, np.arange(rows) % n))
