@@ -46,7 +46,7 @@ enum {
     Q4FC_EALIGN = 3,    /* a pointer or leading dimension misses its alignment */
     Q4FC_EWORKSPACE = 4,/* workspace missing or smaller than q4fc_fc_workspace_bytes() */
     Q4FC_ECUDA = 5,     /* a CUDA runtime call failed (launch, attribute) */
-    Q4FC_EDEVICE = 6,   /* a kernel reported a bounded wait that ran out */
+    Q4FC_EDEVICE = 6,   /* a kernel reported a bounded wait that ran out, or an id out of range */
     Q4FC_ELIMIT = 7     /* size beyond a stated maximum of the entry point */
 };
 
@@ -496,8 +496,8 @@ int q4fc_fc_lora(const q4fc_lora_call* call, const void* wq, int64_t Ng, int64_t
 /* Reads and clears the device status word kept at the start of a workspace
  * (host-synchronous: waits for `stream`).  ws = NULL reads the word that decode
  * calls made without a workspace share (one per device).  Returns Q4FC_OK or
- * Q4FC_EDEVICE (a bounded wait inside a kernel ran out, or an embedding id was out of range; the results
- * are invalid). */
+ * Q4FC_EDEVICE (a bounded wait inside a kernel ran out, or an id of an embedding, an expert or an adapter was
+ * out of range; the results are invalid.  q4fc_last_error() says which of them, all that apply). */
 int q4fc_fc_check_status(void* ws, q4fc_stream_t stream);
 
 #if defined(__GNUC__)

@@ -186,7 +186,7 @@ const char* q4fc_strerror(int code) {
         case Q4FC_EALIGN: return "misaligned pointer or leading dimension";
         case Q4FC_EWORKSPACE: return "workspace missing or too small";
         case Q4FC_ECUDA: return "CUDA runtime error";
-        case Q4FC_EDEVICE: return "device-side wait ran out";
+        case Q4FC_EDEVICE: return "a kernel reported a failure";
         case Q4FC_ELIMIT: return "size beyond a supported maximum";
         default: return "unknown error";
     }
@@ -1008,9 +1008,10 @@ int q4fc_fc_check_status(void* ws, q4fc_stream_t stream) {
     Q4FC_CUDA_OK(cudaStreamSynchronize(s));
     if (status != 0) {
         Q4FC_CUDA_OK(cudaMemsetAsync(ws, 0, sizeof(int), s));
-        const bool bad_id = (status & kStatusBadId) != 0, wait = (status & ~kStatusBadId) != 0;
-        set_error("device status word = 0x%x (%s%s%s)", status, bad_id ? "an embedding id was out of range" : "",
-                  bad_id && wait ? "; " : "", wait ? "a bounded wait ran out" : "");
+        const bool bad_id = (status & kStatusBadId) != 0, bad_group = (status & kStatusBadGroup) != 0, wait = (status & ~kStatusIds) != 0;
+        set_error("device status word = 0x%x (%s%s%s%s%s)", status, bad_id ? "an embedding id was out of range" : "",
+                  bad_id && bad_group ? "; " : "", bad_group ? "an id of an expert or adapter was out of range" : "",
+                  (bad_id || bad_group) && wait ? "; " : "", wait ? "a bounded wait ran out" : "");
         return Q4FC_EDEVICE;
     }
     return Q4FC_OK;

@@ -613,8 +613,7 @@ __global__ void __launch_bounds__(kThreads, 1) fc_prefill_wide_kernel(const Pref
     tc_fence_before();
     __syncthreads();
     if (*aborted) {
-        if (threadIdx.x == 0 && (atomicCAS(p.status, 0, 0x50524546) & ~kStatusBadId) == 0)  // 'PREF': a bounded wait ran out
-            atomicOr(p.status, 0x50524546);
+        if (threadIdx.x == 0) note_wait(p.status, 0x50524546);  // 'PREF': a bounded wait ran out
         // copies that may still be in flight land before the shared memory is handed to another CTA
 #pragma unroll 1
         for (int i = 0; i < 64; i++) __nanosleep(32000);

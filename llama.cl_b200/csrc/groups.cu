@@ -124,7 +124,7 @@ struct GroupArgs {
 };
 __device__ __forceinline__ int bin_of(const GroupArgs& a, int64_t i) {
     const int64_t id = a.i32 ? (int64_t)__ldcg(static_cast<const int*>(a.ids) + i) : (int64_t)__ldcg(static_cast<const long long*>(a.ids) + i);
-    if (id >= a.n) atomicOr(a.status, kStatusBadId);
+    if (id >= a.n) atomicOr(a.status, kStatusBadGroup);
     return id >= 0 && id < a.n ? (int)id : a.n;
 }
 

@@ -41,6 +41,15 @@ __device__ __forceinline__ unsigned long long globaltimer_ns() {
     asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
     return t;
 }
+// The code of a wait that ran out into a status word, beside what bad ids have left there, unless it has one already.
+__device__ __forceinline__ void note_wait(int* status, int code) {
+    int ids = 0;
+    for (int i = 0; i < 3; i++) {  // (two bits can come in between)
+        const int seen = atomicCAS(status, ids, ids | code);
+        if (seen == ids || (seen & ~kStatusIds) != 0) return;
+        ids = seen;
+    }
+}
 // Bounded wait on an mbarrier phase.  Once one wait of the CTA has run out (*fail != 0) all others end at once.
 __device__ __forceinline__ void mbar_wait(uint32_t bar, uint32_t parity, volatile int* fail, int* status, int code) {
     if (mbar_try_wait(bar, parity)) return;
@@ -51,7 +60,7 @@ __device__ __forceinline__ void mbar_wait(uint32_t bar, uint32_t parity, volatil
             if (*fail != 0) return;
             if (globaltimer_ns() - t0 > kWaitLimitNs) {
                 *fail = 1;
-                atomicCAS(status, 0, code);
+                note_wait(status, code);
                 return;
             }
         }

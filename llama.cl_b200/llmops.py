@@ -721,7 +721,8 @@ def lora_add(output: torch.Tensor, input: torch.Tensor, lora_a: torch.Tensor, lo
 
 def check_device_status(device: torch.device | str | int | None = None) -> None:
     """Raises if a kernel launched without a workspace on this device reported a failure (a bounded wait that ran
-    out, an embedding id outside its table).  Host-synchronous on the current stream."""
+    out, an embedding id outside its table, an id of an expert or adapter that does not exist), and says which.
+    Host-synchronous on the current stream."""
     dev = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
     with torch.cuda.device(dev):
         _cabi.check(_cabi.lib().q4fc_fc_check_status(None, _stream_ptr(dev)), "check_device_status")
