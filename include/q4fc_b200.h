@@ -466,8 +466,10 @@ int q4fc_fc_experts(const q4fc_experts_call* call, void* ws, size_t ws_bytes, un
 /* Low-rank adapters of many requests beside a shared projection: for every row m of a group i of the plan
  *   y[m] += scales[i] * lora_b[i] . (lora_a[i] . x[m])
  * with lora_a [adapters][rank][K], lora_b [adapters][N][rank], both of one dtype and dense, x as it is (not quantized) and
- * sums in fp32 (a product of two numbers is off by 2^-20 of it at most; an infinity in x or an adapter reaches the outputs
- * it belongs to as infinity or NaN).  Rows without a group are left as they are.  scales: fp32 [adapters], or NULL for ones.  rank 1..256.
+ * sums in fp32.  Of x, of fp32 weights and of lora_a . x 22 bits are used (a product of two numbers is off by 2^-20 of it at
+ * most), and sixteen terms at a time are summed with bits cut off: outputs are off by 2e-7 to 5e-7 of their size in the 2-norm,
+ * where plain fp32 sums are by 1e-7 to 2e-7.  An infinity in x or an adapter reaches the outputs it belongs to as infinity or
+ * NaN.  Rows without a group are left as they are.  scales: fp32 [adapters], or NULL for ones.  rank 1..256.
  *   q4fc_lora_add  adds to the y that is there, of any projection.
  *   q4fc_fc_lora   q4fc_fc into y and the adapters' part on top: the same results as the two calls.  (The adapters' first
  *                  product runs beside the start of the projection.)  A wait that runs out sets the device status word

@@ -8,7 +8,8 @@
 // With few rows one launch does both; with many, shrink is a launch in front of the projection and expand one behind it.
 // Both on mma.sync.m16n8k8 (tf32 operands, fp32 sums), the adapter's rows on the 16-row side and the call's rows on the
 // 8-column side.  A tf32 operand keeps 11 bits: fp16 and bf16 weights are exact in one, an fp32 number is two (its first 11
-// bits and the next 11), so that a product costs two MMAs, or three with fp32 weights, and is off by 2^-20 at most.
+// bits and the next 11), so that a product costs two MMAs, or four with fp32 weights, and is off by 2^-20 at most.  Outputs are off by 2e-7 to
+// 5e-7 of their size in the 2-norm, about as an fp32 product's are (1e-7 to 2e-7).
 // The order of k in an MMA is free as long as both operands have the same: a lane takes consecutive k of a row (8 of a piece
 // of 32), so that fragments come straight from global memory in 16-byte loads.
 //
@@ -39,6 +40,11 @@ __device__ __forceinline__ void mma_tf32(float (&d)[4], const uint32_t (&a)[4], 
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+__device__ __forceinline__ void mma_tf32_of_zero(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
+}
 // x = hi + lo, cut off to 11 bits each (which cannot overflow; an infinity leaves NaN)
 __device__ __forceinline__ void split(float x, uint32_t& hi, uint32_t& lo) {
     hi = __float_as_uint(x) & 0xffffe000u;
@@ -68,7 +74,7 @@ __device__ __forceinline__ void load_values(const T* p, int64_t valid, T (&v)[NV
         }
     } else {
 #pragma unroll
-        for (int i = 0; i < NV; i++) v[i] = i < valid ? p[i] : T(0.0f);
+        for (int i = 0; i < NV; i++) v[i] = i < (int)valid ? p[i] : T(0.0f);
     }
 }
 
@@ -80,6 +86,24 @@ __device__ __forceinline__ void operand(T a, T b, T c, T d, uint32_t (&hi)[4], u
     for (int i = 0; i < 4; i++)
         if constexpr (sizeof(T) == 4) split(f[i], hi[i], lo[i]);
         else hi[i] = __float_as_uint(f[i]), lo[i] = 0;
+}
+// sum += the products of sixteen terms.  An MMA cuts its sum off, always towards zero, so that a long chain of them shrinks.  So a chain is
+// short: the products with a rest first, while the sum is 2^-11 of the others' size and its cuts too, then two MMAs of the first bits.  An
+// addition, which rounds, joins it to the others.  (Chains over eight or nine pieces of 32 k, or over all of a warp's where warps and CTAs
+// divide K, were off by 1.5e-6 to 8.6e-6, of positive terms by up to 2.4e-5; both products of 2048 rows x 4096 x 4096, rank 32, 37.5 us,
+// so 38.2.  Rests and first bits in turn, chains of eight to sixteen: 4.5e-7 to 1.4e-6.)
+template <typename T>
+__device__ __forceinline__ void add_products(float (&sum)[4], const uint32_t (&wh)[2][4], const uint32_t (&wl)[2][4], const uint4 (&x)[2]) {
+    float part[4];
+    mma_tf32_of_zero(part, wh[0], x[0].z, x[0].w);
+    mma_tf32(part, wh[1], x[1].z, x[1].w);
+    if constexpr (sizeof(T) == 4)
+#pragma unroll
+        for (int j = 0; j < 2; j++) mma_tf32(part, wl[j], x[j].z, x[j].w), mma_tf32(part, wl[j], x[j].x, x[j].y);
+    mma_tf32(part, wh[0], x[0].x, x[0].y);
+    mma_tf32(part, wh[1], x[1].x, x[1].y);
+#pragma unroll
+    for (int i = 0; i < 4; i++) sum[i] += part[i];
 }
 
 // *y += (a, b): nothing comes back, L2 adds.  (One addition for each element: no order to depend on.)
@@ -102,77 +126,85 @@ struct LoraArgs {
 
 // A_i x of eight rows and MB times 16 ranks, by one warp: pieces of 32 k from k0 on, `step` apart, up to k_end.  `x`: the row of lane (g, t)'s
 // g, if `live`; `ranks`: of A that are there.  acc[m][i]: rank m * 16 + 8 (i / 2) + g of row 2t + i % 2.
-template <typename T, int MB, bool VEC, bool LONG>
+template <typename T, int MB, bool VEC>
 __device__ __forceinline__ void shrink_rows(const float* x, bool live, const T* a, int ranks, int64_t K, int64_t k0, int64_t k_end, int64_t step,
                                             float (&acc)[MB][4]) {
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    struct Piece {
-        float v[8];
-        T w[MB][2][8];
+    auto there = [&](int64_t k0) {  // this lane's values of a piece (VEC: whether there are any)
+        const int64_t left = k_end - k0 - 8 * t;
+        return VEC ? left : left < 8 ? left : 8;
     };
-    auto load = [&](int64_t k0, Piece& c) {
-        const int64_t k = k0 + 8 * t, valid = k_end - k;
-        load_values<8, VEC>(x + k, live ? valid : 0, c.v);
+    auto load_x = [&](int64_t k0, float (&v)[8]) { load_values<8, VEC>(x + k0 + 8 * t, live ? there(k0) : 0, v); };
+    auto load_a = [&](int64_t k0, int m, T (&w)[2][8]) {
 #pragma unroll
-        for (int m = 0; m < MB; m++)
-#pragma unroll
-            for (int h = 0; h < 2; h++) {
-                const int r = m * 16 + h * 8 + g;
-                load_values<8, VEC>(a + (int64_t)r * K + k, r < ranks ? valid : 0, c.w[m][h]);
-            }
-    };
-    // An MMA cuts its sum off, always towards zero, so that a long chain of them shrinks.  LONG: after eight or nine pieces the sums move to
-    // where additions round (1270 rows x 2011, fp32: 1.6e-5 of the outputs, so 4e-6; 1 us of 36 at 2048 rows x 4096 x 4096).  Where warps and
-    // CTAs divide K, chains are short.
-    float moved[MB][4];
-    float(&part)[MB][4] = LONG ? moved : acc;
-    auto move = [&] {
-#pragma unroll
-        for (int m = 0; m < MB; m++)
-#pragma unroll
-            for (int i = 0; i < 4; i++) acc[m][i] += moved[m][i], moved[m][i] = 0.0f;
-    };
-    if constexpr (LONG)
-#pragma unroll
-        for (int m = 0; m < MB; m++)
-#pragma unroll
-            for (int i = 0; i < 4; i++) moved[m][i] = 0.0f;
-    auto multiply = [&](const Piece& c) {
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            uint32_t hi0, lo0, hi1, lo1;
-            split(c.v[2 * j], hi0, lo0), split(c.v[2 * j + 1], hi1, lo1);
-#pragma unroll
-            for (int m = 0; m < MB; m++) {
-                uint32_t wh[4], wl[4];
-                operand(c.w[m][0][2 * j], c.w[m][1][2 * j], c.w[m][0][2 * j + 1], c.w[m][1][2 * j + 1], wh, wl);
-                if constexpr (sizeof(T) == 4) mma_tf32(part[m], wl, hi0, hi1);
-                mma_tf32(part[m], wh, lo0, lo1);
-                mma_tf32(part[m], wh, hi0, hi1);
-            }
+        for (int h = 0; h < 2; h++) {
+            const int r = m * 16 + h * 8 + g;
+            load_values<8, VEC>(a + (int64_t)r * K + k0 + 8 * t, r < ranks ? there(k0) : 0, w[h]);
         }
     };
-    // pieces on their way while one is multiplied, as the registers allow
-    constexpr int kDepth = !VEC || MB * sizeof(T) > 8 ? 1 : MB * sizeof(T) > 4 ? 2 : 3;
-    Piece c[kDepth];
-    if constexpr (kDepth > 1) {
+    auto split_x = [&](const float (&v)[8], int j, uint4 (&s)[2]) {
+#pragma unroll
+        for (int i = 0; i < 2; i++) split(v[j + 2 * i], s[i].x, s[i].z), split(v[j + 2 * i + 1], s[i].y, s[i].w);
+    };
+    auto multiply = [&](int m, const T (&w)[2][8], int j, const uint4 (&s)[2]) {
+        uint32_t wh[2][4], wl[2][4];
+#pragma unroll
+        for (int i = 0; i < 2; i++) operand(w[0][j + 2 * i], w[1][j + 2 * i], w[0][j + 2 * i + 1], w[1][j + 2 * i + 1], wh[i], wl[i]);
+        add_products<T>(acc[m], wh, wl, s);
+    };
+    if constexpr (VEC && MB * sizeof(T) == 8) {
+        // one piece; its registers take the next one's weights, 16 ranks after 16 (two pieces do not fit: 61 rows x 4096, 40 fp16
+        // adapters of rank 64, both products 25.3 us, so 23.7)
+        float v[8];
+        T w[MB][2][8];
+        if (k0 < k_end) {
+            load_x(k0, v);
+#pragma unroll
+            for (int m = 0; m < MB; m++) load_a(k0, m, w[m]);
+        }
+#pragma unroll 1
+        for (; k0 < k_end; k0 += step) {
+            uint4 s[2][2];
+            split_x(v, 0, s[0]), split_x(v, 4, s[1]);
+            load_x(k0 + step, v);
+#pragma unroll
+            for (int m = 0; m < MB; m++) {
+                multiply(m, w[m], 0, s[0]), multiply(m, w[m], 4, s[1]);
+                load_a(k0 + step, m, w[m]);
+            }
+        }
+    } else {
+        // pieces on their way while one is multiplied, as the registers allow
+        struct Piece {
+            float v[8];
+            T w[MB][2][8];
+        };
+        auto load = [&](int64_t k0, Piece& c) {
+            load_x(k0, c.v);
+#pragma unroll
+            for (int m = 0; m < MB; m++) load_a(k0, m, c.w[m]);
+        };
+        constexpr int kDepth = VEC && MB * sizeof(T) < 8 ? 3 : 1;
+        Piece c[kDepth];
 #pragma unroll
         for (int d = 0; d + 1 < kDepth; d++)
             if (k0 + d * step < k_end) load(k0 + d * step, c[d]);
-    }
-    constexpr int kMoves = kDepth == 3 ? 3 : 8 / kDepth;
-    int left = kMoves;
-    while (k0 < k_end) {
+        while (k0 < k_end) {
 #pragma unroll
-        for (int d = 0; d < kDepth; d++) {
-            if (k0 >= k_end) break;
-            if (k0 + (kDepth - 1) * step < k_end) load(k0 + (kDepth - 1) * step, c[(d + kDepth - 1) % kDepth]);
-            multiply(c[d]);
-            k0 += step;
+            for (int d = 0; d < kDepth; d++) {
+                if (k0 >= k_end) break;
+                if (k0 + (kDepth - 1) * step < k_end) load(k0 + (kDepth - 1) * step, c[(d + kDepth - 1) % kDepth]);
+#pragma unroll
+                for (int j = 0; j < 8; j += 4) {
+                    uint4 s[2];
+                    split_x(c[d].v, j, s);
+#pragma unroll
+                    for (int m = 0; m < MB; m++) multiply(m, c[d].w[m], j, s);
+                }
+                k0 += step;
+            }
         }
-        if (LONG && --left == 0) move(), left = kMoves;
     }
-    if constexpr (LONG) move();
 }
 
 // y += B t, or without `onto` y = B t, by one warp: 16 columns of NB times eight rows at a time, the next kAcross further; the next
@@ -188,8 +220,10 @@ struct Columns {
         T w[PIECES][2][NV];
     };
     const T* b;          // of the lane's first values of column 0
-    float* y_at[NB][2];  // row nb * 8 + 2t + i at column 0; where there is none, another's
-    int64_t n, N;        // the lane's columns: n and n + 1
+    float* y;
+    int64_t ldy;
+    int y_row[NB][2];    // of row nb * 8 + 2t + i; where there is none, another's
+    int n, N;            // the lane's columns: n and n + 1
     int rank, rows, live;  // rows from this warp's first on, blocks of eight that have any
     bool onto;
     Next c[2];
@@ -203,13 +237,13 @@ struct Columns {
     // rows of the tile from `row0` of its place on, columns from n0 on
     __device__ __forceinline__ void begin(const LoraArgs& p, int4 tile, int tile_rows, int row0, int64_t n0, bool add) {
         const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-        n = n0 + 2 * g, N = p.N, rank = p.rank, rows = tile_rows - row0, live = (rows + 7) / 8, onto = add;
+        y = p.y, ldy = p.ldy, n = (int)n0 + 2 * g, N = (int)p.N, rank = p.rank, rows = tile_rows - row0, live = (rows + 7) / 8, onto = add;
 #pragma unroll
         for (int nb = 0; nb < NB; nb++)
 #pragma unroll
             for (int i = 0; i < 2; i++) {
                 const int row = nb * 8 + 2 * t + i;
-                y_at[nb][i] = p.y + (int64_t)__ldcg(p.order + tile.y + (row < rows ? row0 + row : 0)) * p.ldy;
+                y_row[nb][i] = __ldcg(p.order + tile.y + (row < rows ? row0 + row : 0));
             }
         b = static_cast<const T*>(p.b) + (int64_t)tile.x * p.N * p.rank + NV * t;
     }
@@ -222,19 +256,15 @@ struct Columns {
 #pragma unroll
             for (int h = 0; h < 2; h++) {
                 const int r = r0 + q * kPiece;
-                const int64_t m = n + ahead * kAcross + h;
+                const int m = n + ahead * kAcross + h;
                 if constexpr (VEC)
-                    load_values<NV, VEC>(b + min(m, N - 1) * rank + (r + NV * t < rank ? r : -NV * t), 1, w[q][h]);
+                    load_values<NV, VEC>(b + ((int64_t)min(m, N - 1) * rank + (r + NV * t < rank ? r : -NV * t)), 1, w[q][h]);
                 else
-                    load_values<NV, VEC>(b + m * rank + r, m < N ? rank - r - NV * t : 0, w[q][h]);
+                    load_values<NV, VEC>(b + ((int64_t)m * rank + r), m < N ? rank - r - NV * t : 0, w[q][h]);
             }
     }
     __device__ __forceinline__ void finish(Next& c, const uint4* ts, int pitch) {
-        float acc[NB][4];
-#pragma unroll
-        for (int nb = 0; nb < NB; nb++)
-#pragma unroll
-            for (int j = 0; j < 4; j++) acc[nb][j] = 0.0f;
+        float acc[NB][4] = {};
         const int lane = threadIdx.x & 31;
 #pragma unroll 1
         for (int r0 = 0; r0 < rank; r0 += kChunk) {
@@ -247,16 +277,17 @@ struct Columns {
                     for (int v = 0; v < NV; v++) c.w[q][0][v] = T(0.0f), c.w[q][1][v] = T(0.0f);
                 }
 #pragma unroll
-                for (int j = 0; j < NV / 2; j++) {
-                    uint32_t wh[4], wl[4];
-                    operand(c.w[q][0][2 * j], c.w[q][1][2 * j], c.w[q][0][2 * j + 1], c.w[q][1][2 * j + 1], wh, wl);
+                for (int j = 0; j < NV / 2; j += 2) {
+                    uint32_t wh[2][4], wl[2][4];
+#pragma unroll
+                    for (int i = 0; i < 2; i++)
+                        operand(c.w[q][0][2 * (j + i)], c.w[q][1][2 * (j + i)], c.w[q][0][2 * (j + i) + 1], c.w[q][1][2 * (j + i) + 1], wh[i], wl[i]);
 #pragma unroll
                     for (int nb = 0; nb < NB; nb++) {
                         if (nb >= live) break;
-                        const uint4 u = mine[nb * 8 * pitch + q * (kPiece / 2) + 4 * j];
-                        if constexpr (sizeof(T) == 4) mma_tf32(acc[nb], wl, u.x, u.y);
-                        mma_tf32(acc[nb], wh, u.z, u.w);
-                        mma_tf32(acc[nb], wh, u.x, u.y);
+                        const uint4* at = mine + nb * 8 * pitch + q * (kPiece / 2) + 4 * j;
+                        const uint4 u[2] = {at[0], at[4]};
+                        add_products<T>(acc[nb], wh, wl, u);
                     }
                 }
             }
@@ -267,7 +298,7 @@ struct Columns {
 #pragma unroll
             for (int i = 0; i < 2; i++) {
                 if (nb * 8 + 2 * (lane & 3) + i >= rows) continue;
-                float* y = y_at[nb][i] + n;
+                float* y = this->y + (y_row[nb][i] * ldy + n);
                 if (onto) {
                     if (VEC && n < N) add_to(y, acc[nb][i], acc[nb][i + 2]);
                     if (!VEC && n < N) atomicAdd(y, acc[nb][i]);
@@ -280,7 +311,7 @@ struct Columns {
             }
         n += kAcross;
     }
-    // `times` of them; the first one's B and y have been asked for into c[0]
+    // `times` of them; the first one's B has been asked for into c[0]
     __device__ __forceinline__ void run(int64_t times, const uint4* ts, int pitch) {
 #pragma unroll 1
         for (int64_t k = 0; k < times; k += 2) {
@@ -333,7 +364,7 @@ __global__ void __launch_bounds__(kThreads, 2) lora_few_kernel(const __grid_cons
         const bool live = g < tile.z;
         const float* x = p.x + (live ? (int64_t)__ldcg(p.order + tile.y + g) * p.ldx : 0);
         float acc[MB][4] = {};
-        shrink_rows<T, MB, VEC, false>(x, live, static_cast<const T*>(p.a) + (int64_t)tile.x * p.rank * p.K, p.rank, p.K, k_begin + warp * 32, k_end,
+        shrink_rows<T, MB, VEC>(x, live, static_cast<const T*>(p.a) + (int64_t)tile.x * p.rank * p.K, p.rank, p.K, k_begin + warp * 32, k_end,
                                        kWarps * 32, acc);
         float* mine = by_warp + warp * 8 * kRanks;
 #pragma unroll
@@ -395,7 +426,7 @@ __global__ void __launch_bounds__(kThreads, 2) lora_shrink_kernel(const __grid_c
     const float* x = p.x + (live ? (int64_t)__ldcg(p.order + tile.y + row0 + g) * p.ldx : 0);
     float acc[MB][4] = {};
     if (row0 < tile.z)
-        shrink_rows<T, MB, VEC, !kByK>(x, live, static_cast<const T*>(p.a) + ((int64_t)tile.x * p.rank + rank0) * p.K, p.rank - rank0, p.K,
+        shrink_rows<T, MB, VEC>(x, live, static_cast<const T*>(p.a) + ((int64_t)tile.x * p.rank + rank0) * p.K, p.rank - rank0, p.K,
                                 k_begin + (kByK ? warp * 32 : 0), k_end, kByK ? kWarps * 32 : 32, acc);
     float* mine = kByK ? by_warp + warp * TILE * kRanks : sums + row0 * kRanks;
 #pragma unroll
@@ -425,12 +456,13 @@ __global__ void __launch_bounds__(kThreads, 2) lora_shrink_kernel(const __grid_c
 // The work is pieces of 32 rows of a tile and 64 columns, or of its eight rows and 128, the columns of a tile one behind another; a CTA
 // takes a contiguous share of what the plan has.  (Both launches of lora_add with 2, 3 and 4 CTAs an SM: tiles of 64 rows, 2048 rows x
 // 4096 x 4096, 4 bf16 adapters of rank 32, 37.3, 36.4 and 38.0 us; of eight, 61 rows x 4096 x 11008, 40 fp16 ones of rank 64, with 3 and
-// 4 22.3 and 23.0.  Four times eight rows a warp instead of two: the same.)
+// 4 22.3 and 23.0.  Four times eight rows a warp instead of two: the same.  With fp32 weights of more than 16 ranks 2 hold the tiles of 64
+// rows without spilling: 1024 rows x 4096 x 4096, 8 adapters of rank 128, with 3 and 2 90.3 and 86.3 us.)
 __host__ __device__ constexpr int expand_rows(int tile) { return tile < 32 ? tile : 32; }
 __host__ __device__ constexpr int expand_columns(int tile) { return tile < 32 ? 128 : 64; }
-constexpr int kExpandCtas = 3;  // an SM
+__host__ __device__ constexpr int expand_ctas(int each, int tile, int quads) { return each == 4 && quads == 2 && tile == 64 ? 2 : 3; }  // an SM
 template <typename T, int TILE, int QUADS, int PIECES, bool VEC>
-__global__ void __launch_bounds__(kThreads, kExpandCtas) lora_expand_kernel(const __grid_constant__ LoraArgs p, const bool onto) {
+__global__ void __launch_bounds__(kThreads, expand_ctas(sizeof(T), TILE, QUADS)) lora_expand_kernel(const __grid_constant__ LoraArgs p, const bool onto) {
     constexpr int kRows = expand_rows(TILE), kParts = TILE / kRows, NB = kRows > 8 ? 2 : 1, kAcross = expand_columns(TILE);
     using C = Columns<T, QUADS, PIECES, NB, kAcross, VEC>;
     extern __shared__ uint4 ts[];  // [kRows][pitch]
@@ -536,7 +568,7 @@ int launch_expand(const LoraCall& c, const LoraArgs& p, bool onto, int64_t tiles
     if (!di) return Q4FC_ECUDA;
     const bool vec = expand_vec(c, 4 * QUADS);
     constexpr int kChunk = 16 * QUADS * PIECES;
-    const int64_t pieces = tiles * (TILE / expand_rows(TILE)) * ((c.N + expand_columns(TILE) - 1) / expand_columns(TILE)), most = kExpandCtas * di->sm_count;
+    const int64_t pieces = tiles * (TILE / expand_rows(TILE)) * ((c.N + expand_columns(TILE) - 1) / expand_columns(TILE)), most = expand_ctas(sizeof(T), TILE, QUADS) * di->sm_count;
     DependentLaunch l(dim3((unsigned)(pieces < most ? pieces : most)), kThreads, s);
     auto* fn = vec ? lora_expand_kernel<T, TILE, QUADS, PIECES, true> : lora_expand_kernel<T, TILE, QUADS, PIECES, false>;
     l.cfg.dynamicSmemBytes = expand_rows(TILE) * (size_t)expand_pitch((int)(c.rank + kChunk - 1) / kChunk * kChunk);
@@ -562,8 +594,9 @@ int launch_lora_tile(const LoraCall& c, const LoraArgs& p, const LoraPlan& l, St
         return launch_shrink<T, TILE, 4>(p, vec, grid, l.slices, s);
     }
     if (c.rank <= 16) return launch_expand<T, TILE, 1, 1>(c, p, step == kExpandOnto, tiles, s);
-    if (c.rank <= 32 || sizeof(T) == 4) return launch_expand<T, TILE, 2, 1>(c, p, step == kExpandOnto, tiles, s);
-    return launch_expand<T, TILE, 2, 2>(c, p, step == kExpandOnto, tiles, s);
+    if constexpr (sizeof(T) == 2)
+        if (c.rank > 32) return launch_expand<T, TILE, 2, 2>(c, p, step == kExpandOnto, tiles, s);
+    return launch_expand<T, TILE, 2, 1>(c, p, step == kExpandOnto, tiles, s);
 }
 template <typename T>
 int launch_lora_type(const LoraCall& c, const LoraArgs& p, const LoraPlan& l, Step step, int64_t tiles, cudaStream_t s) {

@@ -244,3 +244,30 @@ def test_ranks_of_several_host_threads(pkg, dtype):
     assert not failed
     for one, x, a, b in sums.values():
         check(one, *added64(x, a, b, None, np.arange(rows) % n))
+
+
+@pytest.mark.parametrize("positive", [False, True])
+@pytest.mark.parametrize("rows,n,r,K,N,dtype", [
+    (1, 1, 16, 4096, 256, torch.bfloat16), (4, 4, 16, 11008, 256, torch.float32), (61, 40, 64, 11008, 256, torch.float16),
+    (61, 3, 200, 11008, 128, torch.float32), (133, 3, 12, 1001, 299, torch.float32), (255, 255, 128, 8192, 96, torch.bfloat16),
+    (255, 255, 128, 8192, 96, torch.float32), (300, 300, 64, 8192, 96, torch.bfloat16), (300, 2, 256, 512, 256, torch.float16),
+    (300, 2, 256, 512, 256, torch.float32), (300, 2, 64, 11008, 256, torch.float32), (1270, 7, 202, 2011, 264, torch.float32),
+    (2048, 4, 32, 11008, 512, torch.bfloat16)])
+def test_long_sums_are_as_good_as_fp32(pkg, rows, n, r, K, N, dtype, positive):
+    """In the 2-norm, in units u = 2^-23 of a number in [1, 2), of which a number is 0.7 in the mean.
+
+    Cut to 11 + 11 of 24 bits an operand loses up to 3 u, 1.4 as a root of the mean of squares: 1.2e-7 of it; there are two such in each
+    product (x or its sum, fp32 weights): 2.4e-7.  Two MMAs of first bits cut up to one u of their sum, half of it in the mean, the first one on
+    0.7 of the sum: 0.7e-7.  At most 128 additions round by 0.3 u, on partial sums of 0.7 of the last or less: 1.9e-7.  Together, as if all had
+    one sign, 5e-7 for each of the two products: 1e-6.  (A warp's whole K as one chain of MMAs is off by several times that.)"""
+    g = torch.Generator("cuda").manual_seed(1)
+    of = torch.abs if positive else (lambda t: t)
+    a = of(torch.randn(n, r, K, device="cuda", generator=g) / K ** 0.5).to(dtype)
+    b = of(torch.randn(n, N, r, device="cuda", generator=g)).to(dtype)
+    x = of(torch.randn(1, rows, K, device="cuda", generator=g))
+    ids = np.arange(rows) % n
+    y = torch.zeros(1, rows, N, device="cuda")
+    pkg.llmops.lora_add(y, x, a, b, groups_of(pkg, ids, n))
+    some = range(min(rows, 3 * n + 60, 400))
+    want = torch.stack([(x[0, k].double() @ a[ids[k]].double().T) @ b[ids[k]].double().T for k in some])
+    assert ((y[0, : len(want)] - want).norm() / want.norm()).item() <= 1e-6
