@@ -134,7 +134,9 @@ int launch_q8c_prefill(const float* x, int64_t rows, int64_t K, int64_t ldx, con
 
 // A launch that may begin before the kernel in front of it has ended: the kernel waits (pdl_wait_prior_grid) before it touches
 // global memory, and lets its own successor begin only after that wait, so that a successor which begins early finds everything
-// in front of this kernel complete.
+// in front of this kernel complete.  What such a successor reads in front of its own wait (weights, a plan, rows, but nothing that this
+// kernel writes) is in L2 then.  It reads it from there: by ld.cg, bulk or tensor copies, or behind pdl_reads_early(), since a line that
+// its SM's L1 has from before may be older.
 struct DependentLaunch {
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr = {};
@@ -197,6 +199,8 @@ __device__ __forceinline__ float4 ld_after_wait(const float4* p) {
     asm volatile("ld.global.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "l"(p) : "memory");
     return v;
 }
+// in front of loads through L1 that come before the wait (see DependentLaunch)
+__device__ __forceinline__ void pdl_reads_early() { __threadfence(); }
 __device__ __forceinline__ void pdl_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 #endif
 

@@ -333,13 +333,15 @@ __device__ __forceinline__ void zero_rows(const LoraArgs& p, int64_t first, int6
 
 // ---- few rows and up to 64 ranks: both products in one launch ---------------------------------------------------------------------------
 // A cluster per tile of eight rows: its CTAs divide K (and their warps that again), their sums meet in every one of them, and then they
-// divide the columns.  With `early` the launch in front computes y alone: all else is complete, and the first product does not wait
-// for it.  CTAs behind those of the tiles quantize x for the decode FC (quant_pre.cuh), which has to be done in front of it anyway.
+// divide the columns.  With `early` (VEC) the launch in front computes y alone: all else is complete, and the first product does not wait
+// for it.  (133 rows x 1000 x 3000, 3 fp32 adapters of rank 12, with the FC 21.9 us, so 19.4.  Value by value, 1001 x 2999, loads behind the
+// fence take longer than the wait, 22.0 and 21.4.)  CTAs behind those of the tiles quantize x for the decode FC (quant_pre.cuh), which has to
+// be done in front of it anyway.
 // Registers: two CTAs on an SM, and up to 16 ranks one beside a CTA of the prefill GEMM (16 rows x 4096 x 4096, 4 bf16 adapters of rank 16, with
 // the FC: 118 registers 19.9 us, 96 18.5).
 template <typename T, int MB, bool VEC>
 __global__ void __maxnreg__(MB == 1 ? 96 : 128) lora_few_kernel(const __grid_constant__ LoraArgs p, const __grid_constant__ QuantPre q, const bool onto,
-                                                               const bool early) {
+                                                               const bool begin_early) {
     constexpr int kRanks = MB * 16, QUADS = MB == 1 ? 1 : 2, PIECES = MB == 4 && sizeof(T) < 4 ? 2 : 1, kAcross = kWarps * 16;
     using C = Columns<T, QUADS, PIECES, 1, kAcross, VEC>;
     constexpr int kPitch = expand_pitch((kRanks + C::kChunk - 1) / C::kChunk * C::kChunk) / 16;
@@ -353,7 +355,9 @@ __global__ void __maxnreg__(MB == 1 ? 96 : 128) lora_few_kernel(const __grid_con
         pdl_wait_prior_grid();
         pdl_launch_dependents();
     };
-    if (!early) others_done();
+    const bool early = VEC && begin_early;
+    if (early) pdl_reads_early();
+    else others_done();
     if ((int)blockIdx.y >= q.first_block) {
         quant_pre_block(q, ((int64_t)(blockIdx.y - q.first_block) * slices + here) * kWarps + warp);
         return;
@@ -470,7 +474,8 @@ __global__ void __launch_bounds__(kThreads, expand_ctas(sizeof(T), TILE, QUADS))
     extern __shared__ uint4 ts[];  // [kRows][pitch]
     const int pairs = (p.rank + C::kChunk - 1) / C::kChunk * C::kChunk / 2, pitch = expand_pitch(2 * pairs) / 16;
     // The launches in front, from shrink on, write t and y.  All else was complete when shrink had waited, and this launch begins only
-    // after that: the plan and B need not wait.
+    // after that: the plan and, VEC, B need not wait.  (Value by value, behind the fence: lora_add, 2048 rows x 4095 x 4095, 4 bf16 adapters of
+    // rank 24, 62.0 us, so 58.4.)
     bool waited = false;
     auto others_done = [&] {
         if (!waited) {
@@ -479,6 +484,8 @@ __global__ void __launch_bounds__(kThreads, expand_ctas(sizeof(T), TILE, QUADS))
         }
         waited = true;
     };
+    if constexpr (VEC) pdl_reads_early();
+    else others_done();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int64_t blocks = (p.N + kAcross - 1) / kAcross, total = (int64_t)__ldcg(p.tile_count) * kParts * blocks;
     int64_t at = total * blockIdx.x / gridDim.x;

@@ -271,3 +271,30 @@ def test_long_sums_are_as_good_as_fp32(pkg, rows, n, r, K, N, dtype, positive):
     some = range(min(rows, 3 * n + 60, 400))
     want = torch.stack([(x[0, k].double() @ a[ids[k]].double().T) @ b[ids[k]].double().T for k in some])
     assert ((y[0, : len(want)] - want).norm() / want.norm()).item() <= 1e-6
+
+
+@pytest.mark.parametrize("rows,n,rank,K,N", [(5, 3, 16, 512, 256), (5, 8, 72, 512, 256), (61, 3, 16, 512, 256), (61, 40, 64, 320, 2048),
+                                             (133, 3, 12, 251, 301), (300, 4, 32, 512, 256)])
+def test_all_inputs_are_written_directly_in_front(pkg, rows, n, rank, K, N):
+    """x, both products' weights, the plan and y change between calls that nothing waits for: a launch that begins early reads the new ones."""
+    ops = pkg.llmops
+    sets = [inputs(rows, n, rank, K, N, torch.bfloat16, seed=s) for s in range(4)]
+    ids = [torch.from_numpy(np.random.default_rng(s).integers(-1, n, rows)).int().cuda()[None] for s in range(4)]
+    wq = ops.offline_FC_quant_Q4A((torch.randn(N, -(-K // 4) * 4, generator=torch.Generator().manual_seed(1)) * 0.02).cuda())
+    want = [ops.fc_Q4A_lora(x, wq, N, a, b, ops.group_rows(i, n), scales=s) for (x, a, b, s), i in zip(sets, ids)]
+    torch.cuda.synchronize()
+    x, a, b, s = (torch.empty_like(t) for t in sets[0])
+    i, out = torch.empty_like(ids[0]), [torch.full_like(want[0], float("nan")) for _ in sets]
+
+    def refill(k):
+        for to, of in zip((x, a, b, s, i), (*sets[k], ids[k])):
+            to.copy_(of)
+
+    for _ in range(20):
+        for k in range(4):
+            refill(k)
+            ops.fc_Q4A_lora(x, wq, N, a, b, ops.group_rows(i, n), scales=s, out=out[k])
+        torch.cuda.synchronize()
+        assert all(torch.equal(o, w) for o, w in zip(out, want))
+        for o in out:
+            o.fill_(float("nan"))
