@@ -298,3 +298,37 @@ def test_all_inputs_are_written_directly_in_front(pkg, rows, n, rank, K, N):
         assert all(torch.equal(o, w) for o, w in zip(out, want))
         for o in out:
             o.fill_(float("nan"))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,n,rank,K,N", [
+    (1, 2, 65, 512, 96), (1, 2, 256, 260, 130), (8, 5, 72, 512, 256), (8, 5, 65, 300, 67), (8, 3, 256, 384, 64), (3, 70, 20, 260, 15361),
+    (8, 300, 16, 512, 16384), (61, 5, 65, 512, 257), (61, 40, 72, 512, 256), (133, 7, 256, 300, 131), (133, 100, 20, 132, 4099), (255, 255, 9, 96, 515)])
+def test_fc_lora_of_many_ranks_or_columns_is_the_two_calls(pkg, rows, n, rank, K, N, dtype):
+    """Where both products are launches of their own: in front of a decode FC, which finds y of the adapters alone and zeros where a row has
+    none, and around the GEMM."""
+    ops = pkg.llmops
+    x, a, b, scales = inputs(rows, n, rank, K, N, dtype)
+    wq = ops.offline_FC_quant_Q4A((torch.randn(N, K, generator=torch.Generator().manual_seed(1)) * 0.02).cuda(), qtype="q4_1", group_k=32)
+    ids = np.random.default_rng(rows).integers(-1, n, rows)
+    ids[rows // 2] = -1
+    for some in (ids, np.full(rows, -1), np.full(rows, n - 1)):
+        groups = groups_of(pkg, some, n)
+        want = ops.fc_Q4A(x, wq, N)
+        ops.lora_add(want, x, a, b, groups, scales=scales)
+        out = torch.full_like(want, float("nan"))
+        assert torch.equal(ops.fc_Q4A_lora(x, wq, N, a, b, groups, scales=scales, out=out), want)
+    ops.check_device_status()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,n,r,K,N", [(257, 1024, 20, 200, 48), (300, 257, 64, 264, 40), (1024, 1024, 12, 96, 64), (2000, 700, 33, 65, 31)])
+def test_as_many_adapters_as_rows_or_more(pkg, rows, n, r, K, N, dtype):
+    """Tiles of 64 rows with one or two in use."""
+    x, a, b, scales = inputs(rows, n, r, K, N, dtype)
+    ids = np.arange(rows) % n
+    ids[5::9] = -1
+    want, bound = added64(x, a, b, scales, ids)
+    y = torch.zeros(1, rows, N, device="cuda")
+    pkg.llmops.lora_add(y, x, a, b, groups_of(pkg, ids, n), scales=scales)
+    check(y, want, bound)
