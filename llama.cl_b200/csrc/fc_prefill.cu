@@ -823,12 +823,15 @@ int launch_prefill_variant(const PrefillParams& p, const CUtensorMap& map, dim3 
     return Q4FC_OK;
 }
 
+template <int FMT, int G, bool GROUPED = false>
+int launch_prefill_64(const PrefillParams& p, const CUtensorMap& map, dim3 grid, cudaStream_t s) {
+    if (p.fold == 0) return launch_prefill_variant<FMT, G, 64, 0, GROUPED>(p, map, grid, s);
+    return p.rows <= 48 ? launch_prefill_variant<FMT, G, 64, kFewRows, GROUPED>(p, map, grid, s)
+                        : launch_prefill_variant<FMT, G, 64, kManyRows, GROUPED>(p, map, grid, s);
+}
 template <int FMT, int G>
 int launch_prefill_tile(int tile, const PrefillParams& p, const CUtensorMap& map, dim3 grid, cudaStream_t s) {
-    if (tile == 128) return launch_prefill_wide(FMT, G, p, map, grid, s);
-    if (p.fold == 0) return launch_prefill_variant<FMT, G, 64>(p, map, grid, s);
-    return p.rows <= 48 ? launch_prefill_variant<FMT, G, 64, kFewRows>(p, map, grid, s)
-                        : launch_prefill_variant<FMT, G, 64, kManyRows>(p, map, grid, s);
+    return tile == 128 ? launch_prefill_wide(FMT, G, p, map, grid, s) : launch_prefill_64<FMT, G>(p, map, grid, s);
 }
 
 // tiles first .. end - 1, K divided by p.split
@@ -1128,7 +1131,7 @@ GroupedPlan grouped_scratch(int64_t rows, int64_t Kg, int G, int64_t n) {
 template <int FMT, int G>
 int launch_grouped(int which, const PrefillParams& p, const CUtensorMap& map, dim3 grid, cudaStream_t s) {
     return which == kTiles128 ? launch_prefill_wide_grouped(FMT, G, p, map, grid, s)
-                              : launch_prefill_variant<FMT, G, 64, 0, true>(p, map, grid, s);
+                              : launch_prefill_64<FMT, G, true>(p, map, grid, s);
 }
 
 }  // namespace
@@ -1159,15 +1162,13 @@ int launch_experts_gemm(const ExpertsCall& c, GroupQuant q, cudaStream_t s) {
     p.Ng = (int)c.Ng, p.Kg = (int)c.Kg, p.n_tiles = (int)n_tiles, p.m_end = (int)m_tiles, p.part = kWhole;
     p.tiles = c.plan.tiles[g.which], p.tile_count = c.plan.counts + g.which, p.order = c.plan.order;
     p.group_bytes = c.Ng * c.Kg * block_bytes(c.qtype, c.G);
-    // few tiles: K divided over clusters, as for as many tiles of one weight tensor
+    // few tiles: K divided over clusters, and running sums moved, as for as many tiles of one weight tensor
     p.split = 1;
     const float tiles = likely_tiles(tile_rows(g.which), c.rows, c.n);
-    const int64_t places = (g.which == kTiles128 ? 1 : 2) * di->sm_count;
-    if (tiles * (float)n_tiles < (float)places) {
-        const TilePlan t = plan_tiles(tile_rows(g.which), fmt, c.G, (int)n_tiles, (int64_t)(tiles + 0.5f) * tile_rows(g.which),
-                                      nstage, cluster_room(di), di->sm_count);
-        p.split = t.split;
-    }
+    const int64_t places = (g.which == kTiles128 ? 1 : 2) * di->sm_count, rows = (int64_t)(tiles + 0.5f) * tile_rows(g.which);
+    if (tiles * (float)n_tiles < (float)places)
+        p.split = plan_tiles(tile_rows(g.which), fmt, c.G, (int)n_tiles, rows, nstage, cluster_room(di), di->sm_count).split;
+    p.fold = fold_of(p.split, least_parts((int)n_tiles, rows, nstage, di->sm_count), nstage);
     const dim3 grid((unsigned)(n_tiles * p.split), (unsigned)m_tiles);
     if (fmt == kQ4_1) return c.G == 32 ? launch_grouped<kQ4_1, 32>(g.which, p, map, grid, s) : launch_grouped<kQ4_1, 128>(g.which, p, map, grid, s);
     if (fmt == kQ4_0) return c.G == 32 ? launch_grouped<kQ4_0, 32>(g.which, p, map, grid, s) : launch_grouped<kQ4_0, 128>(g.which, p, map, grid, s);

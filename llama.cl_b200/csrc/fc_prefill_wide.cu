@@ -627,7 +627,7 @@ __global__ void __launch_bounds__(kThreads, 1) fc_prefill_wide_kernel(const Pref
     }
 }
 
-template <int FMT, int G, bool FOLD, bool GROUPED = false>
+template <int FMT, int G, bool FOLD, bool GROUPED>
 int launch_variant(const PrefillParams& p, const CUtensorMap& map, dim3 grid, cudaStream_t s) {
     using S = WideShape<FMT, G>;
     static std::atomic<bool> attr_done[64] = {};  // set once per device; a second setter repeats the same call
@@ -658,9 +658,9 @@ int launch_variant(const PrefillParams& p, const CUtensorMap& map, dim3 grid, cu
     return Q4FC_OK;
 }
 
-template <int FMT, int G>
+template <int FMT, int G, bool GROUPED = false>
 int launch_fold(const PrefillParams& p, const CUtensorMap& map, dim3 grid, cudaStream_t s) {
-    return p.fold > 0 ? launch_variant<FMT, G, true>(p, map, grid, s) : launch_variant<FMT, G, false>(p, map, grid, s);
+    return p.fold > 0 ? launch_variant<FMT, G, true, GROUPED>(p, map, grid, s) : launch_variant<FMT, G, false, GROUPED>(p, map, grid, s);
 }
 
 }  // namespace
@@ -672,9 +672,9 @@ int launch_prefill_wide(int fmt, int G, const PrefillParams& p, const CUtensorMa
 }
 
 int launch_prefill_wide_grouped(int fmt, int G, const PrefillParams& p, const CUtensorMap& map, dim3 grid, cudaStream_t s) {
-    if (fmt == kQ4_1) return G == 32 ? launch_variant<kQ4_1, 32, false, true>(p, map, grid, s) : launch_variant<kQ4_1, 128, false, true>(p, map, grid, s);
-    if (fmt == kQ4_0) return G == 32 ? launch_variant<kQ4_0, 32, false, true>(p, map, grid, s) : launch_variant<kQ4_0, 128, false, true>(p, map, grid, s);
-    return G == 32 ? launch_variant<kQ4_0Signed, 32, false, true>(p, map, grid, s) : launch_variant<kQ4_0Signed, 128, false, true>(p, map, grid, s);
+    if (fmt == kQ4_1) return G == 32 ? launch_fold<kQ4_1, 32, true>(p, map, grid, s) : launch_fold<kQ4_1, 128, true>(p, map, grid, s);
+    if (fmt == kQ4_0) return G == 32 ? launch_fold<kQ4_0, 32, true>(p, map, grid, s) : launch_fold<kQ4_0, 128, true>(p, map, grid, s);
+    return G == 32 ? launch_fold<kQ4_0Signed, 32, true>(p, map, grid, s) : launch_fold<kQ4_0Signed, 128, true>(p, map, grid, s);
 }
 
 }  // namespace q4fc

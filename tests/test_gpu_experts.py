@@ -241,3 +241,15 @@ def test_refusals(pkg):
     other.buf = other.buf[:-4]
     with pytest.raises(RuntimeError, match="not a plan"):
         call(x, wq, 64, other)
+
+
+@pytest.mark.parametrize("qtype,signed", [(0, False), (0, True), (1, False)])
+@pytest.mark.parametrize("K,N", [(11008, 7040), (11008, 4100), (4096, 9000), (1000, 300)])
+def test_one_expert_for_64_rows_is_the_fc(pkg, K, N, qtype, signed):
+    """The same tiles, K divided as often and long sums moved as often: the same bits."""
+    wq = pkg.llmops.offline_FC_quant_Q4A((torch.randn(N, K, generator=torch.Generator().manual_seed(1)) * 0.02).cuda(), qtype=qtype, group_k=128)
+    x = torch.randn(1, 64, K, generator=torch.Generator().manual_seed(2)).cuda()
+    groups = pkg.llmops.group_rows(torch.zeros(1, 64, 1, dtype=torch.int32, device="cuda"), 1)
+    got = pkg.llmops.fc_Q4A_experts(x, wq[None], N, groups, nibble_signed=signed)
+    assert torch.equal(got[:, :, 0], pkg.llmops.fc_Q4A(x, wq, N, nibble_signed=signed))
+    pkg.llmops.check_device_status()
