@@ -335,3 +335,101 @@ def test_adapters_of_as_many_rows_as_a_plan_holds(pkg):
     want, bound = added64(x[:, some.cuda()], a, b, None, ids[0, some.cuda()].cpu().numpy())
     check(y[0, some.cuda()], want, bound)
     assert not y[0, ids[0] < 0].any()
+
+
+@pytest.mark.parametrize("tokens", [2, 70, 300])
+def test_calls_of_several_host_threads(pkg, tokens):
+    """A step of everything, on a stream of its own for each thread: the bits of one thread alone."""
+    import threading
+
+    ops, n, K, N = pkg.llmops, 6, 256, 160
+    wq = pack(pkg, n, N, K, 1, 128, 3)
+    g = torch.Generator().manual_seed(tokens)
+    a, b = (torch.randn(n, 160, K, generator=g) / 16).half().cuda(), torch.randn(n, N, 160, generator=g).half().cuda()
+    xs = [torch.randn(1, tokens, K, generator=g).cuda() for _ in range(4)]
+    logits = [torch.randn(1, tokens, n, generator=g).cuda() for _ in xs]
+
+    def step(i):
+        rank = (8, 160, 40, 136)[i]
+        la, lb = a[:, :rank].contiguous(), b[..., :rank].contiguous()
+        weights, groups = ops.route_top_k(logits[i], 2)
+        y = ops.fc_Q4A_experts(xs[i], wq, N, groups, weights=weights)
+        rows = ops.group_rows(groups.ids[..., 0].contiguous(), n)
+        y = y + ops.fc_Q4A_lora(xs[i], wq[0], N, la, lb, rows)
+        ops.lora_add(y, xs[i], la, lb, rows)
+        return y
+
+    want = [step(i) for i in range(4)]
+    torch.cuda.synchronize()
+    failed = []
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(40):
+                    got = step(i)
+                torch.cuda.current_stream().synchronize()
+                if not torch.equal(got, want[i]):
+                    failed.append((i, "other bits"))
+        except Exception as e:  # (a thread's error would go nowhere)
+            failed.append((i, str(e)))
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed
+    ops.check_device_status()
+
+
+@pytest.mark.parametrize("tokens", [3, 60, 300])
+def test_branches_of_a_graph(pkg, tokens):
+    """Plans made on a side branch, two branches that read one plan, a copy and a fill directly in front of calls."""
+    ops, n, K, N = pkg.llmops, 5, 512, 192
+    wq, other = pack(pkg, n, N, K, 1, 32, 3), pack(pkg, n, N, K, 0, 128, 4)
+    g = torch.Generator().manual_seed(tokens)
+    a, b = (torch.randn(n, 16, K, generator=g) / 16).half().cuda(), torch.randn(n, N, 16, generator=g).half().cuda()
+    fresh, x = torch.empty(1, tokens, K, device="cuda"), torch.empty(1, tokens, K, device="cuda")
+    logits, ids = torch.empty(1, tokens, n, device="cuda"), torch.empty(1, tokens, dtype=torch.int32, device="cuda")
+    side = torch.cuda.Stream()
+
+    def step(side):
+        main = torch.cuda.current_stream()
+        side.wait_stream(main)
+        with torch.cuda.stream(side):
+            rows = ops.group_rows(ids, n)
+            z = torch.zeros(1, tokens, N, device="cuda")
+            ops.lora_add(z, fresh, a, b, rows)
+        weights, groups = ops.route_top_k(logits, 2)
+        x.copy_(fresh)
+        y = ops.fc_Q4A_experts(x, wq, N, groups, weights=weights)
+        main.wait_stream(side)
+        y = y + ops.fc_Q4A_lora(x, wq[0], N, a, b, rows)
+        side.wait_stream(main)
+        with torch.cuda.stream(side):
+            v = ops.fc_Q4A_experts(x, other, N, groups)
+        w = ops.fc_Q4A_experts(x, wq, N, groups)
+        main.wait_stream(side)
+        return y, z, v, w
+
+    def refill(seed):
+        gen = torch.Generator().manual_seed(seed)
+        fresh.copy_(torch.randn(1, tokens, K, generator=gen))
+        logits.copy_(torch.randn(1, tokens, n, generator=gen))
+        ids.copy_(torch.randint(-1, n, (1, tokens), generator=gen))
+
+    refill(0)
+    step(torch.cuda.current_stream())
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(side)
+    for seed in (1, 2, 3):
+        refill(seed)
+        for _ in range(4):
+            graph.replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for t in out]
+        assert all(torch.equal(u, v) for u, v in zip(got, step(torch.cuda.current_stream())))
+    ops.check_device_status()
