@@ -134,9 +134,10 @@ int launch_q8c_prefill(const float* x, int64_t rows, int64_t K, int64_t ldx, con
 
 // A launch that may begin before the kernel in front of it has ended: the kernel waits (pdl_wait_prior_grid) before it touches
 // global memory, and lets its own successor begin only after that wait, so that a successor which begins early finds everything
-// in front of this kernel complete.  What such a successor reads in front of its own wait (weights, a plan, rows, but nothing that this
-// kernel writes) is in L2 then.  It reads it from there: by ld.cg, bulk or tensor copies, or behind pdl_reads_early(), since a line that
-// its SM's L1 has from before may be older.
+// in front of this kernel complete.  Where such a successor reads in front of its own wait what the kernel in front of this one has written
+// (a plan, codes; never what this kernel writes), this kernel hands on what it saw with a fence between its wait and its release; what lies
+// further back (weights, rows) was complete before this kernel began.  The successor reads it from L2, by ld.cg, bulk or tensor
+// copies, or behind pdl_reads_early(), since a line that its SM's L1 has from before may be older.
 struct DependentLaunch {
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr = {};

@@ -420,6 +420,7 @@ __global__ void __launch_bounds__(kThreads, 2) lora_shrink_kernel(const __grid_c
     __shared__ float by_warp[kByK ? kWarps * TILE * kRanks : 1];
     cg::cluster_group cluster = cg::this_cluster();
     pdl_wait_prior_grid();
+    __threadfence();  // expand reads the plan before this launch has ended (see DependentLaunch)
     pdl_launch_dependents();
     const int slices = (int)cluster.num_blocks(), here = (int)cluster.block_rank(), at = (int)blockIdx.x / slices;  // (clusters lie along x)
     const int4 tile = __ldcg(p.tiles + at);  // (beyond the count: nothing that is used)

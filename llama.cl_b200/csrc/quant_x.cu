@@ -257,7 +257,8 @@ __global__ void __launch_bounds__(kQxWarps * 32) quant_x_tile_kernel(const float
 template <int G, bool F16, int CHUNKS>
 __global__ void __launch_bounds__(kQxWarps * 32) quant_x_group_kernel(const __grid_constant__ GroupQuant a) {
     pdl_wait_prior_grid();
-    pdl_launch_dependents();      // the FC kernels read the plan and their weights meanwhile (from L2)
+    __threadfence();              // what is behind this launch reads the plan, too, before this launch has ended (see DependentLaunch)
+    pdl_launch_dependents();
     const int lane = threadIdx.x & 31;
     const int64_t x_rows = a.rows / a.per_row, row_sets = (x_rows + kQxWarps - 1) / kQxWarps;
     const int64_t set = blockIdx.x / row_sets, c = set * CHUNKS;
