@@ -14,8 +14,8 @@
 // of 32), so that fragments come straight from global memory in 16-byte loads.
 //
 // Bound by the bytes of x, A, B and y where there are many, and in front of that by dependent steps: plan, rows, K, the sums' meeting, columns.
-// Measured, both products: 8 rows x 4096 x 4096, 8 bf16 adapters of rank 16 (2 MB) 6.1 us, 61 rows x 4096 x 11008, 40 fp16 ones of rank 64
-// (65 MB) 22.4, 2048 rows x 4096 x 4096, 4 bf16 ones of rank 32 (34 MB of x, 67 of y) 37.4; shrink alone 7.1 of the second, 16.5 of the third.
+// Measured, both products: 8 rows x 4096 x 4096, 8 bf16 adapters of rank 16 (2 MB) 6.0 us, 61 rows x 4096 x 11008, 40 fp16 ones of rank 64
+// (65 MB) 23.2, 2048 rows x 4096 x 4096, 4 bf16 ones of rank 32 (34 MB of x, 67 of y) 38.7.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 
@@ -209,7 +209,7 @@ __device__ __forceinline__ void shrink_rows(const float* x, bool live, const T* 
 
 // y += B t, or without `onto` y = B t, by one warp: 16 columns of NB times eight rows at a time, the next kAcross further; the next
 // ones' first ranks of B are on their way meanwhile, and y is added to where it is (read and written back, its latency in each step:
-// lora_add, 2048 rows x 4096 x 4096, 4 adapters of rank 32, 41.9 us, so 36.4).  t is in shared memory, as the MMAs want it: two ranks of a
+// lora_add, 2048 rows x 4096 x 4096, 4 adapters of rank 32, 5.5 us more).  t is in shared memory, as the MMAs want it: two ranks of a
 // row in 16 bytes, {hi, hi, lo, lo}, those that a lane reads in turn 64 bytes apart, rows `pitch` apart.
 // QUADS: fours of ranks that a lane takes of a piece of 16 ranks (1, for at most 16) or 32 (2); PIECES of these at a time.
 __host__ __device__ constexpr int expand_pitch(int ranks) { return ranks * 8 / 128 * 128 + 64 + (ranks * 8 % 128 > 64 ? 128 : 0); }  // bytes
@@ -462,12 +462,13 @@ __global__ void __launch_bounds__(kThreads, 2) lora_shrink_kernel(const __grid_c
 
 // The work is pieces of 32 rows of a tile and 64 columns, or of its eight rows and 128, the columns of a tile one behind another; a CTA
 // takes a contiguous share of what the plan has.  (Both launches of lora_add with 2, 3 and 4 CTAs an SM: tiles of 64 rows, 2048 rows x
-// 4096 x 4096, 4 bf16 adapters of rank 32, 37.3, 36.4 and 38.0 us; of eight, 61 rows x 4096 x 11008, 40 fp16 ones of rank 64, with 3 and
-// 4 22.3 and 23.0.  Four times eight rows a warp instead of two: the same.  With fp32 weights of more than 16 ranks 2 hold the tiles of 64
-// rows without spilling: 1024 rows x 4096 x 4096, 8 adapters of rank 128, with 3 and 2 90.3 and 86.3 us.)
+// 4096 x 4096, 4 bf16 adapters of rank 32, 39.0, 38.6 and 38.7 us; of eight, 61 rows x 4096 x 11008, 40 fp16 ones of rank 64, 23.4, 22.8 and
+// 24.3.  Four times eight rows a warp instead of two: the same.  With fp32 weights of more than 16 ranks 2 hold the tiles of 64 rows without
+// spilling: 1024 rows x 4096 x 4096, 8 adapters of rank 128, with 3 and 2 90.3 and 86.3 us.)
 __host__ __device__ constexpr int expand_rows(int tile) { return tile < 32 ? tile : 32; }
 __host__ __device__ constexpr int expand_columns(int tile) { return tile < 32 ? 128 : 64; }
-__host__ __device__ constexpr int expand_ctas(int each, int tile, int quads) { return each == 4 && quads == 2 && tile == 64 ? 2 : 3; }  // an SM
+// CTAs an SM; each: bytes of a weight
+__host__ __device__ constexpr int expand_ctas(int each, int tile, int quads) { return each == 4 && quads == 2 && tile == 64 ? 2 : 3; }
 template <typename T, int TILE, int QUADS, int PIECES, bool VEC>
 __global__ void __launch_bounds__(kThreads, expand_ctas(sizeof(T), TILE, QUADS)) lora_expand_kernel(const __grid_constant__ LoraArgs p, const bool onto) {
     constexpr int kRows = expand_rows(TILE), kParts = TILE / kRows, NB = kRows > 8 ? 2 : 1, kAcross = expand_columns(TILE);
@@ -578,7 +579,8 @@ int launch_expand(const LoraCall& c, const LoraArgs& p, bool onto, int64_t tiles
     if (!di) return Q4FC_ECUDA;
     const bool vec = expand_vec(c, 4 * QUADS);
     constexpr int kChunk = 16 * QUADS * PIECES;
-    const int64_t pieces = tiles * (TILE / expand_rows(TILE)) * ((c.N + expand_columns(TILE) - 1) / expand_columns(TILE)), most = expand_ctas(sizeof(T), TILE, QUADS) * di->sm_count;
+    const int64_t pieces = tiles * (TILE / expand_rows(TILE)) * ((c.N + expand_columns(TILE) - 1) / expand_columns(TILE));
+    const int64_t most = expand_ctas(sizeof(T), TILE, QUADS) * di->sm_count;
     DependentLaunch l(dim3((unsigned)(pieces < most ? pieces : most)), kThreads, s);
     auto* fn = vec ? lora_expand_kernel<T, TILE, QUADS, PIECES, true> : lora_expand_kernel<T, TILE, QUADS, PIECES, false>;
     l.cfg.dynamicSmemBytes = expand_rows(TILE) * (size_t)expand_pitch((int)(c.rank + kChunk - 1) / kChunk * kChunk);
@@ -630,8 +632,9 @@ int launch_lora(const LoraCall& c, Step step, cudaStream_t s) {
     if (c.dtype == Q4FC_F16) return launch_lora_type<__half>(c, p, l, step, tiles, s);
     return launch_lora_type<__nv_bfloat16>(c, p, l, step, tiles, s);
 }
-// Both products in one launch where each CTA of the second would have few of the columns anyway: 133 rows x 1001 x 2999, fp32, rank 12, with
-// the FC 23.4 and 21.5 us, 8 rows x 4096 x 4096, rank 16, 13.7 and 12.9; but 61 rows x 4096 x 11008, rank 64, 45 and 49.
+// Both products in one launch where each CTA of the second would have few of the columns anyway.  In one launch and in two, with the FC: 133
+// rows x 1001 x 2999, fp32, rank 12, 21.2 and 21.8 us, 8 rows x 4096 x 4096, rank 16, 12.7 and 12.7; but 61 rows x 4096 x 11008, rank 64, 48.5
+// and 43.0.
 bool few(const LoraCall& c) {
     if (c.rows >= 256 || c.rank > kRankBlock) return false;
     const DeviceInfo* di = device_info();
