@@ -125,8 +125,8 @@ struct LoraArgs {
 };
 
 // A_i x of eight rows and MB times 16 ranks, by one warp: pieces of 32 k from k0 on, `step` apart, up to k_end.  `x`: the row of lane (g, t)'s
-// g, if `live`; `ranks`: of A that are there.  acc[m][i]: rank m * 16 + 8 (i / 2) + g of row 2t + i % 2.
-template <typename T, int MB, bool VEC>
+// g, if `live`; `ranks`: of A that are there.  DEPTH: pieces at a time of up to 32 ranks.  acc[m][i]: rank m * 16 + 8 (i / 2) + g of row 2t + i % 2.
+template <typename T, int MB, bool VEC, bool PAST_L1, int DEPTH>
 __device__ __forceinline__ void shrink_rows(const float* x, bool live, const T* a, int ranks, int64_t K, int64_t k0, int64_t k_end, int64_t step,
                                             float (&acc)[MB][4]) {
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -134,12 +134,23 @@ __device__ __forceinline__ void shrink_rows(const float* x, bool live, const T* 
         const int64_t left = k_end - k0 - 8 * t;
         return VEC ? left : left < 8 ? left : 8;
     };
-    auto load_x = [&](int64_t k0, float (&v)[8]) { load_values<8, VEC>(x + k0 + 8 * t, live ? there(k0) : 0, v); };
+    // past L1, value by value: every fourth one from t on instead of eight in a row, so that loads share sectors
+    auto load_few = [&](const auto* p, int left, auto& v) {
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+            if (4 * i < left) v[i] = __ldcg(p + 4 * i);
+            else v[i] = 0.0f;
+    };
+    auto load_x = [&](int64_t k0, float (&v)[8]) {
+        if constexpr (PAST_L1) load_few(x + k0 + t, live ? (int)(k_end - k0 < 32 ? k_end - k0 : 32) - t : 0, v);
+        else load_values<8, VEC>(x + k0 + 8 * t, live ? there(k0) : 0, v);
+    };
     auto load_a = [&](int64_t k0, int m, T (&w)[2][8]) {
 #pragma unroll
         for (int h = 0; h < 2; h++) {
             const int r = m * 16 + h * 8 + g;
-            load_values<8, VEC>(a + (int64_t)r * K + k0 + 8 * t, r < ranks ? there(k0) : 0, w[h]);
+            if constexpr (PAST_L1) load_few(a + (int64_t)r * K + k0 + t, r < ranks ? (int)(k_end - k0 < 32 ? k_end - k0 : 32) - t : 0, w[h]);
+            else load_values<8, VEC>(a + (int64_t)r * K + k0 + 8 * t, r < ranks ? there(k0) : 0, w[h]);
         }
     };
     auto split_x = [&](const float (&v)[8], int j, uint4 (&s)[2]) {
@@ -184,7 +195,7 @@ __device__ __forceinline__ void shrink_rows(const float* x, bool live, const T* 
 #pragma unroll
             for (int m = 0; m < MB; m++) load_a(k0, m, c.w[m]);
         };
-        constexpr int kDepth = VEC && MB * sizeof(T) < 8 ? 3 : 1;
+        constexpr int kDepth = VEC && MB * sizeof(T) < 8 ? DEPTH : 1;
         Piece c[kDepth];
 #pragma unroll
         for (int d = 0; d + 1 < kDepth; d++)
@@ -333,17 +344,17 @@ __device__ __forceinline__ void zero_rows(const LoraArgs& p, int64_t first, int6
 
 // ---- few rows and up to 64 ranks: both products in one launch ---------------------------------------------------------------------------
 // A cluster per tile of eight rows: its CTAs divide K (and their warps that again), their sums meet in every one of them, and then they
-// divide the columns.  With `early` (VEC) the launch in front computes y alone: all else is complete, and the first product does not wait
-// for it.  (133 rows x 1000 x 3000, 3 fp32 adapters of rank 12, with the FC 21.9 us, so 19.4.  Value by value, 1001 x 2999, loads behind the
-// fence take longer than the wait, 22.0 and 21.4.)  CTAs behind those of the tiles quantize x for the decode FC (quant_pre.cuh), which has to
-// be done in front of it anyway.
-// Registers: two CTAs on an SM, and up to 16 ranks one beside a CTA of the prefill GEMM (16 rows x 4096 x 4096, 4 bf16 adapters of rank 16, with
-// the FC: 118 registers 19.9 us, 96 18.5).
-template <typename T, int MB, bool VEC>
-__global__ void __maxnreg__(MB == 1 ? 96 : 128) lora_few_kernel(const __grid_constant__ LoraArgs p, const __grid_constant__ QuantPre q, const bool onto,
-                                                               const bool begin_early) {
+// divide the columns.  With `early` the launch in front computes y alone: all else is complete, and the first product does not wait
+// for it (12 rows x 6528 x 3057, 8 bf16 adapters of rank 24, with plan and FC 24.6 us, so 19.9): x and A in wide loads behind a fence, or value
+// by value past L1 (through it, behind a fence, 133 rows x 1001 x 2999, 3 fp32 adapters of rank 12, 22.0 us, waiting 21.4, so 20.5).  CTAs
+// behind those of the tiles quantize x for the decode FC (quant_pre.cuh), which has to be done in front of it anyway.
+// Registers: two CTAs on an SM, and up to 32 ranks one beside a CTA of the prefill GEMM (16 rows x 4096 x 4096, 4 bf16 adapters of rank 16, with
+// the FC: 118 registers 19.9 us, 96 18.5; 64 rows, 16 of rank 32, 128 registers 27.3, 112, and two pieces on their way instead of three, 26.9).
+template <typename T, int MB, bool VEC_A, bool VEC_B>
+__global__ void __maxnreg__(MB == 1 ? 96 : MB == 2 && (sizeof(T) == 2 || !VEC_A) ? 112 : 128)
+    lora_few_kernel(const __grid_constant__ LoraArgs p, const __grid_constant__ QuantPre q, const bool onto, const bool early) {
     constexpr int kRanks = MB * 16, QUADS = MB == 1 ? 1 : 2, PIECES = MB == 4 && sizeof(T) < 4 ? 2 : 1, kAcross = kWarps * 16;
-    using C = Columns<T, QUADS, PIECES, 1, kAcross, VEC>;
+    using C = Columns<T, QUADS, PIECES, 1, kAcross, VEC_B>;
     constexpr int kPitch = expand_pitch((kRanks + C::kChunk - 1) / C::kChunk * C::kChunk) / 16;
     __shared__ float sums[8 * kRanks];                 // this CTA's [row][rank]
     __shared__ float by_warp[kWarps * 8 * kRanks];
@@ -355,9 +366,8 @@ __global__ void __maxnreg__(MB == 1 ? 96 : 128) lora_few_kernel(const __grid_con
         pdl_wait_prior_grid();
         pdl_launch_dependents();
     };
-    const bool early = VEC && begin_early;
-    if (early) pdl_reads_early();
-    else others_done();
+    if (VEC_A && early) pdl_reads_early();  // (value by value x and A come past L1)
+    if (!early) others_done();
     if ((int)blockIdx.y >= q.first_block) {
         quant_pre_block(q, ((int64_t)(blockIdx.y - q.first_block) * slices + here) * kWarps + warp);
         return;
@@ -370,8 +380,8 @@ __global__ void __maxnreg__(MB == 1 ? 96 : 128) lora_few_kernel(const __grid_con
         const bool live = g < tile.z;
         const float* x = p.x + (live ? (int64_t)__ldcg(p.order + tile.y + g) * p.ldx : 0);
         float acc[MB][4] = {};
-        shrink_rows<T, MB, VEC>(x, live, static_cast<const T*>(p.a) + (int64_t)tile.x * p.rank * p.K, p.rank, p.K, k_begin + warp * 32, k_end,
-                                       kWarps * 32, acc);
+        shrink_rows<T, MB, VEC_A, !VEC_A, MB == 2 ? 2 : 3>(x, live, static_cast<const T*>(p.a) + (int64_t)tile.x * p.rank * p.K, p.rank, p.K,
+                                                           k_begin + warp * 32, k_end, kWarps * 32, acc);
         float* mine = by_warp + warp * 8 * kRanks;
 #pragma unroll
         for (int m = 0; m < MB; m++)
@@ -433,7 +443,7 @@ __global__ void __launch_bounds__(kThreads, 2) lora_shrink_kernel(const __grid_c
     const float* x = p.x + (live ? (int64_t)__ldcg(p.order + tile.y + row0 + g) * p.ldx : 0);
     float acc[MB][4] = {};
     if (row0 < tile.z)
-        shrink_rows<T, MB, VEC>(x, live, static_cast<const T*>(p.a) + ((int64_t)tile.x * p.rank + rank0) * p.K, p.rank - rank0, p.K,
+        shrink_rows<T, MB, VEC, false, 3>(x, live, static_cast<const T*>(p.a) + ((int64_t)tile.x * p.rank + rank0) * p.K, p.rank - rank0, p.K,
                                 k_begin + (kByK ? warp * 32 : 0), k_end, kByK ? kWarps * 32 : 32, acc);
     float* mine = kByK ? by_warp + warp * TILE * kRanks : sums + row0 * kRanks;
 #pragma unroll
@@ -563,7 +573,9 @@ struct ClusterLaunch : DependentLaunch {
 template <typename T, int MB>
 int launch_few(const LoraCall& c, const LoraArgs& p, const QuantPre& q, bool onto, bool early, dim3 grid, cudaStream_t s) {
     ClusterLaunch l(grid, (int)grid.x, s);
-    auto* fn = shrink_vec(c) && expand_vec(c, MB == 1 ? 4 : 8) ? lora_few_kernel<T, MB, true> : lora_few_kernel<T, MB, false>;
+    const bool vec_b = expand_vec(c, MB == 1 ? 4 : 8);
+    auto* fn = shrink_vec(c) ? vec_b ? lora_few_kernel<T, MB, true, true> : lora_few_kernel<T, MB, true, false>
+                             : vec_b ? lora_few_kernel<T, MB, false, true> : lora_few_kernel<T, MB, false, false>;
     Q4FC_CUDA_OK(cudaLaunchKernelEx(&l.cfg, fn, p, q, onto, early));
     return Q4FC_OK;
 }
@@ -633,7 +645,7 @@ int launch_lora(const LoraCall& c, Step step, cudaStream_t s) {
     return launch_lora_type<__nv_bfloat16>(c, p, l, step, tiles, s);
 }
 // Both products in one launch where each CTA of the second would have few of the columns anyway.  In one launch and in two, with the FC: 133
-// rows x 1001 x 2999, fp32, rank 12, 21.2 and 21.8 us, 8 rows x 4096 x 4096, rank 16, 12.7 and 12.7; but 61 rows x 4096 x 11008, rank 64, 48.5
+// rows x 1001 x 2999, fp32, rank 12, 20.3 and 21.8 us, 8 rows x 4096 x 4096, rank 16, 12.7 and 12.7; but 61 rows x 4096 x 11008, rank 64, 48.5
 // and 43.0.
 bool few(const LoraCall& c) {
     if (c.rows >= 256 || c.rank > kRankBlock) return false;
