@@ -274,7 +274,8 @@ def test_long_sums_are_as_good_as_fp32(pkg, rows, n, r, K, N, dtype, positive):
 
 
 @pytest.mark.parametrize("rows,n,rank,K,N", [(5, 3, 16, 512, 256), (5, 8, 72, 512, 256), (61, 3, 16, 512, 256), (61, 40, 64, 320, 2048),
-                                             (133, 3, 12, 251, 301), (300, 4, 32, 512, 256)])
+                                             (133, 3, 12, 251, 301), (300, 4, 32, 512, 256), (40, 3, 16, 512, 257), (40, 3, 16, 250, 256),
+                                             (40, 3, 24, 512, 131), (40, 3, 24, 245, 130), (40, 3, 64, 512, 131), (40, 3, 64, 245, 130)])
 def test_all_inputs_are_written_directly_in_front(pkg, rows, n, rank, K, N):
     """x, both products' weights, the plan and y change between calls that nothing waits for: a launch that begins early reads the new ones."""
     ops = pkg.llmops
